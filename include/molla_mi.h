@@ -328,6 +328,107 @@ int mi_decoder_layer_paged(mi_stream stream, const mi_layer_desc* desc, float* r
                            uint16_t* v_pool, const int32_t* kv_index, int64_t index_stride, const int32_t* pos,
                            int32_t max_count, int32_t tokens, void* work, size_t work_bytes);
 
+/* ---- a step over trees of drafted tokens (no counterpart in the reference) -
+ * Several drafted continuations of each sequence verified in one pass: the
+ * tokens of a sequence are the nodes of a tree, each seeing the sequence's
+ * committed positions, its ancestors and itself.  Token rows lie sequence by
+ * sequence: those of sequence b are starts[b] .. starts[b + 1] - 1, so that
+ * every size but the largest is a device value and a captured step serves any
+ * of them.  Node i of a sequence of length n lies at slot n + i of its cache,
+ * whatever its depth; its rotary position is n + its depth. */
+
+/* Block tables and slot maps of a step.  Request b holds lengths[b] positions
+ * and gets news[b] more (below 0: 0), at most 4096 requests.  Position j lies in
+ * cell table[b * table_stride + j / page] * page + j % page.  New pages come off
+ * the end of free_pages (free_count[0] of them, at most free_size) in the order
+ * of the requests and go into the table; where the list runs out, or a position
+ * lies past the table or the list, the cell is -1.  Written: starts[0..batch],
+ * free_left[0..1] (pages left, and pages wanted beyond the list; it may not be
+ * free_count), and for each new token t its cells[t], seq[t] (the request) and
+ * pos[t] (the position; both may be NULL), and its entry of kv_index (may be
+ * NULL), the lists that mi_decoder_layer_paged and mi_attend_tree read.  Token
+ * rows past max_tokens are not planned: starts ends there; rows behind the last
+ * one keep what they held. */
+int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* lengths, const int32_t* news,
+                 int32_t* table, int32_t table_stride, const int32_t* free_pages, int32_t free_size,
+                 const int32_t* free_count, int32_t* free_left, int32_t* kv_index, int64_t index_stride,
+                 int32_t max_tokens, int32_t* starts, int32_t* seq, int32_t* pos, int32_t* cells);
+
+/* uint32 words of a node's mask at trees of up to max_nodes (1..256). */
+int32_t mi_tree_words(int32_t max_nodes);
+
+/* The trees of a step from their parents: parents[t] is the place in its own
+ * sequence of the node that token t follows, or -1 for one that follows the
+ * committed tokens; a parent comes before its node (another value makes a root).
+ * mask[t * words + i / 32] bit i % 32 says whether token t sees node i of its
+ * sequence; pos[t] = lengths[b] + depth (pos may be NULL).  Tokens past
+ * max_nodes of a sequence see no node.  tokens: rows of the buffers. */
+int mi_tree_plan(mi_stream stream, int32_t batch, const int32_t* starts, const int32_t* lengths,
+                 const int32_t* parents, int32_t max_nodes, int32_t tokens, int32_t* pos, uint32_t* mask);
+
+/* Each head of q and k RMS-normed (q_norm and k_norm, device f32[head_dim], or
+ * both NULL), its first rope_dim values rotated as mi_rope does (rope_factors as
+ * in mi_layer_desc, or NULL), in one pass; q to q_out, k to k_out (NULL: not
+ * kept), and k and v to cache rows cells[t] of either form (k_cache, v_cache and
+ * cells, or all three and v NULL).  A negative cell stores nothing.  q_out may be
+ * q and k_out k, at the same stride.  count (device int32, or NULL): rows from
+ * *count on are left alone.  The k/v caches are rows of mi_cache_row(cache_form,
+ * kv_heads * head_dim) halves. */
+typedef struct {
+  int32_t heads, kv_heads, head_dim, rope_dim;
+  int32_t neox;
+  int32_t cache_form;
+  int32_t tokens;
+  float eps;
+  const float* q; /* device f32 rows, q_stride floats apart; likewise k and v */
+  const float* k;
+  const float* v;
+  int64_t q_stride, k_stride, v_stride;
+  float* q_out;
+  float* k_out;
+  int64_t q_out_stride, k_out_stride;
+  const float* q_norm;
+  const float* k_norm;
+  const float* rope_steps; /* device f32[rope_dim/2] from mi_rope_steps */
+  const float* rope_factors;
+  const int32_t* pos; /* device int32[tokens], the rotary positions */
+  const int32_t* count;
+  uint16_t* k_cache;
+  uint16_t* v_cache;
+  const int32_t* cells; /* device int32[tokens] */
+} mi_qk;
+int mi_qk_norm_rope(mi_stream stream, const mi_qk* desc);
+
+/* The trees of a step as attention and the layer read them. */
+typedef struct {
+  int32_t batch;     /* sequences */
+  int32_t tokens;    /* rows of the token buffers: starts[batch] is at most that */
+  int32_t max_nodes; /* tokens of a sequence, at most 256 */
+  int32_t max_count; /* positions of a sequence with its nodes: lengths[b] + nodes is at most that */
+  const int32_t* starts;  /* device int32[batch + 1] */
+  const int32_t* lengths; /* device int32[batch] */
+  const uint32_t* mask;   /* device uint32[tokens * mi_tree_words(max_nodes)] */
+  const int32_t* pos;     /* device int32[tokens], rotary positions: the layer's */
+  const int32_t* cells;   /* device int32[tokens], cache rows (negative: not stored): the layer's */
+} mi_tree;
+
+/* Attention of a step's tokens over the caches, either form: token t of
+ * sequence b sees slots 0 .. lengths[b] - 1 and those slots lengths[b] + i whose
+ * node i its mask has.  Slot j is row j of the sequence's cache, cache_stride
+ * halves from the one before, or with kv_index pool cell kv_index[b *
+ * index_stride + j] (negative: not held, not seen).  q and out are rows of
+ * heads * head_dim floats, q's q_stride apart (16-byte aligned).  A token that
+ * sees nothing gets zeros; rows behind the last sequence keep what they held.
+ * What a token does not see changes no bit of its result, whatever it holds.
+ * GQA groups and head widths as mi_attend.  Workspace:
+ * mi_attend_tree_workspace, 256-byte aligned. */
+size_t mi_attend_tree_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form,
+                                const mi_tree* tree);
+int mi_attend_tree(mi_stream stream, int32_t form, const float* q, int64_t q_stride, const uint16_t* k_cache,
+                   const uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
+                   int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, const mi_tree* tree, float* out,
+                   void* work, size_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

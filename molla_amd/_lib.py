@@ -31,6 +31,19 @@ class MiLayerDesc(ctypes.Structure):
                [("ungated", I32), ("act", I32), ("next_norm", P), ("prenormed", I32)]
 
 
+class MiQk(ctypes.Structure):
+    _fields_ = [(n, I32) for n in ("heads", "kv_heads", "head_dim", "rope_dim", "neox", "cache_form", "tokens")] + \
+               [("eps", F), ("q", P), ("k", P), ("v", P), ("q_stride", I64), ("k_stride", I64), ("v_stride", I64),
+                ("q_out", P), ("k_out", P), ("q_out_stride", I64), ("k_out_stride", I64)] + \
+               [(n, P) for n in ("q_norm", "k_norm", "rope_steps", "rope_factors", "pos", "count", "k_cache", "v_cache",
+                                 "cells")]
+
+
+class MiTree(ctypes.Structure):
+    _fields_ = [(n, I32) for n in ("batch", "tokens", "max_nodes", "max_count")] + \
+               [(n, P) for n in ("starts", "lengths", "mask", "pos", "cells")]
+
+
 # Every symbol include/molla_mi.h declares, with its C signature.
 SIGNATURES = {
     "mi_version": (ctypes.c_int, []),
@@ -64,6 +77,13 @@ SIGNATURES = {
     "mi_decoder_layer": (ctypes.c_int, [P, ctypes.POINTER(MiLayerDesc), P, P, P, I64, P, I32, I32, P, SZ]),
     "mi_decoder_layer_paged": (ctypes.c_int, [P, ctypes.POINTER(MiLayerDesc), P, P, P, P, I64, P, I32, I32, P,
                                               SZ]),
+    "mi_page_plan": (ctypes.c_int, [P, I32, I32, P, P, P, I32, P, I32, P, P, P, I64, I32, P, P, P, P]),
+    "mi_tree_words": (I32, [I32]),
+    "mi_tree_plan": (ctypes.c_int, [P, I32, P, P, P, I32, I32, P, P]),
+    "mi_qk_norm_rope": (ctypes.c_int, [P, ctypes.POINTER(MiQk)]),
+    "mi_attend_tree_workspace": (SZ, [I32, I32, I32, I32, ctypes.POINTER(MiTree)]),
+    "mi_attend_tree": (ctypes.c_int, [P, I32, P, I64, P, P, I64, P, I64, I32, I32, I32, F, ctypes.POINTER(MiTree), P, P,
+                                      SZ]),
 }
 
 _lib = None

@@ -293,6 +293,46 @@ int launch_act(hipStream_t s, float* x, int64_t n, int32_t act);
 int launch_embed(hipStream_t s, const float* emb, int32_t vocab, int32_t width, const int32_t* ids,
                  int32_t tokens, float* out);
 
+// ---- a step over drafted tokens ---------------------------------------------
+// plan.hip
+constexpr int kMaxPlanBatch = 4096;  // requests of a page plan (its scans' LDS)
+constexpr int kMaxTreeNodes = 256;   // drafted tokens of a sequence
+constexpr int kMaxTreeRows = 1 << 30;  // token rows of a step
+constexpr int kMaxHeadsWidth = 1 << 20;  // values of a token's heads
+struct PagePlan {
+  int32_t batch, page, max_tokens, free_size;
+  int64_t table_stride, index_stride, max_pos;  // max_pos: positions the table and the list have room for
+  const int32_t *lengths, *news, *free_pages, *free_count;
+  int32_t *table, *kv_index, *free_left, *starts, *seq, *pos, *cells;
+};
+int launch_page_plan(hipStream_t s, const PagePlan& p);
+int launch_tree_plan(hipStream_t s, int32_t batch, const int32_t* starts, const int32_t* lengths,
+                     const int32_t* parents, int32_t max_nodes, int32_t tokens, int32_t* pos, uint32_t* mask);
+// Each head of q and k normed and rotated, q to q_out and k and v to cache rows
+// (qk_rope.hip).  The row of token t is cells[t], or without cells the one that
+// rope_store takes: kv_index[t * index_stride + pos[t]], or pos[t] of the cache
+// t * cache_stride halves on.  A negative row stores nothing.
+struct QkRope {
+  mi_qk d;
+  int64_t cache_stride, index_stride;
+  const int32_t* kv_index;
+};
+int launch_qk_rope(hipStream_t s, const QkRope& a);
+// attend_tree.hip: attention of trees of drafted tokens (mi_attend_tree).
+struct TreeAttend {
+  const float* q;
+  int64_t q_stride;
+  const uint16_t *k_cache, *v_cache;
+  int64_t cache_stride, index_stride;
+  const int32_t* kv_index;
+  int32_t heads, kv_heads, head_dim, form;
+  float scale;
+  mi_tree tree;
+  float* out;
+};
+size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const mi_tree& tree);
+int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work);
+
 // ---- small device helpers -----------------------------------------------
 
 __device__ __forceinline__ float half_bits_to_float(uint32_t h16) {

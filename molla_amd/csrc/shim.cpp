@@ -406,4 +406,146 @@ int mi_embed(mi_stream stream, const float* embedding, int32_t vocab, int32_t wi
   return launch_embed((hipStream_t)stream, embedding, vocab, width, ids, tokens, out);
 }
 
+// ---- a step over trees of drafted tokens -------------------------------------
+
+int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* lengths, const int32_t* news,
+                 int32_t* table, int32_t table_stride, const int32_t* free_pages, int32_t free_size,
+                 const int32_t* free_count, int32_t* free_left, int32_t* kv_index, int64_t index_stride,
+                 int32_t max_tokens, int32_t* starts, int32_t* seq, int32_t* pos, int32_t* cells) {
+  if (!lengths || !news || !table || !free_count || !free_left || !starts || !cells)
+    return fail(MI_ERR_ARG, "page_plan: null pointer");
+  if (batch < 1 || batch > kMaxPlanBatch) return fail(MI_ERR_SHAPE, "page_plan: batch %d outside 1..%d", batch, kMaxPlanBatch);
+  if (page < 1 || table_stride < 1) return fail(MI_ERR_SHAPE, "page_plan: pages of %d, %d a request", page, table_stride);
+  if (free_size < 0 || (free_size && !free_pages)) return fail(MI_ERR_ARG, "page_plan: a free list of %d pages", free_size);
+  if (free_left == free_count || free_left + 1 == free_count)
+    return fail(MI_ERR_ARG, "page_plan: free_left may not be free_count");
+  if (kv_index && index_stride < 1) return fail(MI_ERR_SHAPE, "page_plan: index stride %lld", (long long)index_stride);
+  if (max_tokens < 1 || max_tokens > kMaxTreeRows)
+    return fail(MI_ERR_SHAPE, "page_plan: max_tokens %d outside 1..%d", max_tokens, kMaxTreeRows);
+  PagePlan p{};
+  p.batch = batch;
+  p.page = page;
+  p.max_tokens = max_tokens;
+  p.free_size = free_size;
+  p.table_stride = table_stride;
+  p.index_stride = index_stride;
+  p.max_pos = std::min<int64_t>((int64_t)table_stride * page, kv_index ? index_stride : INT64_MAX);
+  p.lengths = lengths;
+  p.news = news;
+  p.free_pages = free_pages;
+  p.free_count = free_count;
+  p.table = table;
+  p.kv_index = kv_index;
+  p.free_left = free_left;
+  p.starts = starts;
+  p.seq = seq;
+  p.pos = pos;
+  p.cells = cells;
+  return launch_page_plan((hipStream_t)stream, p);
+}
+
+int32_t mi_tree_words(int32_t max_nodes) {
+  return max_nodes < 1 || max_nodes > kMaxTreeNodes ? -1 : (max_nodes + 31) / 32;
+}
+
+int mi_tree_plan(mi_stream stream, int32_t batch, const int32_t* starts, const int32_t* lengths,
+                 const int32_t* parents, int32_t max_nodes, int32_t tokens, int32_t* pos, uint32_t* mask) {
+  if (!starts || !lengths || !parents || !mask) return fail(MI_ERR_ARG, "tree_plan: null pointer");
+  if (batch < 1) return fail(MI_ERR_SHAPE, "tree_plan: batch %d", batch);
+  if (mi_tree_words(max_nodes) < 0)
+    return fail(MI_ERR_SHAPE, "tree_plan: trees of %d nodes, outside 1..%d", max_nodes, kMaxTreeNodes);
+  if (tokens < 1 || tokens > kMaxTreeRows) return fail(MI_ERR_SHAPE, "tree_plan: %d token rows", tokens);
+  return launch_tree_plan((hipStream_t)stream, batch, starts, lengths, parents, max_nodes, tokens, pos, mask);
+}
+
+int mi_qk_norm_rope(mi_stream stream, const mi_qk* d) {
+  if (!d) return fail(MI_ERR_ARG, "qk_norm_rope: null descriptor");
+  if (!d->q || !d->k || !d->q_out || !d->rope_steps || !d->pos) return fail(MI_ERR_ARG, "qk_norm_rope: null pointer");
+  const int stores = !!d->v + !!d->k_cache + !!d->v_cache + !!d->cells;
+  if (stores != 0 && stores != 4)
+    return fail(MI_ERR_ARG, "qk_norm_rope: v, both caches and the cells come together (%d of 4)", stores);
+  if (!d->q_norm != !d->k_norm) return fail(MI_ERR_ARG, "qk_norm_rope: q and k norms come together");
+  if (d->q_norm && !(d->eps > 0.0f)) return fail(MI_ERR_ARG, "qk_norm_rope: epsilon must be positive");
+  if (d->neox != 0 && d->neox != 1) return fail(MI_ERR_ARG, "qk_norm_rope: neox is 0 or 1, not %d", d->neox);
+  int rc = check_attn("qk_norm_rope", d->heads, d->kv_heads, d->head_dim);
+  if (rc) return rc;
+  if (d->rope_dim <= 0 || d->rope_dim % 2 || d->rope_dim > d->head_dim)
+    return fail(MI_ERR_SHAPE, "qk_norm_rope: rotary dimension %d in heads of %d", d->rope_dim, d->head_dim);
+  if (d->tokens < 1 || d->tokens > kMaxTreeRows) return fail(MI_ERR_SHAPE, "qk_norm_rope: %d tokens", d->tokens);
+  const int64_t qw = (int64_t)d->heads * d->head_dim, kvw = (int64_t)d->kv_heads * d->head_dim;
+  if (qw > kMaxHeadsWidth) return fail(MI_ERR_SHAPE, "qk_norm_rope: rows of %lld values", (long long)qw);
+  if (d->q_stride < qw || d->q_out_stride < qw || d->k_stride < kvw || (d->k_out && d->k_out_stride < kvw) ||
+      (stores && d->v_stride < kvw))
+    return fail(MI_ERR_SHAPE, "qk_norm_rope: row stride too small");
+  if ((d->q_out == d->q && d->q_out_stride != d->q_stride) || (d->k_out == d->k && d->k_out_stride != d->k_stride))
+    return fail(MI_ERR_SHAPE, "qk_norm_rope: in place at another stride");
+  if (stores && cache_row(d->cache_form, (int32_t)kvw) < 0)
+    return fail(MI_ERR_SHAPE, "qk_norm_rope: cache form %d has no row of width %lld", d->cache_form, (long long)kvw);
+  if (stores && (((uintptr_t)d->k_cache | (uintptr_t)d->v_cache) & 15))
+    return fail(MI_ERR_ALIGN, "qk_norm_rope: the caches must be 16-byte aligned");
+  QkRope a{};
+  a.d = *d;
+  return launch_qk_rope((hipStream_t)stream, a);
+}
+
+// A step's trees, for attention and (with `layer`) for a layer.
+int check_tree(const char* name, const mi_tree* t, bool layer) {
+  if (!t || !t->starts || !t->lengths || !t->mask) return fail(MI_ERR_ARG, "%s: null pointer in the trees", name);
+  if (layer && (!t->pos || !t->cells)) return fail(MI_ERR_ARG, "%s: the trees need pos and cells", name);
+  if (t->batch < 1 || t->tokens < 1 || t->tokens > kMaxTreeRows)
+    return fail(MI_ERR_SHAPE, "%s: %d sequences in %d token rows", name, t->batch, t->tokens);
+  if (mi_tree_words(t->max_nodes) < 0)
+    return fail(MI_ERR_SHAPE, "%s: trees of %d nodes, outside 1..%d", name, t->max_nodes, kMaxTreeNodes);
+  if (t->max_count < 1) return fail(MI_ERR_SHAPE, "%s: max_count must be positive", name);
+  return MI_OK;
+}
+
+size_t mi_attend_tree_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form,
+                                const mi_tree* tree) {
+  if (check_attn("attend_tree", heads, kv_heads, head_dim) || (int64_t)heads * head_dim > kMaxHeadsWidth ||
+      cache_row(form, kv_heads * head_dim) < 0 || !tree || tree->batch < 1 || tree->tokens < 1 ||
+      tree->tokens > kMaxTreeRows || mi_tree_words(tree->max_nodes) < 0 || tree->max_count < 1)
+    return 0;
+  return tree_attend_workspace(heads, kv_heads, head_dim, form, *tree);
+}
+
+int mi_attend_tree(mi_stream stream, int32_t form, const float* q, int64_t q_stride, const uint16_t* k_cache,
+                   const uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
+                   int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, const mi_tree* tree, float* out,
+                   void* work, size_t work_bytes) {
+  if (!q || !k_cache || !v_cache || !out) return fail(MI_ERR_ARG, "attend_tree: null pointer");
+  int rc = check_attn("attend_tree", heads, kv_heads, head_dim);
+  if (rc) return rc;
+  if ((int64_t)heads * head_dim > kMaxHeadsWidth)
+    return fail(MI_ERR_SHAPE, "attend_tree: rows of %lld values", (long long)heads * head_dim);
+  const int32_t row = cache_row(form, kv_heads * head_dim);
+  if (row < 0) return fail(MI_ERR_SHAPE, "attend_tree: unknown cache form %d", form);
+  if ((rc = check_tree("attend_tree", tree, false))) return rc;
+  if (q_stride < (int64_t)heads * head_dim) return fail(MI_ERR_SHAPE, "attend_tree: row stride too small");
+  if (kv_index ? index_stride < tree->max_count : (tree->batch > 1 && cache_stride < (int64_t)tree->max_count * row))
+    return fail(MI_ERR_SHAPE, "attend_tree: a sequence's stride holds fewer than %d positions", tree->max_count);
+  if ((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) || q_stride % 4 ||
+      (!kv_index && cache_stride % 8))
+    return fail(MI_ERR_ALIGN, "attend_tree: the queries, the caches and the output must be 16-byte aligned");
+  const size_t need = mi_attend_tree_workspace(heads, kv_heads, head_dim, form, tree);
+  if (!work || ((uintptr_t)work & 255) || work_bytes < need)
+    return fail(MI_ERR_WORKSPACE, "attend_tree: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);
+  TreeAttend a{};
+  a.q = q;
+  a.q_stride = q_stride;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.cache_stride = tree->batch > 1 ? cache_stride : 0;
+  a.index_stride = index_stride;
+  a.kv_index = kv_index;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.head_dim = head_dim;
+  a.form = form;
+  a.scale = scale;
+  a.tree = *tree;
+  a.out = out;
+  return launch_tree_attend((hipStream_t)stream, a, work);
+}
+
 }  // extern "C"

@@ -16,7 +16,7 @@ import ctypes
 import numpy as np
 import torch
 
-from ._lib import MiError, MiLayerDesc, MiWeight, check, lib
+from ._lib import MiError, MiLayerDesc, MiQk, MiTree, MiWeight, check, lib
 
 # ggml type numbers, src/molla/nn/quant.mojo:47-57
 Q_F32, Q_F16, Q_Q4_0, Q_Q4_1, Q_Q5_0, Q_Q5_1, Q_Q8_0, Q_Q4_K, Q_Q5_K, Q_Q6_K = 0, 1, 2, 3, 6, 7, 8, 12, 13, 14
@@ -90,6 +90,7 @@ class DeviceContext:
         self.device = torch.device("cuda", device)
         self.stream = stream if stream is not None else torch.cuda.current_stream(self.device)
         self._work = None
+        self._captured = []  # workspaces that a captured graph replays on
         lib()  # fail now, not at the first launch, if the library is missing
 
     @property
@@ -99,7 +100,11 @@ class DeviceContext:
     def workspace(self, nbytes: int) -> torch.Tensor:
         nbytes = max(int(nbytes), 256)
         if self._work is None or self._work.numel() < nbytes:
-            self._work = torch.empty(nbytes + 256, dtype=torch.uint8, device=self.device)
+            # (of the stream that runs on it, so that one it replaces is reused in that order)
+            with torch.cuda.stream(self.stream):
+                self._work = torch.empty(nbytes + 256, dtype=torch.uint8, device=self.device)
+        if torch.cuda.is_current_stream_capturing() and not any(w is self._work for w in self._captured):
+            self._captured.append(self._work)
         return self._work
 
     def synchronize(self) -> None:
@@ -263,6 +268,154 @@ def device_embed(ctx: DeviceContext, embedding: torch.Tensor, ids: torch.Tensor,
     vocab, width = embedding.shape
     check(lib().mi_embed(ctx.handle, embedding.data_ptr(), vocab, width, ids.data_ptr(), ids.numel(),
                          out.data_ptr()))
+
+
+# ---- a step over trees of drafted tokens (no counterpart in the reference) ----
+def _queue(ctx: DeviceContext, fn, *args) -> None:
+    """A library call on the context's stream, with its device current."""
+    if torch.cuda.current_device() == ctx.device.index:
+        check(fn(ctx.handle, *args))
+    else:
+        with torch.cuda.device(ctx.device):
+            check(fn(ctx.handle, *args))
+
+
+def _on(ctx: DeviceContext, t: torch.Tensor, name: str, dtype: torch.dtype, numel: int = 0) -> int:
+    """The address of a contiguous tensor of the context's device, at least `numel` long."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != ctx.device or not t.is_contiguous():
+        raise ValueError(f"{name} has to be a contiguous {dtype} tensor on {ctx.device}")
+    if t.numel() < numel:
+        raise ValueError(f"{name} has {t.numel()} values where {numel} are needed")
+    return t.data_ptr()
+
+
+def _rows(ctx: DeviceContext, t: torch.Tensor, name: str, tokens: int, width: int) -> int:
+    """The row stride of a float32 tensor of at least `tokens` rows of `width` values, each row contiguous."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != ctx.device or t.dim() != 2 or \
+            t.shape[0] < tokens or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} has to be float32 rows on {ctx.device}, at least {tokens} x {width}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+def device_page_plan(ctx: DeviceContext, page: int, lengths: torch.Tensor, news: torch.Tensor, table: torch.Tensor,
+                     free_pages: torch.Tensor, free_count: torch.Tensor, free_left: torch.Tensor, starts: torch.Tensor,
+                     seq: torch.Tensor | None, pos: torch.Tensor | None, cells: torch.Tensor,
+                     kv_index: torch.Tensor | None = None) -> None:
+    """Block tables and slot maps of a step (mi_page_plan): request b holds
+    lengths[b] positions and gets news[b] more, in pages of `page` off the end of
+    free_pages[:free_count].  Writes starts[batch + 1], the new pages into table
+    [batch, pages], seq, pos and cells of every new token (as many rows as they
+    have; seq and pos may be None), their entries of kv_index [batch, positions],
+    and free_left = (pages left, pages wanted beyond them).  All int32."""
+    i32 = torch.int32
+    batch = lengths.numel()
+    if table.dim() != 2 or table.shape[0] != batch or (kv_index is not None and (kv_index.dim() != 2 or
+                                                                                 kv_index.shape[0] != batch)):
+        raise ValueError(f"page_plan wants a table and a list a request ({batch})")
+    tokens = cells.numel()
+    _queue(ctx, lib().mi_page_plan, batch, page, _on(ctx, lengths, "lengths", i32), _on(ctx, news, "news", i32, batch),
+           _on(ctx, table, "table", i32), table.shape[1], _on(ctx, free_pages, "free_pages", i32), free_pages.numel(),
+           _on(ctx, free_count, "free_count", i32, 1), _on(ctx, free_left, "free_left", i32, 2),
+           None if kv_index is None else _on(ctx, kv_index, "kv_index", i32),
+           0 if kv_index is None else kv_index.shape[1], tokens, _on(ctx, starts, "starts", i32, batch + 1),
+           None if seq is None else _on(ctx, seq, "seq", i32, tokens),
+           None if pos is None else _on(ctx, pos, "pos", i32, tokens), _on(ctx, cells, "cells", i32))
+
+
+def tree_words(max_nodes: int) -> int:
+    """int32 words of a node's mask (mi_tree_words)."""
+    words = lib().mi_tree_words(max_nodes)
+    if words < 0:
+        raise ValueError(f"a tree has 1 to 256 nodes, not {max_nodes}")
+    return words
+
+
+def device_tree_plan(ctx: DeviceContext, starts: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor,
+                     max_nodes: int, pos: torch.Tensor | None, mask: torch.Tensor) -> None:
+    """Ancestor masks and rotary positions of a step's trees (mi_tree_plan):
+    parents[t] is the place in its own sequence of the node that token t follows,
+    -1 for the committed tokens; mask [tokens, tree_words(max_nodes)] and pos
+    [tokens] (or None), int32."""
+    i32 = torch.int32
+    batch, tokens = lengths.numel(), parents.numel()
+    _queue(ctx, lib().mi_tree_plan, batch, _on(ctx, starts, "starts", i32, batch + 1),
+           _on(ctx, lengths, "lengths", i32), _on(ctx, parents, "parents", i32), max_nodes, tokens,
+           None if pos is None else _on(ctx, pos, "pos", i32, tokens),
+           _on(ctx, mask, "mask", i32, tokens * tree_words(max_nodes)))
+
+
+def device_qk_norm_rope(ctx: DeviceContext, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, heads: int,
+                        kv_heads: int, head_dim: int, dim: int, neox: bool, steps: torch.Tensor, pos: torch.Tensor,
+                        q_out: torch.Tensor, k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
+                        cells: torch.Tensor | None = None, form: int = CACHE_F16, k_out: torch.Tensor | None = None,
+                        q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-5,
+                        factors: torch.Tensor | None = None, count: torch.Tensor | None = None) -> None:
+    """Each head of q and k normed and rotated at pos[t], in one pass
+    (mi_qk_norm_rope): q to q_out, k to k_out, and with v, the caches and cells
+    (all four) k and v to the cache rows cells[t].  Rows are 2-D float32 views of
+    any row stride; q_out may be q and k_out k.  count (device int32): rows from
+    count on are left alone."""
+    f32, i32 = torch.float32, torch.int32
+    tokens = pos.numel()
+    qw, kvw = heads * head_dim, kv_heads * head_dim
+    d = MiQk(heads, kv_heads, head_dim, dim, int(neox), form, tokens, eps)
+    d.q, d.q_stride = q.data_ptr(), _rows(ctx, q, "q", tokens, qw)
+    d.k, d.k_stride = k.data_ptr(), _rows(ctx, k, "k", tokens, kvw)
+    d.q_out, d.q_out_stride = q_out.data_ptr(), _rows(ctx, q_out, "q_out", tokens, qw)
+    if k_out is not None:
+        d.k_out, d.k_out_stride = k_out.data_ptr(), _rows(ctx, k_out, "k_out", tokens, kvw)
+    if v is not None:
+        d.v, d.v_stride = v.data_ptr(), _rows(ctx, v, "v", tokens, kvw)
+    if k_cache is not None:
+        d.k_cache = _on(ctx, k_cache, "k_cache", torch.float16)
+    if v_cache is not None:
+        d.v_cache = _on(ctx, v_cache, "v_cache", torch.float16)
+    if cells is not None:
+        d.cells = _on(ctx, cells, "cells", i32, tokens)
+    if q_norm is not None:
+        d.q_norm = _on(ctx, q_norm, "q_norm", f32, head_dim)
+    if k_norm is not None:
+        d.k_norm = _on(ctx, k_norm, "k_norm", f32, head_dim)
+    if factors is not None:
+        d.rope_factors = _on(ctx, factors, "factors", f32, dim // 2)
+    if count is not None:
+        d.count = _on(ctx, count, "count", i32, 1)
+    d.rope_steps, d.pos = _on(ctx, steps, "steps", f32, dim // 2), _on(ctx, pos, "pos", i32)
+    _queue(ctx, lib().mi_qk_norm_rope, ctypes.byref(d))
+
+
+def device_attend_tree(ctx: DeviceContext, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, heads: int,
+                       kv_heads: int, head_dim: int, scale: float, starts: torch.Tensor, lengths: torch.Tensor,
+                       mask: torch.Tensor, max_nodes: int, max_count: int, out: torch.Tensor, cache_stride: int = 0,
+                       kv_index: torch.Tensor | None = None, form: int = CACHE_F16,
+                       work: torch.Tensor | None = None) -> None:
+    """Attention of a step's trees over the caches (mi_attend_tree): q [tokens,
+    heads * head_dim] (rows of any stride), out the same contiguous.  Sequence b's
+    slots are rows of its own cache, cache_stride halves after the one before, or
+    the cells kv_index[b]; lengths[b] of them are committed, its nodes behind."""
+    i32, f16 = torch.int32, torch.float16
+    batch, tokens = lengths.numel(), q.shape[0]
+    qw = heads * head_dim
+    q_stride = _rows(ctx, q, "q", tokens, qw)
+    row = cache_row(form, kv_heads * head_dim)
+    stride = 0
+    if kv_index is not None:
+        if kv_index.dim() != 2 or kv_index.shape[0] < batch:
+            raise ValueError(f"attend_tree wants a list of cells a sequence ({batch})")
+        stride = kv_index.shape[1]
+        least = 1
+    else:
+        least = (batch - 1) * cache_stride + max_count * row
+    tree = MiTree(batch, tokens, max_nodes, max_count, _on(ctx, starts, "starts", i32, batch + 1),
+                  _on(ctx, lengths, "lengths", i32), _on(ctx, mask, "mask", i32, tokens * tree_words(max_nodes)))
+    L = lib()
+    t = ctypes.byref(tree)
+    if work is None:
+        work = ctx.workspace(L.mi_attend_tree_workspace(heads, kv_heads, head_dim, form, t))
+    _queue(ctx, L.mi_attend_tree, form, q.data_ptr(), q_stride, _on(ctx, k_cache, "k_cache", f16, least),
+           _on(ctx, v_cache, "v_cache", f16, least), cache_stride,
+           None if kv_index is None else _on(ctx, kv_index, "kv_index", i32), stride, heads, kv_heads, head_dim, scale,
+           t, _on(ctx, out, "out", torch.float32, tokens * qw), work.data_ptr(), work.numel())
 
 
 __all__ = [n for n in dir() if not n.startswith("_")] + ["MiError"]
