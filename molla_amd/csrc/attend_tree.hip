@@ -3,11 +3,15 @@
 // of several sequences, every token over the sequence's committed positions and
 // the nodes of its own tree that its mask has, over an f16 or a q8_0 cache, GQA.
 //
-// A block takes a tile of one sequence's query rows (row = token, query head of
-// one key head) and a share of the keys, walked in slices with a running maximum
-// and sum, and writes one partial result a row; a second launch folds the
-// shares.  Sizes of the sequences are device values: a block finds its tokens
-// from starts and leaves when there are none.
+// The work is a line of units, one for each (sequence, key head, tile of query
+// rows, slice of keys), slices innermost; a query row is a token and a query head
+// of the key head.  Lengths are device values, so the blocks share the line among
+// themselves: each scans the sequences and takes an equal run of units, walking
+// its slices with a running maximum and sum.  Of the tiles in a run only the first
+// and the last can be another block's too: those leave partial results, two a
+// block, that a second launch folds; the others' rows are finished.  (Shares of
+// the keys fixed by the host leave every block waiting for the longest sequence:
+// eight of 8192 down to 4608 positions 165 us, so 112.)
 #include <math.h>
 
 #include <algorithm>
@@ -18,6 +22,7 @@ namespace mi {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMaxParts = 64;  // blocks that share a tile: the lanes of the fold
 
 // The tokens and keys of sequence b, each held to what the host has checked.
 struct TreeSeq {
@@ -32,6 +37,105 @@ __device__ __forceinline__ TreeSeq tree_seq(const mi_tree& tr, int b) {
   s.count = min(s.len + s.nodes, tr.max_count);
   return s;
 }
+
+__device__ __forceinline__ int tree_tiles(const TreeSeq& s, int group, int rows) {
+  return (s.nodes * group + rows - 1) / rows;
+}
+__device__ __forceinline__ int tree_slices(const TreeSeq& s, int slice) { return (s.count + slice - 1) / slice; }
+
+struct TreeScan {
+  int sum[8], top[8];
+  int b, at;
+};
+
+// Hands this block's units to `take`, a tile's run of slices at a time:
+// take(sequence, b, key head, tile, first slice, end, part), part -1 where the
+// run is the whole tile, else the block's part it goes to.  plan: units a block,
+// then each sequence's first unit (written by block 0, for the fold).
+template <int NT, class F>
+__device__ __forceinline__ void tree_walk(const TreeAttend& a, int rows, int slice, TreeScan& sh,
+                                          int32_t* __restrict__ plan, F take) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int group = a.heads / a.kv_heads, batch = a.tree.batch;
+  const int q = (batch + NT - 1) / NT;
+  auto units_of = [&](int b, int& slices) {
+    const TreeSeq s = tree_seq(a.tree, b);
+    slices = s.nodes ? tree_slices(s, slice) : 0;
+    return tree_tiles(s, group, rows) * a.kv_heads * slices;
+  };
+  int mine = 0, top = 0;
+  for (int b = tid * q; b < min((tid + 1) * q, batch); b++) {
+    int slices;
+    mine += units_of(b, slices);
+    top = max(top, slices);
+  }
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(upto, o);
+    if (lane >= o) upto += u;
+    top = max(top, __shfl_xor(top, o));
+  }
+  if (lane == 63) sh.sum[wave] = upto, sh.top[wave] = top;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; w++) {
+    if (w == wave) upto += total;
+    total += sh.sum[w];
+    top = max(top, sh.top[w]);
+  }
+  total = __builtin_amdgcn_readfirstlane(total);  // (the same in every lane)
+  top = __builtin_amdgcn_readfirstlane(top);
+  const int per = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, (top + kMaxParts - 3) / (kMaxParts - 2)), 1);
+  const int64_t first = (int64_t)blockIdx.x * per;
+  if (blockIdx.x == 0) {
+    if (tid == 0) plan[0] = per;
+    int at = upto - mine, slices;
+    for (int b = tid * q; b < min((tid + 1) * q, batch); b++) {
+      plan[1 + b] = at;
+      at += units_of(b, slices);
+    }
+  }
+  if (first >= total) return;  // (uniform over the block)
+  if (first >= upto - mine && first < upto) {
+    int at = upto - mine, slices;
+    for (int b = tid * q;; b++) {
+      const int u = units_of(b, slices);
+      if (first < at + u) {
+        sh.b = b;
+        sh.at = (int)first - at;
+        break;
+      }
+      at += u;
+    }
+  }
+  __syncthreads();
+  int b = __builtin_amdgcn_readfirstlane(sh.b), at = __builtin_amdgcn_readfirstlane(sh.at);
+  int left = (int)min<int64_t>(per, total - first);
+  while (true) {
+    const TreeSeq s = tree_seq(a.tree, b);
+    const int slices = tree_slices(s, slice), tiles = tree_tiles(s, group, rows);
+    while (at < slices * tiles * a.kv_heads) {
+      const int pair = at / slices, sl = at - pair * slices, n = min(slices - sl, left);
+      const int part = n == slices ? -1 : 2 * (int)blockIdx.x + (sl == 0 ? 1 : 0);
+      take(s, b, pair / tiles, pair % tiles, sl, sl + n, part);
+      left -= n;
+      if (left == 0) return;
+      at += n;
+    }
+    at = 0;
+    do b++;
+    while (tree_seq(a.tree, b).nodes == 0);
+  }
+}
+
+// Where part `part` of a tile's row keeps its sum, and behind all of them its
+// (maximum in base 2, sum).
+struct TreeParts {
+  float* acc;
+  float* ml;
+};
 
 // ---- any head width: the products on the VALU --------------------------------
 // 16 query rows a block, four a wave; a slice's keys and values in LDS as
@@ -48,148 +152,145 @@ __host__ __device__ __forceinline__ size_t rows_lds_bytes(int head_dim) {
 }
 
 template <bool Q8, int ND>
-__global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAttend a, int tiles, int shares,
-                                                                        float* __restrict__ part_acc,
-                                                                        float* __restrict__ part_ml) {
-  const int share = blockIdx.x % shares, rest = blockIdx.x / shares;
-  const int kvh = rest % a.kv_heads, z = rest / a.kv_heads, b = z / tiles, tile = z % tiles;
-  const TreeSeq sq = tree_seq(a.tree, b);
-  const int group = a.heads / a.kv_heads, tq = kRowsTile / group, n0 = tile * tq;
-  if (n0 >= sq.nodes) return;
-  const int D = a.head_dim, kk = rows_slice(D), KS = D + 4;
-  const int words = (a.tree.max_nodes + 31) >> 5;
+__global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAttend a, TreeParts parts,
+                                                                        int32_t* __restrict__ plan) {
+  __shared__ TreeScan scan;
   extern __shared__ float4 lds[];
+  const int D = a.head_dim, kk = rows_slice(D), KS = D + 4;
+  const int words = (a.tree.max_nodes + 31) >> 5, group = a.heads / a.kv_heads;
   float* Ks = (float*)lds;
   float* Vs = Ks + kk * KS;
   float* Qs = Vs + kk * D;
   float* Ps = Qs + kRowsTile * D;  // [wave][key][its 4 rows]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int kvw = a.kv_heads * D, crow = cache_row(a.form, kvw);
-  const __half* kc = (const __half*)a.k_cache + (a.kv_index ? 0 : (int64_t)b * a.cache_stride);
-  const __half* vc = (const __half*)a.v_cache + (a.kv_index ? 0 : (int64_t)b * a.cache_stride);
-  const int32_t* index = a.kv_index ? a.kv_index + (int64_t)b * a.index_stride : nullptr;
-
-  // queries; rows past the sequence repeat its last token (not written)
-  for (int i = tid; i < kRowsTile * D; i += kRowsThreads) {
-    const int r = i / D, e = i - r * D, node = min(n0 + r / group, sq.nodes - 1);
-    Qs[i] = a.q[(int64_t)(sq.t0 + node) * a.q_stride + (int64_t)(kvh * group + r % group) * D + e];
-  }
-  const int r0 = 4 * wave;
-  const uint32_t* mrow[4];
-#pragma unroll
-  for (int r = 0; r < 4; r++)
-    mrow[r] = a.tree.mask + (int64_t)(sq.t0 + min(n0 + (r0 + r) / group, sq.nodes - 1)) * words;
-
-  float m2[4], l[4], o[4][ND];
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    m2[r] = -INFINITY;
-    l[r] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < ND; i++) o[r][i] = 0.0f;
-  }
   const float c2 = a.scale * kLog2e;
-  const int parts = 64 / kk, part = lane / kk, key = lane % kk;
-  const int slices = (sq.count + kk - 1) / kk;
-  for (int sl = share; sl < slices; sl += shares) {
-    const int base = sl * kk;
+  const int split = 64 / kk, part_d = lane / kk, key = lane % kk;
+
+  tree_walk<kRowsThreads>(a, kRowsTile, kk, scan, plan, [&](const TreeSeq& sq, int b, int kvh, int tile, int s0, int s1,
+                                                            int part) {
+    const __half* kc = (const __half*)a.k_cache + (a.kv_index ? 0 : (int64_t)b * a.cache_stride);
+    const __half* vc = (const __half*)a.v_cache + (a.kv_index ? 0 : (int64_t)b * a.cache_stride);
+    const int32_t* index = a.kv_index ? a.kv_index + (int64_t)b * a.index_stride : nullptr;
+    // queries; rows past the sequence repeat its last token (not written)
     __syncthreads();
-    for (int i = tid; i < kk * (D / 8); i += kRowsThreads) {
-      const int k = i / (D / 8), e = 8 * (i - k * (D / 8)), j = min(base + k, sq.count - 1);
-      const int64_t at = (int64_t)(index ? max(index[j], 0) : j) * crow;
-#pragma unroll
-      for (int w = 0; w < 2; w++) {
-        const __half* c = (w ? vc : kc) + at;
-        float* dst = w ? Vs + k * D + e : Ks + k * KS + e;
-        float f[8];
-        if constexpr (Q8) {
-          const uint2 raw = *(const uint2*)((const int8_t*)c + kvh * D + e);
-          const int8_t* q8 = (const int8_t*)&raw;
-          const float fac = __half2float(c[(kvw >> 1) + ((kvh * D + e) >> 5)]);
-#pragma unroll
-          for (int u = 0; u < 8; u++) f[u] = (float)q8[u] * fac;
-        } else {
-          const uint4 raw = *(const uint4*)(c + kvh * D + e);
-          const __half2* h2 = (const __half2*)&raw;
-#pragma unroll
-          for (int u = 0; u < 4; u++) {
-            const float2 g = __half22float2(h2[u]);
-            f[2 * u] = g.x;
-            f[2 * u + 1] = g.y;
-          }
-        }
-        *(float4*)dst = make_float4(f[0], f[1], f[2], f[3]);
-        *(float4*)(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
-      }
+    for (int i = tid; i < kRowsTile * D; i += kRowsThreads) {
+      const int r = tile * kRowsTile + i / D, e = i % D, node = min(r / group, sq.nodes - 1);
+      Qs[i] = a.q[(int64_t)(sq.t0 + node) * a.q_stride + (int64_t)(kvh * group + r % group) * D + e];
     }
-    __syncthreads();
-    // scores of key `key` for the wave's four rows, a part of the dims a lane
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int e = 4 * part; e < D; e += 4 * parts) {
-      const float4 k4 = *(const float4*)(Ks + key * KS + e);
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const float4 q4 = *(const float4*)(Qs + (r0 + r) * D + e);
-        s[r] = fmaf(q4.x, k4.x, s[r]);
-        s[r] = fmaf(q4.y, k4.y, s[r]);
-        s[r] = fmaf(q4.z, k4.z, s[r]);
-        s[r] = fmaf(q4.w, k4.w, s[r]);
-      }
-    }
-    const int j = base + key, node = j - sq.len;
-    const bool there = j < sq.count && (!index || index[min(j, sq.count - 1)] >= 0);
-    bool masked = false;
-    float p[4];
+    const int r0 = 4 * wave;
+    const uint32_t* mrow[4];
+    float m2[4], l[4], o[4][ND];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      for (int x = kk; x < 64; x <<= 1) s[r] += __shfl_xor(s[r], x);
-      const bool sees = there && (node < 0 || ((mrow[r][node >> 5] >> (node & 31)) & 1));
-      masked |= !sees;
-      const float sc = sees ? s[r] * c2 : -INFINITY;
-      float top = sc;
-      for (int x = 1; x < kk; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-      const float mn = fmaxf(m2[r], top);
-      const float old = mn == m2[r] ? 1.0f : exp2f(m2[r] - mn);
-      p[r] = sees ? exp2f(sc - mn) : 0.0f;
-      m2[r] = mn;
-      l[r] *= old;
+      mrow[r] = a.tree.mask + (int64_t)(sq.t0 + min((tile * kRowsTile + r0 + r) / group, sq.nodes - 1)) * words;
+      m2[r] = -INFINITY;
+      l[r] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < ND; i++) o[r][i] *= old;
-      float sum = p[r];
-      for (int x = 1; x < kk; x <<= 1) sum += __shfl_xor(sum, x);
-      l[r] += sum;
-      if (!sees) p[r] = -1.0f;  // (not a weight: what lies there is not read as a value)
+      for (int i = 0; i < ND; i++) o[r][i] = 0.0f;
     }
-    float* pw = Ps + wave * kk * 4;
-    if (part == 0) *(float4*)(pw + 4 * key) = make_float4(p[0], p[1], p[2], p[3]);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const bool some = __any(masked);
-    for (int k = 0; k < kk; k++) {
-      const float4 p4 = *(const float4*)(pw + 4 * k);
-      const float pr[4] = {p4.x, p4.y, p4.z, p4.w};
+    for (int sl = s0; sl < s1; sl++) {
+      const int base = sl * kk;
+      __syncthreads();
+      for (int i = tid; i < kk * (D / 8); i += kRowsThreads) {
+        const int k = i / (D / 8), e = 8 * (i - k * (D / 8)), j = min(base + k, sq.count - 1);
+        const int64_t at = (int64_t)(index ? max(index[j], 0) : j) * crow;
 #pragma unroll
-      for (int i = 0; i < ND; i++) {
-        const int e = lane + 64 * i;
-        const float v = e < D ? Vs[k * D + e] : 0.0f;
+        for (int w = 0; w < 2; w++) {
+          const __half* c = (w ? vc : kc) + at;
+          float* dst = w ? Vs + k * D + e : Ks + k * KS + e;
+          float f[8];
+          if constexpr (Q8) {
+            const uint2 raw = *(const uint2*)((const int8_t*)c + kvh * D + e);
+            const int8_t* q8 = (const int8_t*)&raw;
+            const float fac = __half2float(c[(kvw >> 1) + ((kvh * D + e) >> 5)]);
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-          if (!some || pr[r] >= 0.0f) o[r][i] = fmaf(pr[r], v, o[r][i]);
+            for (int u = 0; u < 8; u++) f[u] = (float)q8[u] * fac;
+          } else {
+            const uint4 raw = *(const uint4*)(c + kvh * D + e);
+            const __half2* h2 = (const __half2*)&raw;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+              const float2 g = __half22float2(h2[u]);
+              f[2 * u] = g.x;
+              f[2 * u + 1] = g.y;
+            }
+          }
+          *(float4*)dst = make_float4(f[0], f[1], f[2], f[3]);
+          *(float4*)(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        }
       }
+      __syncthreads();
+      // scores of key `key` for the wave's four rows, a part of the dims a lane
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int e = 4 * part_d; e < D; e += 4 * split) {
+        const float4 k4 = *(const float4*)(Ks + key * KS + e);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float4 q4 = *(const float4*)(Qs + (r0 + r) * D + e);
+          s[r] = fmaf(q4.x, k4.x, s[r]);
+          s[r] = fmaf(q4.y, k4.y, s[r]);
+          s[r] = fmaf(q4.z, k4.z, s[r]);
+          s[r] = fmaf(q4.w, k4.w, s[r]);
+        }
+      }
+      const int j = base + key, node = j - sq.len;
+      const bool there = j < sq.count && (!index || index[min(j, sq.count - 1)] >= 0);
+      bool masked = false;
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        for (int x = kk; x < 64; x <<= 1) s[r] += __shfl_xor(s[r], x);
+        const bool sees = there && (node < 0 || ((mrow[r][node >> 5] >> (node & 31)) & 1));
+        masked |= !sees;
+        const float sc = sees ? s[r] * c2 : -INFINITY;
+        float top = sc;
+        for (int x = 1; x < kk; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float mn = fmaxf(m2[r], top);
+        const float old = mn == m2[r] ? 1.0f : exp2f(m2[r] - mn);
+        p[r] = sees ? exp2f(sc - mn) : 0.0f;
+        m2[r] = mn;
+        l[r] *= old;
+#pragma unroll
+        for (int i = 0; i < ND; i++) o[r][i] *= old;
+        float sum = p[r];
+        for (int x = 1; x < kk; x <<= 1) sum += __shfl_xor(sum, x);
+        l[r] += sum;
+        if (!sees) p[r] = -1.0f;  // (not a weight: what lies there is not read as a value)
+      }
+      float* pw = Ps + wave * kk * 4;
+      if (part_d == 0) *(float4*)(pw + 4 * key) = make_float4(p[0], p[1], p[2], p[3]);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const bool some = __any(masked);
+      for (int k = 0; k < kk; k++) {
+        const float4 p4 = *(const float4*)(pw + 4 * k);
+        const float pr[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+        for (int i = 0; i < ND; i++) {
+          const int e = lane + 64 * i;
+          const float v = e < D ? Vs[k * D + e] : 0.0f;
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (!some || pr[r] >= 0.0f) o[r][i] = fmaf(pr[r], v, o[r][i]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_wave_barrier();
-  }
 #pragma unroll
-  for (int r = 0; r < 4; r++) {
-    const int node = n0 + (r0 + r) / group;
-    if ((r0 + r) / group >= tq || node >= sq.nodes) continue;
-    const int64_t row = (int64_t)(sq.t0 + node) * a.heads + kvh * group + (r0 + r) % group;
-    const int64_t slot = row * shares + share;
-    if (lane == 0) *(float2*)(part_ml + 2 * slot) = make_float2(m2[r], l[r]);
+    for (int r = 0; r < 4; r++) {
+      const int row = tile * kRowsTile + r0 + r;
+      if (row / group >= sq.nodes) continue;
+      const int64_t slot = (int64_t)part * kRowsTile + r0 + r;
+      float* dst = part < 0 ? a.out + ((int64_t)(sq.t0 + row / group) * a.heads + kvh * group + row % group) * D
+                            : parts.acc + slot * D;
+      const float w = part >= 0 ? 1.0f : l[r] != 0.0f ? 1.0f / l[r] : 0.0f;
 #pragma unroll
-    for (int i = 0; i < ND; i++)
-      if (lane + 64 * i < D) part_acc[slot * D + lane + 64 * i] = o[r][i];
-  }
+      for (int i = 0; i < ND; i++)
+        if (lane + 64 * i < D) dst[lane + 64 * i] = o[r][i] * w;
+      if (part >= 0 && lane == 0) *(float2*)(parts.ml + 2 * slot) = make_float2(m2[r], l[r]);
+    }
+  });
 }
 
 // ---- head widths 64, 128 and 256: the products on the matrix cores -----------
@@ -207,6 +308,11 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 //   largest value is in [2^14, 2^15): every value to 2^-23 of itself (its float
 //   to 2^-24), down to 2^-39 of the largest.  Weights, lifted by 2^14, enter as
 //   two halves as well: to 2^-24 of the largest weight.
+//
+//   A weight is 2^(s c2 - mk), mk = the maximum times c2 rounded once and then
+//   taken as it is, so that the rounding is the same in every weight of a row and
+//   falls out of its quotient (where mk is so large that it could reach a weight's
+//   own size, the difference is taken before the product).
 //
 // q8_0: keys and values enter as their integers, exact halves; a key block's
 // factor multiplies its part of the score, a value block's the weights, which
@@ -293,167 +399,32 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   return (not_finite(w) ? 0u : w & 0xffffu) | (not_finite(w >> 16) ? 0u : w & 0xffff0000u);
 }
 
-__host__ __device__ constexpr int mfma_slice(int D) { return D <= 128 ? 64 : 32; }
+// Sizes by head width and columns: keys of a slice (32 at D = 128 and 256, where
+// the words of 64 on their way cost the registers of a second block's wave; 64 at
+// D = 64), and blocks a compute unit.
+__host__ __device__ constexpr int mfma_slice(int D) { return D == 64 ? 64 : 32; }
+__host__ __device__ constexpr int mfma_blocks(int D, int NC) { return D == 256 || (D == 128 && NC == 2) ? 2 : 3; }
 
 template <int D, int NC, bool Q8, bool PAGED>
-__global__ __launch_bounds__(256, 2) void attend_tree_kernel(TreeAttend a, int tiles, int shares,
-                                                             float* __restrict__ part_acc,
-                                                             float* __restrict__ part_ml) {
+__global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(TreeAttend a, TreeParts parts,
+                                                                              int32_t* __restrict__ plan) {
   constexpr int SL = mfma_slice(D), KS = D / 32, NT = D / 16, PIECES = D / 8;
-  constexpr int PER = Q8 ? SL * D / 16 / 256 : SL * PIECES / 256;  // 16-byte words of K (and of V) a thread
-  constexpr int WPK = Q8 ? D / 16 : PIECES;                       // words a key
+  constexpr int PER = Q8 ? (SL * D / 16 + 255) / 256 : SL * PIECES / 256;  // 16-byte words of K (and of V) a thread
+  constexpr int WPK = Q8 ? D / 16 : PIECES;                               // words a key
   constexpr int ROWS = 64 * NC;
+  static_assert(PER * 256 == SL * WPK, "a slice's words dealt evenly");
   __shared__ __align__(16) _Float16 ks[2][SL * D];
   __shared__ __align__(16) _Float16 vs[2][SL * D];
   __shared__ __align__(16) float fac[Q8 ? 2 : 1][2][Q8 ? KS : 1][Q8 ? SL : 1];  // q8_0 factors of keys and values
-  __shared__ int held[PAGED ? 2 : 1][PAGED ? SL : 1];
-  __shared__ int spoilt;  // some value of a node was not finite
+  __shared__ int holes[2];  // the step whose slice in this buffer has a cell that is not held
+  __shared__ int spoilt;    // the run in which some value of a node was not finite
+  __shared__ TreeScan scan;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lm = lane & 15, lk = lane >> 4;
-  const int share = blockIdx.x % shares, rest = blockIdx.x / shares;
-  const int kvh = rest % a.kv_heads, z = rest / a.kv_heads, b = z / tiles, tile = z % tiles;
-  const TreeSeq sq = tree_seq(a.tree, b);
-  const int group = a.heads / a.kv_heads;
-  if (tile * ROWS >= sq.nodes * group) return;
-  const int words = (a.tree.max_nodes + 31) >> 5;
+  const int group = a.heads / a.kv_heads, words = (a.tree.max_nodes + 31) >> 5;
   const int kvw = a.kv_heads * D, crow = cache_row(a.form, kvw);
-  const __half* kc = (const __half*)a.k_cache + (PAGED ? 0 : (int64_t)b * a.cache_stride);
-  const __half* vc = (const __half*)a.v_cache + (PAGED ? 0 : (int64_t)b * a.cache_stride);
-  const int32_t* index = PAGED ? a.kv_index + (int64_t)b * a.index_stride : nullptr;
-  const int slices = (sq.count + SL - 1) / SL;
-
-  // this lane's columns: rows past the sequence's repeat its last one (not written)
-  const int first_row = tile * ROWS + wave * 16 * NC;
-  const bool busy = first_row < sq.nodes * group;  // (uniform over the wave)
-  int node[NC];
-#pragma unroll
-  for (int c = 0; c < NC; c++) node[c] = (first_row + 16 * c + lm) / group;
-  auto row_of = [&](int c) __attribute__((always_inline)) {
-    return (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * a.heads + kvh * group + (first_row + 16 * c + lm) % group;
-  };
-
-  // staging: words tid + 256 j of a slice's keys, and of its values
-  tu4 kw[PER], vw[PER];
-  int cells[PAGED ? PER : 1], fcell = 0;  // the next slice's (negative: not held)
-  tu4 fw = {0, 0, 0, 0};                  // q8_0: thread = (key or value, key) of the first 2 SL
-  auto cell_at = [&](int j) __attribute__((always_inline)) { return index[min(j, sq.count - 1)]; };
-  auto find = [&](int sl) __attribute__((always_inline)) {
-    if constexpr (PAGED) {
-#pragma unroll
-      for (int j = 0; j < PER; j++) cells[j] = cell_at(sl * SL + (tid + 256 * j) / WPK);
-      if (Q8) fcell = cell_at(sl * SL + tid % SL);
-    }
-  };
-  // (the cells of the slice that is loaded: what is staged where nothing is held is zero)
-  uint32_t dead = 0;
-  auto load = [&](int sl) __attribute__((always_inline)) {
-    dead = 0;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      const int i = tid + 256 * j, key = i / WPK, pc = i % WPK, at = sl * SL + key;
-      const int cell = PAGED ? cells[j] : min(at, sq.count - 1);
-      if (at >= sq.count || (PAGED && cell < 0)) dead |= 1u << j;
-      const int64_t off = (int64_t)(PAGED ? max(cell, 0) : cell) * crow + (Q8 ? (kvh * D + 16 * pc) / 2 : kvh * D + 8 * pc);
-      kw[j] = *(const tu4*)(kc + off);
-      vw[j] = *(const tu4*)(vc + off);
-    }
-    if constexpr (Q8) {
-      const int at = sl * SL + tid % SL, cell = PAGED ? fcell : min(at, sq.count - 1);
-      if (at >= sq.count || (PAGED && cell < 0)) dead |= 1u << 31;
-      if (tid < 2 * SL) {
-        const __half* f = (tid < SL ? kc : vc) + (int64_t)(PAGED ? max(cell, 0) : cell) * crow + (kvw >> 1) + ((kvh * D) >> 5);
-        if constexpr (KS == 2) fw.x = *(const uint32_t*)f;
-        else if constexpr (KS == 4) { fw.x = ((const uint2*)f)->x; fw.y = ((const uint2*)f)->y; }
-        else fw = *(const tu4*)f;
-      }
-    }
-  };
-  auto store = [&](int sl, int buf) __attribute__((always_inline)) {
-    const bool nodes_in = (sl + 1) * SL > sq.len;  // (uniform)
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      const int i = tid + 256 * j, key = i / WPK, pc = i % WPK;
-      tu4 v = vw[j];
-      if ((dead >> j) & 1) v = tu4{0, 0, 0, 0};
-      if constexpr (Q8) {
-        *(th8*)(ks[buf] + key * D + 8 * ((2 * pc) ^ key_swz<D>(key))) = int8_halves(kw[j].x, kw[j].y);
-        *(th8*)(ks[buf] + key * D + 8 * ((2 * pc + 1) ^ key_swz<D>(key))) = int8_halves(kw[j].z, kw[j].w);
-        *(th8*)(vs[buf] + key * D + 8 * ((2 * pc) ^ val_swz<D>(key))) = int8_halves(v.x, v.y);
-        *(th8*)(vs[buf] + key * D + 8 * ((2 * pc + 1) ^ val_swz<D>(key))) = int8_halves(v.z, v.w);
-      } else {
-        if (nodes_in && sl * SL + key >= sq.len) {
-          const tu4 f = {finite_halves(v.x), finite_halves(v.y), finite_halves(v.z), finite_halves(v.w)};
-          if ((f.x ^ v.x) | (f.y ^ v.y) | (f.z ^ v.z) | (f.w ^ v.w)) spoilt = 1;
-          v = f;
-        }
-        *(tu4*)(ks[buf] + key * D + 8 * (pc ^ key_swz<D>(key))) = kw[j];
-        *(tu4*)(vs[buf] + key * D + 8 * (pc ^ val_swz<D>(key))) = v;
-      }
-      if (PAGED && pc == 0) held[buf][key] = !((dead >> j) & 1);
-    }
-    if constexpr (Q8) {
-      if (tid < 2 * SL) {
-        const uint32_t w[4] = {fw.x, fw.y, fw.z, fw.w};
-#pragma unroll
-        for (int u = 0; u < KS; u++)
-          fac[buf][tid / SL][u][tid % SL] = dead >> 31 ? 0.0f : half_bits_to_float(w[u >> 1] >> (16 * (u & 1)));
-      }
-    }
-  };
-
-  if (tid == 0) spoilt = 0;
-  int sl = share;
-  if (sl < slices) {
-    find(sl);
-    load(sl);
-    if (sl + shares < slices) find(sl + shares);
-  }
-  __builtin_amdgcn_sched_barrier(0);
-
-  // the queries as B fragments, each scaled by a power of two that c2 takes back
-  th8 qf[2][NC][KS];
-  float c2[NC];
-#pragma unroll
-  for (int c = 0; c < NC; c++) {
-    const float* qr = a.q + (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * a.q_stride +
-                      (int64_t)(kvh * group + (first_row + 16 * c + lm) % group) * D + 8 * lk;
-    tf4 raw[KS][2];
-    float mx = 0.0f;
-#pragma unroll
-    for (int u = 0; u < KS; u++)
-#pragma unroll
-      for (int w = 0; w < 2; w++) {
-        raw[u][w] = *(const tf4*)(qr + 32 * u + 4 * w);
-#pragma unroll
-        for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(raw[u][w][e]));
-      }
-    mx = across(mx, lanes::Max{});
-    const int e2 = mx > 0.0f ? max(__builtin_amdgcn_frexp_expf(mx) - 15, -126) : 0;
-    c2[c] = ldexpf(fabsf(a.scale) * kLog2e, e2);
-    const float sc = ldexpf(a.scale < 0.0f ? -1.0f : 1.0f, -e2);
-#pragma unroll
-    for (int u = 0; u < KS; u++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float f = raw[u][e >> 2][e & 3] * sc;
-        const _Float16 h = (_Float16)f;
-        qf[0][c][u][e] = h;
-        qf[1][c][u][e] = (_Float16)fmaf((float)h, -1.0f, f);
-      }
-  }
-
-  tf4 o[NC][NT];
-  float mc[NC], l[NC];  // running maximum (of the scores, before c2) and this lane's part of the sum
-  int xo[NC][Q8 ? KS : 1];  // q8_0: the X that a 32-dim block of o is held at
-#pragma unroll
-  for (int c = 0; c < NC; c++) {
-    mc[c] = -1e30f;
-    l[c] = 0.0f;
-#pragma unroll
-    for (int dt = 0; dt < NT; dt++) o[c][dt] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int u = 0; u < (Q8 ? KS : 1); u++) xo[c][u] = -100;
-  }
+  if (tid == 0) holes[0] = holes[1] = spoilt = 0;  // (ahead of the walk's barriers)
+  int turn = 0;  // steps this block has staged, over all its runs
 
   // lane addresses in bytes: a piece's slot is an exclusive or with bits that a
   // row's start leaves free
@@ -467,160 +438,307 @@ __global__ __launch_bounds__(256, 2) void attend_tree_kernel(TreeAttend a, int t
     vat[v] = 2 * row * D + 16 * (((lm & 3) >> 1) ^ val_swz<D>(row)) + 8 * (lm & 1);
   }
 
-  // 32 keys of slice sl
-  auto step = [&](int kt, int buf) __attribute__((always_inline)) {
-    const int base = sl * SL + 32 * kt;
-    const lds_ptr kp = (lds_ptr)&ks[buf][32 * kt * D], vp = (lds_ptr)&vs[buf][32 * kt * D];
-    tf4 s[NC][2];
+  tree_walk<256>(a, ROWS, SL, scan, plan, [&](const TreeSeq& sq, int b, int kvh, int tile, int s0, int s1, int part) {
+    const __half* kc = (const __half*)a.k_cache + (PAGED ? 0 : (int64_t)b * a.cache_stride) + (Q8 ? kvh * D / 2 : kvh * D);
+    const __half* vc = (const __half*)a.v_cache + (PAGED ? 0 : (int64_t)b * a.cache_stride) + (Q8 ? kvh * D / 2 : kvh * D);
+    const int32_t* index = PAGED ? a.kv_index + (int64_t)b * a.index_stride : nullptr;
+    const int run = turn + 1;
+
+    // this lane's columns: rows past the sequence's repeat its last one (not written)
+    const int first_row = tile * ROWS + wave * 16 * NC;
+    const bool busy = first_row < sq.nodes * group;  // (uniform over the wave)
+    int node[NC];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int c = 0; c < NC; c++) node[c] = (first_row + 16 * c + lm) / group;
+    auto mask_row = [&](int c) __attribute__((always_inline)) {
+      return a.tree.mask + (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * words;
+    };
+
+    // staging: words tid + 256 j of a slice's keys, and of its values
+    tu4 kw[PER], vw[PER];
+    int cells[PAGED ? PER : 1], fcell = 0;  // the next slice's (negative: not held)
+    tu4 fw = {0, 0, 0, 0};                  // q8_0: thread = (key or value, key) of the first 2 SL
+    auto cell_at = [&](int j) __attribute__((always_inline)) { return index[min(j, sq.count - 1)]; };
+    auto find = [&](int sl) __attribute__((always_inline)) {
+      if constexpr (PAGED) {
 #pragma unroll
-      for (int c = 0; c < NC; c++) s[c][h] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < PER; j++) cells[j] = cell_at(sl * SL + (tid + 256 * j) / WPK);
+        if (Q8) fcell = cell_at(sl * SL + tid % SL);
+      }
+    };
+    uint32_t dead = 0;  // bit j: nothing is held where word j was loaded
+    auto load = [&](int sl) __attribute__((always_inline)) {
+      dead = 0;
 #pragma unroll
-      for (int u = 0; u < KS; u++) {
-        const th8 k8 = *(lds_h8)(kp + ((kat + 2 * 16 * h * D) ^ (64 * u)));
-        if constexpr (Q8) {
-          const tf4 f = *(const tf4*)&fac[buf][0][u][32 * kt + 16 * h + 4 * lk];
-#pragma unroll
-          for (int c = 0; c < NC; c++) {
-            const tf4 d = mfma16(k8, qf[1][c][u], mfma16(k8, qf[0][c][u], tf4{0.0f, 0.0f, 0.0f, 0.0f}));
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[c][h][i] = fmaf(f[i], d[i], s[c][h][i]);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < NC; c++) s[c][h] = mfma16(k8, qf[1][c][u], mfma16(k8, qf[0][c][u], s[c][h]));
+      for (int j = 0; j < PER; j++) {
+        const int i = tid + 256 * j, at = sl * SL + i / WPK;
+        const int cell = PAGED ? cells[j] : min(at, sq.count - 1);
+        if (PAGED && cell < 0) dead |= 1u << j;
+        const int64_t off = (int64_t)(PAGED ? max(cell, 0) : cell) * crow + 8 * (i % WPK);
+        kw[j] = *(const tu4*)(kc + off);
+        vw[j] = *(const tu4*)(vc + off);
+      }
+      if constexpr (Q8) {
+        const int at = sl * SL + tid % SL, cell = PAGED ? fcell : min(at, sq.count - 1);
+        if (at >= sq.count || (PAGED && cell < 0)) dead |= 1u << 31;
+        if (tid < 2 * SL) {
+          const __half* f = (tid < SL ? kc : vc) + (int64_t)(PAGED ? max(cell, 0) : cell) * crow + (kvw >> 1) -
+                            kvh * D / 2 + ((kvh * D) >> 5);
+          if constexpr (KS == 2) fw.x = *(const uint32_t*)f;
+          else if constexpr (KS == 4) { fw.x = ((const uint2*)f)->x; fw.y = ((const uint2*)f)->y; }
+          else fw = *(const tu4*)f;
         }
       }
-    }
-    uint32_t there = 0xffffffffu;
-    if constexpr (PAGED) there = (uint32_t)__ballot(held[buf][32 * kt + (lane & 31)] != 0);
-    const bool all = base + 32 <= sq.len && there == 0xffffffffu;  // (uniform)
-    th8 ph[NC], pl[NC];
-    float p[NC][8];
-    bool rose[NC];
+    };
+    auto store = [&](int sl, int buf) __attribute__((always_inline)) {
+      turn++;
+      const bool nodes_in = (sl + 1) * SL > sq.len;  // (uniform)
+      if (PAGED && dead) holes[buf] = turn;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        const int i = tid + 256 * j, key = i / WPK, pc = i % WPK;
+        if constexpr (Q8) {
+          *(th8*)(ks[buf] + key * D + 8 * ((2 * pc) ^ key_swz<D>(key))) = int8_halves(kw[j].x, kw[j].y);
+          *(th8*)(ks[buf] + key * D + 8 * ((2 * pc + 1) ^ key_swz<D>(key))) = int8_halves(kw[j].z, kw[j].w);
+          *(th8*)(vs[buf] + key * D + 8 * ((2 * pc) ^ val_swz<D>(key))) = int8_halves(vw[j].x, vw[j].y);
+          *(th8*)(vs[buf] + key * D + 8 * ((2 * pc + 1) ^ val_swz<D>(key))) = int8_halves(vw[j].z, vw[j].w);
+        } else {
+          tu4 v = vw[j];
+          // (what is not held, and what some row may not see, is never more than zero times a weight of zero)
+          if ((nodes_in && sl * SL + key >= sq.len) || (PAGED && dead)) {
+            const tu4 f = {finite_halves(v.x), finite_halves(v.y), finite_halves(v.z), finite_halves(v.w)};
+            if ((f.x ^ v.x) | (f.y ^ v.y) | (f.z ^ v.z) | (f.w ^ v.w)) spoilt = run;
+            v = f;
+          }
+          *(tu4*)(ks[buf] + key * D + 8 * (pc ^ key_swz<D>(key))) = kw[j];
+          *(tu4*)(vs[buf] + key * D + 8 * (pc ^ val_swz<D>(key))) = v;
+        }
+      }
+      if constexpr (Q8) {
+        if (tid < 2 * SL) {
+          const uint32_t w[4] = {fw.x, fw.y, fw.z, fw.w};
+#pragma unroll
+          for (int u = 0; u < KS; u++)
+            fac[buf][tid / SL][u][tid % SL] = dead >> 31 ? 0.0f : half_bits_to_float(w[u >> 1] >> (16 * (u & 1)));
+        }
+      }
+    };
+
+    find(s0);
+    load(s0);
+    if (s0 + 1 < s1) find(s0 + 1);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // the queries as B fragments, each scaled by a power of two that c2 takes back
+    th8 qf[2][NC][KS];
+    float c2[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-      uint32_t mine = 0xffu;
-      if (!all) {
-        const uint32_t* mrow = a.tree.mask + (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * words;
-        mine = (seen_bits(mrow, words, base - sq.len, sq.count - sq.len) & there) >> (4 * lk);
+      const float* qr = a.q + (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * a.q_stride +
+                        (int64_t)(kvh * group + (first_row + 16 * c + lm) % group) * D + 8 * lk;
+      tf4 raw[KS][2];
+      float mx = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-          s[c][i >> 2][i & 3] = (mine >> ((i & 3) + 16 * (i >> 2))) & 1 ? s[c][i >> 2][i & 3] : -INFINITY;
-      }
-      float m = s[c][0][0];
+      for (int u = 0; u < KS; u++)
 #pragma unroll
-      for (int i = 1; i < 8; i++) m = fmaxf(m, s[c][i >> 2][i & 3]);
-      m = across(m, lanes::Max{});
-      const float mn = fmaxf(mc[c], m);
-      rose[c] = mn != mc[c];
-      if (__any(rose[c] && l[c] != 0.0f)) {  // (else there is nothing yet)
-        const float f = __builtin_amdgcn_exp2f((mc[c] - mn) * c2[c]);
-        l[c] *= f;
+        for (int w = 0; w < 2; w++) {
+          raw[u][w] = *(const tf4*)(qr + 32 * u + 4 * w);
 #pragma unroll
-        for (int dt = 0; dt < NT; dt++) o[c][dt] *= f;
-      }
-      mc[c] = mn;
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        // (the difference first: c2 mc of large scores is rounded by more than 1)
-        const float e = __builtin_amdgcn_exp2f((s[c][i >> 2][i & 3] - mn) * c2[c]);
-        p[c][i] = all || (mine >> ((i & 3) + 16 * (i >> 2))) & 1 ? e : -0.0f;
-        l[c] += p[c][i];
-      }
-      if constexpr (!Q8) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          ph[c][i] = (_Float16)fmaf(p[c][i], kLift, 0.0f);  // (one instruction)
-          pl[c][i] = (_Float16)fmaf(p[c][i], kLift, -(float)ph[c][i]);
+          for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(raw[u][w][e]));
         }
-      }
+      mx = across(mx, lanes::Max{});
+      const int e2 = mx > 0.0f ? max(__builtin_amdgcn_frexp_expf(mx) - 15, -126) : 0;
+      c2[c] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e2), 1e-38f);  // (never zero: a key that is not seen scores -inf)
+      const float sc = ldexpf(a.scale < 0.0f ? -1.0f : 1.0f, -e2);
+#pragma unroll
+      for (int u = 0; u < KS; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float f = raw[u][e >> 2][e & 3] * sc;
+          const _Float16 h = (_Float16)f;
+          qf[0][c][u][e] = h;
+          qf[1][c][u][e] = (_Float16)fmaf((float)h, -1.0f, f);
+        }
     }
+
+    tf4 o[NC][NT];
+    // running maximum (of the scores, before c2), the same times c2, and this lane's part of the sum
+    float mc[NC], mk[NC], l[NC];
+    int xo[NC][Q8 ? KS : 1];  // q8_0: the X that a 32-dim block of o is held at
 #pragma unroll
-    for (int dt = 0; dt < NT; dt++) {
-      if constexpr (Q8) {
-        if (dt % 2 == 0) {
-          const int u = dt / 2;
-          const tf4 f0 = *(const tf4*)&fac[buf][1][u][32 * kt + 4 * lk], f1 = *(const tf4*)&fac[buf][1][u][32 * kt + 16 + 4 * lk];
+    for (int c = 0; c < NC; c++) {
+      mc[c] = -1e30f;
+      mk[c] = -3e38f;
+      l[c] = 0.0f;
 #pragma unroll
-          for (int c = 0; c < NC; c++) {
-            float w[8], wm = 0.0f;
+      for (int dt = 0; dt < NT; dt++) o[c][dt] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              // (-0: not seen, whatever its factor)
-              w[i] = __float_as_uint(p[c][i]) != 0x80000000u ? p[c][i] * (i < 4 ? f0[i & 3] : f1[i & 3]) : 0.0f;
-              wm = fmaxf(wm, fabsf(w[i]));
+      for (int u = 0; u < (Q8 ? KS : 1); u++) xo[c][u] = -100;
+    }
+    // a row's mk is too large for a weight's exponent; (uniform) some row's is
+    auto large = [&](int c) __attribute__((always_inline)) { return mc[c] > -1e30f && !(fabsf(mk[c]) <= 4e6f); };
+    bool huge = false;
+
+    // keys 32 kt .. of slice sl
+    auto step = [&](int sl, int kt, int buf) __attribute__((always_inline)) {
+      const int base = sl * SL + 32 * kt;
+      const lds_ptr kp = (lds_ptr)&ks[buf][32 * kt * D], vp = (lds_ptr)&vs[buf][32 * kt * D];
+      tf4 s[NC][2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int c = 0; c < NC; c++) s[c][h] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < KS; u++) {
+          const th8 k8 = *(lds_h8)(kp + ((kat + 2 * 16 * h * D) ^ (64 * u)));
+          if constexpr (Q8) {
+            const tf4 f = *(const tf4*)&fac[buf][0][u][32 * kt + 16 * h + 4 * lk];
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+              const tf4 d = mfma16(k8, qf[1][c][u], mfma16(k8, qf[0][c][u], tf4{0.0f, 0.0f, 0.0f, 0.0f}));
+#pragma unroll
+              for (int i = 0; i < 4; i++) s[c][h][i] = fmaf(f[i], d[i], s[c][h][i]);
             }
-            wm = across(wm, lanes::Max{});
-            const int old = xo[c][u];
-            // (an infinite factor: the finite products are below 2^31)
-            const int xw = wm < INFINITY ? __builtin_amdgcn_frexp_expf(wm) : 31;
-            const int x = wm > 0.0f ? max(max(xw, rose[c] ? old - 60 : old), -100) : old;
-            if (__any(x != old)) {
-              const float f = ldexpf(1.0f, old - x);
-              o[c][dt] *= f;
-              o[c][dt + 1] *= f;
-            }
-            xo[c][u] = x;
-            const float unit = ldexpf(1.0f, 15 - x);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const float v = w[i] * unit;
-              ph[c][i] = (_Float16)v;
-              pl[c][i] = (_Float16)(v - (float)ph[c][i]);
-            }
-            if (__builtin_expect(__any(!(wm < INFINITY)), 0)) {
-#pragma unroll
-              for (int i = 0; i < 8; i++)
-                if (!(fabsf(w[i]) < INFINITY)) pl[c][i] = 0;
-            }
+            for (int c = 0; c < NC; c++) s[c][h] = mfma16(k8, qf[1][c][u], mfma16(k8, qf[0][c][u], s[c][h]));
           }
         }
       }
-      ts8 v;
+      const bool all = base + 32 <= sq.len && !(PAGED && holes[buf] == run + (sl - s0));  // (uniform)
+      uint32_t mine[NC];  // bit (i & 3) + 16 (i >> 2): key 4 lk + that is seen
+      if (!all) {
+        const int key = base + (lane & 31);
+        uint32_t there = 0xffffffffu;
+        if constexpr (PAGED) there = (uint32_t)__ballot(cell_at(key) >= 0);
 #pragma unroll
-      for (int w = 0; w < 2; w++) {
-        const ts4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4*)(vp + (vat[w] ^ (32 * dt))));
+        for (int c = 0; c < NC; c++) {
+          mine[c] = (seen_bits(mask_row(c), words, base - sq.len, sq.count - sq.len) & there) >> (4 * lk);
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[4 * w + e] = x[e];
+          for (int i = 0; i < 8; i++)
+            s[c][i >> 2][i & 3] = (mine[c] >> ((i & 3) + 16 * (i >> 2))) & 1 ? s[c][i >> 2][i & 3] : -INFINITY;
+        }
+      }
+      th8 ph[NC], pl[NC];
+      float p[NC][8];
+      bool rose[NC];
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        float m = s[c][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) m = fmaxf(m, s[c][i >> 2][i & 3]);
+        m = across(m, lanes::Max{});
+        const float mn = fmaxf(mc[c], m);
+        rose[c] = mn != mc[c];
+        if (__any(rose[c])) {
+          const float mkn = rose[c] ? mn * c2[c] : mk[c];
+          const float f = __builtin_amdgcn_exp2f(large(c) ? (mc[c] - mn) * c2[c] : mk[c] - mkn);
+          l[c] *= f;
+#pragma unroll
+          for (int dt = 0; dt < NT; dt++) o[c][dt] *= f;
+          mc[c] = mn;
+          mk[c] = mkn;
+          huge = huge || __any(large(c));
+        }
+        if (__builtin_expect(huge, 0)) {
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            p[c][i] = __builtin_amdgcn_exp2f(large(c) ? (s[c][i >> 2][i & 3] - mc[c]) * c2[c] : fmaf(s[c][i >> 2][i & 3], c2[c], -mk[c]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++) p[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i >> 2][i & 3], c2[c], -mk[c]));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) l[c] += p[c][i];
+        if constexpr (!Q8) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            ph[c][i] = (_Float16)fmaf(p[c][i], kLift, 0.0f);  // (one instruction)
+            pl[c][i] = (_Float16)fmaf(p[c][i], kLift, -(float)ph[c][i]);
+          }
+        }
       }
 #pragma unroll
-      for (int c = 0; c < NC; c++)
-        o[c][dt] = mfma16(__builtin_bit_cast(th8, v), pl[c], mfma16(__builtin_bit_cast(th8, v), ph[c], o[c][dt]));
-    }
-  };
-
-  __syncthreads();  // (spoilt)
-  if (sl < slices) store(sl, 0);
-  __syncthreads();
-  for (int buf = 0; sl < slices; sl += shares, buf ^= 1) {
-    const int next = sl + shares;
-    const bool more = next < slices;  // (uniform)
-    if (more) {
-      load(next);
-      if (next + shares < slices) find(next + shares);
-    }
-    if (busy) {
+      for (int dt = 0; dt < NT; dt++) {
+        if constexpr (Q8) {
+          if (dt % 2 == 0) {
+            const int u = dt / 2;
+            const tf4 f0 = *(const tf4*)&fac[buf][1][u][32 * kt + 4 * lk], f1 = *(const tf4*)&fac[buf][1][u][32 * kt + 16 + 4 * lk];
 #pragma unroll
-      for (int kt = 0; kt < SL / 32; kt++)
-        if (sl * SL + 32 * kt < sq.count) step(kt, buf);
-    }
-    if (more) store(next, buf ^ 1);
-    __syncthreads();
-  }
+            for (int c = 0; c < NC; c++) {
+              float w[8], wm = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 8; i++) w[i] = p[c][i] * (i < 4 ? f0[i & 3] : f1[i & 3]);
+              if (!all) {  // (whatever the factor of a key that is not seen)
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i] = (mine[c] >> ((i & 3) + 16 * (i >> 2))) & 1 ? w[i] : 0.0f;
+              }
+#pragma unroll
+              for (int i = 0; i < 8; i++) wm = fmaxf(wm, fabsf(w[i]));
+              wm = across(wm, lanes::Max{});
+              const int old = xo[c][u];
+              // (an infinite factor: the finite products are below 2^31)
+              const int xw = wm < INFINITY ? __builtin_amdgcn_frexp_expf(wm) : 31;
+              const int x = wm > 0.0f ? max(max(xw, rose[c] ? old - 60 : old), -100) : old;
+              if (__any(x != old)) {
+                const float f = ldexpf(1.0f, old - x);
+                o[c][dt] *= f;
+                o[c][dt + 1] *= f;
+                xo[c][u] = x;
+              }
+              const float unit = ldexpf(1.0f, 15 - x);
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                ph[c][i] = (_Float16)fmaf(w[i], unit, 0.0f);
+                pl[c][i] = (_Float16)fmaf(w[i], unit, -(float)ph[c][i]);
+              }
+              if (__builtin_expect(__any(!(wm < INFINITY)), 0)) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                  if (!(fabsf(w[i]) < INFINITY)) pl[c][i] = 0;
+              }
+            }
+          }
+        }
+        ts8 v;
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          const ts4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4*)(vp + (vat[w] ^ (32 * dt))));
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[4 * w + e] = x[e];
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+          o[c][dt] = mfma16(__builtin_bit_cast(th8, v), pl[c], mfma16(__builtin_bit_cast(th8, v), ph[c], o[c][dt]));
+      }
+    };
 
-  if (!Q8 && __builtin_expect(spoilt, 0) && busy) {
-    for (int s0 = share; s0 < slices; s0 += shares) {
-      for (int j = max(s0 * SL, sq.len); j < min((s0 + 1) * SL, sq.count); j++) {
+    store(s0, 0);
+    __syncthreads();
+    for (int sl = s0, buf = 0; sl < s1; sl++, buf ^= 1) {
+      const bool more = sl + 1 < s1;  // (uniform)
+      if (more) {
+        load(sl + 1);
+        if (sl + 2 < s1) find(sl + 2);
+      }
+      if (busy) {
+#pragma unroll
+        for (int kt = 0; kt < SL / 32; kt++)
+          if (sl * SL + 32 * kt < sq.count) step(sl, kt, buf);
+      }
+      if (more) store(sl + 1, buf ^ 1);
+      __syncthreads();
+    }
+
+    if (!Q8 && __builtin_expect(spoilt == run, 0) && busy) {
+      for (int j = max(s0 * SL, sq.len); j < min(s1 * SL, sq.count); j++) {
         const int cell = PAGED ? index[j] : j;
         if (cell < 0) continue;
-        const __half* vr = vc + (int64_t)cell * crow + kvh * D + 4 * lk;
+        const __half* vr = vc + (int64_t)cell * crow + 4 * lk;
         const int i = j - sq.len;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-          const uint32_t* mrow = a.tree.mask + (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * words;
-          const bool sees = (mrow[i >> 5] >> (i & 31)) & 1;
+          const bool sees = (mask_row(c)[i >> 5] >> (i & 31)) & 1;
 #pragma unroll
           for (int dt = 0; dt < NT; dt++)
 #pragma unroll
@@ -631,63 +749,80 @@ __global__ __launch_bounds__(256, 2) void attend_tree_kernel(TreeAttend a, int t
         }
       }
     }
-  }
-  if (!busy) return;
+    if (!busy) return;
 #pragma unroll
-  for (int c = 0; c < NC; c++) {
-    const float sum = across(l[c], lanes::Add{});
-    if (node[c] >= sq.nodes) continue;
-    const int64_t row = row_of(c);
-    const float w = (shares > 1 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f) * (Q8 ? 1.0f : 1.0f / kLift);
-    float* dst = shares > 1 ? part_acc + (row * shares + share) * D : a.out + row * D;
+    for (int c = 0; c < NC; c++) {
+      const float sum = across(l[c], lanes::Add{});
+      if (node[c] >= sq.nodes) continue;
+      const int64_t slot = (int64_t)part * ROWS + wave * 16 * NC + 16 * c + lm;
+      float* dst = part < 0 ? a.out + ((int64_t)(sq.t0 + node[c]) * a.heads + kvh * group + (first_row + 16 * c + lm) % group) * D
+                            : parts.acc + slot * D;
+      const float w = (part >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f) * (Q8 ? 1.0f : 1.0f / kLift);
 #pragma unroll
-    for (int dt = 0; dt < NT; dt++) {
-      const float f = Q8 ? w * ldexpf(1.0f, xo[c][dt / 2] - 15) : w;
-      *(tf4*)(dst + 16 * dt + 4 * lk) = o[c][dt] * f;
+      for (int dt = 0; dt < NT; dt++) {
+        const float f = Q8 ? w * ldexpf(1.0f, xo[c][dt / 2] - 15) : w;
+        *(tf4*)(dst + 16 * dt + 4 * lk) = o[c][dt] * f;
+      }
+      if (part >= 0 && lk == 0) *(float2*)(parts.ml + 2 * slot) = make_float2(mk[c], sum);
     }
-    if (shares > 1 && lk == 0)
-      *(float2*)(part_ml + 2 * (row * shares + share)) = make_float2(sum != 0.0f ? mc[c] * c2[c] : -INFINITY, sum);
-  }
+  });
 }
 
-// Folds the shares of each (token, head) row: thread = 4 dims.  A share that no
-// key of the row fell in has sum 0 and is left out; a row without any is zero.
-__global__ __launch_bounds__(256) void attend_tree_fold_kernel(const float* __restrict__ part_acc,
-                                                               const float* __restrict__ part_ml, mi_tree tree,
-                                                               int heads, int D, int shares, float* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int tpr = D >> 2, d4 = (int)(i % tpr);
-  const int64_t row = i / tpr;
-  if (row >= (int64_t)min(max(tree.starts[tree.batch], 0), tree.tokens) * heads) return;
-  const float2* ml = (const float2*)part_ml + row * shares;
-  const float4* acc = (const float4*)(part_acc + row * shares * D) + d4;
-  float m = -INFINITY;
-  for (int s = 0; s < shares; s++) {
-    const float2 v = ml[s];
-    if (v.y != 0.0f) m = fmaxf(m, v.x);
+// Folds the parts of each row whose tile several blocks share: a wave a row, up
+// to eight parts' sums on their way at once.  A part that no key of the row fell
+// in has sum 0 and weight 0; a row without any other is zero.
+template <int V>
+__global__ __launch_bounds__(256) void attend_tree_fold_kernel(TreeAttend a, TreeParts parts,
+                                                               const int32_t* __restrict__ plan, int rows, int slice) {
+  typedef float vec __attribute__((ext_vector_type(V)));
+  const int lane = threadIdx.x & 63, D = a.head_dim, group = a.heads / a.kv_heads;
+  const int64_t i = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = (int)(i / ((int64_t)a.tree.max_nodes * a.heads));
+  if (b >= a.tree.batch) return;
+  const int at = (int)(i - (int64_t)b * a.tree.max_nodes * a.heads), node = at / a.heads, h = at - node * a.heads;
+  const TreeSeq sq = tree_seq(a.tree, b);
+  if (node >= sq.nodes) return;
+  const int kvh = h / group, r = node * group + h % group, tile = r / rows, slices = tree_slices(sq, slice);
+  const int per = plan[0], u0 = plan[1 + b] + (kvh * tree_tiles(sq, group, rows) + tile) * slices;
+  const int g0 = u0 / per, n = (u0 + slices - 1) / per - g0 + 1;
+  if (n == 1) return;  // one block's: finished
+  // part k is block g0 + k's: its last one (1) for the block that the tile starts in, else its first (0)
+  auto slot = [&](int k) { return (int64_t)(2 * (g0 + k) + (k == 0 ? 1 : 0)) * rows + r % rows; };
+  const float2 ml = ((const float2*)parts.ml)[slot(min(lane, n - 1))];
+  const bool live = lane < n && ml.y != 0.0f;
+  const float m = lanes::reduce<64>(live ? ml.x : -INFINITY, lanes::Max{});
+  const float w = live ? (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m)) : 0.0f;
+  const float sum = lanes::reduce<64>(live ? ml.y * w : 0.0f, lanes::Add{});
+  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  float* dst = a.out + ((int64_t)(sq.t0 + node) * a.heads + h) * D;
+  for (int d0 = 0; d0 < D; d0 += 64 * V) {
+    const int d = min(d0 + lane * V, D - V);
+    vec o = {};
+    auto add = [&](int k0, auto count) __attribute__((always_inline)) {
+      constexpr int N = decltype(count)::value;
+      vec x[N];
+#pragma unroll
+      for (int k = 0; k < N; k++) x[k] = *(const vec*)(parts.acc + slot(k0 + k) * D + d);
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        o += x[k] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), k0 + k));
+      }
+    };
+    int k = 0;
+    for (; k + 8 <= n; k += 8) add(k, std::integral_constant<int, 8>{});
+    if (n - k >= 4) add(k, std::integral_constant<int, 4>{}), k += 4;
+    if (n - k >= 2) add(k, std::integral_constant<int, 2>{}), k += 2;
+    if (n - k >= 1) add(k, std::integral_constant<int, 1>{});
+    if (d0 + lane * V < D) *(vec*)(dst + d) = o * inv;
   }
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float l = 0.0f;
-  for (int s = 0; s < shares; s++) {
-    const float2 v = ml[s];
-    if (v.y == 0.0f) continue;
-    const float4 x = acc[(int64_t)s * tpr];
-    const float w = v.x == m ? 1.0f : exp2f(v.x - m);
-    l = fmaf(v.y, w, l);
-    o.x = fmaf(x.x, w, o.x);
-    o.y = fmaf(x.y, w, o.y);
-    o.z = fmaf(x.z, w, o.z);
-    o.w = fmaf(x.w, w, o.w);
-  }
-  const float w = l != 0.0f ? 1.0f / l : 0.0f;
-  ((float4*)out)[row * tpr + d4] = make_float4(o.x * w, o.y * w, o.z * w, o.w * w);
 }
 
 struct TreeGrid {
   bool mfma;
   int columns;  // NC of attend_tree_kernel
-  int tiles, shares;
-  int64_t blocks;
+  int rows, slice;
+  int64_t units;  // of the largest step
+  int blocks;
 };
 
 TreeGrid tree_grid(int heads, int kv_heads, int head_dim, const mi_tree& t) {
@@ -695,40 +830,46 @@ TreeGrid tree_grid(int heads, int kv_heads, int head_dim, const mi_tree& t) {
   const int group = heads / kv_heads;
   g.mfma = head_dim == 64 || head_dim == 128 || head_dim == 256;
   g.columns = head_dim <= 128 && t.max_nodes * group > 64 ? 2 : 1;
-  const int rows = g.mfma ? 64 * g.columns : kRowsTile, slice = g.mfma ? mfma_slice(head_dim) : rows_slice(head_dim);
-  g.tiles = (t.max_nodes * group + rows - 1) / rows;
-  const int64_t pairs = (int64_t)t.batch * g.tiles * kv_heads, slices = ((int64_t)t.max_count + slice - 1) / slice;
-  const int64_t room = (g.mfma ? 2 : 4) * (int64_t)cu_count();
-  g.shares = 1;
-  int64_t least = INT64_MAX;
-  for (int n = 1; n <= std::min<int64_t>(slices, 64); n++) {
-    const int64_t cost = 16 * ((n * pairs + room - 1) / room) * ((slices + n - 1) / n + 2) + n;
-    if (cost < least) g.shares = n, least = cost;
-  }
-  g.blocks = pairs * g.shares;
+  g.rows = g.mfma ? 64 * g.columns : kRowsTile;
+  g.slice = g.mfma ? mfma_slice(head_dim) : rows_slice(head_dim);
+  g.units = (int64_t)t.batch * ((t.max_nodes * group + g.rows - 1) / g.rows) * kv_heads *
+            (((int64_t)t.max_count + g.slice - 1) / g.slice);
+  g.blocks = (int)std::min<int64_t>(g.units, (int64_t)cu_count() * (g.mfma ? mfma_blocks(head_dim, g.columns) : 3));
   return g;
+}
+
+// The workspace: each block's two parts of a tile (sums, then maxima and sums),
+// then the plan of the walk.
+struct TreeCarve {
+  size_t ml, plan, total;
+};
+TreeCarve tree_carve(const TreeGrid& g, int head_dim, int batch) {
+  auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
+  TreeCarve c;
+  c.ml = up((size_t)2 * g.blocks * g.rows * head_dim * sizeof(float));
+  c.plan = c.ml + up((size_t)2 * g.blocks * g.rows * 2 * sizeof(float));
+  c.total = c.plan + up(((size_t)batch + 1) * sizeof(int32_t));
+  return c;
 }
 
 }  // namespace
 
-static size_t part_acc_bytes(int heads, int head_dim, const mi_tree& t, int shares) {
-  return ((size_t)t.tokens * heads * shares * head_dim * sizeof(float) + 255) & ~(size_t)255;
-}
-
-size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const mi_tree& t) {
-  (void)form;
-  const TreeGrid g = tree_grid(heads, kv_heads, head_dim, t);
-  return part_acc_bytes(heads, head_dim, t, g.shares) + (size_t)t.tokens * heads * g.shares * 2 * sizeof(float);
+size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, const mi_tree& t) {
+  return tree_carve(tree_grid(heads, kv_heads, head_dim, t), head_dim, t.batch).total;
 }
 
 int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work) {
   const TreeGrid g = tree_grid(a.heads, a.kv_heads, a.head_dim, a.tree);
-  if (g.blocks > 0x7fffffff) return fail(MI_ERR_SHAPE, "attend_tree: %d sequences of %d nodes", a.tree.batch, a.tree.max_nodes);
-  float* part_acc = (float*)work;
-  float* part_ml = (float*)((char*)work + part_acc_bytes(a.heads, a.head_dim, a.tree, g.shares));
-  const dim3 grid((uint32_t)g.blocks);
-#define MI_TREE(D, NC, Q, P)                                                                                       \
-  hipLaunchKernelGGL((attend_tree_kernel<D, NC, Q, P>), grid, dim3(256), 0, s, a, g.tiles, g.shares, part_acc, part_ml)
+  const int64_t fold = ((int64_t)a.tree.batch * a.tree.max_nodes * a.heads + 3) / 4;
+  if (g.units > 0x7fffffff || fold > 0x7fffffff)
+    return fail(MI_ERR_SHAPE, "attend_tree: %d sequences of %d nodes and %d positions are too much work", a.tree.batch,
+                a.tree.max_nodes, a.tree.max_count);
+  const TreeCarve c = tree_carve(g, a.head_dim, a.tree.batch);
+  const TreeParts parts{(float*)work, (float*)((char*)work + c.ml)};
+  int32_t* plan = (int32_t*)((char*)work + c.plan);
+  const dim3 grid(g.blocks);
+#define MI_TREE(D, NC, Q, P) \
+  hipLaunchKernelGGL((attend_tree_kernel<D, NC, Q, P>), grid, dim3(256), 0, s, a, parts, plan)
 #define MI_TREE_F(D, NC)                            \
   if (a.form == MI_CACHE_Q8) {                      \
     if (a.kv_index) MI_TREE(D, NC, true, true);     \
@@ -740,10 +881,10 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work) {
 #define MI_TREE_ROWS(ND)                                                                                             \
   if (a.form == MI_CACHE_Q8)                                                                                         \
     hipLaunchKernelGGL((attend_tree_rows_kernel<true, ND>), grid, dim3(kRowsThreads), rows_lds_bytes(a.head_dim), s,  \
-                       a, g.tiles, g.shares, part_acc, part_ml);                                                     \
+                       a, parts, plan);                                                                              \
   else                                                                                                               \
     hipLaunchKernelGGL((attend_tree_rows_kernel<false, ND>), grid, dim3(kRowsThreads), rows_lds_bytes(a.head_dim), s, \
-                       a, g.tiles, g.shares, part_acc, part_ml)
+                       a, parts, plan)
   if (a.head_dim == 64) {
     if (g.columns == 1) { MI_TREE_F(64, 1) }
     else { MI_TREE_F(64, 2) }
@@ -765,11 +906,12 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work) {
 #undef MI_TREE_F
 #undef MI_TREE_ROWS
   if (int rc = hip_check(hipGetLastError(), "attend_tree launch")) return rc;
-  if (g.mfma && g.shares == 1) return MI_OK;  // (the finished rows)
-  const int64_t threads = (int64_t)a.tree.tokens * a.heads * (a.head_dim / 4), blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffff) return fail(MI_ERR_SHAPE, "attend_tree: %d tokens of %d heads", a.tree.tokens, a.heads);
-  hipLaunchKernelGGL(attend_tree_fold_kernel, dim3((uint32_t)blocks), dim3(256), 0, s, part_acc, part_ml, a.tree,
-                     a.heads, a.head_dim, g.shares, a.out);
+#define MI_TREE_FOLD(V)                                                                                       \
+  hipLaunchKernelGGL((attend_tree_fold_kernel<V>), dim3((uint32_t)fold), dim3(256), 0, s, a, parts, plan, g.rows, g.slice)
+  if (a.head_dim % 256 == 0) MI_TREE_FOLD(4);
+  else if (a.head_dim % 128 == 0) MI_TREE_FOLD(2);
+  else MI_TREE_FOLD(1);
+#undef MI_TREE_FOLD
   return hip_check(hipGetLastError(), "attend_tree fold launch");
 }
 
