@@ -22,7 +22,7 @@ namespace mi {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kMaxParts = 64;  // blocks that share a tile: the lanes of the fold
+constexpr int kMaxParts = 128;  // blocks that share a tile: two for a lane of the fold
 
 // The tokens and keys of sequence b, each held to what the host has checked.
 struct TreeSeq {
@@ -43,90 +43,90 @@ __device__ __forceinline__ int tree_tiles(const TreeSeq& s, int group, int rows)
 }
 __device__ __forceinline__ int tree_slices(const TreeSeq& s, int slice) { return (s.count + slice - 1) / slice; }
 
-struct TreeScan {
-  int sum[8], top[8];
-  int b, at;
+struct IMax {
+  __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
 };
+// the sum over lanes 0 .. this one
+__device__ __forceinline__ int lane_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15 of rows 0 and 2 to the row behind
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+  return v;
+}
 
 // Hands this block's units to `take`, a tile's run of slices at a time:
 // take(sequence, b, key head, tile, first slice, end, part), part -1 where the
-// run is the whole tile, else the block's part it goes to.  plan: units a block,
-// then each sequence's first unit (written by block 0, for the fold).
-template <int NT, class F>
-__device__ __forceinline__ void tree_walk(const TreeAttend& a, int rows, int slice, TreeScan& sh,
-                                          int32_t* __restrict__ plan, F take) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int group = a.heads / a.kv_heads, batch = a.tree.batch;
-  const int q = (batch + NT - 1) / NT;
-  auto units_of = [&](int b, int& slices) {
-    const TreeSeq s = tree_seq(a.tree, b);
-    slices = s.nodes ? tree_slices(s, slice) : 0;
-    return tree_tiles(s, group, rows) * a.kv_heads * slices;
+// run is the whole tile, else the block's part it goes to.  Every wave finds them
+// for itself, 64 sequences at a time in its lanes.  plan: units a block, then each
+// sequence's first unit (written by the first wave, for the fold).
+template <class F>
+__device__ __forceinline__ void tree_walk(const TreeAttend& a, int rows, int slice, int32_t* __restrict__ plan,
+                                          F take) {
+  const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads, batch = a.tree.batch;
+  TreeSeq sq;
+  int units;
+  auto look = [&](int b0) __attribute__((always_inline)) {
+    const int b = b0 + lane;
+    sq = tree_seq(a.tree, min(b, batch - 1));
+    if (b >= batch || sq.nodes == 0) sq.count = 0;
+    units = tree_tiles(sq, group, rows) * a.kv_heads * tree_slices(sq, slice);
   };
-  int mine = 0, top = 0;
-  for (int b = tid * q; b < min((tid + 1) * q, batch); b++) {
-    int slices;
-    mine += units_of(b, slices);
-    top = max(top, slices);
-  }
-  int upto = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(upto, o);
-    if (lane >= o) upto += u;
-    top = max(top, __shfl_xor(top, o));
-  }
-  if (lane == 63) sh.sum[wave] = upto, sh.top[wave] = top;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; w++) {
-    if (w == wave) upto += total;
-    total += sh.sum[w];
-    top = max(top, sh.top[w]);
+  int total = 0, top = 0;
+  for (int b0 = 0; b0 < batch; b0 += 64) {
+    look(b0);
+    total += lanes::reduce<64>(units, lanes::Add{});
+    top = max(top, lanes::reduce<64>(tree_slices(sq, slice), IMax{}));
   }
   total = __builtin_amdgcn_readfirstlane(total);  // (the same in every lane)
   top = __builtin_amdgcn_readfirstlane(top);
-  const int per = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, (top + kMaxParts - 3) / (kMaxParts - 2)), 1);
-  const int64_t first = (int64_t)blockIdx.x * per;
-  if (blockIdx.x == 0) {
-    if (tid == 0) plan[0] = per;
-    int at = upto - mine, slices;
-    for (int b = tid * q; b < min((tid + 1) * q, batch); b++) {
-      plan[1 + b] = at;
-      at += units_of(b, slices);
+  const int blocks = gridDim.x;
+  const int per = max(max((total + blocks - 1) / blocks, (top + kMaxParts - 3) / (kMaxParts - 2)), 1);
+  // blocks go to the 8 XCDs in turn: neighbours in the line, which are one
+  // sequence's tiles over the same keys, to the same L2
+  const int xcd = blockIdx.x & 7, in = blockIdx.x >> 3, many = blocks >> 3, rest = blocks & 7;
+  const int block = xcd * many + min(xcd, rest) + in;
+  const int64_t first = (int64_t)block * per;
+  const bool writes = blockIdx.x == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
+  if (writes && lane == 0) plan[0] = per;
+  int b = -1, at = 0, chunk = 0;
+  for (int b0 = 0, ahead = 0; b0 < batch && (b < 0 || writes); b0 += 64) {
+    if (batch > 64) look(b0);
+    const int upto = ahead + lane_scan(units);
+    if (writes && b0 + lane < batch) plan[1 + b0 + lane] = upto - units;
+    const uint64_t hit = __ballot(first >= upto - units && first < upto);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      b = b0 + l;
+      at = (int)first - __builtin_amdgcn_readlane(upto - units, l);
+      chunk = b0;
     }
+    ahead = __builtin_amdgcn_readlane(upto, 63);
   }
-  if (first >= total) return;  // (uniform over the block)
-  if (first >= upto - mine && first < upto) {
-    int at = upto - mine, slices;
-    for (int b = tid * q;; b++) {
-      const int u = units_of(b, slices);
-      if (first < at + u) {
-        sh.b = b;
-        sh.at = (int)first - at;
-        break;
-      }
-      at += u;
-    }
-  }
-  __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane(sh.b), at = __builtin_amdgcn_readfirstlane(sh.at);
+  if (b < 0) return;  // (no units left for this block)
+  b = __builtin_amdgcn_readfirstlane(b);  // (the same in every lane)
+  at = __builtin_amdgcn_readfirstlane(at);
+  if (batch > 64) look(chunk);
+  TreeSeq s;
+  s.t0 = __builtin_amdgcn_readlane(sq.t0, b - chunk);
+  s.nodes = __builtin_amdgcn_readlane(sq.nodes, b - chunk);
+  s.len = __builtin_amdgcn_readlane(sq.len, b - chunk);
+  s.count = __builtin_amdgcn_readlane(sq.count, b - chunk);
   int left = (int)min<int64_t>(per, total - first);
   while (true) {
-    const TreeSeq s = tree_seq(a.tree, b);
     const int slices = tree_slices(s, slice), tiles = tree_tiles(s, group, rows);
     while (at < slices * tiles * a.kv_heads) {
       const int pair = at / slices, sl = at - pair * slices, n = min(slices - sl, left);
-      const int part = n == slices ? -1 : 2 * (int)blockIdx.x + (sl == 0 ? 1 : 0);
+      const int part = n == slices ? -1 : 2 * block + (sl == 0 ? 1 : 0);
       take(s, b, pair / tiles, pair % tiles, sl, sl + n, part);
       left -= n;
       if (left == 0) return;
       at += n;
     }
     at = 0;
-    do b++;
-    while (tree_seq(a.tree, b).nodes == 0);
+    s = tree_seq(a.tree, ++b);
   }
 }
 
@@ -154,7 +154,6 @@ __host__ __device__ __forceinline__ size_t rows_lds_bytes(int head_dim) {
 template <bool Q8, int ND>
 __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAttend a, TreeParts parts,
                                                                         int32_t* __restrict__ plan) {
-  __shared__ TreeScan scan;
   extern __shared__ float4 lds[];
   const int D = a.head_dim, kk = rows_slice(D), KS = D + 4;
   const int words = (a.tree.max_nodes + 31) >> 5, group = a.heads / a.kv_heads;
@@ -167,8 +166,7 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
   const float c2 = a.scale * kLog2e;
   const int split = 64 / kk, part_d = lane / kk, key = lane % kk;
 
-  tree_walk<kRowsThreads>(a, kRowsTile, kk, scan, plan, [&](const TreeSeq& sq, int b, int kvh, int tile, int s0, int s1,
-                                                            int part) {
+  tree_walk(a, kRowsTile, kk, plan, [&](const TreeSeq& sq, int b, int kvh, int tile, int s0, int s1, int part) {
     const __half* kc = (const __half*)a.k_cache + (a.kv_index ? 0 : (int64_t)b * a.cache_stride);
     const __half* vc = (const __half*)a.v_cache + (a.kv_index ? 0 : (int64_t)b * a.cache_stride);
     const int32_t* index = a.kv_index ? a.kv_index + (int64_t)b * a.index_stride : nullptr;
@@ -316,9 +314,11 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 //
 // q8_0: keys and values enter as their integers, exact halves; a key block's
 // factor multiplies its part of the score, a value block's the weights, which
-// are then split into halves at 2^(15 - X), X the exponent of the column's
-// largest product since its maximum last rose (as in attend_decode.hip): what a
-// column does not see has no part in its X.
+// are then split into halves.  The factors are staged times 2^(15 - X), X the
+// exponent of the largest one so far among committed positions, which every row
+// sees; slices that some row does not see whole leave X as it is, and there each
+// row's products are scaled to its own largest and summed apart: what a row does
+// not see has no part in its result.
 //
 // A value that is not finite in a node that some query does not see would give
 // 0 * inf there: such values are staged as zeros and added at the end to the
@@ -340,17 +340,13 @@ __device__ __forceinline__ tf4 mfma16(th8 a, th8 b, tf4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// 16-byte piece pc of LDS row r lies at slot pc ^ swz(r), so that the lanes
-// served together fall on distinct banks: keys are read one piece of 16 rows,
-// values (transposed) 4 rows x 32 bytes per 16 lanes.
-template <int D>
-__device__ __forceinline__ int key_swz(int r) {
-  return D >= 128 ? (r & 15) : ((r >> 1) & 7);
-}
-template <int D>
-__device__ __forceinline__ int val_swz(int r) {
-  return (D >= 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1)) | ((r >> 2) & 3);
-}
+// LDS rows are padded, so that the lanes served together fall on distinct banks
+// and every fragment is at a fixed distance from a lane's first: keys (16 rows,
+// one 16-byte piece of each) by 16 bytes, values (read transposed, 4 rows x 32
+// bytes per 16 lanes) by 32.  (Pieces permuted by an exclusive or, as in
+// attend_flash.hip, cost an instruction and a register for each.)
+__host__ __device__ constexpr int key_row(int D) { return D + 8; }   // halves
+__host__ __device__ constexpr int val_row(int D) { return D + 16; }
 
 // over the four lanes that share a column
 template <class Op>
@@ -403,46 +399,47 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
 // the words of 64 on their way cost the registers of a second block's wave; 64 at
 // D = 64), and blocks a compute unit.
 __host__ __device__ constexpr int mfma_slice(int D) { return D == 64 ? 64 : 32; }
-__host__ __device__ constexpr int mfma_blocks(int D, int NC) { return D == 256 || (D == 128 && NC == 2) ? 2 : 3; }
+__host__ __device__ constexpr int mfma_blocks(int D, int NC, bool Q8) {
+  return D == 64 ? (Q8 ? 3 : 4) : D == 128 && NC == 1 ? 3 : 2;
+}
 
+#ifndef VGX
+#define VGX 2
+#endif
 template <int D, int NC, bool Q8, bool PAGED>
-__global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(TreeAttend a, TreeParts parts,
+__global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kernel(TreeAttend a, TreeParts parts,
                                                                               int32_t* __restrict__ plan) {
   constexpr int SL = mfma_slice(D), KS = D / 32, NT = D / 16, PIECES = D / 8;
   constexpr int PER = Q8 ? (SL * D / 16 + 255) / 256 : SL * PIECES / 256;  // 16-byte words of K (and of V) a thread
   constexpr int WPK = Q8 ? D / 16 : PIECES;                               // words a key
   constexpr int ROWS = 64 * NC;
+  constexpr int VG = VGX < NT ? VGX : NT;  // 16-dim tiles of values a group of reads
   static_assert(PER * 256 == SL * WPK, "a slice's words dealt evenly");
-  __shared__ __align__(16) _Float16 ks[2][SL * D];
-  __shared__ __align__(16) _Float16 vs[2][SL * D];
+  constexpr int KR = key_row(D), VR = val_row(D);
+  __shared__ __align__(16) _Float16 ks[2][SL * KR];
+  __shared__ __align__(16) _Float16 vs[2][SL * VR];
   __shared__ __align__(16) float fac[Q8 ? 2 : 1][2][Q8 ? KS : 1][Q8 ? SL : 1];  // q8_0 factors of keys and values
+  __shared__ int xs[Q8 ? 2 : 1][Q8 ? KS : 1];                                   // X that the values' factors are at
   __shared__ int holes[2];  // the step whose slice in this buffer has a cell that is not held
-  __shared__ int spoilt;    // the run in which some value of a node was not finite
-  __shared__ TreeScan scan;
+  __shared__ int spoilt[2]; // the last (even, odd) run in which some staged value was not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lm = lane & 15, lk = lane >> 4;
   const int group = a.heads / a.kv_heads, words = (a.tree.max_nodes + 31) >> 5;
   const int kvw = a.kv_heads * D, crow = cache_row(a.form, kvw);
-  if (tid == 0) holes[0] = holes[1] = spoilt = 0;  // (ahead of the walk's barriers)
-  int turn = 0;  // steps this block has staged, over all its runs
+  if (tid == 0) holes[0] = holes[1] = spoilt[0] = spoilt[1] = 0;
+  __syncthreads();
+  int turn = 0, run = 0;  // slices that this block has staged, and runs that it has taken
 
-  // lane addresses in bytes: a piece's slot is an exclusive or with bits that a
-  // row's start leaves free
-  typedef __attribute__((address_space(3))) const char* lds_ptr;
-  typedef __attribute__((address_space(3))) const th8* lds_h8;
-  const uint32_t kat = 2 * lm * D + 16 * (lk ^ key_swz<D>(lm));
-  uint32_t vat[2];
-#pragma unroll
-  for (int v = 0; v < 2; v++) {
-    const int row = 4 * lk + (lm >> 2) + 16 * v;
-    vat[v] = 2 * row * D + 16 * (((lm & 3) >> 1) ^ val_swz<D>(row)) + 8 * (lm & 1);
-  }
+  // a lane's place in a tile of 32 keys, in halves: key lm, values 8 lk .., and for
+  // the transposed reads row 4 lk + lm / 4, dims 4 (lm % 4) ..
+  const int kat = lm * KR + 8 * lk, vat = (4 * lk + (lm >> 2)) * VR + 4 * (lm & 3);
 
-  tree_walk<256>(a, ROWS, SL, scan, plan, [&](const TreeSeq& sq, int b, int kvh, int tile, int s0, int s1, int part) {
+  tree_walk(a, ROWS, SL, plan, [&](const TreeSeq& sq, int b, int kvh, int tile, int s0, int s1, int part) {
     const __half* kc = (const __half*)a.k_cache + (PAGED ? 0 : (int64_t)b * a.cache_stride) + (Q8 ? kvh * D / 2 : kvh * D);
     const __half* vc = (const __half*)a.v_cache + (PAGED ? 0 : (int64_t)b * a.cache_stride) + (Q8 ? kvh * D / 2 : kvh * D);
     const int32_t* index = PAGED ? a.kv_index + (int64_t)b * a.index_stride : nullptr;
-    const int run = turn + 1;
+    run++;
+    const int first_turn = turn + 1;
 
     // this lane's columns: rows past the sequence's repeat its last one (not written)
     const int first_row = tile * ROWS + wave * 16 * NC;
@@ -458,6 +455,10 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
     tu4 kw[PER], vw[PER];
     int cells[PAGED ? PER : 1], fcell = 0;  // the next slice's (negative: not held)
     tu4 fw = {0, 0, 0, 0};                  // q8_0: thread = (key or value, key) of the first 2 SL
+    bool fdead = false;
+    int xrun[Q8 ? KS : 1];  // q8_0: the X of each 32-dim block so far (the wave that stages the values' factors)
+#pragma unroll
+    for (int u = 0; u < (Q8 ? KS : 1); u++) xrun[u] = 0;
     auto cell_at = [&](int j) __attribute__((always_inline)) { return index[min(j, sq.count - 1)]; };
     auto find = [&](int sl) __attribute__((always_inline)) {
       if constexpr (PAGED) {
@@ -466,21 +467,24 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
         if (Q8) fcell = cell_at(sl * SL + tid % SL);
       }
     };
-    uint32_t dead = 0;  // bit j: nothing is held where word j was loaded
+    bool dead = false;  // nothing is held where some word was loaded
     auto load = [&](int sl) __attribute__((always_inline)) {
-      dead = 0;
+      dead = false;
 #pragma unroll
       for (int j = 0; j < PER; j++) {
         const int i = tid + 256 * j, at = sl * SL + i / WPK;
-        const int cell = PAGED ? cells[j] : min(at, sq.count - 1);
-        if (PAGED && cell < 0) dead |= 1u << j;
+        int cell = PAGED ? cells[j] : min(at, sq.count - 1);
+        // (opaque: an address formed ahead of the products would wait for its cell there)
+        if (PAGED) asm volatile("" : "+v"(cell));
+        dead |= PAGED && cell < 0;
         const int64_t off = (int64_t)(PAGED ? max(cell, 0) : cell) * crow + 8 * (i % WPK);
         kw[j] = *(const tu4*)(kc + off);
         vw[j] = *(const tu4*)(vc + off);
       }
       if constexpr (Q8) {
-        const int at = sl * SL + tid % SL, cell = PAGED ? fcell : min(at, sq.count - 1);
-        if (at >= sq.count || (PAGED && cell < 0)) dead |= 1u << 31;
+        int at = sl * SL + tid % SL, cell = PAGED ? fcell : min(at, sq.count - 1);
+        if (PAGED) asm volatile("" : "+v"(cell));
+        fdead = at >= sq.count || (PAGED && cell < 0);
         if (tid < 2 * SL) {
           const __half* f = (tid < SL ? kc : vc) + (int64_t)(PAGED ? max(cell, 0) : cell) * crow + (kvw >> 1) -
                             kvh * D / 2 + ((kvh * D) >> 5);
@@ -494,32 +498,47 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
       turn++;
       const bool nodes_in = (sl + 1) * SL > sq.len;  // (uniform)
       if (PAGED && dead) holes[buf] = turn;
+      // what is not held, and what some row may not see, must be finite: 0 * inf in
+      // the products would reach every row
+      if (!Q8 && (nodes_in || (PAGED && __any(dead)))) {
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const uint32_t f = finite_halves(vw[j][e]);
+            bad |= f != vw[j][e];
+            vw[j][e] = f;
+          }
+        if (bad) spoilt[run & 1] = run;
+      }
 #pragma unroll
       for (int j = 0; j < PER; j++) {
         const int i = tid + 256 * j, key = i / WPK, pc = i % WPK;
         if constexpr (Q8) {
-          *(th8*)(ks[buf] + key * D + 8 * ((2 * pc) ^ key_swz<D>(key))) = int8_halves(kw[j].x, kw[j].y);
-          *(th8*)(ks[buf] + key * D + 8 * ((2 * pc + 1) ^ key_swz<D>(key))) = int8_halves(kw[j].z, kw[j].w);
-          *(th8*)(vs[buf] + key * D + 8 * ((2 * pc) ^ val_swz<D>(key))) = int8_halves(vw[j].x, vw[j].y);
-          *(th8*)(vs[buf] + key * D + 8 * ((2 * pc + 1) ^ val_swz<D>(key))) = int8_halves(vw[j].z, vw[j].w);
+          *(th8*)(ks[buf] + key * KR + 16 * pc) = int8_halves(kw[j].x, kw[j].y);
+          *(th8*)(ks[buf] + key * KR + 16 * pc + 8) = int8_halves(kw[j].z, kw[j].w);
+          *(th8*)(vs[buf] + key * VR + 16 * pc) = int8_halves(vw[j].x, vw[j].y);
+          *(th8*)(vs[buf] + key * VR + 16 * pc + 8) = int8_halves(vw[j].z, vw[j].w);
         } else {
-          tu4 v = vw[j];
-          // (what is not held, and what some row may not see, is never more than zero times a weight of zero)
-          if ((nodes_in && sl * SL + key >= sq.len) || (PAGED && dead)) {
-            const tu4 f = {finite_halves(v.x), finite_halves(v.y), finite_halves(v.z), finite_halves(v.w)};
-            if ((f.x ^ v.x) | (f.y ^ v.y) | (f.z ^ v.z) | (f.w ^ v.w)) spoilt = run;
-            v = f;
-          }
-          *(tu4*)(ks[buf] + key * D + 8 * (pc ^ key_swz<D>(key))) = kw[j];
-          *(tu4*)(vs[buf] + key * D + 8 * (pc ^ val_swz<D>(key))) = v;
+          *(tu4*)(ks[buf] + key * KR + 8 * pc) = kw[j];
+          *(tu4*)(vs[buf] + key * VR + 8 * pc) = vw[j];
         }
       }
       if constexpr (Q8) {
-        if (tid < 2 * SL) {
+        if (tid < 2 * SL) {  // (the values' factors are one wave's, or a half of it)
           const uint32_t w[4] = {fw.x, fw.y, fw.z, fw.w};
 #pragma unroll
-          for (int u = 0; u < KS; u++)
-            fac[buf][tid / SL][u][tid % SL] = dead >> 31 ? 0.0f : half_bits_to_float(w[u >> 1] >> (16 * (u & 1)));
+          for (int u = 0; u < KS; u++) {
+            float f = fdead ? 0.0f : half_bits_to_float(w[u >> 1] >> (16 * (u & 1)));
+            if (tid >= SL) {
+              const float af = fabsf(f), fm = lanes::reduce<SL>(af < INFINITY ? af : 0.0f, lanes::Max{});
+              if (!nodes_in && fm > 0.0f) xrun[u] = max(xrun[u], __builtin_amdgcn_frexp_expf(fm));
+              f = ldexpf(f, 15 - xrun[u]);
+              if (tid == SL) xs[buf][u] = xrun[u];
+            }
+            fac[buf][tid / SL][u][tid % SL] = f;
+          }
         }
       }
     };
@@ -564,7 +583,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
     tf4 o[NC][NT];
     // running maximum (of the scores, before c2), the same times c2, and this lane's part of the sum
     float mc[NC], mk[NC], l[NC];
-    int xo[NC][Q8 ? KS : 1];  // q8_0: the X that a 32-dim block of o is held at
+    int xo[Q8 ? KS : 1];  // q8_0: (uniform) the X that a 32-dim block of o is held at
 #pragma unroll
     for (int c = 0; c < NC; c++) {
       mc[c] = -1e30f;
@@ -572,40 +591,73 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
       l[c] = 0.0f;
 #pragma unroll
       for (int dt = 0; dt < NT; dt++) o[c][dt] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int u = 0; u < (Q8 ? KS : 1); u++) xo[c][u] = -100;
     }
+#pragma unroll
+    for (int u = 0; u < (Q8 ? KS : 1); u++) xo[u] = 0;
     // a row's mk is too large for a weight's exponent; (uniform) some row's is
     auto large = [&](int c) __attribute__((always_inline)) { return mc[c] > -1e30f && !(fabsf(mk[c]) <= 4e6f); };
     bool huge = false;
 
-    // keys 32 kt .. of slice sl
-    auto step = [&](int sl, int kt, int buf) __attribute__((always_inline)) {
-      const int base = sl * SL + 32 * kt;
-      const lds_ptr kp = (lds_ptr)&ks[buf][32 * kt * D], vp = (lds_ptr)&vs[buf][32 * kt * D];
-      tf4 s[NC][2];
+    // the scores of keys 32 kt .. of a slice, and whether all its cells are held
+    auto scores = [&](int sl, int kt, int buf, tf4 (&s)[NC][2], int& hole) __attribute__((always_inline)) {
+      const _Float16* kp = &ks[buf][32 * kt * KR + kat];
+      if (PAGED) hole = holes[buf];
+      // key fragments of as many products as there are registers for on their way
+      // before the first (one at a time, the compiler's order, left each product
+      // waiting for LDS)
+      constexpr int HG = KS <= 4 ? 2 : 1;
+      th8 k8[HG][KS];
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
+      for (int h0 = 0; h0 < 2; h0 += HG) {
 #pragma unroll
-        for (int c = 0; c < NC; c++) s[c][h] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int h = 0; h < HG; h++)
+#pragma unroll
+          for (int u = 0; u < KS; u++) k8[h][u] = *(const th8*)(kp + 16 * (h0 + h) * KR + 32 * u);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int h = 0; h < HG; h++)
+#pragma unroll
+          for (int c = 0; c < NC; c++) s[c][h0 + h] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int u = 0; u < KS; u++) {
-          const th8 k8 = *(lds_h8)(kp + ((kat + 2 * 16 * h * D) ^ (64 * u)));
           if constexpr (Q8) {
-            const tf4 f = *(const tf4*)&fac[buf][0][u][32 * kt + 16 * h + 4 * lk];
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-              const tf4 d = mfma16(k8, qf[1][c][u], mfma16(k8, qf[0][c][u], tf4{0.0f, 0.0f, 0.0f, 0.0f}));
+            for (int h = 0; h < HG; h++) {
+              const tf4 f = *(const tf4*)&fac[buf][0][u][32 * kt + 16 * (h0 + h) + 4 * lk];
 #pragma unroll
-              for (int i = 0; i < 4; i++) s[c][h][i] = fmaf(f[i], d[i], s[c][h][i]);
+              for (int c = 0; c < NC; c++) {
+                const tf4 d = mfma16(k8[h][u], qf[1][c][u], mfma16(k8[h][u], qf[0][c][u], tf4{0.0f, 0.0f, 0.0f, 0.0f}));
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[c][h0 + h][i] = fmaf(f[i], d[i], s[c][h0 + h][i]);
+              }
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < NC; c++) s[c][h] = mfma16(k8, qf[1][c][u], mfma16(k8, qf[0][c][u], s[c][h]));
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+              for (int h = 0; h < HG; h++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) s[c][h0 + h] = mfma16(k8[h][u], qf[k][c][u], s[c][h0 + h]);
           }
         }
       }
-      const bool all = base + 32 <= sq.len && !(PAGED && holes[buf] == run + (sl - s0));  // (uniform)
+      if (PAGED) hole = __builtin_amdgcn_readfirstlane(hole) - (first_turn + sl - s0);
+    };
+    // their softmax and weighted values
+    auto values = [&](int sl, int kt, int buf, tf4 (&s)[NC][2], int hole) __attribute__((always_inline)) {
+      const int base = sl * SL + 32 * kt;
+      const _Float16* vp = &vs[buf][32 * kt * VR + vat];
+      ts4 v4[2][VG][2];
+      auto vread = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 0; d < VG; d++)
+#pragma unroll
+          for (int w = 0; w < 2; w++)
+            v4[g & 1][d][w] =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4*)(vp + 16 * w * VR + 16 * (g * VG + d)));
+      };
+      vread(0);
+      const bool all = base + 32 <= sq.len && !(PAGED && hole == 0);  // (uniform)
       uint32_t mine[NC];  // bit (i & 3) + 16 (i >> 2): key 4 lk + that is seen
       if (!all) {
         const int key = base + (lane & 31);
@@ -621,7 +673,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
       }
       th8 ph[NC], pl[NC];
       float p[NC][8];
-      bool rose[NC];
+      int xc[Q8 ? NC : 1];
 #pragma unroll
       for (int c = 0; c < NC; c++) {
         float m = s[c][0][0];
@@ -629,9 +681,9 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
         for (int i = 1; i < 8; i++) m = fmaxf(m, s[c][i >> 2][i & 3]);
         m = across(m, lanes::Max{});
         const float mn = fmaxf(mc[c], m);
-        rose[c] = mn != mc[c];
-        if (__any(rose[c])) {
-          const float mkn = rose[c] ? mn * c2[c] : mk[c];
+        const bool rose = mn != mc[c];
+        if (__any(rose)) {
+          const float mkn = rose ? mn * c2[c] : mk[c];
           const float f = __builtin_amdgcn_exp2f(large(c) ? (mc[c] - mn) * c2[c] : mk[c] - mkn);
           l[c] *= f;
 #pragma unroll
@@ -648,13 +700,24 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
 #pragma unroll
           for (int i = 0; i < 8; i++) p[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i >> 2][i & 3], c2[c], -mk[c]));
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) l[c] += p[c][i];
+        l[c] += ((p[c][0] + p[c][1]) + (p[c][2] + p[c][3])) + ((p[c][4] + p[c][5]) + (p[c][6] + p[c][7]));
         if constexpr (!Q8) {
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             ph[c][i] = (_Float16)fmaf(p[c][i], kLift, 0.0f);  // (one instruction)
             pl[c][i] = (_Float16)fmaf(p[c][i], kLift, -(float)ph[c][i]);
+          }
+        }
+      }
+      if constexpr (Q8) {  // (uniform) X has risen with this slice's factors
+#pragma unroll
+        for (int u = 0; u < KS; u++) {
+          const int x = __builtin_amdgcn_readfirstlane(xs[buf][u]);
+          if (x != xo[u]) {
+            const float f = ldexpf(1.0f, xo[u] - x);
+#pragma unroll
+            for (int c = 0; c < NC; c++) o[c][2 * u] *= f, o[c][2 * u + 1] *= f;
+            xo[u] = x;
           }
         }
       }
@@ -666,79 +729,103 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
             const tf4 f0 = *(const tf4*)&fac[buf][1][u][32 * kt + 4 * lk], f1 = *(const tf4*)&fac[buf][1][u][32 * kt + 16 + 4 * lk];
 #pragma unroll
             for (int c = 0; c < NC; c++) {
+              if (all) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                  const float f = i < 4 ? f0[i & 3] : f1[i & 3];
+                  ph[c][i] = (_Float16)fmaf(p[c][i], f, 0.0f);
+                  pl[c][i] = (_Float16)fmaf(p[c][i], f, -(float)ph[c][i]);
+                }
+                continue;
+              }
+              // (whatever the factor of a key that is not seen)
               float w[8], wm = 0.0f;
 #pragma unroll
-              for (int i = 0; i < 8; i++) w[i] = p[c][i] * (i < 4 ? f0[i & 3] : f1[i & 3]);
-              if (!all) {  // (whatever the factor of a key that is not seen)
-#pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = (mine[c] >> ((i & 3) + 16 * (i >> 2))) & 1 ? w[i] : 0.0f;
+              for (int i = 0; i < 8; i++) {
+                w[i] = (mine[c] >> ((i & 3) + 16 * (i >> 2))) & 1 ? p[c][i] * (i < 4 ? f0[i & 3] : f1[i & 3]) : 0.0f;
+                wm = fmaxf(wm, fabsf(w[i]));
               }
-#pragma unroll
-              for (int i = 0; i < 8; i++) wm = fmaxf(wm, fabsf(w[i]));
               wm = across(wm, lanes::Max{});
-              const int old = xo[c][u];
-              // (an infinite factor: the finite products are below 2^31)
-              const int xw = wm < INFINITY ? __builtin_amdgcn_frexp_expf(wm) : 31;
-              const int x = wm > 0.0f ? max(max(xw, rose[c] ? old - 60 : old), -100) : old;
-              if (__any(x != old)) {
-                const float f = ldexpf(1.0f, old - x);
-                o[c][dt] *= f;
-                o[c][dt + 1] *= f;
-                xo[c][u] = x;
-              }
-              const float unit = ldexpf(1.0f, 15 - x);
+              xc[c] = wm > 0.0f && wm < INFINITY ? __builtin_amdgcn_frexp_expf(wm) : 0;
+              const float unit = ldexpf(1.0f, 15 - xc[c]);
 #pragma unroll
               for (int i = 0; i < 8; i++) {
                 ph[c][i] = (_Float16)fmaf(w[i], unit, 0.0f);
                 pl[c][i] = (_Float16)fmaf(w[i], unit, -(float)ph[c][i]);
               }
-              if (__builtin_expect(__any(!(wm < INFINITY)), 0)) {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                  if (!(fabsf(w[i]) < INFINITY)) pl[c][i] = 0;
-              }
             }
           }
         }
+        if (dt % VG == 0) {
+          if (dt + VG < NT) vread(dt / VG + 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         ts8 v;
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-          const ts4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4*)(vp + (vat[w] ^ (32 * dt))));
+        for (int w = 0; w < 2; w++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) v[4 * w + e] = x[e];
+          for (int e = 0; e < 4; e++) v[4 * w + e] = v4[(dt / VG) & 1][dt % VG][w][e];
+        if (!Q8 || all) {
+#pragma unroll
+          for (int c = 0; c < NC; c++) o[c][dt] = mfma16(__builtin_bit_cast(th8, v), ph[c], o[c][dt]);
+#pragma unroll
+          for (int c = 0; c < NC; c++) o[c][dt] = mfma16(__builtin_bit_cast(th8, v), pl[c], o[c][dt]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < NC; c++) {
+            const tf4 t = mfma16(__builtin_bit_cast(th8, v), pl[c], mfma16(__builtin_bit_cast(th8, v), ph[c], tf4{0.0f, 0.0f, 0.0f, 0.0f}));
+            const float f = ldexpf(1.0f, xc[c] - 15);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[c][dt][e] = fmaf(t[e], f, o[c][dt][e]);
+          }
         }
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-          o[c][dt] = mfma16(__builtin_bit_cast(th8, v), pl[c], mfma16(__builtin_bit_cast(th8, v), ph[c], o[c][dt]));
       }
     };
 
     store(s0, 0);
+    if (s0 + 1 < s1) {
+      load(s0 + 1);
+      if (s0 + 2 < s1) find(s0 + 2);
+    }
     __syncthreads();
     for (int sl = s0, buf = 0; sl < s1; sl++, buf ^= 1) {
-      const bool more = sl + 1 < s1;  // (uniform)
-      if (more) {
-        load(sl + 1);
-        if (sl + 2 < s1) find(sl + 2);
+      tf4 s[NC][2];
+      int hole = 1;
+      if (busy) scores(sl, 0, buf, s, hole);
+      // the next slice from registers to the other buffer, and the one behind it on
+      // its way (written once for busy and idle waves: with a copy for each the
+      // registers differ, and the busy ones wait for loads at every step)
+      __builtin_amdgcn_sched_barrier(0);
+      if (sl + 1 < s1) {
+        store(sl + 1, buf ^ 1);
+        if (sl + 2 < s1) {
+          load(sl + 2);
+          if (sl + 3 < s1) find(sl + 3);
+        }
       }
       if (busy) {
-#pragma unroll
-        for (int kt = 0; kt < SL / 32; kt++)
-          if (sl * SL + 32 * kt < sq.count) step(sl, kt, buf);
+        values(sl, 0, buf, s, hole);
+        if constexpr (SL > 32) {
+          if (sl * SL + 32 < sq.count) {
+            scores(sl, 1, buf, s, hole);
+            values(sl, 1, buf, s, hole);
+          }
+        }
       }
-      if (more) store(sl + 1, buf ^ 1);
       __syncthreads();
     }
 
-    if (!Q8 && __builtin_expect(spoilt == run, 0) && busy) {
-      for (int j = max(s0 * SL, sq.len); j < min(s1 * SL, sq.count); j++) {
+    // non-finite values of slices that were staged without them, to the rows that
+    // see them (of the other slices', which are in o already, a second time)
+    if (!Q8 && __builtin_expect(spoilt[run & 1] == run, 0) && busy) {
+      for (int j = s0 * SL; j < min(s1 * SL, sq.count); j++) {
         const int cell = PAGED ? index[j] : j;
         if (cell < 0) continue;
         const __half* vr = vc + (int64_t)cell * crow + 4 * lk;
         const int i = j - sq.len;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-          const bool sees = (mask_row(c)[i >> 5] >> (i & 31)) & 1;
+          const bool sees = i < 0 || ((mask_row(c)[max(i, 0) >> 5] >> (i & 31)) & 1);
 #pragma unroll
           for (int dt = 0; dt < NT; dt++)
 #pragma unroll
@@ -760,7 +847,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
       const float w = (part >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f) * (Q8 ? 1.0f : 1.0f / kLift);
 #pragma unroll
       for (int dt = 0; dt < NT; dt++) {
-        const float f = Q8 ? w * ldexpf(1.0f, xo[c][dt / 2] - 15) : w;
+        const float f = Q8 ? w * ldexpf(1.0f, xo[dt / 2] - 15) : w;
         *(tf4*)(dst + 16 * dt + 4 * lk) = o[c][dt] * f;
       }
       if (part >= 0 && lk == 0) *(float2*)(parts.ml + 2 * slot) = make_float2(mk[c], sum);
@@ -768,51 +855,73 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC)) void attend_tree_kernel(Tr
   });
 }
 
-// Folds the parts of each row whose tile several blocks share: a wave a row, up
-// to eight parts' sums on their way at once.  A part that no key of the row fell
-// in has sum 0 and weight 0; a row without any other is zero.
-template <int V>
+// Folds the parts of each row whose tile several blocks share: W waves a row, up
+// to eight parts' sums of each on their way at once.  A part that no key of the
+// row fell in has sum 0 and weight 0; a row without any other is zero.
+template <int V, int W>
 __global__ __launch_bounds__(256) void attend_tree_fold_kernel(TreeAttend a, TreeParts parts,
                                                                const int32_t* __restrict__ plan, int rows, int slice) {
   typedef float vec __attribute__((ext_vector_type(V)));
-  const int lane = threadIdx.x & 63, D = a.head_dim, group = a.heads / a.kv_heads;
-  const int64_t i = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ vec sums[W > 1 ? W : 1][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int D = a.head_dim, group = a.heads / a.kv_heads;
+  const int64_t i = (int64_t)blockIdx.x * (4 / W) + wave / W;
   const int b = (int)(i / ((int64_t)a.tree.max_nodes * a.heads));
-  if (b >= a.tree.batch) return;
+  if (b >= a.tree.batch) return;  // (W > 1: every wave of the block)
   const int at = (int)(i - (int64_t)b * a.tree.max_nodes * a.heads), node = at / a.heads, h = at - node * a.heads;
+  const int per = plan[0], b_first = plan[1 + b];
   const TreeSeq sq = tree_seq(a.tree, b);
   if (node >= sq.nodes) return;
   const int kvh = h / group, r = node * group + h % group, tile = r / rows, slices = tree_slices(sq, slice);
-  const int per = plan[0], u0 = plan[1 + b] + (kvh * tree_tiles(sq, group, rows) + tile) * slices;
+  const int u0 = b_first + (kvh * tree_tiles(sq, group, rows) + tile) * slices;
   const int g0 = u0 / per, n = (u0 + slices - 1) / per - g0 + 1;
   if (n == 1) return;  // one block's: finished
   // part k is block g0 + k's: its last one (1) for the block that the tile starts in, else its first (0)
   auto slot = [&](int k) { return (int64_t)(2 * (g0 + k) + (k == 0 ? 1 : 0)) * rows + r % rows; };
-  const float2 ml = ((const float2*)parts.ml)[slot(min(lane, n - 1))];
-  const bool live = lane < n && ml.y != 0.0f;
-  const float m = lanes::reduce<64>(live ? ml.x : -INFINITY, lanes::Max{});
-  const float w = live ? (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m)) : 0.0f;
-  const float sum = lanes::reduce<64>(live ? ml.y * w : 0.0f, lanes::Add{});
+  const int per_wave = (n + W - 1) / W, k0 = (wave % W) * per_wave, k1 = min(k0 + per_wave, n);
+  float2 ml[2];
+#pragma unroll
+  for (int k = 0; k < 2; k++) ml[k] = ((const float2*)parts.ml)[slot(min(64 * k + lane, n - 1))];
+  // eight parts' sums from k on (past the end the last one again, weight 0)
+  vec x[8];
+  auto send = [&](int k, int d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = *(const vec*)(parts.acc + slot(min(k + j, n - 1)) * D + d);
+  };
+  send(k0, min(lane * V, D - V));  // (behind the maxima, and waited for with them)
+  float w[2], m = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    if (64 * k + lane >= n) ml[k].y = 0.0f;
+    if (ml[k].y != 0.0f) m = fmaxf(m, ml[k].x);
+  }
+  m = lanes::reduce<64>(m, lanes::Max{});
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    w[k] = ml[k].y == 0.0f ? 0.0f : ml[k].x == m ? 1.0f : __builtin_amdgcn_exp2f(ml[k].x - m);
+    sum += ml[k].y == 0.0f ? 0.0f : ml[k].y * w[k];
+  }
+  sum = lanes::reduce<64>(sum, lanes::Add{});
   const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
   float* dst = a.out + ((int64_t)(sq.t0 + node) * a.heads + h) * D;
   for (int d0 = 0; d0 < D; d0 += 64 * V) {
     const int d = min(d0 + lane * V, D - V);
     vec o = {};
-    auto add = [&](int k0, auto count) __attribute__((always_inline)) {
-      constexpr int N = decltype(count)::value;
-      vec x[N];
+    for (int k = k0; k < k1; k += 8) {
+      if (d0 || k != k0) send(k, d);
 #pragma unroll
-      for (int k = 0; k < N; k++) x[k] = *(const vec*)(parts.acc + slot(k0 + k) * D + d);
+      for (int j = 0; j < 8; j++)
+        if (k + j < k1)  // (uniform)
+          o += x[j] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k + j < 64 ? w[0] : w[1]), (k + j) & 63));
+    }
+    if constexpr (W > 1) {
+      if (d0) __syncthreads();
+      sums[wave][lane] = o;
+      __syncthreads();
+      if (wave) continue;
 #pragma unroll
-      for (int k = 0; k < N; k++) {
-        o += x[k] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), k0 + k));
-      }
-    };
-    int k = 0;
-    for (; k + 8 <= n; k += 8) add(k, std::integral_constant<int, 8>{});
-    if (n - k >= 4) add(k, std::integral_constant<int, 4>{}), k += 4;
-    if (n - k >= 2) add(k, std::integral_constant<int, 2>{}), k += 2;
-    if (n - k >= 1) add(k, std::integral_constant<int, 1>{});
+      for (int v = 1; v < W; v++) o += sums[v][lane];
+    }
     if (d0 + lane * V < D) *(vec*)(dst + d) = o * inv;
   }
 }
@@ -825,16 +934,16 @@ struct TreeGrid {
   int blocks;
 };
 
-TreeGrid tree_grid(int heads, int kv_heads, int head_dim, const mi_tree& t) {
+TreeGrid tree_grid(int heads, int kv_heads, int head_dim, int form, const mi_tree& t) {
   TreeGrid g;
   const int group = heads / kv_heads;
   g.mfma = head_dim == 64 || head_dim == 128 || head_dim == 256;
-  g.columns = head_dim <= 128 && t.max_nodes * group > 64 ? 2 : 1;
+  g.columns = head_dim == 128 && form != MI_CACHE_Q8 && t.max_nodes * group > 64 ? 2 : 1;
   g.rows = g.mfma ? 64 * g.columns : kRowsTile;
   g.slice = g.mfma ? mfma_slice(head_dim) : rows_slice(head_dim);
   g.units = (int64_t)t.batch * ((t.max_nodes * group + g.rows - 1) / g.rows) * kv_heads *
             (((int64_t)t.max_count + g.slice - 1) / g.slice);
-  g.blocks = (int)std::min<int64_t>(g.units, (int64_t)cu_count() * (g.mfma ? mfma_blocks(head_dim, g.columns) : 3));
+  g.blocks = (int)std::min<int64_t>(g.units, (int64_t)cu_count() * (g.mfma ? mfma_blocks(head_dim, g.columns, form == MI_CACHE_Q8) : 3));
   return g;
 }
 
@@ -854,13 +963,16 @@ TreeCarve tree_carve(const TreeGrid& g, int head_dim, int batch) {
 
 }  // namespace
 
-size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, const mi_tree& t) {
-  return tree_carve(tree_grid(heads, kv_heads, head_dim, t), head_dim, t.batch).total;
+size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const mi_tree& t) {
+  return tree_carve(tree_grid(heads, kv_heads, head_dim, form, t), head_dim, t.batch).total;
 }
 
 int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work) {
-  const TreeGrid g = tree_grid(a.heads, a.kv_heads, a.head_dim, a.tree);
-  const int64_t fold = ((int64_t)a.tree.batch * a.tree.max_nodes * a.heads + 3) / 4;
+  const TreeGrid g = tree_grid(a.heads, a.kv_heads, a.head_dim, a.form, a.tree);
+  // few rows: four waves each (416 rows of 62 parts 8.4 -> XX us)
+  const int64_t rows = (int64_t)a.tree.batch * a.tree.max_nodes * a.heads;
+  const int waves = rows <= 1024 ? 4 : 1;
+  const int64_t fold = (rows * waves + 3) / 4;
   if (g.units > 0x7fffffff || fold > 0x7fffffff)
     return fail(MI_ERR_SHAPE, "attend_tree: %d sequences of %d nodes and %d positions are too much work", a.tree.batch,
                 a.tree.max_nodes, a.tree.max_count);
@@ -886,11 +998,11 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work) {
     hipLaunchKernelGGL((attend_tree_rows_kernel<false, ND>), grid, dim3(kRowsThreads), rows_lds_bytes(a.head_dim), s, \
                        a, parts, plan)
   if (a.head_dim == 64) {
-    if (g.columns == 1) { MI_TREE_F(64, 1) }
-    else { MI_TREE_F(64, 2) }
+    MI_TREE_F(64, 1)
   } else if (a.head_dim == 128) {
     if (g.columns == 1) { MI_TREE_F(128, 1) }
-    else { MI_TREE_F(128, 2) }
+    else if (a.kv_index) MI_TREE(128, 2, false, true);
+    else MI_TREE(128, 2, false, false);
   } else if (a.head_dim == 256) {
     MI_TREE_F(256, 1)
   } else if (a.head_dim < 64) {
@@ -906,8 +1018,13 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work) {
 #undef MI_TREE_F
 #undef MI_TREE_ROWS
   if (int rc = hip_check(hipGetLastError(), "attend_tree launch")) return rc;
-#define MI_TREE_FOLD(V)                                                                                       \
-  hipLaunchKernelGGL((attend_tree_fold_kernel<V>), dim3((uint32_t)fold), dim3(256), 0, s, a, parts, plan, g.rows, g.slice)
+#define MI_TREE_FOLD(V)                                                                                            \
+  if (waves == 4)                                                                                                  \
+    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 4>), dim3((uint32_t)fold), dim3(256), 0, s, a, parts, plan, g.rows, \
+                       g.slice);                                                                                   \
+  else                                                                                                             \
+    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 1>), dim3((uint32_t)fold), dim3(256), 0, s, a, parts, plan, g.rows, \
+                       g.slice)
   if (a.head_dim % 256 == 0) MI_TREE_FOLD(4);
   else if (a.head_dim % 128 == 0) MI_TREE_FOLD(2);
   else MI_TREE_FOLD(1);

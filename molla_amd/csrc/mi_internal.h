@@ -330,7 +330,7 @@ struct TreeAttend {
   mi_tree tree;
   float* out;
 };
-size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, const mi_tree& tree);
+size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const mi_tree& tree);
 int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work);
 
 // ---- small device helpers -----------------------------------------------

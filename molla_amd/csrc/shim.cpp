@@ -506,7 +506,7 @@ size_t mi_attend_tree_workspace(int32_t heads, int32_t kv_heads, int32_t head_di
       cache_row(form, kv_heads * head_dim) < 0 || !tree || tree->batch < 1 || tree->tokens < 1 ||
       tree->tokens > kMaxTreeRows || mi_tree_words(tree->max_nodes) < 0 || tree->max_count < 1)
     return 0;
-  return tree_attend_workspace(heads, kv_heads, head_dim, *tree);
+  return tree_attend_workspace(heads, kv_heads, head_dim, form, *tree);
 }
 
 int mi_attend_tree(mi_stream stream, int32_t form, const float* q, int64_t q_stride, const uint16_t* k_cache,
