@@ -52,8 +52,10 @@ __global__ __launch_bounds__(kQkThreads) void qk_rope_kernel(QkRope a, int heads
     sn[i] = 0.0f;
     if (turn) {
       const float theta = rope_theta(p, d.rope_steps, d.rope_factors, s);
-      cs[i] = (float)cos((double)theta);
-      sn[i] = (float)sin((double)theta);
+      double sd, cd;
+      sincos((double)theta, &sd, &cd);
+      cs[i] = (float)cd;
+      sn[i] = (float)sd;
     }
     gq[i][0] = d.q_norm && live[i] ? d.q_norm[lo[i]] : 1.0f;
     gq[i][1] = d.q_norm && live[i] ? d.q_norm[hi[i]] : 1.0f;
@@ -147,18 +149,219 @@ __global__ __launch_bounds__(kQkThreads) void qk_rope_kernel(QkRope a, int heads
   }
 }
 
+// The same where a head is a multiple of 64 values up to 256 and everything lies
+// on 16 bytes: two neighbouring slots a lane, so that a lane's values are two
+// words of 8 bytes (half-split pairs) or one of 16 (adjacent pairs), and D / 4
+// lanes a head.  The loads of kAhead heads are sent for together: 4096 tokens of
+// 32 + 2 x 8 heads of 128 68 -> 41 us (184 MB).
+constexpr int kAhead = 4;
+
+struct QkRow {  // of a token, by kind of head
+  const float* src;
+  float* dst;
+  __half* cache;
+};
+
+template <int LPH, bool NEOX, bool Q8>
+__global__ __launch_bounds__(kQkThreads) void qk_rope_vec_kernel(QkRope a, int heads_all, int per, int runs) {
+#pragma clang fp contract(off)
+  constexpr int GROUPS = 64 / LPH, D = 4 * LPH;
+  const mi_qk& d = a.d;
+  const int lane = threadIdx.x & 63, l = lane % LPH, grp = lane / LPH;
+  const int64_t job = (int64_t)blockIdx.x * (kQkThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t64 = job / runs;
+  if (t64 >= d.tokens || (d.count && t64 >= *d.count)) return;
+  const int t = (int)t64, first = (int)(job - t64 * runs) * per, last = min(first + per, heads_all);
+  const int half = d.rope_dim >> 1, p = d.pos[t];
+  // slots 2 l and 2 l + 1: values lo .. and hi .. (two each, or four from lo)
+  const bool turn = 2 * l < half;
+  const int lo = !NEOX ? 4 * l : turn ? 2 * l : d.rope_dim + 2 * (2 * l - half), hi = lo + (NEOX && turn ? half : 2);
+  const int kvw = d.kv_heads * D;
+  int64_t cell = -1, base = 0;
+  if (d.k_cache) {
+    if (d.cells) cell = d.cells[t];
+    else if (a.kv_index) cell = a.kv_index[(int64_t)t * a.index_stride + p];
+    else cell = p, base = (int64_t)t * a.cache_stride;
+  }
+  const int64_t row = base + cell * cache_row(d.cache_form, kvw);
+  auto source = [&](int h) __attribute__((always_inline)) {
+    const int hk = h - d.heads, hv = hk - d.kv_heads;
+    return h < d.heads ? d.q + t * d.q_stride + (int64_t)h * D
+           : hv < 0    ? d.k + t * d.k_stride + (int64_t)hk * D
+                       : d.v + t * d.v_stride + (int64_t)hv * D;
+  };
+  float x[kAhead][4];
+  auto load = [&](int h0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const float* src = source(min(h0 + j * GROUPS + grp, last - 1));
+      if constexpr (NEOX) {
+        const float2 u = *(const float2*)(src + lo), w = *(const float2*)(src + hi);
+        x[j][0] = u.x, x[j][1] = u.y, x[j][2] = w.x, x[j][3] = w.y;
+      } else {
+        const float4 u = *(const float4*)(src + lo);
+        x[j][0] = u.x, x[j][1] = u.y, x[j][2] = u.z, x[j][3] = u.w;
+      }
+    }
+  };
+  load(first);
+  // value e of a lane: slot e % 2 (half-split) or e / 2 (adjacent) of its two, first or second of the pair
+  float cs[2] = {1.0f, 1.0f}, sn[2] = {0.0f, 0.0f}, gq[4], gk[4];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    if (turn) {
+      double sd, cd;
+      sincos((double)rope_theta(p, d.rope_steps, d.rope_factors, 2 * l + i), &sd, &cd);
+      cs[i] = (float)cd;
+      sn[i] = (float)sd;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const int at = e < 2 ? lo + e : hi + e - 2;
+    gq[e] = d.q_norm ? d.q_norm[at] : 1.0f;
+    gk[e] = d.q_norm ? d.k_norm[at] : 1.0f;
+  }
+  for (int h0 = first; h0 < last; h0 += kAhead * GROUPS) {
+    float y[kAhead][4];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[j][e] = x[j][e];
+    if (h0 + kAhead * GROUPS < last) load(h0 + kAhead * GROUPS);
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int h = h0 + j * GROUPS + grp;
+      const bool on = h < last, isq = h < d.heads, isv = h >= d.heads + d.kv_heads;
+      const int hk = isq ? 0 : isv ? h - d.heads - d.kv_heads : h - d.heads;
+      if (d.q_norm) {
+        double acc = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc += (double)y[j][e] * (double)y[j][e];
+        acc = lanes::reduce_sum<LPH>(acc);
+        const float scale = (float)(1.0 / sqrt(acc / (double)D + (double)d.eps));
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (!isv) y[j][e] = y[j][e] * scale * (isq ? gq[e] : gk[e]);
+      }
+      if (!isv && turn) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          float &u = y[j][NEOX ? i : 2 * i], &w = y[j][NEOX ? 2 + i : 2 * i + 1];
+          const float ru = u * cs[i] - w * sn[i], rw = u * sn[i] + w * cs[i];
+          u = ru;
+          w = rw;
+        }
+      }
+      float* dst = !on || isv ? nullptr
+                   : isq      ? d.q_out + t * d.q_out_stride + (int64_t)h * D
+                   : d.k_out  ? d.k_out + t * d.k_out_stride + (int64_t)hk * D
+                              : nullptr;
+      if (dst) {
+        if constexpr (NEOX) {
+          *(float2*)(dst + lo) = make_float2(y[j][0], y[j][1]);
+          *(float2*)(dst + hi) = make_float2(y[j][2], y[j][3]);
+        } else {
+          *(float4*)(dst + lo) = make_float4(y[j][0], y[j][1], y[j][2], y[j][3]);
+        }
+      }
+      if (cell < 0) continue;  // (uniform)
+      __half* rowp = (__half*)(isv ? d.v_cache : d.k_cache) + row;
+      if constexpr (Q8) {
+        // 32 values are 16 lanes' first or second two (half-split: the rotary part is the
+        // whole head), or 8 lanes' four; the rule is q8_store_block's
+        float amax[2];
+#pragma unroll
+        for (int w = 0; w < 2; w++) amax[w] = fmaxf(fabsf(y[j][2 * w]), fabsf(y[j][2 * w + 1]));
+        if constexpr (NEOX) {
+#pragma unroll
+          for (int w = 0; w < 2; w++) amax[w] = lanes::reduce<16>(amax[w], lanes::Max{});
+        } else {
+          amax[0] = amax[1] = lanes::reduce<8>(fmaxf(amax[0], amax[1]), lanes::Max{});
+        }
+        uint32_t bytes[2];
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          const float inv = amax[w] == 0.0f ? 0.0f : 127.0f / amax[w];
+          uint32_t b[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float z = y[j][2 * w + e] * inv, r = z >= 0.0f ? z + 0.5f : z - 0.5f;
+            b[e] = (uint32_t)max(-127, min(127, (int)r)) & 0xffu;
+          }
+          bytes[w] = b[0] | (b[1] << 8);
+        }
+        if (on && !isq) {
+          uint8_t* q8 = (uint8_t*)rowp + hk * D;
+          if constexpr (NEOX) {
+            *(uint16_t*)(q8 + lo) = (uint16_t)bytes[0];
+            *(uint16_t*)(q8 + hi) = (uint16_t)bytes[1];
+            if ((l & 15) == 0) {
+              rowp[(kvw >> 1) + ((hk * D + lo) >> 5)] = __float2half_rn(amax[0] / 127.0f);
+              rowp[(kvw >> 1) + ((hk * D + hi) >> 5)] = __float2half_rn(amax[1] / 127.0f);
+            }
+          } else {
+            *(uint32_t*)(q8 + lo) = bytes[0] | (bytes[1] << 16);
+            if ((l & 7) == 0) rowp[(kvw >> 1) + ((hk * D + lo) >> 5)] = __float2half_rn(amax[0] / 127.0f);
+          }
+        }
+      } else if (on && !isq) {
+        const __half2 u = __floats2half2_rn(y[j][0], y[j][1]), w = __floats2half2_rn(y[j][2], y[j][3]);
+        if constexpr (NEOX) {
+          *(__half2*)(rowp + hk * D + lo) = u;
+          *(__half2*)(rowp + hk * D + hi) = w;
+        } else {
+          __half2 both[2] = {u, w};
+          *(uint2*)(rowp + hk * D + lo) = *(uint2*)both;
+        }
+      }
+    }
+  }
+}
+
 }  // namespace
+
+// Whether the vector kernel takes the shape: its words may not straddle a pair's
+// halves, the rotary part's end or an 8-bit block, and every row starts on 16 bytes.
+static bool qk_vec_fits(const mi_qk& d) {
+  if (d.head_dim != 64 && d.head_dim != 128 && d.head_dim != 256) return false;
+  if (d.rope_dim % 4) return false;
+  if (d.k_cache && d.cache_form == MI_CACHE_Q8 && d.neox && (d.rope_dim != d.head_dim)) return false;
+  const uintptr_t p = (uintptr_t)d.q | (uintptr_t)d.k | (uintptr_t)d.v | (uintptr_t)d.q_out | (uintptr_t)d.k_out;
+  const int64_t st = d.q_stride | d.k_stride | (d.v ? d.v_stride : 0) | d.q_out_stride | (d.k_out ? d.k_out_stride : 0);
+  return !(p & 15) && !(st & 3);
+}
 
 int launch_qk_rope(hipStream_t s, const QkRope& a) {
   const mi_qk& d = a.d;
   const int heads_all = d.heads + d.kv_heads * (d.k_cache ? 2 : 1);
+  const bool q8 = d.k_cache && d.cache_form == MI_CACHE_Q8, vec = qk_vec_fits(d);
   // runs of heads: enough waves for the chip, as few as keep a token's angles together
-  const int64_t waves = (int64_t)cu_count() * 8;
-  const int per = (int)std::max<int64_t>(2, std::min<int64_t>(heads_all, (heads_all * (int64_t)d.tokens + waves - 1) / waves));
+  const int64_t waves = (int64_t)cu_count() * 16;
+  const int least = vec ? 256 / d.head_dim : 2;
+  const int per = (int)std::max<int64_t>(least, std::min<int64_t>(heads_all, (heads_all * (int64_t)d.tokens + waves - 1) / waves));
   const int runs = (heads_all + per - 1) / per;
   const int64_t blocks = ((int64_t)runs * d.tokens + 3) / 4;
   if (blocks > 0x7fffffff) return fail(MI_ERR_SHAPE, "qk_norm_rope: %d tokens of %d heads", d.tokens, heads_all);
-  const bool q8 = d.k_cache && d.cache_form == MI_CACHE_Q8;
+  if (vec) {
+#define MI_QKV(LPH, N, Q)                                                                                             \
+  hipLaunchKernelGGL((qk_rope_vec_kernel<LPH, N, Q>), dim3((uint32_t)blocks), dim3(kQkThreads), 0, s, a, heads_all, \
+                     per, runs)
+#define MI_QKV_F(LPH)                      \
+  if (d.neox) {                            \
+    if (q8) MI_QKV(LPH, true, true);       \
+    else MI_QKV(LPH, true, false);         \
+  } else {                                 \
+    if (q8) MI_QKV(LPH, false, true);      \
+    else MI_QKV(LPH, false, false);        \
+  }
+    if (d.head_dim == 64) { MI_QKV_F(16) }
+    else if (d.head_dim == 128) { MI_QKV_F(32) }
+    else { MI_QKV_F(64) }
+#undef MI_QKV_F
+#undef MI_QKV
+    return hip_check(hipGetLastError(), "qk_norm_rope launch");
+  }
 #define MI_QK(LPH, NS)                                                                                              \
   if (q8)                                                                                                           \
     hipLaunchKernelGGL((qk_rope_kernel<LPH, NS, true>), dim3((uint32_t)blocks), dim3(kQkThreads),                   \

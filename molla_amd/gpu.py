@@ -88,6 +88,7 @@ class DeviceContext:
         if not torch.cuda.is_available():
             raise RuntimeError("no GPU: the molla_amd kernels run only on a ROCm device")
         self.device = torch.device("cuda", device)
+        self.index = self.device.index
         self.stream = stream if stream is not None else torch.cuda.current_stream(self.device)
         self._work = None
         self._captured = []  # workspaces that a captured graph replays on
@@ -273,16 +274,18 @@ def device_embed(ctx: DeviceContext, embedding: torch.Tensor, ids: torch.Tensor,
 # ---- a step over trees of drafted tokens (no counterpart in the reference) ----
 def _queue(ctx: DeviceContext, fn, *args) -> None:
     """A library call on the context's stream, with its device current."""
-    if torch.cuda.current_device() == ctx.device.index:
-        check(fn(ctx.handle, *args))
+    if torch.cuda.current_device() == ctx.index:
+        rc = fn(ctx.stream.cuda_stream, *args)
     else:
-        with torch.cuda.device(ctx.device):
-            check(fn(ctx.handle, *args))
+        with torch.cuda.device(ctx.index):
+            rc = fn(ctx.stream.cuda_stream, *args)
+    if rc:
+        check(rc)
 
 
 def _on(ctx: DeviceContext, t: torch.Tensor, name: str, dtype: torch.dtype, numel: int = 0) -> int:
     """The address of a contiguous tensor of the context's device, at least `numel` long."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != ctx.device or not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != ctx.index or not t.is_contiguous():
         raise ValueError(f"{name} has to be a contiguous {dtype} tensor on {ctx.device}")
     if t.numel() < numel:
         raise ValueError(f"{name} has {t.numel()} values where {numel} are needed")
@@ -291,10 +294,13 @@ def _on(ctx: DeviceContext, t: torch.Tensor, name: str, dtype: torch.dtype, nume
 
 def _rows(ctx: DeviceContext, t: torch.Tensor, name: str, tokens: int, width: int) -> int:
     """The row stride of a float32 tensor of at least `tokens` rows of `width` values, each row contiguous."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != ctx.device or t.dim() != 2 or \
-            t.shape[0] < tokens or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} has to be float32 rows on {ctx.device}, at least {tokens} x {width}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    if t.dtype is not torch.float32 or t.get_device() != ctx.index or t.dim() != 2:
+        raise ValueError(f"{name} has to be float32 rows on {ctx.device}")
+    rows, cols = t.shape
+    stride, step = t.stride()
+    if rows < tokens or cols < width or (step != 1 and cols > 1):
+        raise ValueError(f"{name} has to be at least {tokens} x {width}, its rows contiguous")
+    return stride if rows > 1 or stride > width else width
 
 
 def device_page_plan(ctx: DeviceContext, page: int, lengths: torch.Tensor, news: torch.Tensor, table: torch.Tensor,
@@ -358,29 +364,17 @@ def device_qk_norm_rope(ctx: DeviceContext, q: torch.Tensor, k: torch.Tensor, v:
     f32, i32 = torch.float32, torch.int32
     tokens = pos.numel()
     qw, kvw = heads * head_dim, kv_heads * head_dim
-    d = MiQk(heads, kv_heads, head_dim, dim, int(neox), form, tokens, eps)
-    d.q, d.q_stride = q.data_ptr(), _rows(ctx, q, "q", tokens, qw)
-    d.k, d.k_stride = k.data_ptr(), _rows(ctx, k, "k", tokens, kvw)
-    d.q_out, d.q_out_stride = q_out.data_ptr(), _rows(ctx, q_out, "q_out", tokens, qw)
-    if k_out is not None:
-        d.k_out, d.k_out_stride = k_out.data_ptr(), _rows(ctx, k_out, "k_out", tokens, kvw)
-    if v is not None:
-        d.v, d.v_stride = v.data_ptr(), _rows(ctx, v, "v", tokens, kvw)
-    if k_cache is not None:
-        d.k_cache = _on(ctx, k_cache, "k_cache", torch.float16)
-    if v_cache is not None:
-        d.v_cache = _on(ctx, v_cache, "v_cache", torch.float16)
-    if cells is not None:
-        d.cells = _on(ctx, cells, "cells", i32, tokens)
-    if q_norm is not None:
-        d.q_norm = _on(ctx, q_norm, "q_norm", f32, head_dim)
-    if k_norm is not None:
-        d.k_norm = _on(ctx, k_norm, "k_norm", f32, head_dim)
-    if factors is not None:
-        d.rope_factors = _on(ctx, factors, "factors", f32, dim // 2)
-    if count is not None:
-        d.count = _on(ctx, count, "count", i32, 1)
-    d.rope_steps, d.pos = _on(ctx, steps, "steps", f32, dim // 2), _on(ctx, pos, "pos", i32)
+    def at(t, name, dtype, n=0):
+        return None if t is None else _on(ctx, t, name, dtype, n)
+
+    d = MiQk(heads, kv_heads, head_dim, dim, int(neox), form, tokens, eps, q.data_ptr(), k.data_ptr(),
+             None if v is None else v.data_ptr(), _rows(ctx, q, "q", tokens, qw), _rows(ctx, k, "k", tokens, kvw),
+             0 if v is None else _rows(ctx, v, "v", tokens, kvw), q_out.data_ptr(),
+             None if k_out is None else k_out.data_ptr(), _rows(ctx, q_out, "q_out", tokens, qw),
+             0 if k_out is None else _rows(ctx, k_out, "k_out", tokens, kvw), at(q_norm, "q_norm", f32, head_dim),
+             at(k_norm, "k_norm", f32, head_dim), _on(ctx, steps, "steps", f32, dim // 2),
+             at(factors, "factors", f32, dim // 2), _on(ctx, pos, "pos", i32), at(count, "count", i32, 1),
+             at(k_cache, "k_cache", torch.float16), at(v_cache, "v_cache", torch.float16), at(cells, "cells", i32, tokens))
     _queue(ctx, lib().mi_qk_norm_rope, ctypes.byref(d))
 
 

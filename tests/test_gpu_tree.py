@@ -221,10 +221,10 @@ def q8_values(rows, kvw):
 
 
 def check_qk(tokens, heads, kv, d, dim, neox, norm, with_factors, form, store=True, in_place=False, live=None, scale=1.0,
-             positions=None):
+             positions=None, pad=3):
     rng = np.random.default_rng(tokens * 7 + d)
     qw, kvw = heads * d, kv * d
-    row = (scale * rng.standard_normal((tokens, qw + 2 * kvw + 3))).astype(np.float32)
+    row = (scale * rng.standard_normal((tokens, qw + 2 * kvw + pad))).astype(np.float32)
     steps = gpu.rope_steps(dim, 10000.0)
     gains = [(1 + 0.1 * rng.standard_normal(d)).astype(np.float32) for _ in range(2)] if norm else [None, None]
     factors = np.exp(rng.standard_normal(dim // 2)).astype(np.float32) if with_factors else None
@@ -279,6 +279,17 @@ def check_qk(tokens, heads, kv, d, dim, neox, norm, with_factors, form, store=Tr
                                             (4, 4, 64, 2), (8, 4, 256, 256), (2, 1, 512, 256)])
 def test_qk_heads(form, neox, heads, kv, d, dim):
     check_qk(5, heads, kv, d, dim, neox, True, neox, form)
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("neox", [False, True])
+@pytest.mark.parametrize("heads,kv,d,dim", [(4, 2, 64, 64), (8, 1, 128, 128), (4, 4, 64, 20), (8, 4, 256, 256), (3, 3, 128, 92),
+                                            (1, 1, 128, 64), (16, 8, 64, 32), (2, 2, 256, 4)])
+def test_qk_aligned_rows(form, neox, heads, kv, d, dim):
+    """Rows on 16 bytes (the words of two and four values); head counts that leave a run short."""
+    check_qk(5, heads, kv, d, dim, neox, True, neox, form, pad=4)
+    check_qk(70, heads, kv, d, dim, neox, False, not neox, form, pad=0)
+    check_qk(9, heads, kv, d, dim, neox, True, False, form, pad=4, in_place=True, live=6)
 
 
 @pytest.mark.parametrize("tokens", [1, 2, 63, 300])
