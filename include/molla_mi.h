@@ -429,6 +429,19 @@ int mi_attend_tree(mi_stream stream, int32_t form, const float* q, int64_t q_str
                    int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, const mi_tree* tree, float* out,
                    void* work, size_t work_bytes);
 
+/* mi_decoder_layer over a step's trees, in place on the rows of resid: the same
+ * layer with mi_qk_norm_rope at tree->pos and tree->cells and mi_attend_tree for
+ * its rotation, store and attention, over caches of either layout (kv_index as
+ * there).  cells[t] is the row of the caches that slot lengths[b] + i of its
+ * sequence is (kv_index's cell, or b * cache_stride / mi_cache_row + slot).  Rows
+ * behind the last sequence come out undefined; nothing of them reaches another
+ * row or the caches.  Workspace: mi_layer_tree_workspace, 256-byte aligned;
+ * tree->tokens is at most 65536. */
+size_t mi_layer_tree_workspace(const mi_layer_desc* desc, const mi_tree* tree);
+int mi_decoder_layer_tree(mi_stream stream, const mi_layer_desc* desc, float* resid, uint16_t* k_cache,
+                          uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
+                          const mi_tree* tree, void* work, size_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

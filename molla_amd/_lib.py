@@ -84,6 +84,9 @@ SIGNATURES = {
     "mi_attend_tree_workspace": (SZ, [I32, I32, I32, I32, ctypes.POINTER(MiTree)]),
     "mi_attend_tree": (ctypes.c_int, [P, I32, P, I64, P, P, I64, P, I64, I32, I32, I32, F, ctypes.POINTER(MiTree), P, P,
                                       SZ]),
+    "mi_layer_tree_workspace": (SZ, [ctypes.POINTER(MiLayerDesc), ctypes.POINTER(MiTree)]),
+    "mi_decoder_layer_tree": (ctypes.c_int, [P, ctypes.POINTER(MiLayerDesc), P, P, P, I64, P, I64,
+                                             ctypes.POINTER(MiTree), P, SZ]),
 }
 
 _lib = None

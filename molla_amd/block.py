@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import gpu
-from ._lib import MiLayerDesc, check, lib
+from ._lib import MiLayerDesc, MiTree, check, lib
 
 
 @dataclass
@@ -144,6 +144,38 @@ def device_layer_paged(ctx: gpu.DeviceContext, layer: DeviceLayer, x: torch.Tens
     check(lib().mi_decoder_layer_paged(ctx.handle, ctypes.byref(desc), x.data_ptr(), k_pool.data_ptr(),
                                        v_pool.data_ptr(), kv_index.data_ptr(), index_stride, pos.data_ptr(),
                                        max_count, tokens, work.data_ptr(), work.numel()))
+
+
+def layer_tree_workspace(layer: DeviceLayer, tree: MiTree, form: int = gpu.CACHE_F16) -> int:
+    return lib().mi_layer_tree_workspace(ctypes.byref(with_cache_form(layer.desc, form)), ctypes.byref(tree))
+
+
+def device_layer_tree(ctx: gpu.DeviceContext, layer: DeviceLayer, x: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, mask: torch.Tensor,
+                      pos: torch.Tensor, cells: torch.Tensor, max_nodes: int, max_count: int, cache_stride: int = 0,
+                      kv_index: torch.Tensor | None = None, work: torch.Tensor | None = None,
+                      form: int = gpu.CACHE_F16) -> None:
+    """device_layer over a step's trees of drafted tokens, in place on x
+    ([tokens, width] f32; mi_decoder_layer_tree): token t of sequence b at
+    rotary position pos[t], stored at cache row cells[t], sees the sequence's
+    lengths[b] committed positions and the nodes in its mask (gpu.device_page_plan
+    and gpu.device_tree_plan make the five lists).  Sequence b's slots are rows of
+    its own cache, cache_stride halves after the one before, or the cells
+    kv_index[b].  Rows behind the last sequence come out undefined."""
+    i32, f16, s = torch.int32, torch.float16, layer.spec
+    batch, tokens = lengths.numel(), pos.numel()
+    stride, least = gpu.tree_cache(kv_index, batch, cache_stride, max_count, gpu.cache_row(form, s.kv_width()))
+    on = gpu._on
+    tree = MiTree(batch, tokens, max_nodes, max_count, on(ctx, starts, "starts", i32, batch + 1),
+                  on(ctx, lengths, "lengths", i32), on(ctx, mask, "mask", i32, tokens * gpu.tree_words(max_nodes)),
+                  on(ctx, pos, "pos", i32), on(ctx, cells, "cells", i32, tokens))
+    if work is None:
+        work = ctx.workspace(layer_tree_workspace(layer, tree, form))
+    desc = layer.desc if form == gpu.CACHE_F16 else with_cache_form(layer.desc, form)
+    gpu._queue(ctx, lib().mi_decoder_layer_tree, ctypes.byref(desc), on(ctx, x, "x", torch.float32, tokens * s.width),
+               on(ctx, k_cache, "k_cache", f16, least), on(ctx, v_cache, "v_cache", f16, least), cache_stride,
+               None if kv_index is None else on(ctx, kv_index, "kv_index", i32), stride, ctypes.byref(tree),
+               work.data_ptr(), work.numel())
 
 
 class DeviceModel:

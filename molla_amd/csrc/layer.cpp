@@ -16,7 +16,8 @@
 //   qkv    (q_width + 2 * kv_width) * tokens floats
 //   up     hidden * tokens floats
 //   gate   hidden * tokens floats
-//   attn   attention slices (attend_workspace)
+//   attn   attention slices (attend_workspace); over trees their attention's
+//          workspace and its output in f32
 //   trig   rope (cos, sin) of this position
 //   xq2    4 * hidden * tokens: the down projection's input, when the gate/up
 //          launch writes it (it cannot share xq, which that launch reads)
@@ -30,6 +31,10 @@
 
 namespace mi {
 int check_weight(const char* name, int kind, const void* w, int64_t row_bytes, int32_t rows, int32_t cols);
+int check_tree(const char* name, const mi_tree* t, bool layer);
+int check_tree_caches(const char* name, int32_t form, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                      const uint16_t* k_cache, const uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index,
+                      int64_t index_stride, const mi_tree* tree);
 }
 
 using namespace mi;
@@ -38,11 +43,19 @@ namespace {
 
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
+// The attention's part of a workspace: over trees (with `tree`) theirs.
+size_t tree_part(const mi_layer_desc* d, const mi_tree* tree) {
+  return up256(mi_attend_tree_workspace(d->heads, d->kv_heads, d->head_dim, d->cache_form, tree));
+}
+size_t attend_part(const mi_layer_desc* d, int32_t max_count, int32_t tokens, const mi_tree* tree) {
+  return tree ? tree_part(d, tree) : up256(attend_workspace(d->heads, d->head_dim, max_count, tokens));
+}
+
 struct Carve {
   size_t xq, qkv, up, gate, attn, trig, xq2, part, total;
 };
 
-Carve carve(const mi_layer_desc* d, int32_t max_count, int32_t tokens) {
+Carve carve(const mi_layer_desc* d, int32_t max_count, int32_t tokens, const mi_tree* tree = nullptr) {
   const int64_t qw = (int64_t)d->heads * d->head_dim, kvw = (int64_t)d->kv_heads * d->head_dim;
   const int64_t widest = std::max<int64_t>({d->width, qw, d->hidden});
   Carve c;
@@ -56,7 +69,7 @@ Carve carve(const mi_layer_desc* d, int32_t max_count, int32_t tokens) {
   c.gate = at;
   at += up256(sizeof(float) * (size_t)d->hidden * tokens);
   c.attn = at;
-  at += up256(attend_workspace(d->heads, d->head_dim, max_count, tokens));
+  at += attend_part(d, max_count, tokens, tree) + (tree ? up256(sizeof(float) * (size_t)qw * tokens) : 0);
   c.trig = at;
   at += up256(sizeof(float) * (size_t)d->rope_dim);
   c.xq2 = at;  // down's input; at 2..8 tokens followed by its hx form
@@ -75,7 +88,7 @@ struct PrefillCarve {
   size_t xn, qkv, attn_out, up, h, attn, mm, total;
 };
 
-PrefillCarve prefill_carve(const mi_layer_desc* d, int32_t max_count, int32_t tokens) {
+PrefillCarve prefill_carve(const mi_layer_desc* d, int32_t max_count, int32_t tokens, const mi_tree* tree = nullptr) {
   const int64_t qw = (int64_t)d->heads * d->head_dim, kvw = (int64_t)d->kv_heads * d->head_dim;
   PrefillCarve c;
   size_t at = 0;
@@ -90,7 +103,7 @@ PrefillCarve prefill_carve(const mi_layer_desc* d, int32_t max_count, int32_t to
   c.h = at;
   at += up256(sizeof(float) * (size_t)d->hidden * tokens);
   c.attn = at;
-  at += up256(attend_workspace(d->heads, d->head_dim, max_count, tokens));
+  at += attend_part(d, max_count, tokens, tree);
   c.mm = at;
   size_t mm = 0;
   const int32_t shapes[5][2] = {{(int32_t)(qw + 2 * kvw), d->width}, {(int32_t)qw, d->width},
@@ -153,6 +166,64 @@ bool extended(const mi_layer_desc* d) {
   return d->q_bias || d->q_norm || d->attn_post_norm || d->ffn_post_norm || d->ungated || d->act;
 }
 
+// Where a layer's keys and values are: the caches and, over trees of drafted
+// tokens, the trees (null: a token a sequence, or a sequence's chunk).
+struct LayerCache {
+  uint16_t *k, *v;
+  int64_t stride;
+  const int32_t* kv_index;
+  int64_t index_stride;
+  const mi_tree* tree;
+};
+
+// The q/k norms, the rotation and the cache store of a layer's q|k|v rows over
+// trees, where a node's position is not its slot, then their attention into out
+// (rows of heads * head_dim floats).
+int tree_attention(hipStream_t s, const mi_layer_desc* d, float* qkv, const LayerCache& c, float* out, void* work) {
+  const mi_tree& t = *c.tree;
+  const int64_t qw = (int64_t)d->heads * d->head_dim, kvw = (int64_t)d->kv_heads * d->head_dim;
+  QkRope r{};
+  r.d.heads = d->heads;
+  r.d.kv_heads = d->kv_heads;
+  r.d.head_dim = d->head_dim;
+  r.d.rope_dim = d->rope_dim;
+  r.d.neox = d->neox != 0;
+  r.d.cache_form = d->cache_form;
+  r.d.tokens = t.tokens;
+  r.d.eps = d->eps;
+  r.d.q = r.d.q_out = qkv;
+  r.d.k = qkv + qw;
+  r.d.v = qkv + qw + kvw;
+  r.d.q_stride = r.d.k_stride = r.d.v_stride = r.d.q_out_stride = qw + 2 * kvw;
+  r.d.q_norm = d->q_norm;
+  r.d.k_norm = d->k_norm;
+  r.d.rope_steps = d->rope_steps;
+  r.d.rope_factors = d->rope_factors;
+  r.d.pos = t.pos;
+  r.d.count = t.starts + t.batch;
+  r.d.k_cache = c.k;
+  r.d.v_cache = c.v;
+  r.d.cells = t.cells;
+  const int rc = launch_qk_rope(s, r);
+  if (rc) return rc;
+  TreeAttend a{};
+  a.q = qkv;
+  a.q_stride = qw + 2 * kvw;
+  a.k_cache = c.k;
+  a.v_cache = c.v;
+  a.cache_stride = t.batch > 1 ? c.stride : 0;
+  a.index_stride = c.index_stride;
+  a.kv_index = c.kv_index;
+  a.heads = d->heads;
+  a.kv_heads = d->kv_heads;
+  a.head_dim = d->head_dim;
+  a.form = d->cache_form;
+  a.scale = d->attn_scale;
+  a.tree = t;
+  a.out = out;
+  return launch_tree_attend(s, a, work);
+}
+
 }  // namespace
 
 // The layer with the optional parts of other families at 1..8 tokens, as
@@ -162,8 +233,7 @@ bool extended(const mi_layer_desc* d) {
 // epilogue), norm, up and gate (GLU epilogue, silu or gelu) or up and the
 // activation, down (likewise).  Each part is its own launch; the fused
 // Llama kernels stay for the Llama layer.
-static int extended_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint16_t* k_cache,
-                          uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
+static int extended_layer(hipStream_t s, const mi_layer_desc* d, float* resid, const LayerCache& kv,
                           const int32_t* pos, int32_t max_count, int32_t tokens, char* base, const Carve& c,
                           bool pre) {
   void* xq = base + c.xq;
@@ -187,19 +257,25 @@ static int extended_layer(hipStream_t s, const mi_layer_desc* d, float* resid, u
   if ((rc = launch_matvec(s, d->wv.kind, d->wv.data, d->wv.row_bytes, kvw, d->width, xq, tokens, qkv + qw + kvw,
                           qkv_stride, bias, d->v_bias)))
     return rc;
-  if (d->q_norm) {
-    if ((rc = launch_head_norm(s, qkv, d->heads, d->head_dim, tokens, qkv_stride, d->q_norm, d->eps))) return rc;
-    if ((rc = launch_head_norm(s, qkv + qw, d->kv_heads, d->head_dim, tokens, qkv_stride, d->k_norm, d->eps)))
+  if (kv.tree) {
+    float* out = (float*)((char*)attn + tree_part(d, kv.tree));
+    if ((rc = tree_attention(s, d, qkv, kv, out, attn))) return rc;
+    if ((rc = launch_quantize(s, out, qw, tokens, xq))) return rc;
+  } else {
+    if (d->q_norm) {
+      if ((rc = launch_head_norm(s, qkv, d->heads, d->head_dim, tokens, qkv_stride, d->q_norm, d->eps))) return rc;
+      if ((rc = launch_head_norm(s, qkv + qw, d->kv_heads, d->head_dim, tokens, qkv_stride, d->k_norm, d->eps)))
+        return rc;
+    }
+    if ((rc = launch_rope_store(s, qkv, d->heads, d->kv_heads, d->head_dim, d->rope_dim, d->neox, d->rope_steps, pos,
+                                tokens, qkv_stride, kv.k, kv.v, kv.stride, d->rope_factors, d->cache_form,
+                                kv.kv_index, kv.index_stride)))
+      return rc;
+    if ((rc = launch_attend(s, qkv, qkv_stride, kv.k, kv.v, kv.stride, d->heads, d->kv_heads, d->head_dim,
+                            d->attn_scale, pos, -1, max_count, tokens, nullptr, xq, attn, d->cache_form, kv.kv_index,
+                            kv.index_stride)))
       return rc;
   }
-  if ((rc = launch_rope_store(s, qkv, d->heads, d->kv_heads, d->head_dim, d->rope_dim, d->neox, d->rope_steps, pos,
-                              tokens, qkv_stride, k_cache, v_cache, cache_stride, d->rope_factors, d->cache_form,
-                              kv_index, index_stride)))
-    return rc;
-  if ((rc = launch_attend(s, qkv, qkv_stride, k_cache, v_cache, cache_stride, d->heads, d->kv_heads, d->head_dim,
-                          d->attn_scale, pos, -1, max_count, tokens, nullptr, xq, attn, d->cache_form, kv_index,
-                          index_stride)))
-    return rc;
   if (d->attn_post_norm) {
     // wo into a scratch row (the up buffer is free until the MLP), normed into the stream
     if ((rc = launch_matvec(s, d->wo.kind, d->wo.data, d->wo.row_bytes, d->width, qw, xq, tokens, up, d->width,
@@ -242,10 +318,9 @@ static int extended_layer(hipStream_t s, const mi_layer_desc* d, float* resid, u
 // rows, rope and the cache store per token, attention per token over the
 // positions up to its own (the chunk's earlier tokens included).  The gate
 // projection's GLU epilogue reads the up projection's output.
-static int prefill_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint16_t* k_cache, uint16_t* v_cache,
-                         int64_t cache_stride, const int32_t* kv_index, int64_t index_stride, const int32_t* pos,
-                         int32_t max_count, int32_t tokens, void* work, size_t work_bytes) {
-  const PrefillCarve c = prefill_carve(d, max_count, tokens);
+static int prefill_layer(hipStream_t s, const mi_layer_desc* d, float* resid, const LayerCache& kv,
+                         const int32_t* pos, int32_t max_count, int32_t tokens, void* work, size_t work_bytes) {
+  const PrefillCarve c = prefill_carve(d, max_count, tokens, kv.tree);
   if (work_bytes < c.total)
     return fail(MI_ERR_WORKSPACE, "layer: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, c.total);
   char* base = (char*)work;
@@ -300,19 +375,23 @@ static int prefill_layer(hipStream_t s, const mi_layer_desc* d, float* resid, ui
     if ((rc = mat(d->wk, kvw, d->width, xn, qkv + qw, qkv_stride, MI_EPI_NONE, nullptr))) return rc;
     if ((rc = mat(d->wv, kvw, d->width, xn, qkv + qw + kvw, qkv_stride, MI_EPI_NONE, nullptr))) return rc;
   }
-  if (d->q_norm) {  // each head of q and k normed before rope (block.mojo:367-384)
-    if ((rc = launch_head_norm(s, qkv, d->heads, d->head_dim, tokens, qkv_stride, d->q_norm, d->eps))) return rc;
-    if ((rc = launch_head_norm(s, qkv + qw, d->kv_heads, d->head_dim, tokens, qkv_stride, d->k_norm, d->eps)))
+  if (kv.tree) {
+    if ((rc = tree_attention(s, d, qkv, kv, attn_out, attn))) return rc;
+  } else {
+    if (d->q_norm) {  // each head of q and k normed before rope (block.mojo:367-384)
+      if ((rc = launch_head_norm(s, qkv, d->heads, d->head_dim, tokens, qkv_stride, d->q_norm, d->eps))) return rc;
+      if ((rc = launch_head_norm(s, qkv + qw, d->kv_heads, d->head_dim, tokens, qkv_stride, d->k_norm, d->eps)))
+        return rc;
+    }
+    if ((rc = launch_rope_store(s, qkv, d->heads, d->kv_heads, d->head_dim, d->rope_dim, d->neox, d->rope_steps, pos,
+                                tokens, qkv_stride, kv.k, kv.v, kv.stride, d->rope_factors, d->cache_form,
+                                kv.kv_index, kv.index_stride)))
+      return rc;
+    if ((rc = launch_attend(s, qkv, qkv_stride, kv.k, kv.v, kv.stride, d->heads, d->kv_heads, d->head_dim,
+                            d->attn_scale, pos, -1, max_count, tokens, attn_out, nullptr, attn, d->cache_form,
+                            kv.kv_index, kv.index_stride)))
       return rc;
   }
-  if ((rc = launch_rope_store(s, qkv, d->heads, d->kv_heads, d->head_dim, d->rope_dim, d->neox, d->rope_steps, pos,
-                              tokens, qkv_stride, k_cache, v_cache, cache_stride, d->rope_factors, d->cache_form,
-                              kv_index, index_stride)))
-    return rc;
-  if ((rc = launch_attend(s, qkv, qkv_stride, k_cache, v_cache, cache_stride, d->heads, d->kv_heads, d->head_dim,
-                          d->attn_scale, pos, -1, max_count, tokens, attn_out, nullptr, attn, d->cache_form,
-                          kv_index, index_stride)))
-    return rc;
   if (d->attn_post_norm) {  // wo into xn (free once q, k, v are made), normed into the stream
     if ((rc = mat(d->wo, d->width, qw, attn_out, xn, d->width, MI_EPI_NONE, nullptr))) return rc;
     if ((rc = launch_norm_add(s, resid, xn, d->width, tokens, d->attn_post_norm, d->eps))) return rc;
@@ -401,9 +480,30 @@ static int down_batch(hipStream_t s, const mi_layer_desc* d, const void* xq2, in
                        d->width, MI_EPI_ADD, nullptr);
 }
 
-static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint16_t* k_cache, uint16_t* v_cache,
-                       int64_t cache_stride, const int32_t* kv_index, int64_t index_stride, const int32_t* pos,
+static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, const LayerCache& kv, const int32_t* pos,
                        int32_t max_count, int32_t tokens, char* base, const Carve& c, bool pre, NextNorm* nn);
+
+static int run_layer(hipStream_t s, const mi_layer_desc* d, float* resid, const LayerCache& kv, const int32_t* pos,
+                     int32_t max_count, int32_t tokens, void* work, size_t work_bytes) {
+  if (tokens > kMaxTokens) {
+    if (!work || ((uintptr_t)work & 255)) return fail(MI_ERR_ALIGN, "layer: workspace must be 256-byte aligned");
+    return prefill_layer(s, d, resid, kv, pos, max_count, tokens, work, work_bytes);
+  }
+  const Carve c = carve(d, max_count, tokens, kv.tree);
+  if (!work || ((uintptr_t)work & 255) || work_bytes < c.total)
+    return fail(MI_ERR_WORKSPACE, "layer: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, c.total);
+
+  char* base = (char*)work;
+  // 2..8 tokens: the input's norm may already be in the workspace, and the
+  // next layer's may be asked for (mi_layer_desc next_norm / prenormed)
+  const bool pre = tokens > 1 && d->prenormed;
+  NextNorm nn{tokens > 1 ? d->next_norm : nullptr, false};
+  const int rc = extended(d) ? extended_layer(s, d, resid, kv, pos, max_count, tokens, base, c, pre)
+                             : llama_layer(s, d, resid, kv, pos, max_count, tokens, base, c, pre, &nn);
+  if (rc || !nn.gain || nn.done) return rc;
+  return launch_rms_norm(s, resid, nn.gain, d->width, tokens, d->eps, nullptr, base + c.xq,
+                         (uint8_t*)(base + c.xq) + (size_t)xq_token_bytes(d->width) * tokens);
+}
 
 static int decoder_layer(mi_stream stream, const mi_layer_desc* d, float* resid, uint16_t* k_cache,
                          uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
@@ -426,34 +526,13 @@ static int decoder_layer(mi_stream stream, const mi_layer_desc* d, float* resid,
   if (kv_index && tokens > 1 && index_stride != 0 && index_stride < max_count)
     return fail(MI_ERR_SHAPE, "layer: index stride %lld holds fewer than %d positions", (long long)index_stride,
                 max_count);
-  if (tokens > kMaxTokens) {
-    if (!work || ((uintptr_t)work & 255)) return fail(MI_ERR_ALIGN, "layer: workspace must be 256-byte aligned");
-    return prefill_layer((hipStream_t)stream, d, resid, k_cache, v_cache, cache_stride, kv_index, index_stride, pos,
-                         max_count, tokens, work, work_bytes);
-  }
-  const Carve c = carve(d, max_count, tokens);
-  if (!work || ((uintptr_t)work & 255) || work_bytes < c.total)
-    return fail(MI_ERR_WORKSPACE, "layer: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, c.total);
-
-  hipStream_t s = (hipStream_t)stream;
-  char* base = (char*)work;
-  // 2..8 tokens: the input's norm may already be in the workspace, and the
-  // next layer's may be asked for (mi_layer_desc next_norm / prenormed)
-  const bool pre = tokens > 1 && d->prenormed;
-  NextNorm nn{tokens > 1 ? d->next_norm : nullptr, false};
-  rc = extended(d) ? extended_layer(s, d, resid, k_cache, v_cache, cache_stride, kv_index, index_stride, pos,
-                                    max_count, tokens, base, c, pre)
-                   : llama_layer(s, d, resid, k_cache, v_cache, cache_stride, kv_index, index_stride, pos, max_count,
-                                 tokens, base, c, pre, &nn);
-  if (rc || !nn.gain || nn.done) return rc;
-  return launch_rms_norm(s, resid, nn.gain, d->width, tokens, d->eps, nullptr, base + c.xq,
-                         (uint8_t*)(base + c.xq) + (size_t)xq_token_bytes(d->width) * tokens);
+  const LayerCache kv{k_cache, v_cache, cache_stride, kv_index, index_stride, nullptr};
+  return run_layer((hipStream_t)stream, d, resid, kv, pos, max_count, tokens, work, work_bytes);
 }
 
 // The Llama layer at 1..8 tokens on the fused kernels (pre: the attention
 // norm's xq and hx forms are in the workspace already, 2..8 tokens).
-static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint16_t* k_cache, uint16_t* v_cache,
-                       int64_t cache_stride, const int32_t* kv_index, int64_t index_stride, const int32_t* pos,
+static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, const LayerCache& kv, const int32_t* pos,
                        int32_t max_count, int32_t tokens, char* base, const Carve& c, bool pre, NextNorm* nn) {
   int rc;
   const int64_t kvw = (int64_t)d->kv_heads * d->head_dim;
@@ -484,10 +563,12 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
     sg.nseg = 3;
   }
   const bool q8 = d->cache_form == MI_CACHE_Q8;
+  // the epilogues that rotate take a position for its slot and adjacent pairs
+  const bool epi_rope = !d->neox && !kv.tree;
   // a q8_0 cache takes the folded-norm kernel's q8 form (32-value blocks)
   const bool q8_fold = q8 && qw % 32 == 0 && kvw % 32 == 0 &&
                        q4k_qkv_norm_fits(d->width, d->head_dim, d->rope_dim, resid, d->attn_norm);
-  if (fused_qkv && !d->neox && (!q8 || q8_fold) && q4k_qkv_rope_fits(d->width, d->head_dim, d->rope_dim)) {
+  if (fused_qkv && epi_rope && (!q8 || q8_fold) && q4k_qkv_rope_fits(d->width, d->head_dim, d->rope_dim)) {
     // norm (plus this position's rope table), then q|k|v with the rope and
     // the cache store in its epilogue: no separate rope launch
     float* trig = (float*)(base + c.trig);
@@ -498,9 +579,9 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
     rp.rope_dim = d->rope_dim;
     rp.trig = (const float2*)trig;
     rp.pos = pos;
-    rp.k_cache = (__half*)k_cache;
-    rp.v_cache = (__half*)v_cache;
-    rp.kv_index = kv_index;
+    rp.k_cache = (__half*)kv.k;
+    rp.v_cache = (__half*)kv.v;
+    rp.kv_index = kv.kv_index;
     rp.steps = d->rope_steps;
     rp.factors = d->rope_factors;
     if (q4k_qkv_norm_fits(d->width, d->head_dim, d->rope_dim, resid, d->attn_norm)) {
@@ -512,7 +593,7 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
         return rc;
       if ((rc = launch_q4k_qkv_rope(s, sg, d->width, xq, qkv, rp))) return rc;
     }
-  } else if (tokens == 1 && !kv_index && !d->neox && !q8 && d->wq.kind == MI_Q4_K && d->wk.kind == MI_Q4_K &&
+  } else if (tokens == 1 && !kv.kv_index && epi_rope && !q8 && d->wq.kind == MI_Q4_K && d->wk.kind == MI_Q4_K &&
              d->wv.kind == MI_Q6_K && q4k_rows_fits(d->width) &&
              q4k_qkv_rope_fits(d->width, d->head_dim, d->rope_dim)) {
     // a Q4_K_M file's layer at one token (Q6_K v): the norm with this
@@ -534,8 +615,8 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
     rp.rope_dim = d->rope_dim;
     rp.trig = (const float2*)trig;
     rp.pos = pos;
-    rp.k_cache = (__half*)k_cache;
-    rp.v_cache = (__half*)v_cache;
+    rp.k_cache = (__half*)kv.k;
+    rp.v_cache = (__half*)kv.v;
     rp.steps = d->rope_steps;
     rp.factors = d->rope_factors;
     if ((rc = launch_rms_norm_trig(s, resid, d->attn_norm, d->width, d->eps, xq, pos, d->rope_steps,
@@ -546,7 +627,7 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
     if ((rc = launch_matvec(s, d->wv.kind, d->wv.data, d->wv.row_bytes, (int32_t)kvw, d->width, xq, 1, vrow,
                             (int32_t)kvw, MI_EPI_NONE, nullptr)))
       return rc;
-    if ((rc = launch_store_kv(s, nullptr, vrow, (int32_t)kvw, k_cache, v_cache, pos, 0, 1, qkv_stride, 0)))
+    if ((rc = launch_store_kv(s, nullptr, vrow, (int32_t)kvw, kv.k, kv.v, pos, 0, 1, qkv_stride, 0)))
       return rc;
   } else {
     // at 2..8 tokens the norm also writes the hx form (the f16 tile's input)
@@ -574,9 +655,9 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
     if (fused_qkv) {
       // q, k and v in one launch, straight into the fused row
       if ((rc = launch_q4k_rows_segs(s, sg, d->width, xq, qkv))) return rc;
-    } else if (mixed_qkv && (d->neox || q8)) {
-      // a q8_0 cache or neox pairing: the same two launches, unrotated, for
-      // rope_store (a 4096x14336 layer at 8 tokens 177 us with a launch each
+    } else if (mixed_qkv && (!epi_rope || q8)) {
+      // a q8_0 cache, neox pairing or trees: the same two launches, unrotated, for
+      // the launch behind (a 4096x14336 layer at 8 tokens 177 us with a launch each
       // for q, k and v on the int8 tiles, 139 with these)
       if ((rc = launch_htile(s, MI_Q4_K, qk, qw + (int32_t)kvw, d->width, xq, hxn, tokens, qkv, qkv_stride,
                              MI_EPI_NONE, nullptr)))
@@ -594,13 +675,13 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
       rp.head_dim = d->head_dim;
       rp.rope_dim = d->rope_dim;
       rp.pos = pos;
-      rp.k_cache = (__half*)k_cache;
-      rp.v_cache = (__half*)v_cache;
-      rp.kv_index = kv_index;
+      rp.k_cache = (__half*)kv.k;
+      rp.v_cache = (__half*)kv.v;
+      rp.kv_index = kv.kv_index;
       rp.steps = d->rope_steps;
       rp.factors = d->rope_factors;
-      rp.cache_stride = cache_stride;
-      rp.index_stride = index_stride;
+      rp.cache_stride = kv.stride;
+      rp.index_stride = kv.index_stride;
       if ((rc = launch_htile_qkv_rope(s, qk, d->width, xq, hxn, tokens, qkv, qkv_stride, rp))) return rc;
       QkvRope rv = rp;
       rv.qw = -(int)kvw;
@@ -619,7 +700,7 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
       tg.end[1] = qw + (int32_t)kvw;
       tg.end[2] = qw + 2 * (int32_t)kvw;
       tg.nseg = 3;
-      if (!d->neox && !q8) {
+      if (epi_rope && !q8) {
         // the rope and the f16 cache store in the tile's epilogue
         QkvRope rp{};
         rp.qw = qw;
@@ -627,13 +708,13 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
         rp.head_dim = d->head_dim;
         rp.rope_dim = d->rope_dim;
         rp.pos = pos;
-        rp.k_cache = (__half*)k_cache;
-        rp.v_cache = (__half*)v_cache;
-        rp.kv_index = kv_index;
+        rp.k_cache = (__half*)kv.k;
+        rp.v_cache = (__half*)kv.v;
+        rp.kv_index = kv.kv_index;
         rp.steps = d->rope_steps;
         rp.factors = d->rope_factors;
-        rp.cache_stride = cache_stride;
-        rp.index_stride = index_stride;
+        rp.cache_stride = kv.stride;
+        rp.index_stride = kv.index_stride;
         if (htile_qkv_rope_fits(tg, d->width, tokens, d->head_dim, d->rope_dim))
           rc = launch_htile_qkv_rope(s, tg, d->width, xq, hxn, tokens, qkv, qkv_stride, rp);
         else
@@ -641,8 +722,8 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
         if (rc) return rc;
         roped = true;
       } else {
-        // a q8_0 cache or neox pairing: unrotated q|k|v for rope_store, on
-        // the f16 tile where its segments fit
+        // a q8_0 cache, neox pairing or trees: unrotated q|k|v, on the f16
+        // tile where its segments fit
         if (htile_qkv_rope_fits(tg, d->width, tokens, d->head_dim, d->rope_dim))
           rc = launch_htile(s, MI_Q4_K, tg, qw + 2 * (int32_t)kvw, d->width, xq, hxn, tokens, qkv, qkv_stride,
                             MI_EPI_NONE, nullptr);
@@ -663,16 +744,22 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, uint
     }
     // rotate q and k; k and v into the cache (f16, or q8_0 blocks encoded by
     // the same launch once it holds every rotated key)
-    if (!roped && (rc = launch_rope_store(s, qkv, d->heads, d->kv_heads, d->head_dim, d->rope_dim, d->neox,
-                                d->rope_steps, pos, tokens, qkv_stride, k_cache, v_cache, cache_stride,
-                                d->rope_factors, d->cache_form, kv_index, index_stride)))
+    if (!roped && !kv.tree &&
+        (rc = launch_rope_store(s, qkv, d->heads, d->kv_heads, d->head_dim, d->rope_dim, d->neox, d->rope_steps, pos,
+                                tokens, qkv_stride, kv.k, kv.v, kv.stride, d->rope_factors, d->cache_form,
+                                kv.kv_index, kv.index_stride)))
       return rc;
   }
-  // count = pos + 1 per sequence: the attention kernels read pos and add one.
-  if ((rc = launch_attend(s, qkv, qkv_stride, k_cache, v_cache, cache_stride, d->heads, d->kv_heads,
-                          d->head_dim, d->attn_scale, pos, -1, max_count, tokens, nullptr, xq, attn,
-                          d->cache_form, kv_index, index_stride, hx)))
+  if (kv.tree) {
+    float* out = (float*)((char*)attn + tree_part(d, kv.tree));
+    if ((rc = tree_attention(s, d, qkv, kv, out, attn))) return rc;
+    if ((rc = launch_quantize(s, out, qw, tokens, xq, hx))) return rc;
+  } else if ((rc = launch_attend(s, qkv, qkv_stride, kv.k, kv.v, kv.stride, d->heads, d->kv_heads, d->head_dim,
+                                 d->attn_scale, pos, -1, max_count, tokens, nullptr, xq, attn, d->cache_form,
+                                 kv.kv_index, kv.index_stride, hx))) {
+    // count = pos + 1 per sequence: the attention kernels read pos and add one.
     return rc;
+  }
   const bool glu_tile = tokens >= 4 && d->gate.kind == MI_Q4_K && d->up.kind == MI_Q4_K &&
                         d->gate.row_bytes == d->up.row_bytes && htile_glu_fits(d->hidden, d->width, tokens);
   const bool wo_split = glu_tile && wo_split_norm(d, qw, tokens);
@@ -770,6 +857,28 @@ int mi_decoder_layer_paged(mi_stream stream, const mi_layer_desc* d, float* resi
   if (!kv_index) return fail(MI_ERR_ARG, "layer: a paged layer needs its index");
   return decoder_layer(stream, d, resid, k_pool, v_pool, 0, kv_index, index_stride, pos, max_count, tokens, work,
                        work_bytes);
+}
+
+size_t mi_layer_tree_workspace(const mi_layer_desc* desc, const mi_tree* tree) {
+  if (!desc || !tree || tree->tokens > kMaxPrefill || !tree_part(desc, tree)) return 0;
+  const int32_t n = tree->tokens;
+  return n > kMaxTokens ? prefill_carve(desc, tree->max_count, n, tree).total : carve(desc, tree->max_count, n, tree).total;
+}
+
+int mi_decoder_layer_tree(mi_stream stream, const mi_layer_desc* d, float* resid, uint16_t* k_cache,
+                          uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
+                          const mi_tree* tree, void* work, size_t work_bytes) {
+  int rc = check_desc(d);
+  if (rc) return rc;
+  if (!resid || !k_cache || !v_cache) return fail(MI_ERR_ARG, "layer: null pointer");
+  if ((rc = check_tree("layer", tree, true))) return rc;
+  if ((rc = check_tree_caches("layer", d->cache_form, d->heads, d->kv_heads, d->head_dim, k_cache, v_cache,
+                              cache_stride, kv_index, index_stride, tree)))
+    return rc;
+  if (tree->tokens > kMaxPrefill)
+    return fail(MI_ERR_ARG, "layer: tokens %d outside 1..%d", tree->tokens, kMaxPrefill);
+  const LayerCache kv{k_cache, v_cache, cache_stride, kv_index, index_stride, tree};
+  return run_layer((hipStream_t)stream, d, resid, kv, tree->pos, tree->max_count, tree->tokens, work, work_bytes);
 }
 
 }  // extern "C"

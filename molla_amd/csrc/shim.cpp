@@ -45,6 +45,33 @@ static bool quant_kind(int kind) {
 static bool k_quant(int kind) { return kind == MI_Q4_K || kind == MI_Q5_K || kind == MI_Q6_K; }
 
 // The row geometry the kernels assume, checked once here.
+// A step's trees, for attention and (with `layer`) for a layer.
+int check_tree(const char* name, const mi_tree* t, bool layer) {
+  if (!t || !t->starts || !t->lengths || !t->mask) return fail(MI_ERR_ARG, "%s: null pointer in the trees", name);
+  if (layer && (!t->pos || !t->cells)) return fail(MI_ERR_ARG, "%s: the trees need pos and cells", name);
+  if (t->batch < 1 || t->tokens < 1 || t->tokens > kMaxTreeRows)
+    return fail(MI_ERR_SHAPE, "%s: %d sequences in %d token rows", name, t->batch, t->tokens);
+  if (mi_tree_words(t->max_nodes) < 0)
+    return fail(MI_ERR_SHAPE, "%s: trees of %d nodes, outside 1..%d", name, t->max_nodes, kMaxTreeNodes);
+  if (t->max_count < 1) return fail(MI_ERR_SHAPE, "%s: max_count must be positive", name);
+  return MI_OK;
+}
+
+// The caches of a step over trees (check_tree has passed).
+int check_tree_caches(const char* name, int32_t form, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                      const uint16_t* k_cache, const uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index,
+                      int64_t index_stride, const mi_tree* tree) {
+  if ((int64_t)heads * head_dim > kMaxHeadsWidth)
+    return fail(MI_ERR_SHAPE, "%s: rows of %lld values", name, (long long)heads * head_dim);
+  const int32_t row = cache_row(form, kv_heads * head_dim);
+  if (row < 0) return fail(MI_ERR_SHAPE, "%s: unknown cache form %d", name, form);
+  if (kv_index ? index_stride < tree->max_count : (tree->batch > 1 && cache_stride < (int64_t)tree->max_count * row))
+    return fail(MI_ERR_SHAPE, "%s: a sequence's stride holds fewer than %d positions", name, tree->max_count);
+  if ((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) || (!kv_index && cache_stride % 8))
+    return fail(MI_ERR_ALIGN, "%s: the caches must be 16-byte aligned with a stride of a multiple of 8 halves", name);
+  return MI_OK;
+}
+
 int check_weight(const char* name, int kind, const void* w, int64_t row_bytes, int32_t rows,
                  int32_t cols) {
   if (!quant_kind(kind)) return fail(MI_ERR_KIND, "%s: ggml type %d has no device matvec", name, kind);
@@ -488,18 +515,6 @@ int mi_qk_norm_rope(mi_stream stream, const mi_qk* d) {
   return launch_qk_rope((hipStream_t)stream, a);
 }
 
-// A step's trees, for attention and (with `layer`) for a layer.
-int check_tree(const char* name, const mi_tree* t, bool layer) {
-  if (!t || !t->starts || !t->lengths || !t->mask) return fail(MI_ERR_ARG, "%s: null pointer in the trees", name);
-  if (layer && (!t->pos || !t->cells)) return fail(MI_ERR_ARG, "%s: the trees need pos and cells", name);
-  if (t->batch < 1 || t->tokens < 1 || t->tokens > kMaxTreeRows)
-    return fail(MI_ERR_SHAPE, "%s: %d sequences in %d token rows", name, t->batch, t->tokens);
-  if (mi_tree_words(t->max_nodes) < 0)
-    return fail(MI_ERR_SHAPE, "%s: trees of %d nodes, outside 1..%d", name, t->max_nodes, kMaxTreeNodes);
-  if (t->max_count < 1) return fail(MI_ERR_SHAPE, "%s: max_count must be positive", name);
-  return MI_OK;
-}
-
 size_t mi_attend_tree_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form,
                                 const mi_tree* tree) {
   if (check_attn("attend_tree", heads, kv_heads, head_dim) || (int64_t)heads * head_dim > kMaxHeadsWidth ||
@@ -516,17 +531,13 @@ int mi_attend_tree(mi_stream stream, int32_t form, const float* q, int64_t q_str
   if (!q || !k_cache || !v_cache || !out) return fail(MI_ERR_ARG, "attend_tree: null pointer");
   int rc = check_attn("attend_tree", heads, kv_heads, head_dim);
   if (rc) return rc;
-  if ((int64_t)heads * head_dim > kMaxHeadsWidth)
-    return fail(MI_ERR_SHAPE, "attend_tree: rows of %lld values", (long long)heads * head_dim);
-  const int32_t row = cache_row(form, kv_heads * head_dim);
-  if (row < 0) return fail(MI_ERR_SHAPE, "attend_tree: unknown cache form %d", form);
   if ((rc = check_tree("attend_tree", tree, false))) return rc;
+  if ((rc = check_tree_caches("attend_tree", form, heads, kv_heads, head_dim, k_cache, v_cache, cache_stride, kv_index,
+                              index_stride, tree)))
+    return rc;
   if (q_stride < (int64_t)heads * head_dim) return fail(MI_ERR_SHAPE, "attend_tree: row stride too small");
-  if (kv_index ? index_stride < tree->max_count : (tree->batch > 1 && cache_stride < (int64_t)tree->max_count * row))
-    return fail(MI_ERR_SHAPE, "attend_tree: a sequence's stride holds fewer than %d positions", tree->max_count);
-  if ((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) || q_stride % 4 ||
-      (!kv_index && cache_stride % 8))
-    return fail(MI_ERR_ALIGN, "attend_tree: the queries, the caches and the output must be 16-byte aligned");
+  if ((((uintptr_t)q | (uintptr_t)out) & 15) || q_stride % 4)
+    return fail(MI_ERR_ALIGN, "attend_tree: the queries and the output must be 16-byte aligned");
   const size_t need = mi_attend_tree_workspace(heads, kv_heads, head_dim, form, tree);
   if (!work || ((uintptr_t)work & 255) || work_bytes < need)
     return fail(MI_ERR_WORKSPACE, "attend_tree: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);

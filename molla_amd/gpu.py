@@ -364,6 +364,7 @@ def device_qk_norm_rope(ctx: DeviceContext, q: torch.Tensor, k: torch.Tensor, v:
     f32, i32 = torch.float32, torch.int32
     tokens = pos.numel()
     qw, kvw = heads * head_dim, kv_heads * head_dim
+
     def at(t, name, dtype, n=0):
         return None if t is None else _on(ctx, t, name, dtype, n)
 
@@ -376,6 +377,15 @@ def device_qk_norm_rope(ctx: DeviceContext, q: torch.Tensor, k: torch.Tensor, v:
              at(factors, "factors", f32, dim // 2), _on(ctx, pos, "pos", i32), at(count, "count", i32, 1),
              at(k_cache, "k_cache", torch.float16), at(v_cache, "v_cache", torch.float16), at(cells, "cells", i32, tokens))
     _queue(ctx, lib().mi_qk_norm_rope, ctypes.byref(d))
+
+
+def tree_cache(kv_index: torch.Tensor | None, batch: int, cache_stride: int, max_count: int, row: int) -> tuple:
+    """(entries of a sequence's list of cells or 0, halves a cache holds at least) of a step over trees."""
+    if kv_index is None:
+        return 0, (batch - 1) * cache_stride + max_count * row
+    if kv_index.dim() != 2 or kv_index.shape[0] < batch:
+        raise ValueError(f"a step over trees wants a list of cells a sequence ({batch})")
+    return kv_index.shape[1], 1
 
 
 def device_attend_tree(ctx: DeviceContext, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, heads: int,
@@ -391,15 +401,7 @@ def device_attend_tree(ctx: DeviceContext, q: torch.Tensor, k_cache: torch.Tenso
     batch, tokens = lengths.numel(), q.shape[0]
     qw = heads * head_dim
     q_stride = _rows(ctx, q, "q", tokens, qw)
-    row = cache_row(form, kv_heads * head_dim)
-    stride = 0
-    if kv_index is not None:
-        if kv_index.dim() != 2 or kv_index.shape[0] < batch:
-            raise ValueError(f"attend_tree wants a list of cells a sequence ({batch})")
-        stride = kv_index.shape[1]
-        least = 1
-    else:
-        least = (batch - 1) * cache_stride + max_count * row
+    stride, least = tree_cache(kv_index, batch, cache_stride, max_count, cache_row(form, kv_heads * head_dim))
     tree = MiTree(batch, tokens, max_nodes, max_count, _on(ctx, starts, "starts", i32, batch + 1),
                   _on(ctx, lengths, "lengths", i32), _on(ctx, mask, "mask", i32, tokens * tree_words(max_nodes)))
     L = lib()

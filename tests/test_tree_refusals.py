@@ -107,6 +107,50 @@ def test_attend_refuses_no_trees():
     refused(_lib.lib().mi_attend_tree(*ATTEND.values()), ARG, "trees")
 
 
+def layer_desc(**change):
+    d = _lib.MiLayerDesc(width=512, hidden=1024, heads=8, kv_heads=2, head_dim=64, rope_dim=64, eps=1e-5, attn_scale=0.125,
+                         attn_norm=FAKE, ffn_norm=FAKE, rope_steps=FAKE)
+    for name, rows, cols in (("wq", 512, 512), ("wk", 128, 512), ("wv", 128, 512), ("wo", 512, 512), ("gate", 1024, 512),
+                             ("up", 1024, 512), ("down", 512, 1024)):
+        setattr(d, name, _lib.MiWeight(FAKE, 12, rows, cols, cols // 256 * 144))
+    for name, value in change.items():
+        setattr(d, name, value)
+    return d
+
+
+LAYER = dict(stream=None, desc=None, resid=FAKE, k_cache=FAKE, v_cache=FAKE, cache_stride=12800, kv_index=None,
+             index_stride=0, tree=None, work=FAKE, work_bytes=1 << 30)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(resid=None), ARG, "null"), (dict(k_cache=None), ARG, "null"), (dict(v_cache=None), ARG, "null"),
+    (dict(desc=dict(heads=12)), SHAPE, "1, 2, 4 or 8"), (dict(desc=dict(cache_form=3)), SHAPE, "form"),
+    (dict(desc=dict(q_norm=FAKE)), ARG, "together"), (dict(cache_stride=12799), SHAPE, "fewer"),
+    (dict(kv_index=FAKE, index_stride=99), SHAPE, "fewer"), (dict(cache_stride=12804), ALIGN, "16-byte"),
+    (dict(k_cache=FAKE + 8), ALIGN, "16-byte"), (dict(work=None), ALIGN, "workspace"),
+    (dict(work_bytes=64), WORKSPACE, "needed"), (dict(tree=dict(tokens=8), work_bytes=64), WORKSPACE, "needed"),
+    (dict(tree=dict(tokens=8), work=FAKE + 16), WORKSPACE, "workspace"), (dict(tree=dict(pos=None)), ARG, "pos and cells"),
+    (dict(tree=dict(cells=None)), ARG, "pos and cells"), (dict(tree=dict(mask=None)), ARG, "trees"),
+    (dict(tree=dict(tokens=65537)), ARG, "65536"), (dict(tree=dict(max_nodes=257)), SHAPE, "nodes"),
+    (dict(tree=dict(max_count=0)), SHAPE, "max_count")])
+def test_layer_refusals(change, code, text):
+    tree = _lib.MiTree(**{**TREE, "pos": FAKE, "cells": FAKE, **(change.get("tree") or {})})
+    desc = layer_desc(**(change.get("desc") or {}))
+    args = {**LAYER, **change, "tree": ctypes.byref(tree), "desc": ctypes.byref(desc)}
+    refused(_lib.lib().mi_decoder_layer_tree(*args.values()), code, text)
+
+
+def test_layer_refuses_no_trees():
+    refused(_lib.lib().mi_decoder_layer_tree(*{**LAYER, "desc": ctypes.byref(layer_desc())}.values()), ARG, "trees")
+    refused(_lib.lib().mi_decoder_layer_tree(*LAYER.values()), ARG, "descriptor")
+    size = _lib.lib().mi_layer_tree_workspace
+    tree = _lib.MiTree(**TREE)
+    assert size(ctypes.byref(layer_desc()), ctypes.byref(tree)) > 0
+    assert size(None, ctypes.byref(tree)) == 0 and size(ctypes.byref(layer_desc()), None) == 0
+    assert size(ctypes.byref(layer_desc(head_dim=40)), ctypes.byref(tree)) == 0
+    assert size(ctypes.byref(layer_desc()), ctypes.byref(_lib.MiTree(**{**TREE, "tokens": 65537}))) == 0
+
+
 def test_workspace_of_a_refused_shape_is_zero():
     size = _lib.lib().mi_attend_tree_workspace
     ok = _lib.MiTree(**TREE)
