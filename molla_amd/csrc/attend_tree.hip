@@ -9,9 +9,18 @@
 // themselves: each scans the sequences and takes an equal run of units, walking
 // its slices with a running maximum and sum.  Of the tiles in a run only the first
 // and the last can be another block's too: those leave partial results, two a
-// block, that a second launch folds; the others' rows are finished.  (Shares of
-// the keys fixed by the host leave every block waiting for the longest sequence:
-// eight of 8192 down to 4608 positions 165 us, so 112.)
+// block, that a second launch folds; the others' rows are finished.  (With as many
+// parts for every tile as the longest sequence needs, the fold of 13 nodes over
+// 32768 positions took 46 us, that of 8 over 2048 14; so 5.6 and 4.1.)
+//
+// Measured, products + fold, heads 32 over 8 (over 4 at width 64): 8 sequences of
+// 64 nodes over 8192 down to 4608 positions at width 128 132 + 12.7 us (292
+// TFLOP/s of the formula's products, twice that of the matrix cores', whose steps
+// take turns with the softmax on the VALU at two waves a SIMD); 8 x 48 over 3000
+// down to 1688 at width 64 30 + 9.4 (bound by the VALU); 1 x 13 over 32768 36.6 +
+// 5.6 (3.7 TB/s; 6 once the first slices are there); 4 x 25 over 4099 of q8_0 42.7
+// + 5.8 (a value block's factor makes halves of the weights anew); 1 x 8 over 2048
+// 11.5 + 4.1 (launches and the first loads' latency).
 #include <math.h>
 
 #include <algorithm>
@@ -38,10 +47,15 @@ __device__ __forceinline__ TreeSeq tree_seq(const mi_tree& tr, int b) {
   return s;
 }
 
-__device__ __forceinline__ int tree_tiles(const TreeSeq& s, int group, int rows) {
-  return (s.nodes * group + rows - 1) / rows;
+__device__ __forceinline__ int tree_tiles(const TreeSeq& s, int shift, int rows) {
+  return ((s.nodes << shift) + rows - 1) / rows;
 }
 __device__ __forceinline__ int tree_slices(const TreeSeq& s, int slice) { return (s.count + slice - 1) / slice; }
+// A tile's units: its slices behind kStart that stand for the start of a run in it
+// (queries, first loads), so that a block with two starts gets less of the rest: 1 x
+// 13 over 32768 39.2 us at 0, 36.6 at 3, 39.8 at 6; 4 x 25 of q8_0 46.4, 42.7, 45.9.
+constexpr int kStart = 3;
+__device__ __forceinline__ int tree_units(const TreeSeq& s, int slice) { return kStart + tree_slices(s, slice); }
 
 struct IMax {
   __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
@@ -65,20 +79,20 @@ __device__ __forceinline__ int lane_scan(int v) {
 template <class F>
 __device__ __forceinline__ void tree_walk(const TreeAttend& a, int rows, int slice, int32_t* __restrict__ plan,
                                           F take) {
-  const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads, batch = a.tree.batch;
+  const int lane = threadIdx.x & 63, shift = a.group_shift, batch = a.tree.batch;
   TreeSeq sq;
   int units;
   auto look = [&](int b0) __attribute__((always_inline)) {
     const int b = b0 + lane;
     sq = tree_seq(a.tree, min(b, batch - 1));
     if (b >= batch || sq.nodes == 0) sq.count = 0;
-    units = tree_tiles(sq, group, rows) * a.kv_heads * tree_slices(sq, slice);
+    units = sq.count ? tree_tiles(sq, shift, rows) * a.kv_heads * tree_units(sq, slice) : 0;
   };
   int total = 0, top = 0;
   for (int b0 = 0; b0 < batch; b0 += 64) {
     look(b0);
     total += lanes::reduce<64>(units, lanes::Add{});
-    top = max(top, lanes::reduce<64>(tree_slices(sq, slice), IMax{}));
+    top = max(top, lanes::reduce<64>(sq.count ? tree_units(sq, slice) : 0, IMax{}));
   }
   total = __builtin_amdgcn_readfirstlane(total);  // (the same in every lane)
   top = __builtin_amdgcn_readfirstlane(top);
@@ -116,11 +130,13 @@ __device__ __forceinline__ void tree_walk(const TreeAttend& a, int rows, int sli
   s.count = __builtin_amdgcn_readlane(sq.count, b - chunk);
   int left = (int)min<int64_t>(per, total - first);
   while (true) {
-    const int slices = tree_slices(s, slice), tiles = tree_tiles(s, group, rows);
-    while (at < slices * tiles * a.kv_heads) {
-      const int pair = at / slices, sl = at - pair * slices, n = min(slices - sl, left);
-      const int part = n == slices ? -1 : 2 * block + (sl == 0 ? 1 : 0);
-      take(s, b, pair / tiles, pair % tiles, sl, sl + n, part);
+    const int run = tree_units(s, slice), tiles = tree_tiles(s, shift, rows);
+    while (at < run * tiles * a.kv_heads) {
+      const int pair = at / run, u = at - pair * run, n = min(run - u, left);
+      const int head = tiles == 1 ? pair : pair / tiles;
+      const int s0 = max(u - kStart, 0), s1 = u + n - kStart;
+      const int part = u <= kStart && u + n == run ? -1 : 2 * block + (u <= kStart ? 1 : 0);
+      if (s0 < s1) take(s, b, head, pair - head * tiles, s0, s1, part);
       left -= n;
       if (left == 0) return;
       at += n;
@@ -156,7 +172,7 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
                                                                         int32_t* __restrict__ plan) {
   extern __shared__ float4 lds[];
   const int D = a.head_dim, kk = rows_slice(D), KS = D + 4;
-  const int words = (a.tree.max_nodes + 31) >> 5, group = a.heads / a.kv_heads;
+  const int words = (a.tree.max_nodes + 31) >> 5, shift = a.group_shift, group = 1 << shift;
   float* Ks = (float*)lds;
   float* Vs = Ks + kk * KS;
   float* Qs = Vs + kk * D;
@@ -173,15 +189,15 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
     // queries; rows past the sequence repeat its last token (not written)
     __syncthreads();
     for (int i = tid; i < kRowsTile * D; i += kRowsThreads) {
-      const int r = tile * kRowsTile + i / D, e = i % D, node = min(r / group, sq.nodes - 1);
-      Qs[i] = a.q[(int64_t)(sq.t0 + node) * a.q_stride + (int64_t)(kvh * group + r % group) * D + e];
+      const int r = tile * kRowsTile + i / D, e = i % D, node = min(r >> shift, sq.nodes - 1);
+      Qs[i] = a.q[(int64_t)(sq.t0 + node) * a.q_stride + (int64_t)(kvh * group + (r & (group - 1))) * D + e];
     }
     const int r0 = 4 * wave;
     const uint32_t* mrow[4];
     float m2[4], l[4], o[4][ND];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      mrow[r] = a.tree.mask + (int64_t)(sq.t0 + min((tile * kRowsTile + r0 + r) / group, sq.nodes - 1)) * words;
+      mrow[r] = a.tree.mask + (int64_t)(sq.t0 + min((tile * kRowsTile + r0 + r) >> shift, sq.nodes - 1)) * words;
       m2[r] = -INFINITY;
       l[r] = 0.0f;
 #pragma unroll
@@ -278,9 +294,9 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       const int row = tile * kRowsTile + r0 + r;
-      if (row / group >= sq.nodes) continue;
+      if (row >> shift >= sq.nodes) continue;
       const int64_t slot = (int64_t)part * kRowsTile + r0 + r;
-      float* dst = part < 0 ? a.out + ((int64_t)(sq.t0 + row / group) * a.heads + kvh * group + row % group) * D
+      float* dst = part < 0 ? a.out + ((int64_t)(sq.t0 + (row >> shift)) * a.heads + kvh * group + (row & (group - 1))) * D
                             : parts.acc + slot * D;
       const float w = part >= 0 ? 1.0f : l[r] != 0.0f ? 1.0f / l[r] : 0.0f;
 #pragma unroll
@@ -304,17 +320,20 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 //   leaves them.
 //   Queries enter as two halves, each query scaled by a power of two so that its
 //   largest value is in [2^14, 2^15): every value to 2^-23 of itself (its float
-//   to 2^-24), down to 2^-39 of the largest.  Weights, lifted by 2^14, enter as
-//   two halves as well: to 2^-24 of the largest weight.
+//   to 2^-24), down to 2^-39 of the largest.  Weights enter as two halves as well,
+//   2^14 times their size (f16 caches): to 2^-23 of themselves, down to 2^-39 of
+//   the largest.
 //
-//   A weight is 2^(s c2 - mk), mk = the maximum times c2 rounded once and then
-//   taken as it is, so that the rounding is the same in every weight of a row and
-//   falls out of its quotient (where mk is so large that it could reach a weight's
-//   own size, the difference is taken before the product).
+//   A weight is 2^(s c2 - mk), mk = the maximum times c2 less 14, rounded once and
+//   then taken as it is, so that the rounding is the same in every weight of a row
+//   and falls out of its quotient, as the 14 does (where mk is so large that it
+//   could reach a weight's own size, the difference is taken before the product).
+//   The exponent's own rounding, at most 2^-21, is a weight's 3.3e-7.
 //
 // q8_0: keys and values enter as their integers, exact halves; a key block's
 // factor multiplies its part of the score, a value block's the weights, which
-// are then split into halves.  The factors are staged times 2^(15 - X), X the
+// are then split into halves (the factors' share of 4 x 25 over 4099: 43 us against
+// 30 of f16).  The factors are staged times 2^(15 - X), X the
 // exponent of the largest one so far among committed positions, which every row
 // sees; slices that some row does not see whole leave X as it is, and there each
 // row's products are scaled to its own largest and summed apart: what a row does
@@ -334,7 +353,21 @@ typedef short ts8 __attribute__((ext_vector_type(8)));
 typedef float tf4 __attribute__((ext_vector_type(4)));
 typedef uint32_t tu4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLift = 16384.0f;
+constexpr float kLift = 14.0f;
+
+// w as two halves, pairs of them at a time (one: 1 in a scalar register, so that
+// the difference is one instruction that also rounds it)
+__device__ __forceinline__ void split(const float (&w)[8], float one, th8& hi, th8& lo) {
+  typedef float tf2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const th2 h = __builtin_convertvector((tf2{w[i], w[i + 1]}), th2);
+    hi[i] = h[0];
+    hi[i + 1] = h[1];
+    lo[i] = (_Float16)fmaf(w[i], one, -(float)h[0]);
+    lo[i + 1] = (_Float16)fmaf(w[i + 1], one, -(float)h[1]);
+  }
+}
 
 __device__ __forceinline__ tf4 mfma16(th8 a, th8 b, tf4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -395,26 +428,24 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   return (not_finite(w) ? 0u : w & 0xffffu) | (not_finite(w >> 16) ? 0u : w & 0xffff0000u);
 }
 
-// Sizes by head width and columns: keys of a slice (32 at D = 128 and 256, where
-// the words of 64 on their way cost the registers of a second block's wave; 64 at
-// D = 64), and blocks a compute unit.
+// Sizes by head width: keys of a slice (32 at D = 128 and 256, where the words of 64
+// on their way cost the registers of a second block's wave: 8 x 64 at D = 128 209
+// us, so 165 at the time; 64 at D = 64), and blocks a compute unit (one more at D =
+// 128: q8_0 62 us against 43 for the registers, f16 no faster and 1 us more to fold;
+// at D = 64: no faster).
 __host__ __device__ constexpr int mfma_slice(int D) { return D == 64 ? 64 : 32; }
-__host__ __device__ constexpr int mfma_blocks(int D, int NC, bool Q8) {
-  return D == 64 ? (Q8 ? 3 : 4) : D == 128 && NC == 1 ? 3 : 2;
-}
+__host__ __device__ constexpr int mfma_blocks(int D) { return D == 64 ? 3 : 2; }
 
-#ifndef VGX
-#define VGX 2
-#endif
 template <int D, int NC, bool Q8, bool PAGED>
-__global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kernel(TreeAttend a, TreeParts parts,
+__global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAttend a, TreeParts parts,
                                                                               int32_t* __restrict__ plan) {
   constexpr int SL = mfma_slice(D), KS = D / 32, NT = D / 16, PIECES = D / 8;
   constexpr int PER = Q8 ? (SL * D / 16 + 255) / 256 : SL * PIECES / 256;  // 16-byte words of K (and of V) a thread
   constexpr int WPK = Q8 ? D / 16 : PIECES;                               // words a key
   constexpr int ROWS = 64 * NC;
-  constexpr int VG = VGX < NT ? VGX : NT;  // 16-dim tiles of values a group of reads
-  static_assert(PER * 256 == SL * WPK, "a slice's words dealt evenly");
+  constexpr int VG = 2;  // 16-dim tiles of values a group of reads
+  constexpr int FPER = 2 * SL * KS / 256;                                 // q8_0 factors of K and V a thread
+  static_assert(PER * 256 == SL * WPK && FPER * 256 == 2 * SL * KS, "a slice's words dealt evenly");
   constexpr int KR = key_row(D), VR = val_row(D);
   __shared__ __align__(16) _Float16 ks[2][SL * KR];
   __shared__ __align__(16) _Float16 vs[2][SL * VR];
@@ -424,7 +455,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
   __shared__ int spoilt[2]; // the last (even, odd) run in which some staged value was not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lm = lane & 15, lk = lane >> 4;
-  const int group = a.heads / a.kv_heads, words = (a.tree.max_nodes + 31) >> 5;
+  const int shift = a.group_shift, group = 1 << shift, words = (a.tree.max_nodes + 31) >> 5;
   const int kvw = a.kv_heads * D, crow = cache_row(a.form, kvw);
   if (tid == 0) holes[0] = holes[1] = spoilt[0] = spoilt[1] = 0;
   __syncthreads();
@@ -443,72 +474,76 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
 
     // this lane's columns: rows past the sequence's repeat its last one (not written)
     const int first_row = tile * ROWS + wave * 16 * NC;
-    const bool busy = first_row < sq.nodes * group;  // (uniform over the wave)
+    const bool busy = first_row < sq.nodes << shift;  // (uniform over the wave)
     int node[NC];
 #pragma unroll
-    for (int c = 0; c < NC; c++) node[c] = (first_row + 16 * c + lm) / group;
+    for (int c = 0; c < NC; c++) node[c] = (first_row + 16 * c + lm) >> shift;
     auto mask_row = [&](int c) __attribute__((always_inline)) {
       return a.tree.mask + (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * words;
     };
 
     // staging: words tid + 256 j of a slice's keys, and of its values
-    tu4 kw[PER], vw[PER];
-    int cells[PAGED ? PER : 1], fcell = 0;  // the next slice's (negative: not held)
-    tu4 fw = {0, 0, 0, 0};                  // q8_0: thread = (key or value, key) of the first 2 SL
-    bool fdead = false;
-    int xrun[Q8 ? KS : 1];  // q8_0: the X of each 32-dim block so far (the wave that stages the values' factors)
+    struct Stage {
+      tu4 kw[PER], vw[PER];
+      int cells[PAGED ? PER : 1], fcell[PAGED && Q8 ? FPER : 1];  // (negative: not held)
+      uint16_t f[Q8 ? FPER : 1];  // q8_0: factor tid + 256 j of (key or value, 32-dim block, key)
+      bool dead;                  // nothing is held where some word was loaded
+    };
+    Stage st;
+    int xrun[Q8 ? FPER : 1];  // q8_0: the X so far of the blocks whose values' factors this thread stages
 #pragma unroll
-    for (int u = 0; u < (Q8 ? KS : 1); u++) xrun[u] = 0;
+    for (int j = 0; j < (Q8 ? FPER : 1); j++) xrun[j] = 0;
     auto cell_at = [&](int j) __attribute__((always_inline)) { return index[min(j, sq.count - 1)]; };
-    auto find = [&](int sl) __attribute__((always_inline)) {
+    auto find = [&](int sl, Stage& st) __attribute__((always_inline)) {
       if constexpr (PAGED) {
 #pragma unroll
-        for (int j = 0; j < PER; j++) cells[j] = cell_at(sl * SL + (tid + 256 * j) / WPK);
-        if (Q8) fcell = cell_at(sl * SL + tid % SL);
-      }
-    };
-    bool dead = false;  // nothing is held where some word was loaded
-    auto load = [&](int sl) __attribute__((always_inline)) {
-      dead = false;
+        for (int j = 0; j < PER; j++) st.cells[j] = cell_at(sl * SL + (tid + 256 * j) / WPK);
+        if constexpr (Q8) {
 #pragma unroll
-      for (int j = 0; j < PER; j++) {
-        const int i = tid + 256 * j, at = sl * SL + i / WPK;
-        int cell = PAGED ? cells[j] : min(at, sq.count - 1);
-        // (opaque: an address formed ahead of the products would wait for its cell there)
-        if (PAGED) asm volatile("" : "+v"(cell));
-        dead |= PAGED && cell < 0;
-        const int64_t off = (int64_t)(PAGED ? max(cell, 0) : cell) * crow + 8 * (i % WPK);
-        kw[j] = *(const tu4*)(kc + off);
-        vw[j] = *(const tu4*)(vc + off);
-      }
-      if constexpr (Q8) {
-        int at = sl * SL + tid % SL, cell = PAGED ? fcell : min(at, sq.count - 1);
-        if (PAGED) asm volatile("" : "+v"(cell));
-        fdead = at >= sq.count || (PAGED && cell < 0);
-        if (tid < 2 * SL) {
-          const __half* f = (tid < SL ? kc : vc) + (int64_t)(PAGED ? max(cell, 0) : cell) * crow + (kvw >> 1) -
-                            kvh * D / 2 + ((kvh * D) >> 5);
-          if constexpr (KS == 2) fw.x = *(const uint32_t*)f;
-          else if constexpr (KS == 4) { fw.x = ((const uint2*)f)->x; fw.y = ((const uint2*)f)->y; }
-          else fw = *(const tu4*)f;
+          for (int j = 0; j < FPER; j++) st.fcell[j] = cell_at(sl * SL + (tid + 256 * j) % SL);
         }
       }
     };
-    auto store = [&](int sl, int buf) __attribute__((always_inline)) {
+    auto load = [&](int sl, Stage& st) __attribute__((always_inline)) {
+      st.dead = false;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        const int i = tid + 256 * j, at = sl * SL + i / WPK;
+        int cell = PAGED ? st.cells[j] : min(at, sq.count - 1);
+        // (opaque: an address formed ahead of the products would wait for its cell there)
+        if (PAGED) asm volatile("" : "+v"(cell));
+        st.dead |= PAGED && cell < 0;
+        const int64_t off = (int64_t)(PAGED ? max(cell, 0) : cell) * crow + 8 * (i % WPK);
+        st.kw[j] = *(const tu4*)(kc + off);
+        st.vw[j] = *(const tu4*)(vc + off);
+      }
+      if constexpr (Q8) {
+#pragma unroll
+        for (int j = 0; j < FPER; j++) {
+          const int i = tid + 256 * j, at = sl * SL + i % SL;
+          int cell = PAGED ? st.fcell[j] : min(at, sq.count - 1);
+          if (PAGED) asm volatile("" : "+v"(cell));
+          st.f[j] = *(const uint16_t*)((i < SL * KS ? kc : vc) + (int64_t)(PAGED ? max(cell, 0) : cell) * crow + (kvw >> 1) -
+                                       kvh * D / 2 + ((kvh * D) >> 5) + i / SL % KS);
+          if (at >= sq.count || (PAGED && cell < 0)) st.f[j] = 0;
+        }
+      }
+    };
+    auto store = [&](int sl, int buf, Stage& st) __attribute__((always_inline)) {
       turn++;
       const bool nodes_in = (sl + 1) * SL > sq.len;  // (uniform)
-      if (PAGED && dead) holes[buf] = turn;
+      if (PAGED && st.dead) holes[buf] = turn;
       // what is not held, and what some row may not see, must be finite: 0 * inf in
       // the products would reach every row
-      if (!Q8 && (nodes_in || (PAGED && __any(dead)))) {
+      if (!Q8 && (nodes_in || (PAGED && __any(st.dead)))) {
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < PER; j++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const uint32_t f = finite_halves(vw[j][e]);
-            bad |= f != vw[j][e];
-            vw[j][e] = f;
+            const uint32_t f = finite_halves(st.vw[j][e]);
+            bad |= f != st.vw[j][e];
+            st.vw[j][e] = f;
           }
         if (bad) spoilt[run & 1] = run;
       }
@@ -516,36 +551,51 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
       for (int j = 0; j < PER; j++) {
         const int i = tid + 256 * j, key = i / WPK, pc = i % WPK;
         if constexpr (Q8) {
-          *(th8*)(ks[buf] + key * KR + 16 * pc) = int8_halves(kw[j].x, kw[j].y);
-          *(th8*)(ks[buf] + key * KR + 16 * pc + 8) = int8_halves(kw[j].z, kw[j].w);
-          *(th8*)(vs[buf] + key * VR + 16 * pc) = int8_halves(vw[j].x, vw[j].y);
-          *(th8*)(vs[buf] + key * VR + 16 * pc + 8) = int8_halves(vw[j].z, vw[j].w);
+          *(th8*)(ks[buf] + key * KR + 16 * pc) = int8_halves(st.kw[j].x, st.kw[j].y);
+          *(th8*)(ks[buf] + key * KR + 16 * pc + 8) = int8_halves(st.kw[j].z, st.kw[j].w);
+          *(th8*)(vs[buf] + key * VR + 16 * pc) = int8_halves(st.vw[j].x, st.vw[j].y);
+          *(th8*)(vs[buf] + key * VR + 16 * pc + 8) = int8_halves(st.vw[j].z, st.vw[j].w);
         } else {
-          *(tu4*)(ks[buf] + key * KR + 8 * pc) = kw[j];
-          *(tu4*)(vs[buf] + key * VR + 8 * pc) = vw[j];
+          *(tu4*)(ks[buf] + key * KR + 8 * pc) = st.kw[j];
+          *(tu4*)(vs[buf] + key * VR + 8 * pc) = st.vw[j];
         }
       }
       if constexpr (Q8) {
-        if (tid < 2 * SL) {  // (the values' factors are one wave's, or a half of it)
-          const uint32_t w[4] = {fw.x, fw.y, fw.z, fw.w};
 #pragma unroll
-          for (int u = 0; u < KS; u++) {
-            float f = fdead ? 0.0f : half_bits_to_float(w[u >> 1] >> (16 * (u & 1)));
-            if (tid >= SL) {
-              const float af = fabsf(f), fm = lanes::reduce<SL>(af < INFINITY ? af : 0.0f, lanes::Max{});
-              if (!nodes_in && fm > 0.0f) xrun[u] = max(xrun[u], __builtin_amdgcn_frexp_expf(fm));
-              f = ldexpf(f, 15 - xrun[u]);
-              if (tid == SL) xs[buf][u] = xrun[u];
-            }
-            fac[buf][tid / SL][u][tid % SL] = f;
+        for (int j = 0; j < FPER; j++) {
+          const int i = tid + 256 * j, u = i / SL % KS;
+          float f = half_bits_to_float(st.f[j]);
+          if (i >= SL * KS) {  // (uniform: the second half of the threads, or of a thread's factors)
+            const float af = fabsf(f), fm = lanes::reduce<SL>(af < INFINITY ? af : 0.0f, lanes::Max{});
+            if (!nodes_in && fm > 0.0f) xrun[j] = max(xrun[j], __builtin_amdgcn_frexp_expf(fm));
+            f = ldexpf(f, 15 - xrun[j]);
+            if (i % SL == 0) xs[buf][u] = xrun[j];
           }
+          fac[buf][i / (SL * KS)][u][i % SL] = f;
         }
       }
     };
 
-    find(s0);
-    load(s0);
-    if (s0 + 1 < s1) find(s0 + 1);
+    // the first two slices and the queries at once
+    find(s0, st);
+    Stage ahead;
+    if (s0 + 1 < s1) find(s0 + 1, ahead);
+    tf4 raw[NC][KS][2];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      const float* qr = a.q + (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * a.q_stride +
+                        (int64_t)(kvh * group + ((first_row + 16 * c + lm) & (group - 1))) * D + 8 * lk;
+#pragma unroll
+      for (int u = 0; u < KS; u++)
+#pragma unroll
+        for (int w = 0; w < 2; w++) raw[c][u][w] = *(const tf4*)(qr + 32 * u + 4 * w);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load(s0, st);
+    if (s0 + 1 < s1) {
+      load(s0 + 1, ahead);
+      if (s0 + 2 < s1) find(s0 + 2, ahead);
+    }
     __builtin_amdgcn_sched_barrier(0);
 
     // the queries as B fragments, each scaled by a power of two that c2 takes back
@@ -553,18 +603,13 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
     float c2[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-      const float* qr = a.q + (int64_t)(sq.t0 + min(node[c], sq.nodes - 1)) * a.q_stride +
-                        (int64_t)(kvh * group + (first_row + 16 * c + lm) % group) * D + 8 * lk;
-      tf4 raw[KS][2];
       float mx = 0.0f;
 #pragma unroll
       for (int u = 0; u < KS; u++)
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-          raw[u][w] = *(const tf4*)(qr + 32 * u + 4 * w);
+        for (int w = 0; w < 2; w++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(raw[u][w][e]));
-        }
+          for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(raw[c][u][w][e]));
       mx = across(mx, lanes::Max{});
       const int e2 = mx > 0.0f ? max(__builtin_amdgcn_frexp_expf(mx) - 15, -126) : 0;
       c2[c] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e2), 1e-38f);  // (never zero: a key that is not seen scores -inf)
@@ -573,7 +618,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
       for (int u = 0; u < KS; u++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const float f = raw[u][e >> 2][e & 3] * sc;
+          const float f = raw[c][u][e >> 2][e & 3] * sc;
           const _Float16 h = (_Float16)f;
           qf[0][c][u][e] = h;
           qf[1][c][u][e] = (_Float16)fmaf((float)h, -1.0f, f);
@@ -597,6 +642,9 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
     // a row's mk is too large for a weight's exponent; (uniform) some row's is
     auto large = [&](int c) __attribute__((always_inline)) { return mc[c] > -1e30f && !(fabsf(mk[c]) <= 4e6f); };
     bool huge = false;
+    constexpr float lift = Q8 ? 0.0f : kLift;
+    float one = 1.0f;
+    asm("" : "+s"(one));
 
     // the scores of keys 32 kt .. of a slice, and whether all its cells are held
     auto scores = [&](int sl, int kt, int buf, tf4 (&s)[NC][2], int& hole) __attribute__((always_inline)) {
@@ -605,40 +653,71 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
       // key fragments of as many products as there are registers for on their way
       // before the first (one at a time, the compiler's order, left each product
       // waiting for LDS)
-      constexpr int HG = KS <= 4 ? 2 : 1;
-      th8 k8[HG][KS];
+      if constexpr (Q8) {
+        // a group: the products of 16 keys over up to four 32-dim blocks, each with
+        // its keys' factors; the next group's fragments on their way (at D = 256 there
+        // are no registers for them)
+        constexpr int UG = KS < 4 ? KS : 4, G = 2 * KS / UG, AH = KS <= 4 ? 2 : 1;
+        th8 k8[AH][UG];
+        tf4 f[AH][UG];  // the factors of lane group lk's four keys
+        auto read = [&](int g) __attribute__((always_inline)) {
+          const int h = g * UG / KS, u0 = g * UG % KS;
 #pragma unroll
-      for (int h0 = 0; h0 < 2; h0 += HG) {
+          for (int u = 0; u < UG; u++) k8[g % AH][u] = *(const th8*)(kp + 16 * h * KR + 32 * (u0 + u));
 #pragma unroll
-        for (int h = 0; h < HG; h++)
+          for (int u = 0; u < UG; u++) f[g % AH][u] = *(const tf4*)&fac[buf][0][u0 + u][32 * kt + 16 * h + 4 * lk];
+        };
+        if (AH == 2) read(0);
 #pragma unroll
-          for (int u = 0; u < KS; u++) k8[h][u] = *(const th8*)(kp + 16 * (h0 + h) * KR + 32 * u);
+        for (int g = 0; g < G; g++) {
+          const int h = g * UG / KS, u0 = g * UG % KS;
+          if (g + AH - 1 < G) read(g + AH - 1);
+          __builtin_amdgcn_sched_barrier(0);
+          tf4 d[NC][UG];
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int u = 0; u < UG; u++)
+#pragma unroll
+              for (int c = 0; c < NC; c++)
+                d[c][u] = mfma16(k8[g % AH][u], qf[k][c][u0 + u], k ? d[c][u] : tf4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+          for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int u = 0; u < UG; u++)
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                s[c][h][i] = u0 + u ? fmaf(f[g % AH][u][i], d[c][u][i], s[c][h][i]) : f[g % AH][u][i] * d[c][u][i];
+        }
+      } else {
+        constexpr bool both = KS <= 4;
+        th8 k8[2][KS];
+        auto kread = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+          for (int u = 0; u < KS; u++) k8[h][u] = *(const th8*)(kp + 16 * h * KR + 32 * u);
+        };
+        kread(0);
+        if (both) kread(1);
         __builtin_amdgcn_sched_barrier(0);
+        constexpr int HG = both ? 2 : 1;
 #pragma unroll
-        for (int h = 0; h < HG; h++)
+        for (int h0 = 0; h0 < 2; h0 += HG) {
+          if (!both && h0) {
+            kread(1);
+            __builtin_amdgcn_sched_barrier(0);
+          }
 #pragma unroll
-          for (int c = 0; c < NC; c++) s[c][h0 + h] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
+          for (int h = h0; h < h0 + HG; h++)
 #pragma unroll
-        for (int u = 0; u < KS; u++) {
-          if constexpr (Q8) {
+            for (int c = 0; c < NC; c++) s[c][h] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int h = 0; h < HG; h++) {
-              const tf4 f = *(const tf4*)&fac[buf][0][u][32 * kt + 16 * (h0 + h) + 4 * lk];
-#pragma unroll
-              for (int c = 0; c < NC; c++) {
-                const tf4 d = mfma16(k8[h][u], qf[1][c][u], mfma16(k8[h][u], qf[0][c][u], tf4{0.0f, 0.0f, 0.0f, 0.0f}));
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[c][h0 + h][i] = fmaf(f[i], d[i], s[c][h0 + h][i]);
-              }
-            }
-          } else {
+          for (int u = 0; u < KS; u++)
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-              for (int h = 0; h < HG; h++)
+              for (int h = h0; h < h0 + HG; h++)
 #pragma unroll
-                for (int c = 0; c < NC; c++) s[c][h0 + h] = mfma16(k8[h][u], qf[k][c][u], s[c][h0 + h]);
-          }
+                for (int c = 0; c < NC; c++) s[c][h] = mfma16(k8[h][u], qf[k][c][u], s[c][h]);
         }
       }
       if (PAGED) hole = __builtin_amdgcn_readfirstlane(hole) - (first_turn + sl - s0);
@@ -673,7 +752,6 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
       }
       th8 ph[NC], pl[NC];
       float p[NC][8];
-      int xc[Q8 ? NC : 1];
 #pragma unroll
       for (int c = 0; c < NC; c++) {
         float m = s[c][0][0];
@@ -683,7 +761,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
         const float mn = fmaxf(mc[c], m);
         const bool rose = mn != mc[c];
         if (__any(rose)) {
-          const float mkn = rose ? mn * c2[c] : mk[c];
+          const float mkn = rose ? fmaf(mn, c2[c], -lift) : mk[c];
           const float f = __builtin_amdgcn_exp2f(large(c) ? (mc[c] - mn) * c2[c] : mk[c] - mkn);
           l[c] *= f;
 #pragma unroll
@@ -695,19 +773,13 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
         if (__builtin_expect(huge, 0)) {
 #pragma unroll
           for (int i = 0; i < 8; i++)
-            p[c][i] = __builtin_amdgcn_exp2f(large(c) ? (s[c][i >> 2][i & 3] - mc[c]) * c2[c] : fmaf(s[c][i >> 2][i & 3], c2[c], -mk[c]));
+            p[c][i] = __builtin_amdgcn_exp2f(large(c) ? fmaf(s[c][i >> 2][i & 3] - mc[c], c2[c], lift) : fmaf(s[c][i >> 2][i & 3], c2[c], -mk[c]));
         } else {
 #pragma unroll
           for (int i = 0; i < 8; i++) p[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i >> 2][i & 3], c2[c], -mk[c]));
         }
         l[c] += ((p[c][0] + p[c][1]) + (p[c][2] + p[c][3])) + ((p[c][4] + p[c][5]) + (p[c][6] + p[c][7]));
-        if constexpr (!Q8) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            ph[c][i] = (_Float16)fmaf(p[c][i], kLift, 0.0f);  // (one instruction)
-            pl[c][i] = (_Float16)fmaf(p[c][i], kLift, -(float)ph[c][i]);
-          }
-        }
+        if constexpr (!Q8) split(p[c], one, ph[c], pl[c]);
       }
       if constexpr (Q8) {  // (uniform) X has risen with this slice's factors
 #pragma unroll
@@ -721,72 +793,94 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
           }
         }
       }
-#pragma unroll
-      for (int dt = 0; dt < NT; dt++) {
-        if constexpr (Q8) {
-          if (dt % 2 == 0) {
-            const int u = dt / 2;
-            const tf4 f0 = *(const tf4*)&fac[buf][1][u][32 * kt + 4 * lk], f1 = *(const tf4*)&fac[buf][1][u][32 * kt + 16 + 4 * lk];
-#pragma unroll
-            for (int c = 0; c < NC; c++) {
-              if (all) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                  const float f = i < 4 ? f0[i & 3] : f1[i & 3];
-                  ph[c][i] = (_Float16)fmaf(p[c][i], f, 0.0f);
-                  pl[c][i] = (_Float16)fmaf(p[c][i], f, -(float)ph[c][i]);
-                }
-                continue;
-              }
-              // (whatever the factor of a key that is not seen)
-              float w[8], wm = 0.0f;
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                w[i] = (mine[c] >> ((i & 3) + 16 * (i >> 2))) & 1 ? p[c][i] * (i < 4 ? f0[i & 3] : f1[i & 3]) : 0.0f;
-                wm = fmaxf(wm, fabsf(w[i]));
-              }
-              wm = across(wm, lanes::Max{});
-              xc[c] = wm > 0.0f && wm < INFINITY ? __builtin_amdgcn_frexp_expf(wm) : 0;
-              const float unit = ldexpf(1.0f, 15 - xc[c]);
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                ph[c][i] = (_Float16)fmaf(w[i], unit, 0.0f);
-                pl[c][i] = (_Float16)fmaf(w[i], unit, -(float)ph[c][i]);
-              }
-            }
-          }
-        }
-        if (dt % VG == 0) {
-          if (dt + VG < NT) vread(dt / VG + 1);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+      // value fragments of group dt / VG, the next group's on their way
+      auto vtile = [&](int dt) __attribute__((always_inline)) {
         ts8 v;
 #pragma unroll
         for (int w = 0; w < 2; w++)
 #pragma unroll
           for (int e = 0; e < 4; e++) v[4 * w + e] = v4[(dt / VG) & 1][dt % VG][w][e];
-        if (!Q8 || all) {
+        return __builtin_bit_cast(th8, v);
+      };
+      if constexpr (Q8) {
+        static_assert(VG == 2, "a group is a 32-dim block");
+        tf4 f[2][2];  // a block's factors, the next one's on their way
+        auto fread = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
-          for (int c = 0; c < NC; c++) o[c][dt] = mfma16(__builtin_bit_cast(th8, v), ph[c], o[c][dt]);
+          for (int w = 0; w < 2; w++) f[u & 1][w] = *(const tf4*)&fac[buf][1][u][32 * kt + 16 * w + 4 * lk];
+        };
+        fread(0);
+        if (all) {
 #pragma unroll
-          for (int c = 0; c < NC; c++) o[c][dt] = mfma16(__builtin_bit_cast(th8, v), pl[c], o[c][dt]);
+          for (int u = 0; u < KS; u++) {
+            if (u + 1 < KS) {
+              vread(u + 1);
+              fread(u + 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                ph[c][i] = (_Float16)fmaf(p[c][i], f[u & 1][i >> 2][i & 3], 0.0f);
+                pl[c][i] = (_Float16)fmaf(p[c][i], f[u & 1][i >> 2][i & 3], -(float)ph[c][i]);
+              }
+#pragma unroll
+              for (int dt = 2 * u; dt < 2 * u + 2; dt++) o[c][dt] = mfma16(vtile(dt), ph[c], o[c][dt]);
+#pragma unroll
+              for (int dt = 2 * u; dt < 2 * u + 2; dt++) o[c][dt] = mfma16(vtile(dt), pl[c], o[c][dt]);
+            }
+          }
         } else {
 #pragma unroll
-          for (int c = 0; c < NC; c++) {
-            const tf4 t = mfma16(__builtin_bit_cast(th8, v), pl[c], mfma16(__builtin_bit_cast(th8, v), ph[c], tf4{0.0f, 0.0f, 0.0f, 0.0f}));
-            const float f = ldexpf(1.0f, xc[c] - 15);
+          for (int u = 0; u < KS; u++) {
+            if (u) {
+              vread(u);
+              fread(u);
+            }
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[c][dt][e] = fmaf(t[e], f, o[c][dt][e]);
+            for (int c = 0; c < NC; c++) {
+              // (whatever the factor of a key that is not seen)
+              float w[8], wm = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                w[i] = (mine[c] >> ((i & 3) + 16 * (i >> 2))) & 1 ? p[c][i] * f[u & 1][i >> 2][i & 3] : 0.0f;
+                wm = fmaxf(wm, fabsf(w[i]));
+              }
+              wm = across(wm, lanes::Max{});
+              const int xc = wm > 0.0f && wm < INFINITY ? __builtin_amdgcn_frexp_expf(wm) : 0;
+              const float unit = ldexpf(1.0f, 15 - xc), back = ldexpf(1.0f, xc - 15);
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                ph[c][i] = (_Float16)fmaf(w[i], unit, 0.0f);
+                pl[c][i] = (_Float16)fmaf(w[i], unit, -(float)ph[c][i]);
+              }
+#pragma unroll
+              for (int dt = 2 * u; dt < 2 * u + 2; dt++) {
+                const tf4 t = mfma16(vtile(dt), pl[c], mfma16(vtile(dt), ph[c], tf4{0.0f, 0.0f, 0.0f, 0.0f}));
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[c][dt][e] = fmaf(t[e], back, o[c][dt][e]);
+              }
+            }
           }
+        }
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < NT; dt++) {
+          if (dt % VG == 0) {
+            if (dt + VG < NT) vread(dt / VG + 1);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int c = 0; c < NC; c++) o[c][dt] = mfma16(vtile(dt), ph[c], o[c][dt]);
+#pragma unroll
+          for (int c = 0; c < NC; c++) o[c][dt] = mfma16(vtile(dt), pl[c], o[c][dt]);
         }
       }
     };
 
-    store(s0, 0);
-    if (s0 + 1 < s1) {
-      load(s0 + 1);
-      if (s0 + 2 < s1) find(s0 + 2);
-    }
+    store(s0, 0, st);
+    if (s0 + 1 < s1) st = ahead;
     __syncthreads();
     for (int sl = s0, buf = 0; sl < s1; sl++, buf ^= 1) {
       tf4 s[NC][2];
@@ -797,10 +891,10 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
       // registers differ, and the busy ones wait for loads at every step)
       __builtin_amdgcn_sched_barrier(0);
       if (sl + 1 < s1) {
-        store(sl + 1, buf ^ 1);
+        store(sl + 1, buf ^ 1, st);
         if (sl + 2 < s1) {
-          load(sl + 2);
-          if (sl + 3 < s1) find(sl + 3);
+          load(sl + 2, st);
+          if (sl + 3 < s1) find(sl + 3, st);
         }
       }
       if (busy) {
@@ -842,9 +936,9 @@ __global__ __launch_bounds__(256, mfma_blocks(D, NC, Q8)) void attend_tree_kerne
       const float sum = across(l[c], lanes::Add{});
       if (node[c] >= sq.nodes) continue;
       const int64_t slot = (int64_t)part * ROWS + wave * 16 * NC + 16 * c + lm;
-      float* dst = part < 0 ? a.out + ((int64_t)(sq.t0 + node[c]) * a.heads + kvh * group + (first_row + 16 * c + lm) % group) * D
+      float* dst = part < 0 ? a.out + ((int64_t)(sq.t0 + node[c]) * a.heads + kvh * group + ((first_row + 16 * c + lm) & (group - 1))) * D
                             : parts.acc + slot * D;
-      const float w = (part >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f) * (Q8 ? 1.0f : 1.0f / kLift);
+      const float w = part >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
       for (int dt = 0; dt < NT; dt++) {
         const float f = Q8 ? w * ldexpf(1.0f, xo[dt / 2] - 15) : w;
@@ -864,16 +958,16 @@ __global__ __launch_bounds__(256) void attend_tree_fold_kernel(TreeAttend a, Tre
   typedef float vec __attribute__((ext_vector_type(V)));
   __shared__ vec sums[W > 1 ? W : 1][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int D = a.head_dim, group = a.heads / a.kv_heads;
-  const int64_t i = (int64_t)blockIdx.x * (4 / W) + wave / W;
-  const int b = (int)(i / ((int64_t)a.tree.max_nodes * a.heads));
+  const int D = a.head_dim, shift = a.group_shift;
+  const uint32_t i = blockIdx.x * (4 / W) + wave / W, step = (uint32_t)a.tree.max_nodes * a.heads;  // (both below 2^31)
+  const int b = (int)(i / step);
   if (b >= a.tree.batch) return;  // (W > 1: every wave of the block)
-  const int at = (int)(i - (int64_t)b * a.tree.max_nodes * a.heads), node = at / a.heads, h = at - node * a.heads;
+  const int at = (int)(i - b * step), node = at / a.heads, h = at - node * a.heads;
   const int per = plan[0], b_first = plan[1 + b];
   const TreeSeq sq = tree_seq(a.tree, b);
   if (node >= sq.nodes) return;
-  const int kvh = h / group, r = node * group + h % group, tile = r / rows, slices = tree_slices(sq, slice);
-  const int u0 = b_first + (kvh * tree_tiles(sq, group, rows) + tile) * slices;
+  const int kvh = h >> shift, r = (node << shift) + (h & ((1 << shift) - 1)), tile = r / rows, slices = tree_slices(sq, slice);
+  const int u0 = b_first + (kvh * tree_tiles(sq, shift, rows) + tile) * tree_units(sq, slice) + kStart;
   const int g0 = u0 / per, n = (u0 + slices - 1) / per - g0 + 1;
   if (n == 1) return;  // one block's: finished
   // part k is block g0 + k's: its last one (1) for the block that the tile starts in, else its first (0)
@@ -938,12 +1032,16 @@ TreeGrid tree_grid(int heads, int kv_heads, int head_dim, int form, const mi_tre
   TreeGrid g;
   const int group = heads / kv_heads;
   g.mfma = head_dim == 64 || head_dim == 128 || head_dim == 256;
+  // two columns a lane read each key fragment once for twice the rows, but only
+  // where a sequence has more rows than one column's 64: 8 x 32 nodes at D = 128 74
+  // us with two and 89 with one, 8 x 16 62 and 50, 1 x 13 47 and 37 (at D = 64 the
+  // registers cost the third block, with q8_0 they spill)
   g.columns = head_dim == 128 && form != MI_CACHE_Q8 && t.max_nodes * group > 64 ? 2 : 1;
   g.rows = g.mfma ? 64 * g.columns : kRowsTile;
   g.slice = g.mfma ? mfma_slice(head_dim) : rows_slice(head_dim);
   g.units = (int64_t)t.batch * ((t.max_nodes * group + g.rows - 1) / g.rows) * kv_heads *
-            (((int64_t)t.max_count + g.slice - 1) / g.slice);
-  g.blocks = (int)std::min<int64_t>(g.units, (int64_t)cu_count() * (g.mfma ? mfma_blocks(head_dim, g.columns, form == MI_CACHE_Q8) : 3));
+            (((int64_t)t.max_count + g.slice - 1) / g.slice + kStart);
+  g.blocks = (int)std::min<int64_t>(g.units, (int64_t)cu_count() * (g.mfma ? mfma_blocks(head_dim) : 3));
   return g;
 }
 
@@ -967,13 +1065,16 @@ size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, 
   return tree_carve(tree_grid(heads, kv_heads, head_dim, form, t), head_dim, t.batch).total;
 }
 
-int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work) {
+int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
+  TreeAttend a = step;
+  a.group_shift = __builtin_ctz(a.heads / a.kv_heads);  // (1, 2, 4 or 8 query heads a key head)
   const TreeGrid g = tree_grid(a.heads, a.kv_heads, a.head_dim, a.form, a.tree);
-  // few rows: four waves each (416 rows of 62 parts 8.4 -> XX us)
+  // few rows: four waves each (416 rows of 62 parts 8.5 us with one, 5.6 with four;
+  // 3200 of 10 5.8 and 12.2)
   const int64_t rows = (int64_t)a.tree.batch * a.tree.max_nodes * a.heads;
   const int waves = rows <= 1024 ? 4 : 1;
-  const int64_t fold = (rows * waves + 3) / 4;
-  if (g.units > 0x7fffffff || fold > 0x7fffffff)
+  const uint32_t fold = (uint32_t)((rows * waves + 3) / 4);
+  if (g.units > 0x7fffffff || rows > 0x7ffffff0)
     return fail(MI_ERR_SHAPE, "attend_tree: %d sequences of %d nodes and %d positions are too much work", a.tree.batch,
                 a.tree.max_nodes, a.tree.max_count);
   const TreeCarve c = tree_carve(g, a.head_dim, a.tree.batch);
@@ -1020,10 +1121,10 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work) {
   if (int rc = hip_check(hipGetLastError(), "attend_tree launch")) return rc;
 #define MI_TREE_FOLD(V)                                                                                            \
   if (waves == 4)                                                                                                  \
-    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 4>), dim3((uint32_t)fold), dim3(256), 0, s, a, parts, plan, g.rows, \
+    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 4>), dim3(fold), dim3(256), 0, s, a, parts, plan, g.rows, \
                        g.slice);                                                                                   \
   else                                                                                                             \
-    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 1>), dim3((uint32_t)fold), dim3(256), 0, s, a, parts, plan, g.rows, \
+    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 1>), dim3(fold), dim3(256), 0, s, a, parts, plan, g.rows, \
                        g.slice)
   if (a.head_dim % 256 == 0) MI_TREE_FOLD(4);
   else if (a.head_dim % 128 == 0) MI_TREE_FOLD(2);
