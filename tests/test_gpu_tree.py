@@ -387,8 +387,8 @@ class Step:
     def want(self):
         out = torch.full((self.tokens, self.heads * self.d), -3.0, dtype=torch.float64)
         t = 0
+        k, v = self.values(self.k), self.values(self.v)
         for b, (n, m) in enumerate(zip(self.lens, self.counts)):
-            k, v = self.values(self.k), self.values(self.v)
             for _ in range(m):
                 slots = list(range(n)) + [n + i for i in sorted(self.seen[t])]
                 rows = [int(self.index[b, j]) for j in slots if int(self.index[b, j]) >= 0]
@@ -539,6 +539,105 @@ def test_attend_scales(form, d, nodes):
     s.q[0] *= 1e-6
     s.q[1] = 0
     s.check(s.run())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d,nodes", [(64, 3), (128, 40), (96, 5), (256, 2)])
+def test_attend_without_a_scale(form, d, nodes):
+    """Every key weighs the same."""
+    s = Step(form, [50, 0], [nodes, 1], 2, 1, d)
+    s.scale = 0.0
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d,nodes", [(64, 4), (128, 4), (128, 70), (256, 4), (96, 4)])
+def test_attend_scores_past_an_exponent(form, d, nodes):
+    """One query whose scores are near 1e8, where a weight's exponent has no
+    fraction left: the key it points at takes all of it, the other queries are as
+    without it."""
+    s = Step(form, [700], [nodes], 1, 1, d)
+    s.k[333] = encode(torch.full((1, d), 4.0), form)[0]
+    plain = s.run()
+    s.check(plain)
+    s.q[2] = 1e7
+    got = s.run()
+    others = [t for t in range(nodes) if t != 2]
+    assert torch.equal(got[others], plain[others])
+    assert (got[2].double() - s.values(s.v)[333]).abs().max() <= 1e-5 * float(s.values(s.v).abs().max())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d,nodes", [(64, 5), (128, 5), (128, 70), (256, 5), (96, 5)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attend_of_a_query_that_is_not_finite(form, d, nodes, bad):
+    s = Step(form, [90], [nodes], 2, 1, d)
+    clean = s.run()
+    s.q[1, d + 3] = bad  # (token 1, head 1)
+    got = s.run()
+    assert torch.isnan(got[1, d:]).all() and torch.equal(got[1, :d], clean[1, :d])
+    others = [t for t in range(s.tokens) if t != 1]
+    assert torch.equal(got[others], clean[others])
+
+
+@pytest.mark.parametrize("form,heads,kv,d", [("f16", 2, 1, 64), ("q8", 2, 1, 128), ("f16", 4, 2, 128), ("f16", 2, 2, 96), ("q8", 1, 1, 256)])
+@pytest.mark.parametrize("batch", [64, 65, 200])
+def test_attend_many_sequences(form, heads, kv, d, batch):
+    """More sequences than a wave has lanes; some without nodes, some without a context."""
+    rng = np.random.default_rng(batch)
+    lens, counts = rng.integers(0, 70, batch), rng.integers(0, 4, batch)
+    lens[::7], counts[3::5], counts[-1] = 0, 0, 2
+    s = Step(form, lens.tolist(), counts.tolist(), heads, kv, d, paged=True)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("only", [0, 63, 64, 150, 299])
+def test_attend_one_of_many(form, only):
+    counts = [0] * 300
+    counts[only] = 7
+    s = Step(form, [20] * only + [900] + [20] * (299 - only), counts, 2, 1, 64)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("d", [128, 96])
+def test_cache_past_32_bits(form, paged, d):
+    """Cache rows whose offsets pass 2^31 halves and 2^32 bytes, stored and attended."""
+    ctx = gpu.DeviceContext(0)
+    row = gpu.cache_row(FORMS[form], d)
+    cells = (1 << 31) // row + 2000
+    pool = [torch.empty(cells, row, dtype=torch.float16, device="cuda") for _ in range(2)]
+    s = Step(form, [70, 40], [5, 6], 2, 1, d, paged=True)
+    base = [cells - s.room, 5] if paged else [0, cells - s.room]
+    for b in range(2):
+        at = s.index[b].long()
+        pool[0][base[b]:base[b] + s.room] = s.k[at].cuda()
+        pool[1][base[b]:base[b] + s.room] = s.v[at].cuda()
+    index = torch.stack([torch.arange(s.room) + base[b] for b in range(2)]).to(torch.int32).cuda()
+    # the last node's key and value of both sequences by the store
+    tokens = torch.randn(2, 4 * d, generator=torch.Generator().manual_seed(3)).cuda()
+    last = [n + m - 1 for n, m in zip(s.lens, s.counts)]
+    to = ints([int(index[b, last[b]]) for b in range(2)])
+    steps = torch.from_numpy(gpu.rope_steps(d, 10000.0)).cuda()
+    gpu.device_qk_norm_rope(ctx, tokens[:, :2 * d], tokens[:, 2 * d:3 * d], tokens[:, 3 * d:], 2, 1, d, d, False, steps, ints([0, 0]),
+                            torch.empty(2, 2 * d, device="cuda"), pool[0], pool[1], to, FORMS[form])
+    ctx.synchronize()
+    for b in range(2):
+        cell = int(s.index[b, last[b]])
+        for c, have, part in ((s.k, pool[0], tokens[b, 2 * d:3 * d]), (s.v, pool[1], tokens[b, 3 * d:])):
+            c[cell] = encode(part.cpu()[None], form)[0]
+            used = d if form == "f16" else d // 2 + d // 32
+            assert torch.equal(have[int(to[b])][:used].cpu().view(torch.int16), c[cell][:used].view(torch.int16))
+    words = gpu.tree_words(s.max_nodes)
+    mask = ints(np.concatenate([words_of(s.seen, words), np.full((s.tokens - len(s.seen), words), -1, np.int32)]))
+    out = torch.full((s.tokens, 2 * d), -3.0, device="cuda")
+    gpu.device_attend_tree(ctx, s.q.cuda(), pool[0], pool[1], 2, 1, d, s.scale, starts_of(s.counts), ints(s.lens), mask, s.max_nodes,
+                           s.max_count, out, cache_stride=0 if paged else base[1] * row, kv_index=index if paged else None,
+                           form=FORMS[form])
+    ctx.synchronize()
+    s.check(out.cpu())
 
 
 def test_attend_workspace_contents():
