@@ -17,10 +17,11 @@
 // 64 nodes over 8192 down to 4608 positions at width 128 132 + 12.7 us (292
 // TFLOP/s of the formula's products, twice that of the matrix cores', whose steps
 // take turns with the softmax on the VALU at two waves a SIMD); 8 x 48 over 3000
-// down to 1688 at width 64 30 + 9.4 (bound by the VALU); 1 x 13 over 32768 36.6 +
-// 5.6 (3.7 TB/s; 6 once the first slices are there); 4 x 25 over 4099 of q8_0 42.7
-// + 5.8 (a value block's factor makes halves of the weights anew); 1 x 8 over 2048
-// 11.5 + 4.1 (launches and the first loads' latency).
+// down to 1688 at width 64 29.9 + 9.3 (bound by a step's chain of latencies at three
+// waves a SIMD); 1 x 13 over 32768 36.6 + 5.6 (3.7 TB/s; 6 once the first slices are
+// there); 4 x 25 over 4099 of q8_0 41.8 + 5.7 (a value block's factor makes halves
+// of the weights anew); 1 x 8 over 2048 11.5 + 4.1 (launches and the first loads'
+// latency).
 #include <math.h>
 
 #include <algorithm>
@@ -53,7 +54,7 @@ __device__ __forceinline__ int tree_tiles(const TreeSeq& s, int shift, int rows)
 __device__ __forceinline__ int tree_slices(const TreeSeq& s, int slice) { return (s.count + slice - 1) / slice; }
 // A tile's units: its slices behind kStart that stand for the start of a run in it
 // (queries, first loads), so that a block with two starts gets less of the rest: 1 x
-// 13 over 32768 39.2 us at 0, 36.6 at 3, 39.8 at 6; 4 x 25 of q8_0 46.4, 42.7, 45.9.
+// 13 over 32768 39.2 us at 0, 36.6 at 3, 39.8 at 6; 4 x 25 of q8_0 46.4, 42.7, 45.9 (at the time).
 constexpr int kStart = 3;
 __device__ __forceinline__ int tree_units(const TreeSeq& s, int slice) { return kStart + tree_slices(s, slice); }
 
@@ -332,8 +333,8 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 //
 // q8_0: keys and values enter as their integers, exact halves; a key block's
 // factor multiplies its part of the score, a value block's the weights, which
-// are then split into halves (the factors' share of 4 x 25 over 4099: 43 us against
-// 30 of f16).  The factors are staged times 2^(15 - X), X the
+// are then split into halves (the factors' share of 4 x 25 over 4099: 42 us against
+// 30 of f16; at D = 256 107 against 48, where they do not fit the registers).  The factors are staged times 2^(15 - X), X the
 // exponent of the largest one so far among committed positions, which every row
 // sees; slices that some row does not see whole leave X as it is, and there each
 // row's products are scaled to its own largest and summed apart: what a row does
@@ -350,22 +351,28 @@ typedef _Float16 th2 __attribute__((ext_vector_type(2)));
 typedef _Float16 th8 __attribute__((ext_vector_type(8)));
 typedef short ts4 __attribute__((ext_vector_type(4)));
 typedef short ts8 __attribute__((ext_vector_type(8)));
+typedef float tf2 __attribute__((ext_vector_type(2)));
 typedef float tf4 __attribute__((ext_vector_type(4)));
 typedef uint32_t tu4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLift = 14.0f;
 
-// w as two halves, pairs of them at a time (one: 1 in a scalar register, so that
-// the difference is one instruction that also rounds it)
-__device__ __forceinline__ void split(const float (&w)[8], float one, th8& hi, th8& lo) {
-  typedef float tf2 __attribute__((ext_vector_type(2)));
+// w f as two halves (ONE: f is 1, in a scalar register that the compiler takes for
+// any value): an instruction each or less, the higher halves opaque so that the
+// lower ones are taken from them where they lie in their pair
+template <bool ONE, class F>
+__device__ __forceinline__ void split(const float (&w)[8], F f, th8& hi, th8& lo) {
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const th2 h = __builtin_convertvector((tf2{w[i], w[i + 1]}), th2);
+    th2 h;
+    if constexpr (ONE) h = __builtin_convertvector((tf2{w[i], w[i + 1]}), th2);
+    else h = th2{(_Float16)fmaf(w[i], f(i), 0.0f), (_Float16)fmaf(w[i + 1], f(i + 1), 0.0f)};
+    asm("" : "+v"(h));
+    const th2 l = {(_Float16)fmaf(w[i], f(i), -(float)h[0]), (_Float16)fmaf(w[i + 1], f(i + 1), -(float)h[1])};
     hi[i] = h[0];
     hi[i + 1] = h[1];
-    lo[i] = (_Float16)fmaf(w[i], one, -(float)h[0]);
-    lo[i + 1] = (_Float16)fmaf(w[i + 1], one, -(float)h[1]);
+    lo[i] = l[0];
+    lo[i + 1] = l[1];
   }
 }
 
@@ -779,7 +786,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
           for (int i = 0; i < 8; i++) p[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i >> 2][i & 3], c2[c], -mk[c]));
         }
         l[c] += ((p[c][0] + p[c][1]) + (p[c][2] + p[c][3])) + ((p[c][4] + p[c][5]) + (p[c][6] + p[c][7]));
-        if constexpr (!Q8) split(p[c], one, ph[c], pl[c]);
+        if constexpr (!Q8) split<true>(p[c], [&](int) __attribute__((always_inline)) { return one; }, ph[c], pl[c]);
       }
       if constexpr (Q8) {  // (uniform) X has risen with this slice's factors
 #pragma unroll
@@ -820,11 +827,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                ph[c][i] = (_Float16)fmaf(p[c][i], f[u & 1][i >> 2][i & 3], 0.0f);
-                pl[c][i] = (_Float16)fmaf(p[c][i], f[u & 1][i >> 2][i & 3], -(float)ph[c][i]);
-              }
+              split<false>(p[c], [&](int i) __attribute__((always_inline)) { return f[u & 1][i >> 2][i & 3]; }, ph[c], pl[c]);
 #pragma unroll
               for (int dt = 2 * u; dt < 2 * u + 2; dt++) o[c][dt] = mfma16(vtile(dt), ph[c], o[c][dt]);
 #pragma unroll
@@ -883,9 +886,12 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
     if (s0 + 1 < s1) st = ahead;
     __syncthreads();
     for (int sl = s0, buf = 0; sl < s1; sl++, buf ^= 1) {
-      tf4 s[NC][2];
+      tf4 s[SL / 32][NC][2];
       int hole = 1;
-      if (busy) scores(sl, 0, buf, s, hole);
+      if (busy) {
+        scores(sl, 0, buf, s[0], hole);
+        if constexpr (SL > 32) scores(sl, 1, buf, s[1], hole);
+      }
       // the next slice from registers to the other buffer, and the one behind it on
       // its way (written once for busy and idle waves: with a copy for each the
       // registers differ, and the busy ones wait for loads at every step)
@@ -898,12 +904,9 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
         }
       }
       if (busy) {
-        values(sl, 0, buf, s, hole);
+        values(sl, 0, buf, s[0], hole);
         if constexpr (SL > 32) {
-          if (sl * SL + 32 < sq.count) {
-            scores(sl, 1, buf, s, hole);
-            values(sl, 1, buf, s, hole);
-          }
+          if (sl * SL + 32 < sq.count) values(sl, 1, buf, s[1], hole);
         }
       }
       __syncthreads();
