@@ -8,11 +8,9 @@
 namespace mi {
 namespace {
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanPer = kMaxPlanBatch / kPlanThreads;  // requests a thread scans
-
-// Inclusive sum over a block of 1024, each partial sum at most `most` (with
-// values at least 0 the capped sum is associative); wsum: 16 ints of LDS.
+// Inclusive sum over a block of T threads, each partial sum at most `most` (with
+// values at least 0 the capped sum is associative); wsum: an int a wave, of LDS.
+template <int T>
 __device__ __forceinline__ int scan_block(int v, int most, int* wsum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -24,22 +22,27 @@ __device__ __forceinline__ int scan_block(int v, int most, int* wsum) {
   if (lane == 63) wsum[wave] = v;
   __syncthreads();
   int before = 0;
-  for (int w = 0; w < wave; w++) before = min(before + wsum[w], most);
+#pragma unroll
+  for (int w = 0; w < T / 64 - 1; w++) before = min(before + (w < wave ? wsum[w] : 0), most);
   return min(before + v, most);
 }
 
-// Every block scans all requests (at most 4096, four a thread, from the cache)
+// Every block of T threads scans all requests (at most T * PER, from the cache)
 // and then fills its share of the token rows: no second launch, and nothing
 // between blocks.  A position that is a multiple of the page opens a new page:
-// pages a request holds are full up to its length, but for the last one.
-__global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PagePlan p) {
-  __shared__ int start[kMaxPlanBatch + 1];   // of each request's new tokens
-  __shared__ int before[kMaxPlanBatch + 1];  // new pages of the requests ahead
-  __shared__ int wsum[kPlanThreads / 64];
-  const int tid = threadIdx.x, b0 = tid * kPlanPer;
-  int len[kPlanPer], n[kPlanPer], sum = 0;
+// pages a request holds are full up to its length, but for the last one.  (All
+// positions are below 2^32: a length and a row of tokens are below 2^31.)
+template <int T, int PER>
+__global__ __launch_bounds__(T) void page_plan_kernel(PagePlan p) {
+  __shared__ int start[T * PER + 1];   // of each request's new tokens
+  __shared__ int before[T * PER + 1];  // new pages of the requests ahead
+  __shared__ int wsum[T / 64];
+  const int tid = threadIdx.x, b0 = tid * PER;
+  const uint32_t page = p.page, cap = (uint32_t)min<int64_t>(p.max_pos, 0xffffffff);  // positions there is room for
+  auto pages_of = [&](uint32_t n) { return min(n, cap) / page + (min(n, cap) % page != 0); };
+  int len[PER], n[PER], sum = 0;
 #pragma unroll
-  for (int i = 0; i < kPlanPer; i++) {
+  for (int i = 0; i < PER; i++) {
     const bool live = b0 + i < p.batch;
     len[i] = live ? max(p.lengths[b0 + i], 0) : 0;
     n[i] = live ? min(max(p.news[b0 + i], 0), p.max_tokens) : 0;
@@ -47,48 +50,45 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PagePlan p) {
   }
   const int free0 = min(max(p.free_count[0], 0), p.free_size);
   // token rows: what does not fit into max_tokens is not planned
-  int at = scan_block(sum, p.max_tokens, wsum);
+  int at = scan_block<T>(sum, p.max_tokens, wsum);
   {
     // (the capped total cannot be taken back: the exclusive sum again from the left)
     const int up = __shfl_up(at, 1);
-    __shared__ int last[kPlanThreads / 64];
+    __shared__ int last[T / 64];
     if ((tid & 63) == 63) last[tid >> 6] = at;
     __syncthreads();
     at = (tid & 63) ? up : (tid ? last[(tid >> 6) - 1] : 0);
   }
-  int grow[kPlanPer], pages = 0;
+  int grow[PER], pages = 0;
 #pragma unroll
-  for (int i = 0; i < kPlanPer; i++) {
-    const int end = min(at + n[i], p.max_tokens);
-    const int64_t cap = p.max_pos;  // positions the table and the list have room for
-    const int64_t have = (min<int64_t>(len[i], cap) + p.page - 1) / p.page;
-    const int64_t need = (min<int64_t>((int64_t)len[i] + (end - at), cap) + p.page - 1) / p.page;
+  for (int i = 0; i < PER; i++) {
+    const int end = (int)min((uint32_t)at + n[i], (uint32_t)p.max_tokens);
     start[b0 + i] = at;
-    grow[i] = (int)(need - have);
+    grow[i] = (int)(pages_of((uint32_t)len[i] + (end - at)) - pages_of(len[i]));
     pages += grow[i];
     at = end;
   }
-  if (tid == kPlanThreads - 1) start[kMaxPlanBatch] = at;
+  if (tid == T - 1) start[T * PER] = at;
   // (a new page holds at least one new token, so their sum is below 2^31 too)
-  const int upto = scan_block(pages, 0x7fffffff, wsum);
+  const int upto = scan_block<T>(pages, 0x7fffffff, wsum);
   int ahead = upto - pages;
 #pragma unroll
-  for (int i = 0; i < kPlanPer; i++) {
+  for (int i = 0; i < PER; i++) {
     before[b0 + i] = ahead;
     ahead += grow[i];
   }
-  if (tid == kPlanThreads - 1) before[kMaxPlanBatch] = ahead;
+  if (tid == T - 1) before[T * PER] = ahead;
   __syncthreads();
-  const int total = start[kMaxPlanBatch];
+  const int total = start[T * PER];
   if (blockIdx.x == 0) {
-    for (int b = tid; b <= p.batch; b += kPlanThreads) p.starts[b] = b < p.batch ? start[b] : total;
+    for (int b = tid; b <= p.batch; b += T) p.starts[b] = b < p.batch ? start[b] : total;
     if (tid == 0) {
-      const int want = before[kMaxPlanBatch];
+      const int want = before[T * PER];
       p.free_left[0] = max(free0 - want, 0);
       p.free_left[1] = max(want - free0, 0);
     }
   }
-  for (int64_t t64 = (int64_t)blockIdx.x * kPlanThreads + tid; t64 < total; t64 += (int64_t)gridDim.x * kPlanThreads) {
+  for (int64_t t64 = (int64_t)blockIdx.x * T + tid; t64 < total; t64 += (int64_t)gridDim.x * T) {
     const int t = (int)t64;
     int lo = 0, hi = p.batch;  // the last request that starts at or ahead of t
     while (hi - lo > 1) {
@@ -96,26 +96,25 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PagePlan p) {
       if (start[mid] <= t) lo = mid;
       else hi = mid;
     }
-    const int64_t held = max(p.lengths[lo], 0);
-    const int64_t pos = held + (t - start[lo]);
+    const uint32_t held = max(p.lengths[lo], 0), pos = held + (t - start[lo]);
     int cell = -1;
-    if (pos < p.max_pos) {
-      const int64_t col = pos / p.page, off = pos - col * p.page, have = (held + p.page - 1) / p.page;
-      int32_t* entry = p.table + lo * p.table_stride + col;
-      int page;
+    if (pos < cap) {
+      const uint32_t col = pos / page, off = pos - col * page, have = held / page + (held % page != 0);
+      int32_t* entry = p.table + (int64_t)lo * p.table_stride + col;
+      int got;
       if (col < have) {
-        page = *entry;
+        got = *entry;
       } else {
         const int take = free0 - 1 - (before[lo] + (int)(col - have));
-        page = take >= 0 ? p.free_pages[take] : -1;
-        if (off == 0) *entry = page;
+        got = take >= 0 ? p.free_pages[take] : -1;
+        if (off == 0) *entry = got;
       }
-      const int64_t c = (int64_t)page * p.page + off;
-      if (page >= 0 && c <= 0x7fffffff) cell = (int)c;
+      const int64_t c = (int64_t)got * page + off;
+      if (got >= 0 && c <= 0x7fffffff) cell = (int)c;
       if (p.kv_index) p.kv_index[lo * p.index_stride + pos] = cell;
     }
     if (p.seq) p.seq[t] = lo;
-    if (p.pos) p.pos[t] = (int)min<int64_t>(pos, 0x7fffffff);
+    if (p.pos) p.pos[t] = (int)min(pos, 0x7fffffffu);
     p.cells[t] = cell;
   }
 }
@@ -180,10 +179,16 @@ __global__ __launch_bounds__(kMaxTreeNodes) void tree_plan_kernel(const int32_t*
 }  // namespace
 
 int launch_page_plan(hipStream_t s, const PagePlan& p) {
-  // a block for each 4096 token rows, at most one a compute unit
-  const int64_t want = ((int64_t)p.max_tokens + 4 * kPlanThreads - 1) / (4 * kPlanThreads);
-  const int blocks = (int)(want < cu_count() ? want : cu_count());
-  hipLaunchKernelGGL(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), 0, s, p);
+  // up to 256 requests: one a thread of four waves, whose scan is short (64 requests
+  // of a token 3.6 us, 5.7 with the larger block; 200 prompts of 282000 tokens 6.2 and
+  // 8.8); a block for each T token rows, at most four (or one) a compute unit (for
+  // each 4 T of them the 200 prompts take 7.4)
+  const bool few = p.batch <= 256;
+  const int T = few ? 256 : 1024;
+  const int64_t want = ((int64_t)p.max_tokens + T - 1) / T, most = (int64_t)cu_count() * (few ? 4 : 1);
+  const int blocks = (int)(want < most ? want : most);
+  if (few) hipLaunchKernelGGL((page_plan_kernel<256, 1>), dim3(blocks), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((page_plan_kernel<1024, kMaxPlanBatch / 1024>), dim3(blocks), dim3(1024), 0, s, p);
   return hip_check(hipGetLastError(), "page_plan launch");
 }
 

@@ -134,6 +134,17 @@ def test_page_plan_many_requests():
     check_plan(16, lens.tolist(), news.tolist(), 20, 3000, 3500, 12288)
 
 
+@pytest.mark.parametrize("batch", [255, 256, 257, 1024, 1025])
+@pytest.mark.parametrize("page", [1, 16])
+def test_page_plan_of_as_many_requests_as_threads(batch, page):
+    """One request a thread, and several; each token its own row or many rows a request."""
+    rng = np.random.default_rng(batch)
+    lens, news = rng.integers(0, 40, batch), rng.integers(0, 9, batch)
+    news[::3] = 0
+    check_plan(page, lens.tolist(), news.tolist(), -(-48 // page), 9 * batch // page, 9 * batch, int(news.sum()) + 3)
+    check_plan(page, lens.tolist(), news.tolist(), -(-48 // page), batch // page, 9 * batch, int(news.sum()) - 3)  # too few of both
+
+
 def test_page_plan_over_several_blocks():
     rng = np.random.default_rng(4)
     lens, news = rng.integers(0, 300, 37), rng.integers(0, 1500, 37)
