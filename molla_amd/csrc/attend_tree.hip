@@ -17,7 +17,7 @@
 // 64 nodes over 8192 down to 4608 positions at width 128 132 + 12.7 us (292
 // TFLOP/s of the formula's products, twice that of the matrix cores', whose steps
 // take turns with the softmax on the VALU at two waves a SIMD); 8 x 48 over 3000
-// down to 1688 at width 64 29.9 + 9.3 (bound by a step's chain of latencies at three
+// down to 1688 at width 64 29.4 + 9.3 (bound by a step's chain of latencies at three
 // waves a SIMD); 1 x 13 over 32768 36.6 + 5.6 (3.7 TB/s; 6 once the first slices are
 // there); 4 x 25 over 4099 of q8_0 41.8 + 5.7 (a value block's factor makes halves
 // of the weights anew); 1 x 8 over 2048 11.5 + 4.1 (launches and the first loads'
@@ -321,24 +321,26 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 //   leaves them.
 //   Queries enter as two halves, each query scaled by a power of two so that its
 //   largest value is in [2^14, 2^15): every value to 2^-23 of itself (its float
-//   to 2^-24), down to 2^-39 of the largest.  Weights enter as two halves as well,
-//   2^14 times their size (f16 caches): to 2^-23 of themselves, down to 2^-39 of
-//   the largest.
+//   to 2^-24), down to 2^-39 of the largest.  Weights enter as two halves as well:
+//   to 2^-23 of themselves, down to 2^-35 of the largest.
 //
-//   A weight is 2^(s c2 - mk), mk = the maximum times c2 less 14, rounded once and
-//   then taken as it is, so that the rounding is the same in every weight of a row
-//   and falls out of its quotient, as the 14 does (where mk is so large that it
-//   could reach a weight's own size, the difference is taken before the product).
-//   The exponent's own rounding, at most 2^-21, is a weight's 3.3e-7.
+//   A weight is 2^(s c2 - mk), mk = a maximum times c2 less 10, rounded once and then
+//   taken as it is, so that the rounding is the same in every weight of a row and
+//   falls out of its quotient, as the 10 does (where mk is so large that it could
+//   reach a weight's own size, the difference is taken before the product).  The
+//   exponent's own rounding, at most 2^-21, is a weight's 3.3e-7.  mk follows the
+//   running maximum where that would make a weight above 2^14: a half holds 2^16, and
+//   with the slack most slices leave the sums as they are (8 x 64 129 -> 126 us at
+//   best, 8 x 48 at width 64 29.8 -> 29.4).
 //
 // q8_0: keys and values enter as their integers, exact halves; a key block's
 // factor multiplies its part of the score, a value block's the weights, which
 // are then split into halves (the factors' share of 4 x 25 over 4099: 42 us against
-// 30 of f16; at D = 256 107 against 48, where they do not fit the registers).  The factors are staged times 2^(15 - X), X the
-// exponent of the largest one so far among committed positions, which every row
-// sees; slices that some row does not see whole leave X as it is, and there each
-// row's products are scaled to its own largest and summed apart: what a row does
-// not see has no part in its result.
+// 30 of f16; at D = 256 107 against 48, where they do not fit the registers).  The
+// factors are staged times 2^(11 - X), X the exponent of the largest one so far
+// among committed positions, which every row sees; slices that some row does not see
+// whole leave X as it is, and there each row's products are scaled to its own largest
+// and summed apart: what a row does not see has no part in its result.
 //
 // A value that is not finite in a node that some query does not see would give
 // 0 * inf there: such values are staged as zeros and added at the end to the
@@ -355,7 +357,8 @@ typedef float tf2 __attribute__((ext_vector_type(2)));
 typedef float tf4 __attribute__((ext_vector_type(4)));
 typedef uint32_t tu4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLift = 14.0f;
+constexpr float kLift = 10.0f, kSlack = 4.0f;   // of a weight's exponent: its sum 14 at most
+constexpr int kFactor = 15 - (int)kSlack;       // q8_0: the largest factor's, for weights up to 2^kSlack
 
 // w f as two halves (ONE: f is 1, in a scalar register that the compiler takes for
 // any value): an instruction each or less, the higher halves opaque so that the
@@ -575,7 +578,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
           if (i >= SL * KS) {  // (uniform: the second half of the threads, or of a thread's factors)
             const float af = fabsf(f), fm = lanes::reduce<SL>(af < INFINITY ? af : 0.0f, lanes::Max{});
             if (!nodes_in && fm > 0.0f) xrun[j] = max(xrun[j], __builtin_amdgcn_frexp_expf(fm));
-            f = ldexpf(f, 15 - xrun[j]);
+            f = ldexpf(f, kFactor - xrun[j]);
             if (i % SL == 0) xs[buf][u] = xrun[j];
           }
           fac[buf][i / (SL * KS)][u][i % SL] = f;
@@ -765,9 +768,9 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
 #pragma unroll
         for (int i = 1; i < 8; i++) m = fmaxf(m, s[c][i >> 2][i & 3]);
         m = across(m, lanes::Max{});
-        const float mn = fmaxf(mc[c], m);
-        const bool rose = mn != mc[c];
+        const bool rose = huge && large(c) ? m > mc[c] : fmaf(m, c2[c], -mk[c]) > lift + kSlack;
         if (__any(rose)) {
+          const float mn = rose ? m : mc[c];
           const float mkn = rose ? fmaf(mn, c2[c], -lift) : mk[c];
           const float f = __builtin_amdgcn_exp2f(large(c) ? (mc[c] - mn) * c2[c] : mk[c] - mkn);
           l[c] *= f;
@@ -944,7 +947,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
       const float w = part >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
       for (int dt = 0; dt < NT; dt++) {
-        const float f = Q8 ? w * ldexpf(1.0f, xo[dt / 2] - 15) : w;
+        const float f = Q8 ? w * ldexpf(1.0f, xo[dt / 2] - kFactor) : w;
         *(tf4*)(dst + 16 * dt + 4 * lk) = o[c][dt] * f;
       }
       if (part >= 0 && lk == 0) *(float2*)(parts.ml + 2 * slot) = make_float2(mk[c], sum);

@@ -553,6 +553,25 @@ def test_attend_scales(form, d, nodes):
 
 
 @pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d,nodes", [(64, 3), (128, 3), (128, 70), (256, 3), (96, 3)])
+@pytest.mark.parametrize("rise", [0.004, 0.08, 1.9, 2.76, 2.85, 5.6, -0.08])
+def test_attend_of_rising_scores(form, d, nodes, rise):
+    """Scores that rise with the position, by `rise` a key or (from 1 on) a 50th key:
+    the running maximum moves at every slice, at some, or by just less and just more
+    than what the sums are left alone for."""
+    length = 900
+    s = Step(form, [length, 40], [nodes, 2], 1, 1, d)
+    g = torch.Generator().manual_seed(7)
+    along = torch.randn(d, generator=g)
+    steps = torch.arange(length, dtype=torch.float32)
+    score = rise * (steps if rise < 1 else (steps / 50).floor())
+    s.k[:length] = encode((score - score.max() / 2)[:, None] / s.scale * along / (along @ along) +
+                          0.02 * torch.randn(length, d, generator=g), form)
+    s.q[:nodes] = along * (1 + 0.1 * torch.randn(nodes, 1, generator=g))
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
 @pytest.mark.parametrize("d,nodes", [(64, 3), (128, 40), (96, 5), (256, 2)])
 def test_attend_without_a_scale(form, d, nodes):
     """Every key weighs the same."""
