@@ -14,12 +14,12 @@
 // 32768 positions took 46 us, that of 8 over 2048 14; so 5.6 and 4.1.)
 //
 // Measured, products + fold, heads 32 over 8 (over 4 at width 64): 8 sequences of
-// 64 nodes over 8192 down to 4608 positions at width 128 132 + 12.7 us (292
+// 64 nodes over 8192 down to 4608 positions at width 128 132 + 8.6 us (292
 // TFLOP/s of the formula's products, twice that of the matrix cores', whose steps
 // take turns with the softmax on the VALU at two waves a SIMD); 8 x 48 over 3000
-// down to 1688 at width 64 29.4 + 9.3 (bound by a step's chain of latencies at three
+// down to 1688 at width 64 29.4 + 5.1 (bound by a step's chain of latencies at three
 // waves a SIMD); 1 x 13 over 32768 36.6 + 5.6 (3.7 TB/s; 6 once the first slices are
-// there); 4 x 25 over 4099 of q8_0 41.8 + 5.7 (a value block's factor makes halves
+// there); 4 x 25 over 4099 of q8_0 41.8 + 5.5 (a value block's factor makes halves
 // of the weights anew); 1 x 8 over 2048 11.5 + 4.1 (launches and the first loads'
 // latency).
 #include <math.h>
@@ -1026,6 +1026,68 @@ __global__ __launch_bounds__(256) void attend_tree_fold_kernel(TreeAttend a, Tre
   }
 }
 
+// The same for rows of 64 and 128 values where there are many: 64 / L rows a wave,
+// L lanes of four values each.  They are consecutive rows of a tile, so that their
+// parts lie in the same blocks (12288 rows of 64 in 5 parts 9.3 us with a wave each,
+// 5.1; 16384 of 128 13 and 8.6).
+template <int L>
+__global__ __launch_bounds__(256) void attend_tree_fold_rows_kernel(TreeAttend a, TreeParts parts,
+                                                                    const int32_t* __restrict__ plan, int rows,
+                                                                    int slice) {
+  constexpr int R = 64 / L, D = 4 * L, J = kMaxParts / L;
+  const int lane = threadIdx.x & 63, l = lane % L, shift = a.group_shift;
+  const uint32_t job = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t runs = ((a.tree.max_nodes << shift) + R - 1) / R, pair = job / runs;
+  const int b = (int)(pair / a.kv_heads), kvh = (int)(pair - b * a.kv_heads), r0 = (int)(job - pair * runs) * R;
+  if (b >= a.tree.batch) return;
+  const int per = plan[0], b_first = plan[1 + b];
+  const TreeSeq sq = tree_seq(a.tree, b);
+  if (r0 >= sq.nodes << shift) return;
+  const int slices = tree_slices(sq, slice);
+  const int u0 = b_first + (kvh * tree_tiles(sq, shift, rows) + r0 / rows) * tree_units(sq, slice) + kStart;
+  const int g0 = u0 / per, n = (u0 + slices - 1) / per - g0 + 1;
+  if (n == 1) return;
+  const int r = r0 + lane / L;
+  auto slot = [&](int k) { return (int64_t)(2 * (g0 + k) + (k == 0 ? 1 : 0)) * rows + r % rows; };
+  tf4 x[8];
+  auto send = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = *(const tf4*)(parts.acc + slot(min(k + j, n - 1)) * D + 4 * l);
+  };
+  // part L j + l of the row: its maximum and sum, then its weight
+  float2 ml[J];
+#pragma unroll
+  for (int j = 0; j < J; j++)
+    if (j == 0 || L * j < n) ml[j] = ((const float2*)parts.ml)[slot(min(L * j + l, n - 1))];
+  send(0);
+  float w[J], m = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < J; j++) {
+    if (L * j + l >= n) ml[j].y = 0.0f;
+    if (ml[j].y != 0.0f) m = fmaxf(m, ml[j].x);
+  }
+  m = lanes::reduce<L>(m, lanes::Max{});
+#pragma unroll
+  for (int j = 0; j < J; j++) {
+    w[j] = ml[j].y == 0.0f ? 0.0f : ml[j].x == m ? 1.0f : __builtin_amdgcn_exp2f(ml[j].x - m);
+    sum += ml[j].y == 0.0f ? 0.0f : ml[j].y * w[j];
+  }
+  sum = lanes::reduce<L>(sum, lanes::Add{});
+  tf4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < J; j++)
+    for (int k = L * j; k < min(L * (j + 1), n); k += 8) {
+      if (k) send(k);
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (k + i < n) o += x[i] * __shfl(w[j], (lane & ~(L - 1)) + k + i - L * j);  // (uniform)
+    }
+  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  const int node = r >> shift;
+  if (node < sq.nodes)
+    *(tf4*)(a.out + ((int64_t)(sq.t0 + node) * a.heads + (kvh << shift) + (r & ((1 << shift) - 1))) * D + 4 * l) = o * inv;
+}
+
 struct TreeGrid {
   bool mfma;
   int columns;  // NC of attend_tree_kernel
@@ -1076,7 +1138,7 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   a.group_shift = __builtin_ctz(a.heads / a.kv_heads);  // (1, 2, 4 or 8 query heads a key head)
   const TreeGrid g = tree_grid(a.heads, a.kv_heads, a.head_dim, a.form, a.tree);
   // few rows: four waves each (416 rows of 62 parts 8.5 us with one, 5.6 with four;
-  // 3200 of 10 5.8 and 12.2)
+  // 3200 of 10 5.8 and 12.2), else several rows a wave where a row is 64 or 128 values
   const int64_t rows = (int64_t)a.tree.batch * a.tree.max_nodes * a.heads;
   const int waves = rows <= 1024 ? 4 : 1;
   const uint32_t fold = (uint32_t)((rows * waves + 3) / 4);
@@ -1132,7 +1194,15 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   else                                                                                                             \
     hipLaunchKernelGGL((attend_tree_fold_kernel<V, 1>), dim3(fold), dim3(256), 0, s, a, parts, plan, g.rows, \
                        g.slice)
-  if (a.head_dim % 256 == 0) MI_TREE_FOLD(4);
+  if (waves == 1 && (a.head_dim == 64 || a.head_dim == 128)) {
+    const int per_wave = a.head_dim == 64 ? 4 : 2;
+    const int64_t runs = ((int64_t)a.tree.max_nodes * a.heads / a.kv_heads + per_wave - 1) / per_wave;
+    const dim3 folds((uint32_t)((a.tree.batch * a.kv_heads * runs + 3) / 4));
+    if (a.head_dim == 64)
+      hipLaunchKernelGGL(attend_tree_fold_rows_kernel<16>, folds, dim3(256), 0, s, a, parts, plan, g.rows, g.slice);
+    else
+      hipLaunchKernelGGL(attend_tree_fold_rows_kernel<32>, folds, dim3(256), 0, s, a, parts, plan, g.rows, g.slice);
+  } else if (a.head_dim % 256 == 0) MI_TREE_FOLD(4);
   else if (a.head_dim % 128 == 0) MI_TREE_FOLD(2);
   else MI_TREE_FOLD(1);
 #undef MI_TREE_FOLD

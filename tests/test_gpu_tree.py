@@ -462,6 +462,16 @@ def test_attend_long(form, heads, kv, d, nodes):
     s.check(s.run())
 
 
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("heads,kv,d", [(8, 2, 64), (8, 8, 64), (8, 2, 128), (5, 5, 128), (4, 2, 96), (8, 1, 256)])
+@pytest.mark.parametrize("length", [500, 2500, 20001])
+def test_attend_many_parts(form, heads, kv, d, length):
+    """Room for many rows and few of them there: a row in up to 128 parts, folded by
+    the kernel for many rows."""
+    s = Step(form, [length, 30], [3, 2], heads, kv, d, seed=5, max_nodes=256)
+    s.check(s.run())
+
+
 @pytest.mark.parametrize("kind", ["chain", "roots"])
 @pytest.mark.parametrize("form", ["f16", "q8"])
 def test_attend_chains_and_roots(kind, form):
