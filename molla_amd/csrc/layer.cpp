@@ -182,28 +182,28 @@ struct LayerCache {
 int tree_attention(hipStream_t s, const mi_layer_desc* d, float* qkv, const LayerCache& c, float* out, void* work) {
   const mi_tree& t = *c.tree;
   const int64_t qw = (int64_t)d->heads * d->head_dim, kvw = (int64_t)d->kv_heads * d->head_dim;
-  QkRope r{};
-  r.d.heads = d->heads;
-  r.d.kv_heads = d->kv_heads;
-  r.d.head_dim = d->head_dim;
-  r.d.rope_dim = d->rope_dim;
-  r.d.neox = d->neox != 0;
-  r.d.cache_form = d->cache_form;
-  r.d.tokens = t.tokens;
-  r.d.eps = d->eps;
-  r.d.q = r.d.q_out = qkv;
-  r.d.k = qkv + qw;
-  r.d.v = qkv + qw + kvw;
-  r.d.q_stride = r.d.k_stride = r.d.v_stride = r.d.q_out_stride = qw + 2 * kvw;
-  r.d.q_norm = d->q_norm;
-  r.d.k_norm = d->k_norm;
-  r.d.rope_steps = d->rope_steps;
-  r.d.rope_factors = d->rope_factors;
-  r.d.pos = t.pos;
-  r.d.count = t.starts + t.batch;
-  r.d.k_cache = c.k;
-  r.d.v_cache = c.v;
-  r.d.cells = t.cells;
+  mi_qk r{};
+  r.heads = d->heads;
+  r.kv_heads = d->kv_heads;
+  r.head_dim = d->head_dim;
+  r.rope_dim = d->rope_dim;
+  r.neox = d->neox != 0;
+  r.cache_form = d->cache_form;
+  r.tokens = t.tokens;
+  r.eps = d->eps;
+  r.q = r.q_out = qkv;
+  r.k = qkv + qw;
+  r.v = qkv + qw + kvw;
+  r.q_stride = r.k_stride = r.v_stride = r.q_out_stride = qw + 2 * kvw;
+  r.q_norm = d->q_norm;
+  r.k_norm = d->k_norm;
+  r.rope_steps = d->rope_steps;
+  r.rope_factors = d->rope_factors;
+  r.pos = t.pos;
+  r.count = t.starts + t.batch;
+  r.k_cache = c.k;
+  r.v_cache = c.v;
+  r.cells = t.cells;
   const int rc = launch_qk_rope(s, r);
   if (rc) return rc;
   TreeAttend a{};

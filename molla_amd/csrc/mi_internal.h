@@ -308,16 +308,8 @@ struct PagePlan {
 int launch_page_plan(hipStream_t s, const PagePlan& p);
 int launch_tree_plan(hipStream_t s, int32_t batch, const int32_t* starts, const int32_t* lengths,
                      const int32_t* parents, int32_t max_nodes, int32_t tokens, int32_t* pos, uint32_t* mask);
-// Each head of q and k normed and rotated, q to q_out and k and v to cache rows
-// (qk_rope.hip).  The row of token t is cells[t], or without cells the one that
-// rope_store takes: kv_index[t * index_stride + pos[t]], or pos[t] of the cache
-// t * cache_stride halves on.  A negative row stores nothing.
-struct QkRope {
-  mi_qk d;
-  int64_t cache_stride, index_stride;
-  const int32_t* kv_index;
-};
-int launch_qk_rope(hipStream_t s, const QkRope& a);
+// mi_qk_norm_rope, checked (qk_rope.hip).
+int launch_qk_rope(hipStream_t s, const mi_qk& d);
 // attend_tree.hip: attention of trees of drafted tokens (mi_attend_tree).
 struct TreeAttend {
   const float* q;

@@ -25,11 +25,10 @@ constexpr int kQkThreads = 256;
 // A wave takes runs of `per` heads of one token (q's, then k's, then v's,
 // numbered end to end), its cosines and sines kept in registers for all of them.
 template <int LPH, int NS, bool Q8>
-__global__ __launch_bounds__(kQkThreads) void qk_rope_kernel(QkRope a, int heads_all, int per, int runs) {
+__global__ __launch_bounds__(kQkThreads) void qk_rope_kernel(mi_qk d, int heads_all, int per, int runs) {
 #pragma clang fp contract(off)
   constexpr int GROUPS = 64 / LPH;
   extern __shared__ float stage[];  // Q8: a head's values a lane group
-  const mi_qk& d = a.d;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane % LPH, grp = lane / LPH;
   const int64_t job = (int64_t)blockIdx.x * (kQkThreads / 64) + wave;
@@ -63,13 +62,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_rope_kernel(QkRope a, int heads
     gk[i][1] = d.k_norm && live[i] ? d.k_norm[hi[i]] : 1.0f;
   }
   const int kvw = d.kv_heads * D;
-  int64_t cell = -1, base = 0;
-  if (d.k_cache) {
-    if (d.cells) cell = d.cells[t];
-    else if (a.kv_index) cell = a.kv_index[(int64_t)t * a.index_stride + p];
-    else cell = p, base = (int64_t)t * a.cache_stride;
-  }
-  const int64_t row = base + cell * cache_row(d.cache_form, kvw);
+  const int64_t cell = d.k_cache ? d.cells[t] : -1, row = cell * cache_row(d.cache_form, kvw);
   // (every lane of the wave walks the same number of heads: the sums and the
   // 8-bit blocks exchange lanes)
   for (int h0 = first; h0 < last; h0 += GROUPS) {
@@ -163,10 +156,9 @@ struct QkRow {  // of a token, by kind of head
 };
 
 template <int LPH, bool NEOX, bool Q8>
-__global__ __launch_bounds__(kQkThreads) void qk_rope_vec_kernel(QkRope a, int heads_all, int per, int runs) {
+__global__ __launch_bounds__(kQkThreads) void qk_rope_vec_kernel(mi_qk d, int heads_all, int per, int runs) {
 #pragma clang fp contract(off)
   constexpr int GROUPS = 64 / LPH, D = 4 * LPH;
-  const mi_qk& d = a.d;
   const int lane = threadIdx.x & 63, l = lane % LPH, grp = lane / LPH;
   const int64_t job = (int64_t)blockIdx.x * (kQkThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t64 = job / runs;
@@ -177,13 +169,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_rope_vec_kernel(QkRope a, int h
   const bool turn = 2 * l < half;
   const int lo = !NEOX ? 4 * l : turn ? 2 * l : d.rope_dim + 2 * (2 * l - half), hi = lo + (NEOX && turn ? half : 2);
   const int kvw = d.kv_heads * D;
-  int64_t cell = -1, base = 0;
-  if (d.k_cache) {
-    if (d.cells) cell = d.cells[t];
-    else if (a.kv_index) cell = a.kv_index[(int64_t)t * a.index_stride + p];
-    else cell = p, base = (int64_t)t * a.cache_stride;
-  }
-  const int64_t row = base + cell * cache_row(d.cache_form, kvw);
+  const int64_t cell = d.k_cache ? d.cells[t] : -1, row = cell * cache_row(d.cache_form, kvw);
   auto source = [&](int h) __attribute__((always_inline)) {
     const int hk = h - d.heads, hv = hk - d.kv_heads;
     return h < d.heads ? d.q + t * d.q_stride + (int64_t)h * D
@@ -332,8 +318,7 @@ static bool qk_vec_fits(const mi_qk& d) {
   return !(p & 15) && !(st & 3);
 }
 
-int launch_qk_rope(hipStream_t s, const QkRope& a) {
-  const mi_qk& d = a.d;
+int launch_qk_rope(hipStream_t s, const mi_qk& d) {
   const int heads_all = d.heads + d.kv_heads * (d.k_cache ? 2 : 1);
   const bool q8 = d.k_cache && d.cache_form == MI_CACHE_Q8, vec = qk_vec_fits(d);
   // runs of heads: enough waves for the chip, as few as keep a token's angles together
@@ -345,7 +330,7 @@ int launch_qk_rope(hipStream_t s, const QkRope& a) {
   if (blocks > 0x7fffffff) return fail(MI_ERR_SHAPE, "qk_norm_rope: %d tokens of %d heads", d.tokens, heads_all);
   if (vec) {
 #define MI_QKV(LPH, N, Q)                                                                                             \
-  hipLaunchKernelGGL((qk_rope_vec_kernel<LPH, N, Q>), dim3((uint32_t)blocks), dim3(kQkThreads), 0, s, a, heads_all, \
+  hipLaunchKernelGGL((qk_rope_vec_kernel<LPH, N, Q>), dim3((uint32_t)blocks), dim3(kQkThreads), 0, s, d, heads_all, \
                      per, runs)
 #define MI_QKV_F(LPH)                      \
   if (d.neox) {                            \
@@ -365,9 +350,9 @@ int launch_qk_rope(hipStream_t s, const QkRope& a) {
 #define MI_QK(LPH, NS)                                                                                              \
   if (q8)                                                                                                           \
     hipLaunchKernelGGL((qk_rope_kernel<LPH, NS, true>), dim3((uint32_t)blocks), dim3(kQkThreads),                   \
-                       sizeof(float) * d.head_dim * (kQkThreads / LPH), s, a, heads_all, per, runs);                \
+                       sizeof(float) * d.head_dim * (kQkThreads / LPH), s, d, heads_all, per, runs);                \
   else                                                                                                              \
-    hipLaunchKernelGGL((qk_rope_kernel<LPH, NS, false>), dim3((uint32_t)blocks), dim3(kQkThreads), 0, s, a, heads_all, \
+    hipLaunchKernelGGL((qk_rope_kernel<LPH, NS, false>), dim3((uint32_t)blocks), dim3(kQkThreads), 0, s, d, heads_all, \
                        per, runs)
   if (d.head_dim <= 64) MI_QK(32, 1);
   else if (d.head_dim <= 128) MI_QK(64, 1);

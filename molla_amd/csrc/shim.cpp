@@ -510,9 +510,7 @@ int mi_qk_norm_rope(mi_stream stream, const mi_qk* d) {
     return fail(MI_ERR_SHAPE, "qk_norm_rope: cache form %d has no row of width %lld", d->cache_form, (long long)kvw);
   if (stores && (((uintptr_t)d->k_cache | (uintptr_t)d->v_cache) & 15))
     return fail(MI_ERR_ALIGN, "qk_norm_rope: the caches must be 16-byte aligned");
-  QkRope a{};
-  a.d = *d;
-  return launch_qk_rope((hipStream_t)stream, a);
+  return launch_qk_rope((hipStream_t)stream, *d);
 }
 
 size_t mi_attend_tree_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form,
