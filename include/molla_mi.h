@@ -418,7 +418,7 @@ typedef struct {
  * node i its mask has.  Slot j is row j of the sequence's cache, cache_stride
  * halves from the one before, or with kv_index pool cell kv_index[b *
  * index_stride + j] (negative: not held, not seen).  q and out are rows of
- * heads * head_dim floats, q's q_stride apart (16-byte aligned).  A token that
+ * heads * head_dim floats, q's q_stride apart (16-byte aligned), out apart from them.  A token that
  * sees nothing gets zeros; rows behind the last sequence keep what they held.
  * What a token does not see changes no bit of its result, whatever it holds.
  * GQA groups and head widths as mi_attend.  Workspace:

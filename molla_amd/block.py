@@ -175,7 +175,7 @@ def device_layer_tree(ctx: gpu.DeviceContext, layer: DeviceLayer, x: torch.Tenso
     gpu._queue(ctx, lib().mi_decoder_layer_tree, ctypes.byref(desc), on(ctx, x, "x", torch.float32, tokens * s.width),
                on(ctx, k_cache, "k_cache", f16, least), on(ctx, v_cache, "v_cache", f16, least), cache_stride,
                None if kv_index is None else on(ctx, kv_index, "kv_index", i32), stride, ctypes.byref(tree),
-               work.data_ptr(), work.numel())
+               on(ctx, work, "work", torch.uint8), work.numel())
 
 
 class DeviceModel:

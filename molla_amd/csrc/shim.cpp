@@ -536,6 +536,10 @@ int mi_attend_tree(mi_stream stream, int32_t form, const float* q, int64_t q_str
   if (q_stride < (int64_t)heads * head_dim) return fail(MI_ERR_SHAPE, "attend_tree: row stride too small");
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || q_stride % 4)
     return fail(MI_ERR_ALIGN, "attend_tree: the queries and the output must be 16-byte aligned");
+  // (a tile's queries are read by several blocks, one of which may have written its rows)
+  const float* q_end = q + (tree->tokens - 1) * q_stride + (int64_t)heads * head_dim;
+  if (out < q_end && q < out + (int64_t)tree->tokens * heads * head_dim)
+    return fail(MI_ERR_ARG, "attend_tree: the output may not lie among the queries");
   const size_t need = mi_attend_tree_workspace(heads, kv_heads, head_dim, form, tree);
   if (!work || ((uintptr_t)work & 255) || work_bytes < need)
     return fail(MI_ERR_WORKSPACE, "attend_tree: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);

@@ -285,11 +285,11 @@ def _queue(ctx: DeviceContext, fn, *args) -> None:
 
 def _on(ctx: DeviceContext, t: torch.Tensor, name: str, dtype: torch.dtype, numel: int = 0) -> int:
     """The address of a contiguous tensor of the context's device, at least `numel` long."""
-    if t.dtype is not dtype or t.get_device() != ctx.index or not t.is_contiguous():
-        raise ValueError(f"{name} has to be a contiguous {dtype} tensor on {ctx.device}")
-    if t.numel() < numel:
+    if t.dtype is dtype and t.get_device() == ctx.index and t.is_contiguous() and (not numel or t.numel() >= numel):
+        return t.data_ptr()
+    if t.dtype is dtype and t.get_device() == ctx.index and t.is_contiguous():
         raise ValueError(f"{name} has {t.numel()} values where {numel} are needed")
-    return t.data_ptr()
+    raise ValueError(f"{name} has to be a contiguous {dtype} tensor on {ctx.device}")
 
 
 def _rows(ctx: DeviceContext, t: torch.Tensor, name: str, tokens: int, width: int) -> int:
@@ -411,7 +411,7 @@ def device_attend_tree(ctx: DeviceContext, q: torch.Tensor, k_cache: torch.Tenso
     _queue(ctx, L.mi_attend_tree, form, q.data_ptr(), q_stride, _on(ctx, k_cache, "k_cache", f16, least),
            _on(ctx, v_cache, "v_cache", f16, least), cache_stride,
            None if kv_index is None else _on(ctx, kv_index, "kv_index", i32), stride, heads, kv_heads, head_dim, scale,
-           t, _on(ctx, out, "out", torch.float32, tokens * qw), work.data_ptr(), work.numel())
+           t, _on(ctx, out, "out", torch.float32, tokens * qw), _on(ctx, work, "work", torch.uint8), work.numel())
 
 
 __all__ = [n for n in dir() if not n.startswith("_")] + ["MiError"]

@@ -883,7 +883,8 @@ def test_python_refusals():
     for bad in (dict(q=e["q"].cpu()), dict(q=e["q"].half()), dict(q=e["q"].t()), dict(k_cache=e["k"][:3].contiguous()),
                 dict(v_cache=e["v"].float()), dict(starts=e["starts"].long()), dict(starts=e["starts"][:1]),
                 dict(mask=e["mask"][:1].contiguous()), dict(out=out[:2]), dict(out=out.t()), dict(max_nodes=300),
-                dict(kv_index=ints([1, 2, 3]))):
+                dict(kv_index=ints([1, 2, 3])), dict(out=e["q"]),
+                dict(work=torch.empty(1 << 24, dtype=torch.uint8)), dict(work=torch.empty(1 << 22, device="cuda"))):
         with pytest.raises((ValueError, gpu.MiError)):
             attend(**bad)
     with pytest.raises(ValueError):

@@ -253,6 +253,7 @@ def test_python_refusals():
     ctx.synchronize()
     for bad in (dict(x=s.xd[:2]), dict(x=s.xd.double()), dict(cells=i["cells"][:2]), dict(mask=i["mask"][:1]),
                 dict(kv_index=s.index[0]), dict(kv_index=None, max_count=1000), dict(starts=i["starts"][:1]), dict(max_nodes=0),
-                dict(pos=i["pos"].long()), dict(k_cache=s.k[0].float()), dict(work=torch.empty(64, dtype=torch.uint8, device="cuda"))):
+                dict(pos=i["pos"].long()), dict(k_cache=s.k[0].float()), dict(work=torch.empty(64, dtype=torch.uint8, device="cuda")),
+                dict(work=torch.empty(1 << 26, dtype=torch.uint8))):
         with pytest.raises((ValueError, gpu.MiError)):
             block.device_layer_tree(ctx, layer, **{**good, **bad})

@@ -81,7 +81,7 @@ def test_qk_refuses_no_descriptor():
 
 TREE = dict(batch=3, tokens=24, max_nodes=8, max_count=100, starts=FAKE, lengths=FAKE, mask=FAKE)
 ATTEND = dict(stream=None, form=0, q=FAKE, q_stride=512, k_cache=FAKE, v_cache=FAKE, cache_stride=12800, kv_index=None,
-              index_stride=0, heads=8, kv_heads=2, head_dim=64, scale=0.125, tree=None, out=FAKE, work=FAKE,
+              index_stride=0, heads=8, kv_heads=2, head_dim=64, scale=0.125, tree=None, out=FAKE + 24 * 2048, work=FAKE,
               work_bytes=1 << 30)
 
 
@@ -92,6 +92,7 @@ ATTEND = dict(stream=None, form=0, q=FAKE, q_stride=512, k_cache=FAKE, v_cache=F
     (dict(cache_stride=12799), SHAPE, "fewer"), (dict(kv_index=FAKE, index_stride=99), SHAPE, "fewer"),
     (dict(q=FAKE + 4), ALIGN, "16-byte"), (dict(q_stride=514), ALIGN, "16-byte"), (dict(cache_stride=12804), ALIGN, "16-byte"),
     (dict(out=FAKE + 8), ALIGN, "16-byte"), (dict(work=None), WORKSPACE, "workspace"),
+    (dict(out=FAKE), ARG, "among"), (dict(out=FAKE + 24 * 2048 - 16), ARG, "among"), (dict(out=FAKE - 24 * 2048 + 16), ARG, "among"),
     (dict(work=FAKE + 16), WORKSPACE, "workspace"), (dict(work_bytes=64), WORKSPACE, "needed"),
     (dict(tree=dict(starts=None)), ARG, "trees"), (dict(tree=dict(lengths=None)), ARG, "trees"),
     (dict(tree=dict(mask=None)), ARG, "trees"), (dict(tree=dict(batch=0)), SHAPE, "sequences"),
