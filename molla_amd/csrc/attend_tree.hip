@@ -14,10 +14,10 @@
 // 32768 positions took 46 us, that of 8 over 2048 14; so 5.6 and 4.1.)
 //
 // Measured, products + fold, heads 32 over 8 (over 4 at width 64): 8 sequences of
-// 64 nodes over 8192 down to 4608 positions at width 128 132 + 8.6 us (292
+// up to 64 nodes over 8192 down to 4608 positions at width 128 132 + 8.6 us (292
 // TFLOP/s of the formula's products, twice that of the matrix cores', whose steps
 // take turns with the softmax on the VALU at two waves a SIMD); 8 x 48 over 3000
-// down to 1688 at width 64 29.4 + 5.1 (bound by a step's chain of latencies at three
+// down to 1691 at width 64 29.4 + 5.1 (bound by a step's chain of latencies at three
 // waves a SIMD); 1 x 13 over 32768 36.6 + 5.6 (3.7 TB/s; 6 once the first slices are
 // there); 4 x 25 over 4099 of q8_0 41.8 + 5.5 (a value block's factor makes halves
 // of the weights anew); 1 x 8 over 2048 11.5 + 4.1 (launches and the first loads'

@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kMaxTreeNodes) void tree_plan_kernel(const int32_t*
 
 int launch_page_plan(hipStream_t s, const PagePlan& p) {
   // up to 256 requests: one a thread of four waves, whose scan is short (64 requests
-  // of a token 3.6 us, 5.7 with the larger block; 200 prompts of 282000 tokens 6.2 and
+  // of a token 3.6 us, 5.7 with the larger block; 200 prompts of 274000 tokens 6.2 and
   // 8.8); a block for each T token rows, at most four (or one) a compute unit (for
   // each 4 T of them the 200 prompts take 7.4)
   const bool few = p.batch <= 256;
