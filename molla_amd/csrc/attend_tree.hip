@@ -1142,7 +1142,7 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   const int64_t rows = (int64_t)a.tree.batch * a.tree.max_nodes * a.heads;
   const int waves = rows <= 1024 ? 4 : 1;
   const uint32_t fold = (uint32_t)((rows * waves + 3) / 4);
-  if (g.units > 0x7fffffff || rows > 0x7ffffff0)
+  if (g.units > 1 << 30 || rows > 1 << 30)  // (sums of them in 32 bits on the device)
     return fail(MI_ERR_SHAPE, "attend_tree: %d sequences of %d nodes and %d positions are too much work", a.tree.batch,
                 a.tree.max_nodes, a.tree.max_count);
   const TreeCarve c = tree_carve(g, a.head_dim, a.tree.batch);

@@ -104,6 +104,15 @@ def test_attend_refusals(change, code, text):
     refused(_lib.lib().mi_attend_tree(*args.values()), code, text)
 
 
+@pytest.mark.parametrize("tree", [dict(batch=1, max_nodes=256, max_count=2 ** 31 - 1), dict(batch=40000, max_nodes=256, max_count=2 ** 20),
+                                  dict(batch=10 ** 6, max_nodes=256, max_count=1)])
+def test_attend_refuses_more_work_than_32_bits_count(tree):
+    tree = _lib.MiTree(**{**TREE, **tree})
+    args = {**ATTEND, "heads": 64, "kv_heads": 64, "q_stride": 4096, "kv_index": FAKE, "index_stride": 2 ** 31, "out": FAKE << 8,
+            "work_bytes": 1 << 50, "tree": ctypes.byref(tree)}
+    refused(_lib.lib().mi_attend_tree(*args.values()), SHAPE, "too much work")
+
+
 def test_attend_refuses_no_trees():
     refused(_lib.lib().mi_attend_tree(*ATTEND.values()), ARG, "trees")
 
