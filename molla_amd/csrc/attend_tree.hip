@@ -89,16 +89,16 @@ __device__ __forceinline__ void tree_walk(const TreeAttend& a, int rows, int sli
     if (b >= batch || sq.nodes == 0) sq.count = 0;
     units = sq.count ? tree_tiles(sq, shift, rows) * a.kv_heads * tree_units(sq, slice) : 0;
   };
-  int total = 0, top = 0;
+  int total = 0, top = 0, upto = 0;  // upto: of the lanes up to this one
   for (int b0 = 0; b0 < batch; b0 += 64) {
     look(b0);
-    total += lanes::reduce<64>(units, lanes::Add{});
+    upto = lane_scan(units);
+    total += __builtin_amdgcn_readlane(upto, 63);
     top = max(top, lanes::reduce<64>(sq.count ? tree_units(sq, slice) : 0, IMax{}));
   }
-  total = __builtin_amdgcn_readfirstlane(total);  // (the same in every lane)
-  top = __builtin_amdgcn_readfirstlane(top);
-  const int blocks = gridDim.x;
-  const int per = max(max((total + blocks - 1) / blocks, (top + kMaxParts - 3) / (kMaxParts - 2)), 1);
+  top = __builtin_amdgcn_readfirstlane(top);  // (the same in every lane)
+  const uint32_t blocks = gridDim.x;
+  const int per = max(max((int)(((uint32_t)total + blocks - 1) / blocks), (top + kMaxParts - 3) / (kMaxParts - 2)), 1);
   // blocks go to the 8 XCDs in turn: neighbours in the line, which are one
   // sequence's tiles over the same keys, to the same L2
   const int xcd = blockIdx.x & 7, in = blockIdx.x >> 3, many = blocks >> 3, rest = blocks & 7;
@@ -108,8 +108,10 @@ __device__ __forceinline__ void tree_walk(const TreeAttend& a, int rows, int sli
   if (writes && lane == 0) plan[0] = per;
   int b = -1, at = 0, chunk = 0;
   for (int b0 = 0, ahead = 0; b0 < batch && (b < 0 || writes); b0 += 64) {
-    if (batch > 64) look(b0);
-    const int upto = ahead + lane_scan(units);
+    if (batch > 64) {
+      look(b0);
+      upto = ahead + lane_scan(units);
+    }
     if (writes && b0 + lane < batch) plan[1 + b0 + lane] = upto - units;
     const uint64_t hit = __ballot(first >= upto - units && first < upto);
     if (hit) {
@@ -133,8 +135,8 @@ __device__ __forceinline__ void tree_walk(const TreeAttend& a, int rows, int sli
   while (true) {
     const int run = tree_units(s, slice), tiles = tree_tiles(s, shift, rows);
     while (at < run * tiles * a.kv_heads) {
-      const int pair = at / run, u = at - pair * run, n = min(run - u, left);
-      const int head = tiles == 1 ? pair : pair / tiles;
+      const int pair = (uint32_t)at / (uint32_t)run, u = at - pair * run, n = min(run - u, left);
+      const int head = tiles == 1 ? pair : (uint32_t)pair / (uint32_t)tiles;
       const int s0 = max(u - kStart, 0), s1 = u + n - kStart;
       const int part = u <= kStart && u + n == run ? -1 : 2 * block + (u <= kStart ? 1 : 0);
       if (s0 < s1) take(s, b, head, pair - head * tiles, s0, s1, part);
