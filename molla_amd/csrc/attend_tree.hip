@@ -1135,6 +1135,12 @@ size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, 
   return tree_carve(tree_grid(heads, kv_heads, head_dim, form, t), head_dim, t.batch).total;
 }
 
+// Whether units and rows, whose sums the device takes in 32 bits, are few enough.
+bool tree_attend_fits(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const mi_tree& t) {
+  return tree_grid(heads, kv_heads, head_dim, form, t).units <= 1 << 30 &&
+         (int64_t)t.batch * t.max_nodes * heads <= 1 << 30;
+}
+
 int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   TreeAttend a = step;
   a.group_shift = __builtin_ctz(a.heads / a.kv_heads);  // (1, 2, 4 or 8 query heads a key head)
@@ -1144,9 +1150,6 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   const int64_t rows = (int64_t)a.tree.batch * a.tree.max_nodes * a.heads;
   const int waves = rows <= 1024 ? 4 : 1;
   const uint32_t fold = (uint32_t)((rows * waves + 3) / 4);
-  if (g.units > 1 << 30 || rows > 1 << 30)  // (sums of them in 32 bits on the device)
-    return fail(MI_ERR_SHAPE, "attend_tree: %d sequences of %d nodes and %d positions are too much work", a.tree.batch,
-                a.tree.max_nodes, a.tree.max_count);
   const TreeCarve c = tree_carve(g, a.head_dim, a.tree.batch);
   const TreeParts parts{(float*)work, (float*)((char*)work + c.ml)};
   int32_t* plan = (int32_t*)((char*)work + c.plan);

@@ -324,6 +324,7 @@ struct TreeAttend {
   int32_t group_shift;  // log2 of heads / kv_heads (set by the launch)
 };
 size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const mi_tree& tree);
+bool tree_attend_fits(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const mi_tree& tree);
 int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work);
 
 // ---- small device helpers -----------------------------------------------

@@ -69,6 +69,9 @@ int check_tree_caches(const char* name, int32_t form, int32_t heads, int32_t kv_
     return fail(MI_ERR_SHAPE, "%s: a sequence's stride holds fewer than %d positions", name, tree->max_count);
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) || (!kv_index && cache_stride % 8))
     return fail(MI_ERR_ALIGN, "%s: the caches must be 16-byte aligned with a stride of a multiple of 8 halves", name);
+  if (!tree_attend_fits(heads, kv_heads, head_dim, form, *tree))
+    return fail(MI_ERR_SHAPE, "%s: %d sequences of %d nodes and %d positions are too much work", name, tree->batch,
+                tree->max_nodes, tree->max_count);
   return MI_OK;
 }
 

@@ -191,6 +191,49 @@ def test_rows_behind_the_last_sequence(counts, spare):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("counts", [[3, 2], [4, 4], [9, 2]])
+def test_chained_layers(counts):
+    """Layers that norm for the next one give the same bits."""
+    spec = spec_of(512, 1024, 8, 2, 64)
+    outs = []
+    for chained in (False, True):
+        ctx = gpu.DeviceContext(0)
+        layers = [device_layer_from(make_layer_weights(spec, 50 + i), spec)[1] for i in range(3)]
+        if chained:
+            block.chain_layers([layer.desc for layer in layers])
+        s = Trees(ctx, spec, [12, 30], counts, "f16", True, layers=3)
+        s.plan()
+        for i, layer in enumerate(layers):
+            s.layer(layer, i)
+        ctx.synchronize()
+        outs.append([s.xd] + s.k + s.v)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    """Two contexts' layers in turn on streams of their own, each as it is alone."""
+    spec = spec_of(512, 1024, 8, 2, 64)
+    _, layer = device_layer_from(make_layer_weights(spec, 60), spec)
+    want = []
+    for seed in (3, 4):
+        ctx = gpu.DeviceContext(0)
+        s = Trees(ctx, spec, [200, 900], [20, 13], "f16", True, seed=seed)
+        s.plan()
+        s.layer(layer)
+        ctx.synchronize()
+        want.append(s.xd.clone())
+    sets = [Trees(gpu.DeviceContext(0, torch.cuda.Stream()), spec, [200, 900], [20, 13], "f16", True, seed=seed) for seed in (3, 4)]
+    torch.cuda.synchronize()
+    for s in sets:
+        s.plan()
+    for s in sets:
+        s.layer(layer)
+    for s, w in zip(sets, want):
+        s.ctx.synchronize()
+        assert torch.equal(s.xd, w)
+
+
 @pytest.mark.parametrize("counts", [[3, 2], [8, 6]])
 def test_step_captured_and_replayed(counts):
     """Plans and two layers as one graph: other lengths and trees between the

@@ -113,6 +113,13 @@ def test_attend_refuses_more_work_than_32_bits_count(tree):
     refused(_lib.lib().mi_attend_tree(*args.values()), SHAPE, "too much work")
 
 
+def test_layer_refuses_it_before_its_first_launch():
+    tree = _lib.MiTree(**{**TREE, "batch": 200000, "max_nodes": 256, "max_count": 2 ** 20, "pos": FAKE, "cells": FAKE})
+    args = {**LAYER, "kv_index": FAKE, "index_stride": 2 ** 20, "work_bytes": 1 << 50, "desc": ctypes.byref(layer_desc()),
+            "tree": ctypes.byref(tree)}
+    refused(_lib.lib().mi_decoder_layer_tree(*args.values()), SHAPE, "too much work")
+
+
 def test_attend_refuses_no_trees():
     refused(_lib.lib().mi_attend_tree(*ATTEND.values()), ARG, "trees")
 
