@@ -1105,7 +1105,8 @@ TreeGrid tree_grid(int heads, int kv_heads, int head_dim, int form, const mi_tre
   // two columns a lane read each key fragment once for twice the rows, but only
   // where a sequence has more rows than one column's 64: 8 x 32 nodes at D = 128 74
   // us with two and 89 with one, 8 x 16 62 and 50, 1 x 13 47 and 37 (at D = 64 the
-  // registers cost the third block, with q8_0 they spill)
+  // registers cost the third block: 8 x 48 over 3000 31 us for 29, over 12000 80 for
+  // 83; with q8_0 they spill)
   g.columns = head_dim == 128 && form != MI_CACHE_Q8 && t.max_nodes * group > 64 ? 2 : 1;
   g.rows = g.mfma ? 64 * g.columns : kRowsTile;
   g.slice = g.mfma ? mfma_slice(head_dim) : rows_slice(head_dim);
