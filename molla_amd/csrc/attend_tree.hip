@@ -340,9 +340,9 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 // are then split into halves (the factors' share of 4 x 25 over 4099: 42 us against
 // 30 of f16; at D = 256 107 against 48, where they do not fit the registers).  The
 // factors are staged times 2^(11 - X), X the exponent of the largest one so far
-// among committed positions, which every row sees; slices that some row does not see
-// whole leave X as it is, and there each row's products are scaled to its own largest
-// and summed apart: what a row does not see has no part in its result.
+// among committed positions, which every row sees.  In 32 keys that some row does not
+// see whole each row's products are scaled to its own largest and summed apart: what
+// a row does not see has no part in its result.
 //
 // A value that is not finite in a node that some query does not see would give
 // 0 * inf there: such values are staged as zeros and added at the end to the
@@ -578,8 +578,9 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
           const int i = tid + 256 * j, u = i / SL % KS;
           float f = half_bits_to_float(st.f[j]);
           if (i >= SL * KS) {  // (uniform: the second half of the threads, or of a thread's factors)
-            const float af = fabsf(f), fm = lanes::reduce<SL>(af < INFINITY ? af : 0.0f, lanes::Max{});
-            if (!nodes_in && fm > 0.0f) xrun[j] = max(xrun[j], __builtin_amdgcn_frexp_expf(fm));
+            const float af = fabsf(f);
+            const float fm = lanes::reduce<SL>(sl * SL + i % SL < sq.len && af < INFINITY ? af : 0.0f, lanes::Max{});
+            if (fm > 0.0f) xrun[j] = max(xrun[j], __builtin_amdgcn_frexp_expf(fm));
             f = ldexpf(f, kFactor - xrun[j]);
             if (i % SL == 0) xs[buf][u] = xrun[j];
           }

@@ -582,6 +582,19 @@ def test_attend_of_rising_scores(form, d, nodes, rise):
 
 
 @pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d,nodes", [(64, 3), (64, 20), (128, 3), (128, 20), (256, 3), (96, 3)])
+@pytest.mark.parametrize("length", [0, 20, 40, 64, 100, 130])
+@pytest.mark.parametrize("size", [1e4, 1e-3])
+def test_attend_of_large_and_small_values(form, d, nodes, length, size):
+    """Values far from 1, with a context that ends anywhere in a slice."""
+    s = Step(form, [length, 70], [nodes, 2], 4, 2, d, seed=length, paged=True)
+    g = torch.Generator().manual_seed(2)
+    s.v = encode(size * torch.randn(len(s.v), 2 * d, generator=g).clamp(-6, 6), form)
+    s.k = encode(2 * torch.randn(len(s.k), 2 * d, generator=g), form)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
 @pytest.mark.parametrize("d,nodes", [(64, 3), (128, 40), (96, 5), (256, 2)])
 def test_attend_without_a_scale(form, d, nodes):
     """Every key weighs the same."""
