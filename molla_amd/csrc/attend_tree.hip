@@ -448,13 +448,13 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
 __host__ __device__ constexpr int mfma_slice(int D) { return D == 64 ? 64 : 32; }
 __host__ __device__ constexpr int mfma_blocks(int D) { return D == 64 ? 3 : 2; }
 
-template <int D, int NC, bool Q8, bool PAGED>
+template <int D, int NC, bool Q8, bool PAGED, int KW = 1>
 __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAttend a, TreeParts parts,
                                                                               int32_t* __restrict__ plan) {
-  constexpr int SL = mfma_slice(D), KS = D / 32, NT = D / 16, PIECES = D / 8;
+  constexpr int SL = KW == 2 ? 64 : mfma_slice(D), KS = D / 32, NT = D / 16, PIECES = D / 8;
   constexpr int PER = Q8 ? (SL * D / 16 + 255) / 256 : SL * PIECES / 256;  // 16-byte words of K (and of V) a thread
   constexpr int WPK = Q8 ? D / 16 : PIECES;                               // words a key
-  constexpr int ROWS = 64 * NC;
+  constexpr int ROWS = 64 * NC / KW;
   constexpr int VG = 2;  // 16-dim tiles of values a group of reads
   constexpr int FPER = 2 * SL * KS / 256;                                 // q8_0 factors of K and V a thread
   static_assert(PER * 256 == SL * WPK && FPER * 256 == 2 * SL * KS, "a slice's words dealt evenly");
@@ -462,10 +462,12 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
   __shared__ __align__(16) _Float16 ks[2][SL * KR];
   __shared__ __align__(16) _Float16 vs[2][SL * VR];
   __shared__ __align__(16) float fac[Q8 ? 2 : 1][2][Q8 ? KS : 1][Q8 ? SL : 1];  // q8_0 factors of keys and values
-  __shared__ int xs[Q8 ? 2 : 1][Q8 ? KS : 1];                                   // X that the values' factors are at
+  __shared__ __align__(16) int xs[Q8 ? 2 : 1][Q8 ? KS : 1];                                 // X that the values' factors are at
   __shared__ int holes[2];  // the step whose slice in this buffer has a cell that is not held
   __shared__ int spoilt[2]; // the last (even, odd) run in which some staged value was not finite
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, wave_all = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // KW = 2: waves 2 and 3 have the rows of 0 and 1, and each slice's other 32 keys
+  const int wave = wave_all % (4 / KW), half = wave_all / (4 / KW);
   const int lm = lane & 15, lk = lane >> 4;
   const int shift = a.group_shift, group = 1 << shift, words = (a.tree.max_nodes + 31) >> 5;
   const int kvw = a.kv_heads * D, crow = cache_row(a.form, kvw);
@@ -660,9 +662,14 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
     asm("" : "+s"(one));
 
     // the scores of keys 32 kt .. of a slice, and whether all its cells are held
-    auto scores = [&](int sl, int kt, int buf, tf4 (&s)[NC][2], int& hole) __attribute__((always_inline)) {
+    // and (q8_0) the X that its values' factors are at
+    auto scores = [&](int sl, int kt, int buf, tf4 (&s)[NC][2], int& hole, int (&xv)[Q8 ? KS : 1]) __attribute__((always_inline)) {
       const _Float16* kp = &ks[buf][32 * kt * KR + kat];
       if (PAGED) hole = holes[buf];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int u = 0; u < KS; u++) xv[u] = xs[buf][u];
+      }
       // key fragments of as many products as there are registers for on their way
       // before the first (one at a time, the compiler's order, left each product
       // waiting for LDS)
@@ -736,7 +743,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
       if (PAGED) hole = __builtin_amdgcn_readfirstlane(hole) - (first_turn + sl - s0);
     };
     // their softmax and weighted values
-    auto values = [&](int sl, int kt, int buf, tf4 (&s)[NC][2], int hole) __attribute__((always_inline)) {
+    auto values = [&](int sl, int kt, int buf, tf4 (&s)[NC][2], int hole, int (&xv)[Q8 ? KS : 1]) __attribute__((always_inline)) {
       const int base = sl * SL + 32 * kt;
       const _Float16* vp = &vs[buf][32 * kt * VR + vat];
       ts4 v4[2][VG][2];
@@ -795,10 +802,13 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
         if constexpr (!Q8) split<true>(p[c], [&](int) __attribute__((always_inline)) { return one; }, ph[c], pl[c]);
       }
       if constexpr (Q8) {  // (uniform) X has risen with this slice's factors
+        int rise = 0;
 #pragma unroll
-        for (int u = 0; u < KS; u++) {
-          const int x = __builtin_amdgcn_readfirstlane(xs[buf][u]);
-          if (x != xo[u]) {
+        for (int u = 0; u < KS; u++) rise |= __builtin_amdgcn_readfirstlane(xv[u]) ^ xo[u];
+        if (rise) {
+#pragma unroll
+          for (int u = 0; u < KS; u++) {
+            const int x = __builtin_amdgcn_readfirstlane(xv[u]);
             const float f = ldexpf(1.0f, xo[u] - x);
 #pragma unroll
             for (int c = 0; c < NC; c++) o[c][2 * u] *= f, o[c][2 * u + 1] *= f;
@@ -893,10 +903,12 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
     __syncthreads();
     for (int sl = s0, buf = 0; sl < s1; sl++, buf ^= 1) {
       tf4 s[SL / 32][NC][2];
-      int hole = 1;
-      if (busy) {
-        scores(sl, 0, buf, s[0], hole);
-        if constexpr (SL > 32) scores(sl, 1, buf, s[1], hole);
+      int hole = 1, xv[Q8 ? KS : 1];
+      if constexpr (KW == 2) {
+        if (busy && sl * SL + 32 * half < sq.count) scores(sl, half, buf, s[0], hole, xv);
+      } else if (busy) {
+        scores(sl, 0, buf, s[0], hole, xv);
+        if constexpr (SL > 32) scores(sl, 1, buf, s[1], hole, xv);
       }
       // the next slice from registers to the other buffer, and the one behind it on
       // its way (written once for busy and idle waves: with a copy for each the
@@ -909,10 +921,12 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
           if (sl + 3 < s1) find(sl + 3, st);
         }
       }
-      if (busy) {
-        values(sl, 0, buf, s[0], hole);
+      if constexpr (KW == 2) {
+        if (busy && sl * SL + 32 * half < sq.count) values(sl, half, buf, s[0], hole, xv);
+      } else if (busy) {
+        values(sl, 0, buf, s[0], hole, xv);
         if constexpr (SL > 32) {
-          if (sl * SL + 32 < sq.count) values(sl, 1, buf, s[1], hole);
+          if (sl * SL + 32 < sq.count) values(sl, 1, buf, s[1], hole, xv);
         }
       }
       __syncthreads();
@@ -939,7 +953,28 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
         }
       }
     }
-    if (!busy) return;
+    if constexpr (KW == 2) {
+      // the two waves of a row to one, by way of the keys' buffers (no more in use; the
+      // next run's first slice waits behind the second barrier)
+      static_assert(Q8 && NC == 1 && sizeof(ks) >= 2 * 64 * (NT + 1) * sizeof(tf4), "room for two waves' sums");
+      tf4* put = (tf4*)ks + (wave * 64 + lane) * (NT + 1);
+      if (half && busy) {
+#pragma unroll
+        for (int dt = 0; dt < NT; dt++) put[dt] = o[0][dt] * ldexpf(1.0f, xo[dt / 2] - kFactor);
+        put[NT] = tf4{mk[0], l[0], 0.0f, 0.0f};
+      }
+      __syncthreads();
+      if (!half && busy) {
+        const float om = put[NT][0], m = fmaxf(mk[0], om);
+        const float f0 = mk[0] == m ? 1.0f : __builtin_amdgcn_exp2f(mk[0] - m), f1 = om == m ? 1.0f : __builtin_amdgcn_exp2f(om - m);
+#pragma unroll
+        for (int dt = 0; dt < NT; dt++) o[0][dt] = o[0][dt] * (ldexpf(f0, xo[dt / 2] - kFactor)) + put[dt] * f1;
+        l[0] = l[0] * f0 + put[NT][1] * f1;
+        mk[0] = m;
+      }
+      __syncthreads();
+    }
+    if (!busy || half) return;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
       const float sum = across(l[c], lanes::Add{});
@@ -950,7 +985,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
       const float w = part >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
       for (int dt = 0; dt < NT; dt++) {
-        const float f = Q8 ? w * ldexpf(1.0f, xo[dt / 2] - kFactor) : w;
+        const float f = Q8 && KW == 1 ? w * ldexpf(1.0f, xo[dt / 2] - kFactor) : w;
         *(tf4*)(dst + 16 * dt + 4 * lk) = o[c][dt] * f;
       }
       if (part >= 0 && lk == 0) *(float2*)(parts.ml + 2 * slot) = make_float2(mk[c], sum);
@@ -1093,7 +1128,7 @@ __global__ __launch_bounds__(256) void attend_tree_fold_rows_kernel(TreeAttend a
 
 struct TreeGrid {
   bool mfma;
-  int columns;  // NC of attend_tree_kernel
+  int columns, split;  // NC and KW of attend_tree_kernel
   int rows, slice;
   int64_t units;  // of the largest step
   int blocks;
@@ -1109,8 +1144,9 @@ TreeGrid tree_grid(int heads, int kv_heads, int head_dim, int form, const mi_tre
   // registers cost the third block: 8 x 48 over 3000 31 us for 29, over 12000 80 for
   // 83; with q8_0 they spill)
   g.columns = head_dim == 128 && form != MI_CACHE_Q8 && t.max_nodes * group > 64 ? 2 : 1;
-  g.rows = g.mfma ? 64 * g.columns : kRowsTile;
-  g.slice = g.mfma ? mfma_slice(head_dim) : rows_slice(head_dim);
+  g.split = form == MI_CACHE_Q8 && (head_dim == 64 || head_dim == 128) && t.max_nodes * group <= 32 ? 2 : 1;
+  g.rows = g.mfma ? 64 * g.columns / g.split : kRowsTile;
+  g.slice = g.split == 2 ? 64 : g.mfma ? mfma_slice(head_dim) : rows_slice(head_dim);
   g.units = (int64_t)t.batch * ((t.max_nodes * group + g.rows - 1) / g.rows) * kv_heads *
             (((int64_t)t.max_count + g.slice - 1) / g.slice + kStart);
   g.blocks = (int)std::min<int64_t>(g.units, (int64_t)cu_count() * (g.mfma ? mfma_blocks(head_dim) : 3));
@@ -1173,7 +1209,15 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   else                                                                                                               \
     hipLaunchKernelGGL((attend_tree_rows_kernel<false, ND>), grid, dim3(kRowsThreads), rows_lds_bytes(a.head_dim), s, \
                        a, parts, plan)
-  if (a.head_dim == 64) {
+#define MI_TREE_SPLIT(D)                                                                                         \
+  if (a.kv_index)                                                                                                \
+    hipLaunchKernelGGL((attend_tree_kernel<D, 1, true, true, 2>), grid, dim3(256), 0, s, a, parts, plan);        \
+  else                                                                                                           \
+    hipLaunchKernelGGL((attend_tree_kernel<D, 1, true, false, 2>), grid, dim3(256), 0, s, a, parts, plan)
+  if (g.split == 2) {
+    if (a.head_dim == 64) MI_TREE_SPLIT(64);
+    else MI_TREE_SPLIT(128);
+  } else if (a.head_dim == 64) {
     MI_TREE_F(64, 1)
   } else if (a.head_dim == 128) {
     if (g.columns == 1) { MI_TREE_F(128, 1) }
@@ -1192,6 +1236,7 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   }
 #undef MI_TREE
 #undef MI_TREE_F
+#undef MI_TREE_SPLIT
 #undef MI_TREE_ROWS
   if (int rc = hip_check(hipGetLastError(), "attend_tree launch")) return rc;
 #define MI_TREE_FOLD(V)                                                                                            \
