@@ -19,7 +19,7 @@
 // take turns with the softmax on the VALU at two waves a SIMD); 8 x 48 over 3000
 // down to 1691 at width 64 29.4 + 5.1 (bound by a step's chain of latencies at three
 // waves a SIMD); 1 x 13 over 32768 36.6 + 5.6 (3.7 TB/s; 6 once the first slices are
-// there); 4 x 25 over 4099 of q8_0 41.8 + 5.5 (a value block's factor makes halves
+// there); 4 x 25 over 4099 of q8_0 39.9 + 5.5 (a value block's factor makes halves
 // of the weights anew); 1 x 8 over 2048 11.5 + 4.1 (launches and the first loads'
 // latency).
 #include <math.h>
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 }
 
 // ---- head widths 64, 128 and 256: the products on the matrix cores -----------
-// v_mfma_f32_16x16x32_f16.  A block is 64 NC query rows, 16 NC to a wave, and
+// v_mfma_f32_16x16x32_f16.  A block is 64 NC / KW query rows, 16 NC to a wave, and
 // stages slices of 64 keys (32 at D = 256) in LDS for its four waves, the next
 // slice's words on their way in registers behind the present one's products.
 //
@@ -337,8 +337,8 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 //
 // q8_0: keys and values enter as their integers, exact halves; a key block's
 // factor multiplies its part of the score, a value block's the weights, which
-// are then split into halves (the factors' share of 4 x 25 over 4099: 42 us against
-// 30 of f16; at D = 256 107 against 48, where they do not fit the registers).  The
+// are then split into halves (the factors' share of 4 x 25 over 4099: 40 us against
+// 30 of f16; at D = 256 112 against 48, where they do not fit the registers).  The
 // factors are staged times 2^(11 - X), X the exponent of the largest one so far
 // among committed positions, which every row sees.  In 32 keys that some row does not
 // see whole each row's products are scaled to its own largest and summed apart: what
@@ -466,7 +466,8 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
   __shared__ int holes[2];  // the step whose slice in this buffer has a cell that is not held
   __shared__ int spoilt[2]; // the last (even, odd) run in which some staged value was not finite
   const int tid = threadIdx.x, lane = tid & 63, wave_all = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // KW = 2: waves 2 and 3 have the rows of 0 and 1, and each slice's other 32 keys
+  // KW = 2 (few rows): waves 2 and 3 have the rows of 0 and 1, and each slice's other
+  // 32 keys
   const int wave = wave_all % (4 / KW), half = wave_all / (4 / KW);
   const int lm = lane & 15, lk = lane >> 4;
   const int shift = a.group_shift, group = 1 << shift, words = (a.tree.max_nodes + 31) >> 5;
@@ -500,13 +501,25 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
     struct Stage {
       tu4 kw[PER], vw[PER];
       int cells[PAGED ? PER : 1], fcell[PAGED && Q8 ? FPER : 1];  // (negative: not held)
-      uint16_t f[Q8 ? FPER : 1];  // q8_0: factor tid + 256 j of (key or value, 32-dim block, key)
+      uint16_t f[Q8 ? FPER : 1];  // q8_0: factors
       bool dead;                  // nothing is held where some word was loaded
     };
     Stage st;
     int xrun[Q8 ? FPER : 1];  // q8_0: the X so far of the blocks whose values' factors this thread stages
 #pragma unroll
     for (int j = 0; j < (Q8 ? FPER : 1); j++) xrun[j] = 0;
+    // q8_0: factor tid + 256 j of a slice: the keys' first, then the values', the keys of
+    // a 32-dim block in SL lanes, whose largest X takes.  With KW = 2, where loads are
+    // what a step waits for, the keys' with a key's blocks in neighbouring lanes, so that
+    // their line is asked for once (182 -> 173 us; elsewhere the registers cost more)
+    auto fkey = [&](int j) __attribute__((always_inline)) {
+      const int i = tid + 256 * j;
+      return KW == 2 && i < SL * KS ? i / KS : i % SL;
+    };
+    auto fblock = [&](int j) __attribute__((always_inline)) {
+      const int i = tid + 256 * j;
+      return KW == 2 && i < SL * KS ? i % KS : i / SL % KS;
+    };
     auto cell_at = [&](int j) __attribute__((always_inline)) { return index[min(j, sq.count - 1)]; };
     auto find = [&](int sl, Stage& st) __attribute__((always_inline)) {
       if constexpr (PAGED) {
@@ -514,7 +527,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
         for (int j = 0; j < PER; j++) st.cells[j] = cell_at(sl * SL + (tid + 256 * j) / WPK);
         if constexpr (Q8) {
 #pragma unroll
-          for (int j = 0; j < FPER; j++) st.fcell[j] = cell_at(sl * SL + (tid + 256 * j) % SL);
+          for (int j = 0; j < FPER; j++) st.fcell[j] = cell_at(sl * SL + fkey(j));
         }
       }
     };
@@ -534,11 +547,11 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
       if constexpr (Q8) {
 #pragma unroll
         for (int j = 0; j < FPER; j++) {
-          const int i = tid + 256 * j, at = sl * SL + i % SL;
+          const int i = tid + 256 * j, at = sl * SL + fkey(j);
           int cell = PAGED ? st.fcell[j] : min(at, sq.count - 1);
           if (PAGED) asm volatile("" : "+v"(cell));
           st.f[j] = *(const uint16_t*)((i < SL * KS ? kc : vc) + (int64_t)(PAGED ? max(cell, 0) : cell) * crow + (kvw >> 1) -
-                                       kvh * D / 2 + ((kvh * D) >> 5) + i / SL % KS);
+                                       kvh * D / 2 + ((kvh * D) >> 5) + fblock(j));
           if (at >= sq.count || (PAGED && cell < 0)) st.f[j] = 0;
         }
       }
@@ -577,16 +590,16 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
       if constexpr (Q8) {
 #pragma unroll
         for (int j = 0; j < FPER; j++) {
-          const int i = tid + 256 * j, u = i / SL % KS;
+          const int i = tid + 256 * j, u = fblock(j);
           float f = half_bits_to_float(st.f[j]);
           if (i >= SL * KS) {  // (uniform: the second half of the threads, or of a thread's factors)
             const float af = fabsf(f);
-            const float fm = lanes::reduce<SL>(sl * SL + i % SL < sq.len && af < INFINITY ? af : 0.0f, lanes::Max{});
+            const float fm = lanes::reduce<SL>(sl * SL + fkey(j) < sq.len && af < INFINITY ? af : 0.0f, lanes::Max{});
             if (fm > 0.0f) xrun[j] = max(xrun[j], __builtin_amdgcn_frexp_expf(fm));
             f = ldexpf(f, kFactor - xrun[j]);
             if (i % SL == 0) xs[buf][u] = xrun[j];
           }
-          fac[buf][i / (SL * KS)][u][i % SL] = f;
+          fac[buf][i / (SL * KS)][u][fkey(j)] = f;
         }
       }
     };
@@ -1144,6 +1157,9 @@ TreeGrid tree_grid(int heads, int kv_heads, int head_dim, int form, const mi_tre
   // registers cost the third block: 8 x 48 over 3000 31 us for 29, over 12000 80 for
   // 83; with q8_0 they spill)
   g.columns = head_dim == 128 && form != MI_CACHE_Q8 && t.max_nodes * group > 64 ? 2 : 1;
+  // up to 32 rows are two waves' work, at q8_0 long enough for the other two to take
+  // half of each slice's keys: 64 x 1 nodes over 4096 212 us, so 173; 8 x 8 over 16384
+  // 122 and 101 (f16 waits for its loads, 150 us and 5.4 TB/s)
   g.split = form == MI_CACHE_Q8 && (head_dim == 64 || head_dim == 128) && t.max_nodes * group <= 32 ? 2 : 1;
   g.rows = g.mfma ? 64 * g.columns / g.split : kRowsTile;
   g.slice = g.split == 2 ? 64 : g.mfma ? mfma_slice(head_dim) : rows_slice(head_dim);
