@@ -164,7 +164,7 @@ def device_layer_tree(ctx: gpu.DeviceContext, layer: DeviceLayer, x: torch.Tenso
     kv_index[b].  Rows behind the last sequence come out undefined."""
     i32, f16, s = torch.int32, torch.float16, layer.spec
     batch, tokens = lengths.numel(), pos.numel()
-    stride, least = gpu.tree_cache(kv_index, batch, cache_stride, max_count, gpu.cache_row(form, s.kv_width()))
+    stride, least = gpu.tree_cache(kv_index, batch, cache_stride, max_count, form, s.kv_width())
     on = gpu._on
     tree = MiTree(batch, tokens, max_nodes, max_count, on(ctx, starts, "starts", i32, batch + 1),
                   on(ctx, lengths, "lengths", i32), on(ctx, mask, "mask", i32, tokens * gpu.tree_words(max_nodes)),

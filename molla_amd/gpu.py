@@ -379,10 +379,11 @@ def device_qk_norm_rope(ctx: DeviceContext, q: torch.Tensor, k: torch.Tensor, v:
     _queue(ctx, lib().mi_qk_norm_rope, ctypes.byref(d))
 
 
-def tree_cache(kv_index: torch.Tensor | None, batch: int, cache_stride: int, max_count: int, row: int) -> tuple:
+def tree_cache(kv_index: torch.Tensor | None, batch: int, cache_stride: int, max_count: int, form: int,
+               width: int) -> tuple:
     """(entries of a sequence's list of cells or 0, halves a cache holds at least) of a step over trees."""
     if kv_index is None:
-        return 0, (batch - 1) * cache_stride + max_count * row
+        return 0, (batch - 1) * cache_stride + max_count * cache_row(form, width)
     if kv_index.dim() != 2 or kv_index.shape[0] < batch:
         raise ValueError(f"a step over trees wants a list of cells a sequence ({batch})")
     return kv_index.shape[1], 1
@@ -401,17 +402,19 @@ def device_attend_tree(ctx: DeviceContext, q: torch.Tensor, k_cache: torch.Tenso
     batch, tokens = lengths.numel(), q.shape[0]
     qw = heads * head_dim
     q_stride = _rows(ctx, q, "q", tokens, qw)
-    stride, least = tree_cache(kv_index, batch, cache_stride, max_count, cache_row(form, kv_heads * head_dim))
+    stride, least = tree_cache(kv_index, batch, cache_stride, max_count, form, kv_heads * head_dim)
     tree = MiTree(batch, tokens, max_nodes, max_count, _on(ctx, starts, "starts", i32, batch + 1),
                   _on(ctx, lengths, "lengths", i32), _on(ctx, mask, "mask", i32, tokens * tree_words(max_nodes)))
     L = lib()
     t = ctypes.byref(tree)
     if work is None:
         work = ctx.workspace(L.mi_attend_tree_workspace(heads, kv_heads, head_dim, form, t))
+    else:
+        _on(ctx, work, "work", torch.uint8)
     _queue(ctx, L.mi_attend_tree, form, q.data_ptr(), q_stride, _on(ctx, k_cache, "k_cache", f16, least),
            _on(ctx, v_cache, "v_cache", f16, least), cache_stride,
            None if kv_index is None else _on(ctx, kv_index, "kv_index", i32), stride, heads, kv_heads, head_dim, scale,
-           t, _on(ctx, out, "out", torch.float32, tokens * qw), _on(ctx, work, "work", torch.uint8), work.numel())
+           t, _on(ctx, out, "out", torch.float32, tokens * qw), work.data_ptr(), work.numel())
 
 
 __all__ = [n for n in dir() if not n.startswith("_")] + ["MiError"]
