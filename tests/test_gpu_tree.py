@@ -595,6 +595,31 @@ def test_attend_of_large_and_small_values(form, d, nodes, length, size):
 
 
 @pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d,nodes", [(64, 3), (64, 30), (128, 3), (128, 30), (128, 70), (256, 3), (96, 3)])
+@pytest.mark.parametrize("first,last", [(1e-4, 3e3), (3e3, 1e-4)])
+def test_attend_of_values_whose_size_moves(form, d, nodes, first, last):
+    """Values that grow or shrink along the positions, in each 32 of them at a place of
+    its own; a few queries look at the small ones alone, held to those."""
+    length = 700
+    s = Step(form, [length, 33], [nodes, 3], 2, 1, d, seed=11)
+    g = torch.Generator().manual_seed(12)
+    cells, blocks = len(s.v), d // 32
+    place = (torch.arange(cells)[:, None] + 40 * torch.arange(blocks)[None, :]).clamp(max=length) / length
+    size = first * (last / first) ** place
+    s.v = encode((torch.randn(cells, blocks, 32, generator=g) * size[..., None]).reshape(cells, d), form)
+    s.check(s.run())
+    small = slice(0, 60) if first < last else slice(640, length)
+    s.k[:length] = encode(0.01 * torch.randn(length, d, generator=g), form)
+    along = torch.randn(d, generator=g)
+    s.k[small] = encode(along * (50 / s.scale) / (along @ along) + 0.01 * torch.randn(60, d, generator=g), form)
+    s.q[0] = along.repeat(2)
+    got, want = s.run(), s.want()
+    s.check(got)
+    # the others' weights are 2^-72 of these
+    assert (got[0].double() - want[0]).abs().max() <= 1e-5 * float(s.values(s.v)[small].abs().max())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
 @pytest.mark.parametrize("d,nodes", [(64, 3), (128, 40), (96, 5), (256, 2)])
 def test_attend_without_a_scale(form, d, nodes):
     """Every key weighs the same."""
