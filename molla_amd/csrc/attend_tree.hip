@@ -340,7 +340,9 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 // are then split into halves (the factors' share of 4 x 25 over 4099: 40 us against
 // 30 of f16; at D = 256 112 against 48, where they do not fit the registers).  The
 // factors are staged times 2^(11 - X), X the exponent of the largest one so far
-// among committed positions, which every row sees.  In 32 keys that some row does not
+// among committed positions, which every row sees (a weight's lower half ends at
+// 2^-24: with X held at 0 or above, values near 4e-6 whose weights are 2^-12 of the
+// largest came out 6e-3 of their size off; so 3.6e-7).  In 32 keys that some row does not
 // see whole each row's products are scaled to its own largest and summed apart: what
 // a row does not see has no part in its result.
 //
@@ -361,6 +363,7 @@ typedef uint32_t tu4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLift = 10.0f, kSlack = 4.0f;   // of a weight's exponent: its sum 14 at most
 constexpr int kFactor = 15 - (int)kSlack;       // q8_0: the largest factor's, for weights up to 2^kSlack
+constexpr int kNoFactor = -24;                  // X ahead of the first factor, which is 2^-24 (X = -23) or more
 
 // w f as two halves (ONE: f is 1, in a scalar register that the compiler takes for
 // any value): an instruction each or less, the higher halves opaque so that the
@@ -507,7 +510,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
     Stage st;
     int xrun[Q8 ? FPER : 1];  // q8_0: the X so far of the blocks whose values' factors this thread stages
 #pragma unroll
-    for (int j = 0; j < (Q8 ? FPER : 1); j++) xrun[j] = 0;
+    for (int j = 0; j < (Q8 ? FPER : 1); j++) xrun[j] = kNoFactor;
     // q8_0: factor tid + 256 j of a slice: the keys' first, then the values', the keys of
     // a 32-dim block in SL lanes, whose largest X takes.  With KW = 2, where loads are
     // what a step waits for, the keys' with a key's blocks in neighbouring lanes, so that
@@ -666,7 +669,7 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
       for (int dt = 0; dt < NT; dt++) o[c][dt] = tf4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 #pragma unroll
-    for (int u = 0; u < (Q8 ? KS : 1); u++) xo[u] = 0;
+    for (int u = 0; u < (Q8 ? KS : 1); u++) xo[u] = kNoFactor;
     // a row's mk is too large for a weight's exponent; (uniform) some row's is
     auto large = [&](int c) __attribute__((always_inline)) { return mc[c] > -1e30f && !(fabsf(mk[c]) <= 4e6f); };
     bool huge = false;
