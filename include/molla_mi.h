@@ -370,8 +370,9 @@ int mi_tree_plan(mi_stream stream, int32_t batch, const int32_t* starts, const i
  * both NULL), its first rope_dim values rotated as mi_rope does (rope_factors as
  * in mi_layer_desc, or NULL), in one pass; q to q_out, k to k_out (NULL: not
  * kept), and k and v to cache rows cells[t] of either form (k_cache, v_cache and
- * cells, or all three and v NULL).  A negative cell stores nothing; of
- * tokens with the same cell one is kept.  q_out may be q and k_out k, at the same
+ * cells, or all three and v NULL).  A negative cell stores nothing; a
+ * cell that two tokens name holds no row of either (heads of both, in no order),
+ * every other row is as without them.  q_out may be q and k_out k, at the same
  * stride.  count (device int32, or NULL): rows from
  * *count on are left alone.  The k/v caches are rows of mi_cache_row(cache_form,
  * kv_heads * head_dim) halves. */
