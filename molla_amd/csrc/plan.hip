@@ -8,6 +8,11 @@
 namespace mi {
 namespace {
 
+// a + b of values from 0 to `most`, at most that (their sum may pass 31 bits)
+__device__ __forceinline__ int capped(int a, int b, int most) {
+  return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)most);
+}
+
 // Inclusive sum over a block of T threads, each partial sum at most `most` (with
 // values at least 0 the capped sum is associative); wsum: an int a wave, of LDS.
 template <int T>
@@ -16,15 +21,15 @@ __device__ __forceinline__ int scan_block(int v, int most, int* wsum) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int u = __shfl_up(v, o);
-    if (lane >= o) v = min(v + u, most);
+    if (lane >= o) v = capped(v, u, most);
   }
   __syncthreads();  // (wsum of an earlier scan has been read)
   if (lane == 63) wsum[wave] = v;
   __syncthreads();
   int before = 0;
 #pragma unroll
-  for (int w = 0; w < T / 64 - 1; w++) before = min(before + (w < wave ? wsum[w] : 0), most);
-  return min(before + v, most);
+  for (int w = 0; w < T / 64 - 1; w++) before = capped(before, w < wave ? wsum[w] : 0, most);
+  return capped(before, v, most);
 }
 
 // Every block of T threads scans all requests (at most T * PER, from the cache)
@@ -46,7 +51,7 @@ __global__ __launch_bounds__(T) void page_plan_kernel(PagePlan p) {
     const bool live = b0 + i < p.batch;
     len[i] = live ? max(p.lengths[b0 + i], 0) : 0;
     n[i] = live ? min(max(p.news[b0 + i], 0), p.max_tokens) : 0;
-    sum = min(sum + n[i], p.max_tokens);
+    sum = capped(sum, n[i], p.max_tokens);
   }
   const int free0 = min(max(p.free_count[0], 0), p.free_size);
   // token rows: what does not fit into max_tokens is not planned

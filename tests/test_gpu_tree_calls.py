@@ -36,3 +36,22 @@ def test_cells_that_two_tokens_name(form, d, pad):
     unnamed = [i for i in range(rows) if i not in cells.tolist()] + [int(cells[t]) for t in (7, 30, 31)]
     for a, b in zip(outs[0][2:], outs[1][2:]):
         assert torch.equal(a[own].view(torch.int16), b[own].view(torch.int16)) and (b[unnamed] == 0).all()
+
+
+@pytest.mark.parametrize("batch", [3, 300])
+def test_page_plan_of_the_most_token_rows(batch):
+    """Requests that want 2^30 rows each, of 2^30 rows (4 GiB): the sum of two passes 31 bits."""
+    rows, ctx = 1 << 30, gpu.DeviceContext(0)
+    news = [rows, rows, 5] + [rows] * (batch - 3)
+    table = torch.arange(4 * batch, dtype=torch.int32, device="cuda").reshape(batch, 4)
+    starts, cells, left = ints([-9] * (batch + 1)), torch.full((rows,), -3, dtype=torch.int32, device="cuda"), ints([-5, -5])
+    for first in (0, 7):  # (7: the second request's sum is cut inside it)
+        gpu.device_page_plan(ctx, 16, ints([64] * batch), ints([rows - first] + news[1:]), table, ints([1]), ints([0]), left,
+                             starts, None, None, cells)
+        ctx.synchronize()
+        assert starts.tolist() == [0, rows - first] + [rows] * (batch - 1) and left.tolist() == [0, 0]
+        assert bool((cells == -1).all())  # (the table has no room behind the 64 positions)
+    gpu.device_page_plan(ctx, 16, ints([60] * batch), ints(news), table, ints([1]), ints([0]), left, starts, None, None, cells)
+    ctx.synchronize()
+    assert starts.tolist() == [0] + [rows] * batch
+    assert cells[:4].tolist() == [60, 61, 62, 63] and bool((cells[4:] == -1).all())
