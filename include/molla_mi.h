@@ -348,7 +348,14 @@ int mi_decoder_layer_paged(mi_stream stream, const mi_layer_desc* desc, float* r
  * pos[t] (the position; both may be NULL), and its entry of kv_index (may be
  * NULL), the lists that mi_decoder_layer_paged and mi_attend_tree read.  Token
  * rows past max_tokens are not planned: starts ends there; rows behind the last
- * one keep what they held. */
+ * one keep what they held.
+ * A request holds the pages of its table's first ceil(lengths[b] / page) entries
+ * and no others: what the entries behind them hold is not looked at, and a new page
+ * takes their place.  Where a step's positions are taken back (drafts that were
+ * rejected), the caller puts the pages behind the kept ones, those of entries
+ * ceil(kept / page) to ceil((lengths[b] + news[b]) / page) - 1 that are not -1, back
+ * on the list, from free_pages[free_left[0]] on, ahead of the next plan: else they
+ * are lost. */
 int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* lengths, const int32_t* news,
                  int32_t* table, int32_t table_stride, const int32_t* free_pages, int32_t free_size,
                  const int32_t* free_count, int32_t* free_left, int32_t* kv_index, int64_t index_stride,

@@ -312,7 +312,10 @@ def device_page_plan(ctx: DeviceContext, page: int, lengths: torch.Tensor, news:
     free_pages[:free_count].  Writes starts[batch + 1], the new pages into table
     [batch, pages], seq, pos and cells of every new token (as many rows as they
     have; seq and pos may be None), their entries of kv_index [batch, positions],
-    and free_left = (pages left, pages wanted beyond them).  All int32."""
+    and free_left = (pages left, pages wanted beyond them).  All int32.
+    A request holds its table's first ceil(lengths[b] / page) pages and no others:
+    after drafts were rejected the caller puts the pages behind the kept ones back,
+    from free_pages[free_left[0]] on, ahead of the next plan."""
     i32 = torch.int32
     batch = lengths.numel()
     if table.dim() != 2 or table.shape[0] != batch or (kv_index is not None and (kv_index.dim() != 2 or

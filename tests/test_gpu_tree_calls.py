@@ -55,3 +55,40 @@ def test_page_plan_of_the_most_token_rows(batch):
     ctx.synchronize()
     assert starts.tolist() == [0] + [rows] * batch
     assert cells[:4].tolist() == [60, 61, 62, 63] and bool((cells[4:] == -1).all())
+
+
+@pytest.mark.parametrize("page", [1, 4, 16])
+def test_pages_of_rejected_drafts_go_back(page):
+    """Steps of which a part is taken back, in the header's way and without a look from
+    the host: no page is lost, none is held twice, and kept positions keep their cells."""
+    batch, width, new, pages = 5, 24 if page > 1 else 130, 9, 5 * 130 // page
+    g = torch.Generator().manual_seed(page)
+    ctx = gpu.DeviceContext(0)
+    table = torch.full((batch, width), -1, dtype=torch.int32, device="cuda")
+    free = torch.cat([torch.randperm(pages, generator=g), torch.zeros(1, dtype=torch.int64)]).to(torch.int32).cuda()
+    count, left, lengths = ints([pages]), ints([0, 0]), ints([0] * batch)
+    index = torch.full((batch, width * page), -1, dtype=torch.int32, device="cuda")
+    starts, cells = ints([0] * (batch + 1)), ints([-1] * (batch * new))
+    col = torch.arange(width, device="cuda")
+    held_cells = [[] for _ in range(batch)]
+    for step in range(20):
+        news = torch.randint(0, new + 1, (batch,), generator=g).to(torch.int32).cuda()
+        kept = torch.minimum(torch.randint(0, 6, (batch,), generator=g).to(torch.int32).cuda(), news)
+        gpu.device_page_plan(ctx, page, lengths, news, table, free[:pages], count, left, starts, None, None, cells, index)
+        # the pages behind the kept positions go back: a place on the list each, the others to the spare slot
+        keep, had = -(-(lengths + kept) // page), -(-(lengths + news) // page)
+        back = ((col >= keep[:, None]) & (col < had[:, None])).flatten()
+        place = torch.where(back, left[0] + torch.cumsum(back, 0) - 1, pages)
+        free.index_put_((place,), table.flatten())
+        count.copy_(left[:1] + back.sum())
+        lengths += kept
+        ctx.synchronize()
+        assert left[1] == 0
+        on_list = free[:int(count)].tolist()
+        in_use = [table[b, c].item() for b in range(batch) for c in range(-(-int(lengths[b]) // page))]
+        assert sorted(on_list + in_use) == list(range(pages)), step
+        for b in range(batch):
+            n = int(lengths[b])
+            assert index[b, :len(held_cells[b])].tolist() == held_cells[b]
+            held_cells[b] = index[b, :n].tolist()
+            assert min(held_cells[b], default=0) >= 0
