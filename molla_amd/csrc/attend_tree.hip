@@ -348,7 +348,7 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 //
 // A value that is not finite in a node that some query does not see would give
 // 0 * inf there: such values are staged as zeros and added at the end to the
-// queries that see them.
+// queries that see them, as are those of committed positions.
 //
 // MFMA fragments (16x16x32): lane l holds row / column l % 16 and values
 // 8 (l / 16) .. +8 of the 32; result element i of lane l is row 4 (l / 16) + i,
@@ -948,27 +948,6 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
       __syncthreads();
     }
 
-    // non-finite values of slices that were staged without them, to the rows that
-    // see them (of the other slices', which are in o already, a second time)
-    if (!Q8 && __builtin_expect(spoilt[run & 1] == run, 0) && busy) {
-      for (int j = s0 * SL; j < min(s1 * SL, sq.count); j++) {
-        const int cell = PAGED ? index[j] : j;
-        if (cell < 0) continue;
-        const __half* vr = vc + (int64_t)cell * crow + 4 * lk;
-        const int i = j - sq.len;
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-          const bool sees = i < 0 || ((mask_row(c)[max(i, 0) >> 5] >> (i & 31)) & 1);
-#pragma unroll
-          for (int dt = 0; dt < NT; dt++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const float v = __half2float(vr[16 * dt + e]);
-              if (sees && !(fabsf(v) < INFINITY)) o[c][dt][e] += v;
-            }
-        }
-      }
-    }
     if constexpr (KW == 2) {
       // the two waves of a row to one, by way of the keys' buffers (no more in use; the
       // next run's first slice waits behind the second barrier)
@@ -991,20 +970,67 @@ __global__ __launch_bounds__(256, mfma_blocks(D)) void attend_tree_kernel(TreeAt
       __syncthreads();
     }
     if (!busy || half) return;
+    float sum[NC];
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-      const float sum = across(l[c], lanes::Add{});
-      if (node[c] >= sq.nodes) continue;
-      const int64_t slot = (int64_t)part * ROWS + wave * 16 * NC + 16 * c + lm;
-      float* dst = part < 0 ? a.out + ((int64_t)(sq.t0 + node[c]) * a.heads + kvh * group + ((first_row + 16 * c + lm) & (group - 1))) * D
-                            : parts.acc + slot * D;
-      const float w = part >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
+    for (int c = 0; c < NC; c++) sum[c] = across(l[c], lanes::Add{});
+    auto write = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int dt = 0; dt < NT; dt++) {
-        const float f = Q8 && KW == 1 ? w * ldexpf(1.0f, xo[dt / 2] - kFactor) : w;
-        *(tf4*)(dst + 16 * dt + 4 * lk) = o[c][dt] * f;
+      for (int c = 0; c < NC; c++) {
+        if (node[c] >= sq.nodes) continue;
+        const int64_t slot = (int64_t)part * ROWS + wave * 16 * NC + 16 * c + lm;
+        float* dst = part < 0 ? a.out + ((int64_t)(sq.t0 + node[c]) * a.heads + kvh * group + ((first_row + 16 * c + lm) & (group - 1))) * D
+                              : parts.acc + slot * D;
+        const float w = part >= 0 ? 1.0f : sum[c] != 0.0f ? 1.0f / sum[c] : 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < NT; dt++) {
+          const float f = Q8 && KW == 1 ? w * ldexpf(1.0f, xo[dt / 2] - kFactor) : w;
+          *(tf4*)(dst + 16 * dt + 4 * lk) = o[c][dt] * f;
+        }
+        if (part >= 0 && lk == 0) *(float2*)(parts.ml + 2 * slot) = make_float2(mk[c], sum[c]);
       }
-      if (part >= 0 && lk == 0) *(float2*)(parts.ml + 2 * slot) = make_float2(mk[c], sum);
+    };
+    write();
+    // Values that are not finite.  Of slices that were staged without them they are
+    // missing in o; of the others the halves' products have made NaN (inf times a lower
+    // half of zero): each such sum starts anew from the values that the row sees.  Where
+    // the weights are NaN so is their sum, and the result with it, whatever o is.  (Behind
+    // the stores, which need not wait for the look: 1 x 8 over 2048 15.2 us ahead of them.)
+    if constexpr (!Q8) {
+      bool lost = spoilt[run & 1] == run;
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        tf4 none = {0.0f, 0.0f, 0.0f, 0.0f};  // (zero, or NaN)
+#pragma unroll
+        for (int dt = 0; dt < NT; dt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) none[e] = fmaf(o[c][dt][e], 0.0f, none[e]);
+        lost |= (none[0] + none[1]) + (none[2] + none[3]) != 0.0f && sum[c] == sum[c];
+      }
+      if (__builtin_expect(!__any(lost), 1)) return;
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int dt = 0; dt < NT; dt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[c][dt][e] = fabsf(o[c][dt][e]) < INFINITY ? o[c][dt][e] : 0.0f;
+      for (int j = s0 * SL; j < min(s1 * SL, sq.count); j++) {
+        const int cell = PAGED ? index[j] : j;
+        if (cell < 0) continue;
+        const __half* vr = vc + (int64_t)cell * crow + 4 * lk;
+        const int i = j - sq.len;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          const bool sees = i < 0 || ((mask_row(c)[max(i, 0) >> 5] >> (i & 31)) & 1);
+#pragma unroll
+          for (int dt = 0; dt < NT; dt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float v = __half2float(vr[16 * dt + e]);
+              if (sees && !(fabsf(v) < INFINITY)) o[c][dt][e] += v;
+            }
+        }
+      }
+      write();
     }
   });
 }

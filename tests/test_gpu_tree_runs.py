@@ -107,3 +107,31 @@ def test_sizes_that_move_within_a_run(form, d, nodes, falls, nodes_only):
     for at in (3, 7777, 15001, 20000):
         pointed(s, nodes, 60.0, at)
         check_own_size(s, s.run())
+
+
+@pytest.mark.parametrize("d,nodes", [(64, 3), (64, 40), (128, 3), (128, 70), (256, 3), (96, 3)])
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("length", [70, LENGTH])
+def test_infinities_that_are_seen(d, nodes, paged, length):
+    """An infinite value gives its sign's infinity to whoever sees it, wherever it lies,
+    both signs or a NaN give NaN; every other place of the result keeps its bits."""
+    s = Step("f16", [length, 40], [nodes, 3], 2, 1, d, seed=d, paged=paged)
+    clean = s.run()
+    inf, nan = float("inf"), float("nan")
+    cells = s.index[0].long()
+    for place, v in ((5, inf), (65, -inf), (length // 2 + 1, nan)):  # committed
+        s.v[cells[place], place % d] = v
+    s.v[cells[2], 7], s.v[cells[length - 3], 7] = inf, -inf
+    s.v[cells[3], 9], s.v[cells[length - 1], 9] = -inf, -inf
+    s.v[cells[length], 11] = inf  # the first node: itself and its descendants
+    s.v[cells[length - 2], 12], s.v[cells[length], 12] = inf, -inf
+    want = clean.clone().reshape(s.tokens, 2, d)
+    for place, v in ((5, inf), (65, -inf), (length // 2 + 1, nan)):
+        want[:nodes, :, place % d] = v
+    want[:nodes, :, 7], want[:nodes, :, 9] = nan, -inf
+    sees = torch.tensor([0 in s.seen[t] for t in range(nodes)])
+    want[:nodes, :, 11] = torch.where(sees[:, None], inf, want[:nodes, :, 11])
+    want[:nodes, :, 12] = torch.where(sees[:, None], nan, inf)
+    got = s.run().reshape(s.tokens, 2, d)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got, 0, 1e38, -1e38), torch.nan_to_num(want, 0, 1e38, -1e38))
