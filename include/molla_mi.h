@@ -380,7 +380,8 @@ int mi_tree_plan(mi_stream stream, int32_t batch, const int32_t* starts, const i
  * cells, or all three and v NULL).  A negative cell stores nothing; a
  * cell that two tokens name holds no row of either (heads of both, in no order),
  * every other row is as without them.  q_out may be q and k_out k, at the same
- * stride.  count (device int32, or NULL): rows from
+ * stride; else they share no value with q, k, v or each other (rows of one stride
+ * may lie between one another, as in a fused q|k|v row), nor the caches.  count (device int32, or NULL): rows from
  * *count on are left alone.  The k/v caches are rows of mi_cache_row(cache_form,
  * kv_heads * head_dim) halves. */
 typedef struct {

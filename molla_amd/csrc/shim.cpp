@@ -488,6 +488,16 @@ int mi_tree_plan(mi_stream stream, int32_t batch, const int32_t* starts, const i
   return launch_tree_plan((hipStream_t)stream, batch, starts, lengths, parents, max_nodes, tokens, pos, mask);
 }
 
+// Whether two buffers' rows share a value: `rows` rows of wa values at a, sa apart,
+// and of wb at b.  Rows at one stride may lie between one another (a fused row's
+// parts); at two strides they are taken to meet where their ranges do.
+static bool rows_meet(const float* a, int64_t sa, int64_t wa, const float* b, int64_t sb, int64_t wb, int64_t rows) {
+  if (b >= a + (rows - 1) * sa + wa || a >= b + (rows - 1) * sb + wb) return false;
+  if (sa != sb || rows == 1) return true;
+  const int64_t from = ((b - a) % sa + sa) % sa;
+  return from < wa || from + wb > sa;
+}
+
 int mi_qk_norm_rope(mi_stream stream, const mi_qk* d) {
   if (!d) return fail(MI_ERR_ARG, "qk_norm_rope: null descriptor");
   if (!d->q || !d->k || !d->q_out || !d->rope_steps || !d->pos) return fail(MI_ERR_ARG, "qk_norm_rope: null pointer");
@@ -513,6 +523,23 @@ int mi_qk_norm_rope(mi_stream stream, const mi_qk* d) {
     return fail(MI_ERR_SHAPE, "qk_norm_rope: cache form %d has no row of width %lld", d->cache_form, (long long)kvw);
   if (stores && (((uintptr_t)d->k_cache | (uintptr_t)d->v_cache) & 15))
     return fail(MI_ERR_ALIGN, "qk_norm_rope: the caches must be 16-byte aligned");
+  // (a token's heads are several blocks' work, in no order)
+  struct Rows {
+    const char* name;
+    const float* at;
+    int64_t stride, width;
+  };
+  const Rows in[] = {{"q", d->q, d->q_stride, qw}, {"k", d->k, d->k_stride, kvw}, {"v", d->v, d->v_stride, kvw}};
+  const Rows out[] = {{"q_out", d->q_out, d->q_out_stride, qw}, {"k_out", d->k_out, d->k_out_stride, kvw}};
+  for (int o = 0; o < 2; o++)
+    for (int i = 0; out[o].at && i < 3; i++) {
+      if (!in[i].at || (i == o && in[i].at == out[o].at)) continue;  // (in place)
+      if (rows_meet(out[o].at, out[o].stride, out[o].width, in[i].at, in[i].stride, in[i].width, d->tokens))
+        return fail(MI_ERR_ARG, "qk_norm_rope: %s lies among the rows of %s", out[o].name, in[i].name);
+    }
+  if (d->k_out && rows_meet(d->q_out, d->q_out_stride, qw, d->k_out, d->k_out_stride, kvw, d->tokens))
+    return fail(MI_ERR_ARG, "qk_norm_rope: k_out lies among the rows of q_out");
+  if (stores && d->k_cache == d->v_cache) return fail(MI_ERR_ARG, "qk_norm_rope: one cache for keys and values");
   return launch_qk_rope((hipStream_t)stream, *d);
 }
 

@@ -92,3 +92,30 @@ def test_pages_of_rejected_drafts_go_back(page):
             assert index[b, :len(held_cells[b])].tolist() == held_cells[b]
             held_cells[b] = index[b, :n].tolist()
             assert min(held_cells[b], default=0) >= 0
+
+
+def test_qk_outputs_between_rows():
+    """Outputs at one stride with the inputs, in what those leave free, and in place: as outputs apart."""
+    heads, kv, d, tokens = 8, 2, 64, 50
+    qw, kvw = heads * d, kv * d
+    g = torch.Generator().manual_seed(2)
+    steps = torch.from_numpy(gpu.rope_steps(d, 10000.0)).cuda()
+    data = torch.randn(tokens, qw + 2 * kvw, generator=g).cuda()
+    ctx, outs = gpu.DeviceContext(0), []
+    for how in ("apart", "between", "in place"):
+        row = torch.zeros(tokens, 2 * qw + 3 * kvw, device="cuda")
+        # q | q_out | k | k_out | v
+        q, q_out, k, k_out, v = torch.split(row, [qw, qw, kvw, kvw, kvw], 1)
+        if how == "apart":
+            q_out, k_out = torch.zeros(tokens, qw, device="cuda"), torch.zeros(tokens, kvw, device="cuda")
+        elif how == "in place":
+            q_out, k_out = q, k
+        q.copy_(data[:, :qw]), k.copy_(data[:, qw:qw + kvw]), v.copy_(data[:, qw + kvw:])
+        kc, vc = (torch.zeros(tokens, kvw, dtype=torch.float16, device="cuda") for _ in range(2))
+        gpu.device_qk_norm_rope(ctx, q, k, v, heads, kv, d, d, True, steps, ints(range(tokens)), q_out, kc, vc,
+                                ints(range(tokens)), k_out=k_out)
+        ctx.synchronize()
+        outs.append([t.clone() for t in (q_out, k_out, kc, vc, v)])
+    for other in outs[1:]:
+        for a, b in zip(outs[0], other):
+            assert torch.equal(a, b)
