@@ -355,7 +355,9 @@ int mi_decoder_layer_paged(mi_stream stream, const mi_layer_desc* desc, float* r
  * rejected), the caller puts the pages behind the kept ones, those of entries
  * ceil(kept / page) to ceil((lengths[b] + news[b]) / page) - 1 that are not -1, back
  * on the list, from free_pages[free_left[0]] on, ahead of the next plan: else they
- * are lost. */
+ * are lost.
+ * Nothing that is written may lie in lengths, news, free_pages, free_count or the
+ * table (but that kv_index may be the table where page is 1). */
 int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* lengths, const int32_t* news,
                  int32_t* table, int32_t table_stride, const int32_t* free_pages, int32_t free_size,
                  const int32_t* free_count, int32_t* free_left, int32_t* kv_index, int64_t index_stride,
@@ -369,7 +371,9 @@ int32_t mi_tree_words(int32_t max_nodes);
  * committed tokens; a parent comes before its node (another value makes a root).
  * mask[t * words + i / 32] bit i % 32 says whether token t sees node i of its
  * sequence; pos[t] = lengths[b] + depth (pos may be NULL).  Tokens past
- * max_nodes of a sequence see no node.  tokens: rows of the buffers. */
+ * max_nodes of a sequence see no node.  tokens: rows of the buffers.  pos and mask
+ * lie apart from each other and from the rest, but that either may be parents (mask
+ * where it is a word a token). */
 int mi_tree_plan(mi_stream stream, int32_t batch, const int32_t* starts, const int32_t* lengths,
                  const int32_t* parents, int32_t max_nodes, int32_t tokens, int32_t* pos, uint32_t* mask);
 

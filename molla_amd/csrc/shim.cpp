@@ -438,6 +438,16 @@ int mi_embed(mi_stream stream, const float* embedding, int32_t vocab, int32_t wi
 
 // ---- a step over trees of drafted tokens -------------------------------------
 
+// A buffer of int32 (none where `at` is null), and whether two share a value.
+struct Ints {
+  const char* name;
+  const int32_t* at;
+  int64_t count;
+};
+static bool ints_meet(const Ints& a, const Ints& b) {
+  return a.at && b.at && a.at < b.at + b.count && b.at < a.at + a.count;
+}
+
 int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* lengths, const int32_t* news,
                  int32_t* table, int32_t table_stride, const int32_t* free_pages, int32_t free_size,
                  const int32_t* free_count, int32_t* free_left, int32_t* kv_index, int64_t index_stride,
@@ -452,6 +462,20 @@ int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* l
   if (kv_index && index_stride < 1) return fail(MI_ERR_SHAPE, "page_plan: index stride %lld", (long long)index_stride);
   if (max_tokens < 1 || max_tokens > kMaxTreeRows)
     return fail(MI_ERR_SHAPE, "page_plan: max_tokens %d outside 1..%d", max_tokens, kMaxTreeRows);
+  // (every block reads all of the inputs, in no order with the others' stores)
+  const int64_t room = (int64_t)table_stride * page, list = kv_index ? std::min<int64_t>(index_stride, room) : 0;
+  const Ints in[] = {{"lengths", lengths, batch}, {"news", news, batch}, {"free_pages", free_pages, free_size},
+                     {"free_count", free_count, 1}, {"the table", table, (int64_t)batch * table_stride}};
+  const Ints out[] = {{"the table", table, in[4].count}, {"starts", starts, (int64_t)batch + 1}, {"free_left", free_left, 2},
+                      {"seq", seq, max_tokens}, {"pos", pos, max_tokens}, {"cells", cells, max_tokens},
+                      {"kv_index", kv_index, kv_index ? (batch - 1) * index_stride + list : 0}};
+  for (const Ints& o : out)
+    for (const Ints& i : in) {
+      if (&o == out && &i == in + 4) continue;
+      // (with pages of one position a request's table is its list)
+      if (o.at == kv_index && i.at == table && o.at == i.at && page == 1 && index_stride == table_stride) continue;
+      if (ints_meet(o, i)) return fail(MI_ERR_ARG, "page_plan: %s lies in %s", o.name, i.name);
+    }
   PagePlan p{};
   p.batch = batch;
   p.page = page;
@@ -485,6 +509,17 @@ int mi_tree_plan(mi_stream stream, int32_t batch, const int32_t* starts, const i
   if (mi_tree_words(max_nodes) < 0)
     return fail(MI_ERR_SHAPE, "tree_plan: trees of %d nodes, outside 1..%d", max_nodes, kMaxTreeNodes);
   if (tokens < 1 || tokens > kMaxTreeRows) return fail(MI_ERR_SHAPE, "tree_plan: %d token rows", tokens);
+  // (a sequence's block reads its parents ahead of its first store, so that a row of one
+  // value may take its parent's place)
+  const int64_t words = mi_tree_words(max_nodes);
+  const Ints in[] = {{"starts", starts, (int64_t)batch + 1}, {"lengths", lengths, batch}, {"parents", parents, tokens}};
+  const Ints out[] = {{"pos", pos, tokens}, {"mask", (const int32_t*)mask, tokens * words}};
+  for (const Ints& o : out)
+    for (const Ints& i : in) {
+      if (i.at == parents && o.at == i.at && o.count == i.count) continue;
+      if (ints_meet(o, i)) return fail(MI_ERR_ARG, "tree_plan: %s lies in %s", o.name, i.name);
+    }
+  if (ints_meet(out[0], out[1])) return fail(MI_ERR_ARG, "tree_plan: pos lies in the mask");
   return launch_tree_plan((hipStream_t)stream, batch, starts, lengths, parents, max_nodes, tokens, pos, mask);
 }
 

@@ -1,11 +1,12 @@
 """Calls of a step over trees of drafted tokens that the header allows and the tests
 of its results do not make."""
 
+import numpy as np
 import pytest
 import torch
 
 from molla_amd import gpu
-from tests.test_gpu_tree import FORMS, ints
+from tests.test_gpu_tree import FORMS, draft, ints, starts_of, words_of
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +120,39 @@ def test_qk_outputs_between_rows():
     for other in outs[1:]:
         for a, b in zip(outs[0], other):
             assert torch.equal(a, b)
+
+
+def test_tree_plan_in_the_place_of_parents():
+    """pos, or a mask of one word, where the parents were."""
+    ctx = gpu.DeviceContext(0)
+    counts, lens = [20, 0, 31], [5, 6, 7]
+    parents, seen, depth = draft(counts, 3)
+    words = words_of(seen, 1)
+    first = np.repeat(lens, counts)
+    for which in ("pos", "mask"):
+        p, other = ints(parents), ints([0] * len(parents))
+        pos, mask = (p, other) if which == "pos" else (other, p)
+        gpu.device_tree_plan(ctx, starts_of(counts), ints(lens), p, 31, pos, mask)
+        ctx.synchronize()
+        assert pos.tolist() == [int(n) + d for n, d in zip(first, depth)]
+        assert mask.tolist() == words[:, 0].tolist()
+
+
+def test_page_plan_of_one_position_a_page():
+    """With pages of one position the table and the list are one buffer."""
+    lens, news, width = [3, 0, 7], [4, 5, 0], 12
+    free = torch.randperm(40).to(torch.int32)[:20]
+    table = torch.full((3, width), -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        table[b, :n] = torch.arange(n) + 50 + 10 * b
+    outs = []
+    for shared in (False, True):
+        t = table.cuda()
+        index = t if shared else table.cuda()
+        starts, cells, left = ints([0] * 4), ints([-1] * 9), ints([0, 0])
+        gpu.device_page_plan(gpu.DeviceContext(0), 1, ints(lens), ints(news), t, free.cuda(), ints([20]), left, starts, None,
+                             None, cells, index)
+        torch.cuda.synchronize()
+        outs.append((t, index, starts, cells, left))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
