@@ -437,6 +437,7 @@ typedef struct {
  * An f16 value that it sees and that is not finite gives its place of the result
  * its infinity, or NaN (for NaN, and for both signs); a key or a q8_0 factor that it
  * sees and that is not finite leaves the heads over it undefined.
+ * The scale is finite.
  * GQA groups and head widths as mi_attend.  Workspace:
  * mi_attend_tree_workspace, 256-byte aligned. */
 size_t mi_attend_tree_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form,

@@ -33,8 +33,8 @@ namespace mi {
 int check_weight(const char* name, int kind, const void* w, int64_t row_bytes, int32_t rows, int32_t cols);
 int check_tree(const char* name, const mi_tree* t, bool layer);
 int check_tree_caches(const char* name, int32_t form, int32_t heads, int32_t kv_heads, int32_t head_dim,
-                      const uint16_t* k_cache, const uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index,
-                      int64_t index_stride, const mi_tree* tree);
+                      float scale, const uint16_t* k_cache, const uint16_t* v_cache, int64_t cache_stride,
+                      const int32_t* kv_index, int64_t index_stride, const mi_tree* tree);
 }
 
 using namespace mi;
@@ -872,7 +872,7 @@ int mi_decoder_layer_tree(mi_stream stream, const mi_layer_desc* d, float* resid
   if (rc) return rc;
   if (!resid || !k_cache || !v_cache) return fail(MI_ERR_ARG, "layer: null pointer");
   if ((rc = check_tree("layer", tree, true))) return rc;
-  if ((rc = check_tree_caches("layer", d->cache_form, d->heads, d->kv_heads, d->head_dim, k_cache, v_cache,
+  if ((rc = check_tree_caches("layer", d->cache_form, d->heads, d->kv_heads, d->head_dim, d->attn_scale, k_cache, v_cache,
                               cache_stride, kv_index, index_stride, tree)))
     return rc;
   if (tree->tokens > kMaxPrefill)

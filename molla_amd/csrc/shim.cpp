@@ -7,6 +7,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "mi_internal.h"
 
@@ -57,10 +58,12 @@ int check_tree(const char* name, const mi_tree* t, bool layer) {
   return MI_OK;
 }
 
-// The caches of a step over trees (check_tree has passed).
+// The caches of a step over trees and the scores' scale, of which a NaN would be taken for
+// the least one (check_tree has passed).
 int check_tree_caches(const char* name, int32_t form, int32_t heads, int32_t kv_heads, int32_t head_dim,
-                      const uint16_t* k_cache, const uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index,
-                      int64_t index_stride, const mi_tree* tree) {
+                      float scale, const uint16_t* k_cache, const uint16_t* v_cache, int64_t cache_stride,
+                      const int32_t* kv_index, int64_t index_stride, const mi_tree* tree) {
+  if (!std::isfinite(scale)) return fail(MI_ERR_ARG, "%s: the scale of the scores has to be finite", name);
   if ((int64_t)heads * head_dim > kMaxHeadsWidth)
     return fail(MI_ERR_SHAPE, "%s: rows of %lld values", name, (long long)heads * head_dim);
   const int32_t row = cache_row(form, kv_heads * head_dim);
@@ -595,8 +598,8 @@ int mi_attend_tree(mi_stream stream, int32_t form, const float* q, int64_t q_str
   int rc = check_attn("attend_tree", heads, kv_heads, head_dim);
   if (rc) return rc;
   if ((rc = check_tree("attend_tree", tree, false))) return rc;
-  if ((rc = check_tree_caches("attend_tree", form, heads, kv_heads, head_dim, k_cache, v_cache, cache_stride, kv_index,
-                              index_stride, tree)))
+  if ((rc = check_tree_caches("attend_tree", form, heads, kv_heads, head_dim, scale, k_cache, v_cache, cache_stride,
+                              kv_index, index_stride, tree)))
     return rc;
   if (q_stride < (int64_t)heads * head_dim) return fail(MI_ERR_SHAPE, "attend_tree: row stride too small");
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || q_stride % 4)
