@@ -1045,7 +1045,7 @@ __global__ __launch_bounds__(256) void attend_tree_fold_kernel(TreeAttend a, Tre
   __shared__ vec sums[W > 1 ? W : 1][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int D = a.head_dim, shift = a.group_shift;
-  const uint32_t i = blockIdx.x * (4 / W) + wave / W, step = (uint32_t)a.tree.max_nodes * a.heads;  // (both below 2^31)
+  const uint32_t i = grid_block() * (4 / W) + wave / W, step = (uint32_t)a.tree.max_nodes * a.heads;  // (both below 2^31)
   const int b = (int)(i / step);
   if (b >= a.tree.batch) return;  // (W > 1: every wave of the block)
   const int at = (int)(i - b * step), node = at / a.heads, h = at - node * a.heads;
@@ -1116,7 +1116,7 @@ __global__ __launch_bounds__(256) void attend_tree_fold_rows_kernel(TreeAttend a
                                                                     int slice) {
   constexpr int R = 64 / L, D = 4 * L, J = kMaxParts / L;
   const int lane = threadIdx.x & 63, l = lane % L, shift = a.group_shift;
-  const uint32_t job = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t job = grid_block() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t runs = ((a.tree.max_nodes << shift) + R - 1) / R, pair = job / runs;
   const int b = (int)(pair / a.kv_heads), kvh = (int)(pair - b * a.kv_heads), r0 = (int)(job - pair * runs) * R;
   if (b >= a.tree.batch) return;
@@ -1232,7 +1232,7 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   // 3200 of 10 5.8 and 12.2), else several rows a wave where a row is 64 or 128 values
   const int64_t rows = (int64_t)a.tree.batch * a.tree.max_nodes * a.heads;
   const int waves = rows <= 1024 ? 4 : 1;
-  const uint32_t fold = (uint32_t)((rows * waves + 3) / 4);
+  const dim3 fold = grid_of((rows * waves + 3) / 4);
   const TreeCarve c = tree_carve(g, a.head_dim, a.tree.batch);
   const TreeParts parts{(float*)work, (float*)((char*)work + c.ml)};
   int32_t* plan = (int32_t*)((char*)work + c.plan);
@@ -1286,15 +1286,15 @@ int launch_tree_attend(hipStream_t s, const TreeAttend& step, void* work) {
   if (int rc = hip_check(hipGetLastError(), "attend_tree launch")) return rc;
 #define MI_TREE_FOLD(V)                                                                                            \
   if (waves == 4)                                                                                                  \
-    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 4>), dim3(fold), dim3(256), 0, s, a, parts, plan, g.rows, \
+    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 4>), fold, dim3(256), 0, s, a, parts, plan, g.rows, \
                        g.slice);                                                                                   \
   else                                                                                                             \
-    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 1>), dim3(fold), dim3(256), 0, s, a, parts, plan, g.rows, \
+    hipLaunchKernelGGL((attend_tree_fold_kernel<V, 1>), fold, dim3(256), 0, s, a, parts, plan, g.rows, \
                        g.slice)
   if (waves == 1 && (a.head_dim == 64 || a.head_dim == 128)) {
     const int per_wave = a.head_dim == 64 ? 4 : 2;
     const int64_t runs = ((int64_t)a.tree.max_nodes * a.heads / a.kv_heads + per_wave - 1) / per_wave;
-    const dim3 folds((uint32_t)((a.tree.batch * a.kv_heads * runs + 3) / 4));
+    const dim3 folds = grid_of(((int64_t)a.tree.batch * a.kv_heads * runs + 3) / 4);
     if (a.head_dim == 64)
       hipLaunchKernelGGL(attend_tree_fold_rows_kernel<16>, folds, dim3(256), 0, s, a, parts, plan, g.rows, g.slice);
     else

@@ -327,7 +327,17 @@ size_t tree_attend_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, 
 bool tree_attend_fits(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const mi_tree& tree);
 int launch_tree_attend(hipStream_t s, const TreeAttend& a, void* work);
 
+// A launch has fewer than 2^32 threads a dimension: more than 2^22 blocks (of up to 512
+// threads) in rows of 2^22, the last of which may be longer than what is left.
+constexpr int kGridRow = 22;
+inline dim3 grid_of(int64_t blocks) {
+  const int64_t row = 1 << kGridRow;
+  return blocks <= row ? dim3((uint32_t)blocks) : dim3((uint32_t)row, (uint32_t)((blocks + row - 1) / row));
+}
+
 // ---- small device helpers -----------------------------------------------
+
+__device__ __forceinline__ uint32_t grid_block() { return blockIdx.x + (blockIdx.y << kGridRow); }
 
 __device__ __forceinline__ float half_bits_to_float(uint32_t h16) {
   return __half2float(__ushort_as_half((unsigned short)(h16 & 0xFFFFu)));

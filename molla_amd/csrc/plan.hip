@@ -131,11 +131,13 @@ __global__ __launch_bounds__(T) void page_plan_kernel(PagePlan p) {
 __global__ __launch_bounds__(kMaxTreeNodes) void tree_plan_kernel(const int32_t* __restrict__ starts,
                                                                   const int32_t* __restrict__ lengths,
                                                                   const int32_t* __restrict__ parents, int max_nodes,
-                                                                  int words, int tokens, int32_t* __restrict__ pos,
-                                                                  uint32_t* __restrict__ mask) {
+                                                                  int words, int batch, int tokens,
+                                                                  int32_t* __restrict__ pos, uint32_t* __restrict__ mask) {
   __shared__ uint32_t set[kMaxTreeNodes / 32][kMaxTreeNodes];
   __shared__ int jump[kMaxTreeNodes], depth[kMaxTreeNodes];
-  const int b = blockIdx.x, i = threadIdx.x;
+  const int i = threadIdx.x;
+  const uint32_t b = grid_block();
+  if (b >= (uint32_t)batch) return;  // (the whole block)
   const int s0 = min(max(starts[b], 0), tokens), s1 = min(max(starts[b + 1], s0), tokens);
   const int n = s1 - s0;
   const bool node = i < min(n, max_nodes);
@@ -199,8 +201,8 @@ int launch_page_plan(hipStream_t s, const PagePlan& p) {
 
 int launch_tree_plan(hipStream_t s, int32_t batch, const int32_t* starts, const int32_t* lengths,
                      const int32_t* parents, int32_t max_nodes, int32_t tokens, int32_t* pos, uint32_t* mask) {
-  hipLaunchKernelGGL(tree_plan_kernel, dim3(batch), dim3((max_nodes + 63) / 64 * 64), 0, s, starts, lengths, parents,
-                     max_nodes, (max_nodes + 31) / 32, tokens, pos, mask);
+  hipLaunchKernelGGL(tree_plan_kernel, grid_of(batch), dim3((max_nodes + 63) / 64 * 64), 0, s, starts, lengths, parents,
+                     max_nodes, (max_nodes + 31) / 32, batch, tokens, pos, mask);
   return hip_check(hipGetLastError(), "tree_plan launch");
 }
 

@@ -31,7 +31,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_rope_kernel(mi_qk d, int heads_
   extern __shared__ float stage[];  // Q8: a head's values a lane group
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane % LPH, grp = lane / LPH;
-  const int64_t job = (int64_t)blockIdx.x * (kQkThreads / 64) + wave;
+  const int64_t job = (int64_t)grid_block() * (kQkThreads / 64) + wave;
   const int64_t t64 = job / runs;
   if (t64 >= d.tokens || (d.count && t64 >= *d.count)) return;
   const int t = (int)t64, first = (int)(job - t64 * runs) * per, last = min(first + per, heads_all);
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(kQkThreads) void qk_rope_vec_kernel(mi_qk d, int he
 #pragma clang fp contract(off)
   constexpr int GROUPS = 64 / LPH, D = 4 * LPH;
   const int lane = threadIdx.x & 63, l = lane % LPH, grp = lane / LPH;
-  const int64_t job = (int64_t)blockIdx.x * (kQkThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t job = (int64_t)grid_block() * (kQkThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t64 = job / runs;
   if (t64 >= d.tokens || (d.count && t64 >= *d.count)) return;
   const int t = (int)t64, first = (int)(job - t64 * runs) * per, last = min(first + per, heads_all);
@@ -330,7 +330,7 @@ int launch_qk_rope(hipStream_t s, const mi_qk& d) {
   if (blocks > 0x7fffffff) return fail(MI_ERR_SHAPE, "qk_norm_rope: %d tokens of %d heads", d.tokens, heads_all);
   if (vec) {
 #define MI_QKV(LPH, N, Q)                                                                                             \
-  hipLaunchKernelGGL((qk_rope_vec_kernel<LPH, N, Q>), dim3((uint32_t)blocks), dim3(kQkThreads), 0, s, d, heads_all, \
+  hipLaunchKernelGGL((qk_rope_vec_kernel<LPH, N, Q>), grid_of(blocks), dim3(kQkThreads), 0, s, d, heads_all, \
                      per, runs)
 #define MI_QKV_F(LPH)                      \
   if (d.neox) {                            \
@@ -349,10 +349,10 @@ int launch_qk_rope(hipStream_t s, const mi_qk& d) {
   }
 #define MI_QK(LPH, NS)                                                                                              \
   if (q8)                                                                                                           \
-    hipLaunchKernelGGL((qk_rope_kernel<LPH, NS, true>), dim3((uint32_t)blocks), dim3(kQkThreads),                   \
+    hipLaunchKernelGGL((qk_rope_kernel<LPH, NS, true>), grid_of(blocks), dim3(kQkThreads),                   \
                        sizeof(float) * d.head_dim * (kQkThreads / LPH), s, d, heads_all, per, runs);                \
   else                                                                                                              \
-    hipLaunchKernelGGL((qk_rope_kernel<LPH, NS, false>), dim3((uint32_t)blocks), dim3(kQkThreads), 0, s, d, heads_all, \
+    hipLaunchKernelGGL((qk_rope_kernel<LPH, NS, false>), grid_of(blocks), dim3(kQkThreads), 0, s, d, heads_all, \
                        per, runs)
   if (d.head_dim <= 64) MI_QK(32, 1);
   else if (d.head_dim <= 128) MI_QK(64, 1);

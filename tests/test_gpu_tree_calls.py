@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from molla_amd import gpu
-from tests.test_gpu_tree import FORMS, draft, ints, starts_of, words_of
+from tests.test_gpu_tree import FORMS, Step, draft, ints, starts_of, words_of
 
 pytestmark = pytest.mark.gpu
 
@@ -156,3 +156,60 @@ def test_page_plan_of_one_position_a_page():
         outs.append((t, index, starts, cells, left))
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+# ---- launches of more than 2^32 threads ------------------------------------------
+@pytest.mark.parametrize("d", [32, 64])
+def test_qk_of_many_tokens(d):
+    """More than 2^26 rows: each as in a short call."""
+    tokens, ctx = (1 << 26) + 9, gpu.DeviceContext(0)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(d)
+    q = torch.randn(tokens, d, generator=g, device="cuda")
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    steps = torch.from_numpy(gpu.rope_steps(d, 10000.0)).cuda()
+    out = torch.full((tokens, d), -3.0, device="cuda")
+    gpu.device_qk_norm_rope(ctx, q, q, None, 1, 1, d, d, True, steps, pos, out)
+    for first in (0, tokens // 2, tokens - 1000):
+        part = torch.full((1000, d), -4.0, device="cuda")
+        at = slice(first, first + 1000)
+        gpu.device_qk_norm_rope(ctx, q[at], q[at], None, 1, 1, d, d, True, steps, pos[at], part)
+        ctx.synchronize()
+        assert torch.equal(out[at], part)
+    assert not bool((out == -3.0).all(1).any())
+
+
+def test_tree_plan_of_many_sequences():
+    batch, ctx = (1 << 24) + 5, gpu.DeviceContext(0)
+    counts = torch.zeros(batch, dtype=torch.int32)
+    live = [0, 77, 1 << 23, batch - 2, batch - 1]
+    sizes = [256, 3, 40, 1, 100]
+    for b, n in zip(live, sizes):
+        counts[b] = n
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), torch.cumsum(counts, 0)]).to(torch.int32).cuda()
+    lengths = torch.arange(batch, dtype=torch.int32).cuda()
+    parents, seen, depth = draft(sizes, 6)
+    pos, mask = ints([-3] * len(parents)), ints([[-3] * 8] * len(parents))
+    gpu.device_tree_plan(ctx, starts, lengths, ints(parents), 256, pos, mask)
+    ctx.synchronize()
+    assert pos.tolist() == [int(n) + d for n, d in zip(np.repeat(live, sizes), depth)]
+    assert (mask.cpu().numpy() == words_of(seen, 8)).all()
+
+
+@pytest.mark.parametrize("heads,kv,d,batch", [(8, 1, 256, 40000), (8, 1, 64, 131100), (8, 1, 128, 65600), (8, 2, 96, 40000)])
+def test_attend_of_many_sequences(heads, kv, d, batch):
+    """Room for more rows than a launch has threads; the rows that are there are shared by blocks."""
+    s = Step("f16", [300, 41, 290, 7], [5, 0, 9, 2], heads, kv, d, seed=1, paged=True)
+    live = [0, 500, batch - 2, batch - 1]
+    lens, counts = torch.zeros(batch, dtype=torch.int32), torch.zeros(batch, dtype=torch.int64)
+    index = torch.full((batch, s.room), -1, dtype=torch.int32)
+    for i, b in enumerate(live):
+        lens[b], counts[b], index[b] = s.lens[i], s.counts[i], s.index[i]
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), torch.cumsum(counts, 0)]).to(torch.int32)
+    mask = np.concatenate([words_of(s.seen, 8), np.full((s.tokens - len(s.seen), 8), -1, np.int32)])
+    out = torch.full((s.tokens, heads * d), -3.0, device="cuda")
+    ctx = gpu.DeviceContext(0)
+    gpu.device_attend_tree(ctx, s.q.cuda(), s.k.cuda(), s.v.cuda(), heads, kv, d, s.scale, starts.cuda(), lens.cuda(), ints(mask),
+                           256, s.max_count, out, kv_index=index.cuda())
+    ctx.synchronize()
+    s.check(out.cpu())
