@@ -135,3 +135,77 @@ def test_infinities_that_are_seen(d, nodes, paged, length):
     got = s.run().reshape(s.tokens, 2, d)
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     assert torch.equal(torch.nan_to_num(got, 0, 1e38, -1e38), torch.nan_to_num(want, 0, 1e38, -1e38))
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d,nodes", NODES + [(128, 70), (32, 3), (512, 3)])
+@pytest.mark.parametrize("rise", [0.004, 0.08, 1.9, 2.76, 2.85, 5.6, -0.08])
+def test_rising_scores_within_a_run(form, d, nodes, rise):
+    """Scores that rise over each 450 positions, by `rise` a key or (from 1 on) a 50th
+    key: the running maximum moves inside a block's run at every slice, at some, or by
+    just less and just more than what the sums are left alone for."""
+    s = Step(form, [LENGTH, 40], [nodes, 2], 1, 1, d)
+    g = torch.Generator().manual_seed(7)
+    along = torch.randn(d, generator=g)
+    steps = torch.arange(LENGTH, dtype=torch.float32) % 450
+    score = rise * (steps if rise < 1 else (steps / 50).floor())
+    s.k[:LENGTH] = encode((score - (score.max() + score.min()) / 2)[:, None] / s.scale * along / (along @ along) +
+                          0.02 * torch.randn(LENGTH, d, generator=g), form)
+    s.q[:nodes] = along * (1 + 0.01 * torch.randn(nodes, 1, generator=g))
+    check_own_size(s, s.run())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d,nodes", NODES + [(128, 70), (32, 20), (512, 3)])
+def test_positions_not_held_within_a_run(form, d, nodes):
+    """Cells that are not held: one in seven, whole slices, the ends of some, all of a sequence's."""
+    s = Step(form, [LENGTH, 300, 90], [nodes, 3, 2], 2, 1, d, seed=d, paged=True)
+    s.index[0, 5:LENGTH - 900:7] = -1
+    for a, n in ((0, 32), (640, 64), (3000, 1000), (8000 - 3, 70), (LENGTH - 500, 40), (LENGTH - 2, 1)):
+        s.index[0, a:a + n] = -1
+    s.index[1, 40:200] = -1
+    s.index[2, :90] = -1
+    check_own_size(s, s.run())
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("heads,kv,d,nodes", [(4, 2, 96, 6), (4, 4, 32, 20), (2, 1, 512, 5), (4, 2, 64, 6), (2, 1, 128, 40),
+                                              (2, 1, 256, 6)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -65504.0])
+@pytest.mark.parametrize("length,paged", [(70, False), (70, True), (LENGTH, True)])
+def test_what_is_not_seen(form, heads, kv, d, nodes, bad, length, paged):
+    """What lies in nodes that a token does not see, in slots behind the sequence and in
+    cells that are not held changes no bit of its result, at every kind of head width
+    and where a block walks several slices."""
+    s = Step(form, [length, 30], [nodes, nodes], heads, kv, d, seed=d, paged=paged)
+    for t in range(2 * nodes):  # the last node is seen by itself alone, the one before by nobody
+        s.seen[t] -= {nodes - 2}
+        if t % nodes != nodes - 1:
+            s.seen[t] -= {nodes - 1}
+    if paged:
+        s.index[0, 11::23] = -1
+        s.index[1, 0] = -1
+    clean = s.run()
+    check_own_size(s, clean)
+    kvw = kv * d
+    held = {int(s.index[b, j]) for b, n in enumerate(s.lens) for j in range(n + nodes) if j != n + nodes - 2}
+    hidden = torch.tensor([i for i in range(len(s.k)) if i not in held])
+    for c in (s.k, s.v):
+        if form == "f16":
+            c[hidden] = bad
+        else:
+            c[hidden, kvw // 2:kvw // 2 + kvw // 32] = bad
+    assert torch.equal(s.run(), clean)
+    # the last node's own value (not its key) goes to itself alone
+    for b, n in enumerate(s.lens):
+        i = int(s.index[b, n + nodes - 1])
+        if form == "f16":
+            s.v[i] = bad
+        else:
+            s.v[i, kvw // 2:kvw // 2 + kvw // 32] = bad
+    got = s.run()
+    last = [nodes - 1, 2 * nodes - 1]
+    others = [t for t in range(s.tokens) if t not in last]
+    assert torch.equal(got[others], clean[others])
+    if not abs(bad) < float("inf"):
+        assert not torch.isfinite(got[last]).any()
