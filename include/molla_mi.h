@@ -435,8 +435,9 @@ typedef struct {
  * sees nothing gets zeros; rows behind the last sequence keep what they held.
  * What a token does not see changes no bit of its result, whatever it holds.
  * An f16 value that it sees and that is not finite gives its place of the result
- * its infinity, or NaN (for NaN, and for both signs); a key or a q8_0 factor that it
- * sees and that is not finite leaves the heads over it undefined.
+ * its infinity, or NaN (for NaN, for both signs, and where its weight may be below
+ * 2^-126 of the largest); a key or a q8_0 factor that it sees and that is not finite
+ * leaves the heads over it undefined.
  * The scale is finite.
  * GQA groups and head widths as mi_attend.  Workspace:
  * mi_attend_tree_workspace, 256-byte aligned. */

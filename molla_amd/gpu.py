@@ -82,7 +82,9 @@ def row_bytes(kind: int, cols: int) -> int:
 class DeviceContext:
     """One device and one stream, like MAX's DeviceContext in the reference
     (one per process, tests/main.mojo:52-60).  Holds the workspace the
-    library draws scratch from; it grows on demand and is reused."""
+    library draws scratch from; it grows on demand and is reused.  Calls of one
+    context and the graphs captured on it share that workspace and run one after
+    the other: what is to overlap takes a context each, or workspaces of its own."""
 
     def __init__(self, device: int = 0, stream: torch.cuda.Stream | None = None):
         if not torch.cuda.is_available():

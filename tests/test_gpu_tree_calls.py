@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from molla_amd import gpu
-from tests.test_gpu_tree import FORMS, Step, draft, ints, starts_of, words_of
+from tests.test_gpu_tree import FORMS, Draft, Step, draft, ints, starts_of, words_of
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +213,61 @@ def test_attend_of_many_sequences(heads, kv, d, batch):
                            256, s.max_count, out, kv_index=index.cuda())
     ctx.synchronize()
     s.check(out.cpu())
+
+
+# ---- captured calls --------------------------------------------------------------
+@pytest.mark.parametrize("form,heads,kv,d", [("f16", 4, 2, 256), ("q8", 4, 2, 96)])
+def test_a_first_call_that_is_captured(form, heads, kv, d):
+    """A context whose first calls are a capture, its workspace made there: each replay as
+    the eager calls between them, and the workspace outlives the graph."""
+    stream = torch.cuda.Stream()
+    ctx = gpu.DeviceContext(0, stream)
+    s = Draft(ctx, form, heads, kv, d)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        s.step()
+    for _ in range(3):
+        s.out.fill_(-3.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        ctx.synchronize()
+        replayed = s.check()
+        s.out.fill_(-3.0)
+        torch.cuda.synchronize()
+        s.step()
+        ctx.synchronize()
+        assert torch.equal(s.out, replayed)
+    del graph
+    other = torch.full((1 << 22,), 7.0, device="cuda")
+    s.out.fill_(-3.0)
+    torch.cuda.synchronize()
+    s.step()
+    ctx.synchronize()
+    assert torch.equal(s.out, replayed) and bool((other == 7.0).all())
+
+
+def test_two_graphs_of_one_context():
+    """Captured on one context they share its workspace, and run one after the other."""
+    stream = torch.cuda.Stream()
+    ctx = gpu.DeviceContext(0, stream)
+    steps, graphs, want = [Draft(ctx, "f16"), Draft(ctx, "q8", 8, 8, 128)], [], []
+    torch.cuda.synchronize()
+    for s in steps:
+        s.step()
+        ctx.synchronize()
+        want.append(s.check())
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            s.step()
+    for order in ((0, 1, 0), (1, 1, 0, 1)):
+        for s in steps:
+            s.out.fill_(-3.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for i in order:
+                graphs[i].replay()
+        ctx.synchronize()
+        for s, w in zip(steps, want):
+            assert torch.equal(s.out, w)
