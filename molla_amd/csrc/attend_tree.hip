@@ -13,15 +13,18 @@
 // parts for every tile as the longest sequence needs, the fold of 13 nodes over
 // 32768 positions took 46 us, that of 8 over 2048 14; so 5.6 and 4.1.)
 //
-// Measured, products + fold, heads 32 over 8 (over 4 at width 64): 8 sequences of
-// up to 64 nodes over 8192 down to 4608 positions at width 128 132 + 8.6 us (292
-// TFLOP/s of the formula's products, twice that of the matrix cores', whose steps
-// take turns with the softmax on the VALU at two waves a SIMD); 8 x 48 over 3000
-// down to 1691 at width 64 29.4 + 5.1 (bound by a step's chain of latencies at three
-// waves a SIMD); 1 x 13 over 32768 36.6 + 5.6 (3.7 TB/s; 6 once the first slices are
-// there); 4 x 25 over 4099 of q8_0 39.9 + 5.5 (a value block's factor makes halves
-// of the weights anew); 1 x 8 over 2048 11.5 + 4.1 (launches and the first loads'
-// latency).
+// Measured, products + fold under the profiler, heads 32 over 8 (over 4 at width 64):
+// 8 sequences of up to 64 nodes over 8192 down to 4608 positions at width 128 122 to
+// 147 + 8.7 us, the whole call among others 119 (324 TFLOP/s of the formula's products,
+// twice that of the matrix cores', whose steps take turns with the softmax on the VALU
+// at two waves a SIMD); 8 x 48 over 3000 down to 1691 at width 64 29 + 5.5 (bound by a
+// step's chain of latencies at three waves a SIMD); 1 x 13 over 32768 36.3 + 5.6 (3.7
+// TB/s; 6 once the first slices are there); 4 x 25 over 4099 of q8_0 40.5 + 5.4 (a
+// barrier and a chain of latencies every 32 keys at two waves a SIMD: the VALU issues
+// for about 15 us of it, the matrix cores are busy for 11 %); 1 x 8 over 2048 11.5 + 4.2
+// (launches and the first loads' latency).  The kernel for the other widths has its
+// products on the VALU: at width 160 8 x 64 3480 + 18 us, 1 x 13 773 + 6, 4 x 25 459 + 8
+// (q8_0 452); at width 96 with 16 over 4 heads 8 x 64 1127 + 9 (at width 128 70 + 8).
 #include <math.h>
 
 #include <algorithm>
@@ -53,8 +56,12 @@ __device__ __forceinline__ int tree_tiles(const TreeSeq& s, int shift, int rows)
 }
 __device__ __forceinline__ int tree_slices(const TreeSeq& s, int slice) { return (s.count + slice - 1) / slice; }
 // A tile's units: its slices behind kStart that stand for the start of a run in it
-// (queries, first loads), so that a block with two starts gets less of the rest: 1 x
-// 13 over 32768 39.2 us at 0, 36.6 at 3, 39.8 at 6; 4 x 25 of q8_0 46.4, 42.7, 45.9 (at the time).
+// (queries, first loads), so that a block with two starts gets less of the rest.  us at
+// 0, 3 and 6: 1 x 8 over 2048 13.8, 11.2, 11.4; 1 x 13 over 5000 17.2, 14.4, 14.6, over
+// 32768 38.7, 36.0, 36.1, at width 64 23.7, 23.1, 23.2; 4 x 25 over 4099 34.0, 29.7,
+// 29.0, of q8_0 43.5, 40.4, 43.1; 8 x 48 over 12000 at width 64 86.6, 81.1, 83.6; 64 x 1
+// over 4096 of q8_0 174, 172, 180; no difference for 8 x 48 over 3000, 64 x 1 of f16 and
+// 8 x 8 over 16384 of q8_0.
 constexpr int kStart = 3;
 __device__ __forceinline__ int tree_units(const TreeSeq& s, int slice) { return kStart + tree_slices(s, slice); }
 
@@ -338,7 +345,7 @@ __global__ __launch_bounds__(kRowsThreads) void attend_tree_rows_kernel(TreeAtte
 // q8_0: keys and values enter as their integers, exact halves; a key block's
 // factor multiplies its part of the score, a value block's the weights, which
 // are then split into halves (the factors' share of 4 x 25 over 4099: 40 us against
-// 30 of f16; at D = 256 112 against 48, where they do not fit the registers).  The
+// 30 of f16; at D = 256 115 against 47, where they do not fit the registers).  The
 // factors are staged times 2^(11 - X), X the exponent of the largest one so far
 // among committed positions, which every row sees (a weight's lower half ends at
 // 2^-24: with X held at 0 or above, values near 4e-6 whose weights are 2^-12 of the

@@ -45,7 +45,6 @@ static bool quant_kind(int kind) {
 }
 static bool k_quant(int kind) { return kind == MI_Q4_K || kind == MI_Q5_K || kind == MI_Q6_K; }
 
-// The row geometry the kernels assume, checked once here.
 // A step's trees, for attention and (with `layer`) for a layer.
 int check_tree(const char* name, const mi_tree* t, bool layer) {
   if (!t || !t->starts || !t->lengths || !t->mask) return fail(MI_ERR_ARG, "%s: null pointer in the trees", name);
@@ -78,6 +77,7 @@ int check_tree_caches(const char* name, int32_t form, int32_t heads, int32_t kv_
   return MI_OK;
 }
 
+// The row geometry the kernels assume, checked once here.
 int check_weight(const char* name, int kind, const void* w, int64_t row_bytes, int32_t rows,
                  int32_t cols) {
   if (!quant_kind(kind)) return fail(MI_ERR_KIND, "%s: ggml type %d has no device matvec", name, kind);
