@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from molla_amd import gpu
-from tests.test_gpu_tree import FORMS, Draft, Step, draft, ints, starts_of, words_of
+from tests.test_gpu_tree import FORMS, Draft, Step, check_qk, draft, ints, starts_of, words_of
 
 pytestmark = pytest.mark.gpu
 
@@ -271,3 +271,45 @@ def test_two_graphs_of_one_context():
         ctx.synchronize()
         for s, w in zip(steps, want):
             assert torch.equal(s.out, w)
+
+
+# ---- the widths and sizes between the others' ---------------------------------------
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d", [160, 192, 224, 288, 320, 352, 384, 416, 448, 480])
+def test_every_head_width(form, d):
+    """Attention, then norm, rotation and store, at the widths that no other test has."""
+    for paged, heads, kv in ((False, 2, 1), (True, 4, 1)):
+        s = Step(form, [70, 0, 41], [5, 3, 0], heads, kv, d, seed=d, paged=paged)
+        s.check(s.run())
+    check_qk(5, 4, 1, d, d, True, True, False, form)
+    check_qk(6, 2, 2, d, d // 2, False, True, True, form, pad=0)
+    check_qk(3, 1, 1, d, 2, True, False, False, form, pad=4, in_place=True)
+
+
+@pytest.mark.parametrize("form", ["f16", "q8"])
+@pytest.mark.parametrize("d", [256, 512, 32])
+def test_eight_query_heads_a_key_head(form, d):
+    s = Step(form, [50, 300], [33, 2], 16, 2, d, seed=d, paged=True)
+    s.check(s.run())
+
+
+def test_tree_plan_without_positions():
+    ctx = gpu.DeviceContext(0)
+    parents, seen, _ = draft([9, 2], 1)
+    mask = ints([[-3]] * 12)
+    gpu.device_tree_plan(ctx, starts_of([9, 2]), ints([4, 5]), ints(parents + [0]), 9, None, mask)
+    ctx.synchronize()
+    assert (mask.cpu().numpy()[:11] == words_of(seen, 1)).all() and int(mask[11]) == -3
+
+
+def test_rows_that_start_behind_the_first():
+    """starts[0] may be past 0: the rows ahead of it keep what they held."""
+    s = Step("f16", [40, 33], [5, 6], 4, 2, 64, spare=7)
+    want, ctx = s.run(), gpu.DeviceContext(0)
+    e = s.dev
+    q, mask = torch.roll(e["q"], 4, 0), torch.roll(e["mask"], 4, 0)
+    out = torch.full_like(q, -3.0)
+    gpu.device_attend_tree(ctx, q, e["k"], e["v"], 4, 2, 64, s.scale, e["starts"] + 4, e["lengths"], mask, s.max_nodes,
+                           s.max_count, out, cache_stride=s.room * s.k.shape[1])
+    ctx.synchronize()
+    assert torch.equal(out.cpu()[4:15], want[:11]) and bool((out[:4] == -3.0).all()) and bool((out[15:] == -3.0).all())

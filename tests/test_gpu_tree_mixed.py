@@ -52,3 +52,11 @@ def test_chained_mixed_layers(counts):
         outs.append([s.xd] + s.k + s.v)
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+def test_layer_of_many_sequences():
+    """More sequences than a wave has lanes, a token each, some without one."""
+    spec = spec_of(512, 1024, 8, 2, 64)
+    host = make_layer_weights(spec, 25)
+    _, layer = device_layer_from(host, spec)
+    run(spec, host, layer, [(7 * i) % 40 for i in range(70)], [int(i % 9 != 4) for i in range(70)], "f16", True)
