@@ -357,7 +357,7 @@ int mi_decoder_layer_paged(mi_stream stream, const mi_layer_desc* desc, float* r
  * on the list, from free_pages[free_left[0]] on, ahead of the next plan: else they
  * are lost.
  * Nothing that is written may lie in lengths, news, free_pages, free_count or the
- * table (but that kv_index may be the table where page is 1). */
+ * table (but that kv_index may be the table, at its stride, where page is 1). */
 int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* lengths, const int32_t* news,
                  int32_t* table, int32_t table_stride, const int32_t* free_pages, int32_t free_size,
                  const int32_t* free_count, int32_t* free_left, int32_t* kv_index, int64_t index_stride,
@@ -385,7 +385,8 @@ int mi_tree_plan(mi_stream stream, int32_t batch, const int32_t* starts, const i
  * cell that two tokens name holds no row of either (heads of both, in no order),
  * every other row is as without them.  q_out may be q and k_out k, at the same
  * stride; else they share no value with q, k, v or each other (rows of one stride
- * may lie between one another, as in a fused q|k|v row), nor the caches.  count (device int32, or NULL): rows from
+ * may lie between one another, as in a fused q|k|v row), nor with the caches.
+ * count (device int32, or NULL): rows from
  * *count on are left alone.  The k/v caches are rows of mi_cache_row(cache_form,
  * kv_heads * head_dim) halves. */
 typedef struct {

@@ -441,14 +441,14 @@ int mi_embed(mi_stream stream, const float* embedding, int32_t vocab, int32_t wi
 
 // ---- a step over trees of drafted tokens -------------------------------------
 
-// A buffer of int32 (none where `at` is null), and whether two share a value.
+// A buffer of int32 (none where `at` is null or it has no value), and whether two share one.
 struct Ints {
   const char* name;
   const int32_t* at;
   int64_t count;
 };
 static bool ints_meet(const Ints& a, const Ints& b) {
-  return a.at && b.at && a.at < b.at + b.count && b.at < a.at + a.count;
+  return a.at && b.at && a.count > 0 && b.count > 0 && a.at < b.at + b.count && b.at < a.at + a.count;
 }
 
 int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* lengths, const int32_t* news,
@@ -471,7 +471,7 @@ int mi_page_plan(mi_stream stream, int32_t batch, int32_t page, const int32_t* l
                      {"free_count", free_count, 1}, {"the table", table, (int64_t)batch * table_stride}};
   const Ints out[] = {{"the table", table, in[4].count}, {"starts", starts, (int64_t)batch + 1}, {"free_left", free_left, 2},
                       {"seq", seq, max_tokens}, {"pos", pos, max_tokens}, {"cells", cells, max_tokens},
-                      {"kv_index", kv_index, kv_index ? (batch - 1) * index_stride + list : 0}};
+                      {"kv_index", kv_index, (batch - 1) * std::min<int64_t>(index_stride, (int64_t)1 << 40) + list}};
   for (const Ints& o : out)
     for (const Ints& i : in) {
       if (&o == out && &i == in + 4) continue;

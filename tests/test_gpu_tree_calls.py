@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from molla_amd import gpu
+from molla_amd._lib import check, lib
 from tests.test_gpu_tree import FORMS, Draft, Step, check_qk, draft, ints, starts_of, words_of
 
 pytestmark = pytest.mark.gpu
@@ -300,6 +301,16 @@ def test_tree_plan_without_positions():
     gpu.device_tree_plan(ctx, starts_of([9, 2]), ints([4, 5]), ints(parents + [0]), 9, None, mask)
     ctx.synchronize()
     assert (mask.cpu().numpy()[:11] == words_of(seen, 1)).all() and int(mask[11]) == -3
+
+
+def test_page_plan_of_an_empty_free_list():
+    """A list of no pages lies nowhere, whatever its address."""
+    starts, cells, left, table = ints([0] * 3), ints([-3] * 4), ints([0, 0]), ints([[7, -1], [3, -1]])
+    lens, news, none = ints([5, 15]), ints([1, 3]), ints([0])
+    check(lib().mi_page_plan(None, 2, 16, lens.data_ptr(), news.data_ptr(), table.data_ptr(), 2, cells.data_ptr() + 8, 0,
+                             none.data_ptr(), left.data_ptr(), None, 0, 4, starts.data_ptr(), None, None, cells.data_ptr()))
+    torch.cuda.synchronize()
+    assert cells.tolist() == [7 * 16 + 5, 3 * 16 + 15, -1, -1] and left.tolist() == [0, 1]
 
 
 def test_rows_that_start_behind_the_first():
