@@ -462,6 +462,54 @@ int mi_decoder_layer_tree(mi_stream stream, const mi_layer_desc* desc, float* re
                           uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
                           const mi_tree* tree, void* work, size_t work_bytes);
 
+/* ---- sparse experts (no counterpart in the reference) ----------------------
+ * An MLP of many experts, of which each token takes a few.  Experts are stacked
+ * as a file's ffn_*_exps tensors hold them: expert e's matrix is rows e * rows ..
+ * of one tensor of experts * rows rows, 16-byte aligned.  At most 512 experts,
+ * 64 of them a token, 2^20 (token, expert) pairs a call. */
+
+enum { MI_ROUTER_SIGMOID = 1, MI_ROUTER_NORM = 2 };
+
+/* Which experts a token takes: with logits l = router . x[t] (router: f32 rows of
+ * `width`, a multiple of 4, one an expert; products and sums in float64), p =
+ * softmax(l) over the experts, or with MI_ROUTER_SIGMOID 1 / (1 + exp(-l)) of
+ * each; ids[t * used ..] are the `used` experts of the largest p + bias (bias:
+ * f32[experts], or NULL), largest first, the lower one of two equal ones; a value
+ * that is not a number is the least.  weights[t * used + k] is scale * p of that
+ * expert, with MI_ROUTER_NORM divided by the sum of the token's (by 1 where that
+ * is 0).  Workspace: mi_router_workspace, 256-byte aligned.  x and router 16-byte
+ * aligned. */
+size_t mi_router_workspace(int32_t experts, int32_t tokens);
+int mi_router(mi_stream stream, const float* x, const float* router, const float* bias, int32_t width, int32_t experts,
+              int32_t used, int32_t tokens, int32_t flags, float scale, int32_t* ids, float* weights, void* work,
+              size_t work_bytes);
+
+/* Matrix products grouped by expert: y[p * rows ..] = W[ids[p]] . x[p / share] for
+ * p < pairs (a multiple of share), x of pairs / share rows; to the accuracy of
+ * mi_matvec.  A row whose id is no expert keeps what it held.  The kinds and
+ * columns of mi_matvec.  x and y 16-byte aligned, apart from each other.
+ * Workspace: mi_experts_matmul_workspace, 256-byte aligned. */
+size_t mi_experts_matmul_workspace(int32_t experts, int32_t cols, int32_t share, int32_t pairs);
+int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_bytes, int32_t experts, int32_t rows,
+                      int32_t cols, const float* x, int32_t share, const int32_t* ids, int32_t pairs, float* y,
+                      void* work, size_t work_bytes);
+
+/* The experts' gated MLP: out[t] = sum over k < used of weights[t * used + k] *
+ * down[e](act(gate[e] x[t]) * (up[e] x[t])), e = ids[t * used + k]; with MI_EPI_ADD
+ * added to out.  A pair whose id is no expert takes no part; the sum runs in the
+ * order of k.  gate and up are of one kind, their rows experts * hidden, down's
+ * experts * width.  out may be x.  Workspace: mi_experts_workspace, 256-byte
+ * aligned; x and out 16-byte aligned. */
+typedef struct {
+  int32_t experts;
+  int32_t width, hidden; /* of one expert, multiples of 64 (256 for the K-quants) */
+  int32_t act;           /* 0 silu, MI_ACT_GELU gelu */
+  mi_weight gate, up, down;
+} mi_experts;
+size_t mi_experts_workspace(const mi_experts* experts, int32_t tokens, int32_t used);
+int mi_experts_mlp(mi_stream stream, const mi_experts* experts, const float* x, int32_t tokens, int32_t used,
+                   const int32_t* ids, const float* weights, float* out, int32_t epi, void* work, size_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

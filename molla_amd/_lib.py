@@ -44,6 +44,11 @@ class MiTree(ctypes.Structure):
                [(n, P) for n in ("starts", "lengths", "mask", "pos", "cells")]
 
 
+class MiExperts(ctypes.Structure):
+    _fields_ = [(n, I32) for n in ("experts", "width", "hidden", "act")] + \
+               [(n, MiWeight) for n in ("gate", "up", "down")]
+
+
 # Every symbol include/molla_mi.h declares, with its C signature.
 SIGNATURES = {
     "mi_version": (ctypes.c_int, []),
@@ -87,6 +92,12 @@ SIGNATURES = {
     "mi_layer_tree_workspace": (SZ, [ctypes.POINTER(MiLayerDesc), ctypes.POINTER(MiTree)]),
     "mi_decoder_layer_tree": (ctypes.c_int, [P, ctypes.POINTER(MiLayerDesc), P, P, P, I64, P, I64,
                                              ctypes.POINTER(MiTree), P, SZ]),
+    "mi_router_workspace": (SZ, [I32, I32]),
+    "mi_router": (ctypes.c_int, [P, P, P, P, I32, I32, I32, I32, I32, F, P, P, P, SZ]),
+    "mi_experts_matmul_workspace": (SZ, [I32, I32, I32, I32]),
+    "mi_experts_matmul": (ctypes.c_int, [P, ctypes.c_int, P, I64, I32, I32, I32, P, I32, P, I32, P, P, SZ]),
+    "mi_experts_workspace": (SZ, [ctypes.POINTER(MiExperts), I32, I32]),
+    "mi_experts_mlp": (ctypes.c_int, [P, ctypes.POINTER(MiExperts), P, I32, I32, P, P, P, I32, P, SZ]),
 }
 
 _lib = None

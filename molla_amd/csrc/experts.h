@@ -1,0 +1,64 @@
+// experts.h -- what the sparse-expert kernels and their callers share.
+#pragma once
+
+#include "mi_internal.h"
+
+namespace mi {
+
+constexpr int kMaxExperts = 512;       // a plan's thread each
+constexpr int kMaxUsed = 64;           // of a token: a lane each
+constexpr int kMaxPairs = 1 << 20;     // of a call
+constexpr int kFewPairs = 64;          // up to here the row kernel: a lane each
+
+int launch_router(hipStream_t s, const float* x, const float* router, const float* bias, int32_t width, int32_t experts,
+                  int32_t used, int32_t tokens, int32_t flags, float scale, int32_t* ids, float* weights, void* work);
+
+// A few pairs' products (experts.hip): y[p] = W[ids[p]] . x[p / share], x in
+// matvec form; with w1, act(w0) * w1 in matvec form to xq_out instead.
+struct ExpertRows {
+  const void *w0, *w1;
+  int64_t row_bytes;
+  int32_t rows, cols, experts;
+  const void* xq;
+  int32_t share, pairs, act;
+  const int32_t* ids;
+  float* y;
+  void* xq_out;
+};
+int launch_expert_rows(hipStream_t s, int kind, const ExpertRows& a);
+int launch_expert_sum(hipStream_t s, const float* part, const int32_t* ids, const float* weights, int32_t width,
+                      int32_t tokens, int32_t used, int32_t experts, bool add, float* out);
+
+// The lists of many pairs by expert: slot[pair] (below 0: no expert), order[slot]
+// (the pair), and the blocks' tiles (experts_tile.hip).
+struct GroupPlan {
+  int32_t *slot, *order, *count;
+  void* tiles;
+  int32_t slots;   // the most that are numbered, whole tiles of 32
+  int32_t blocks;  // the most tile lists
+  size_t bytes;
+};
+int launch_group_plan(hipStream_t s, const int32_t* ids, int32_t pairs, int32_t experts, int32_t tiles_a_block,
+                      const GroupPlan& g);
+
+// Products of many pairs on the matrix cores: a plan, the activations by slot,
+// then the products.  group_plan lays a plan out in `work` (null: sizes only).
+GroupPlan group_plan(void* work, int32_t pairs, int32_t experts, int32_t tiles_a_block);
+int group_tiles(int kind, int32_t pairs, int32_t experts);  // 32-slot tiles a block
+size_t group_prep_bytes(int32_t cols, const GroupPlan& g);
+int launch_group_prep(hipStream_t s, const float* x, int32_t cols, int32_t pairs, int32_t share, const GroupPlan& g,
+                      void* prep);
+// y[p] = W[expert of p] . x; with w1, act(w0) * w1.  tiles_a_block as the plan's.
+int launch_group_tile(hipStream_t s, int kind, const void* w0, const void* w1, int64_t row_bytes, int32_t rows,
+                      int32_t cols, int32_t act, const GroupPlan& g, int32_t tiles_a_block, const void* prep, float* y);
+
+// experts_api.cpp: the MLP, checked, and its checks for the layer.
+size_t experts_workspace(int32_t experts, int32_t width, int32_t hidden, int32_t tokens, int32_t used);
+int launch_experts_mlp(hipStream_t s, const mi_experts& d, const float* x, int32_t tokens, int32_t used,
+                       const int32_t* ids, const float* weights, float* out, bool add, void* work);
+int check_experts(const char* name, const mi_experts* d);
+int check_router(const char* name, const float* router, int32_t width, int32_t experts, int32_t used, int32_t tokens,
+                 int32_t flags, float scale);
+size_t router_workspace(int32_t experts, int32_t tokens);
+
+}  // namespace mi

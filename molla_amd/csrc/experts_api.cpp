@@ -1,0 +1,271 @@
+// experts_api.cpp -- the C ABI of the sparse-expert entry points
+// (include/molla_mi.h): argument checks, workspaces, the launches of a call.
+#include <algorithm>
+#include <cmath>
+
+#include "experts.h"
+
+namespace mi {
+int check_weight(const char* name, int kind, const void* w, int64_t row_bytes, int32_t rows, int32_t cols);
+
+namespace {
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// Whether two buffers share a byte.
+bool meet(const void* a, size_t an, const void* b, size_t bn) {
+  return a && b && (const char*)a < (const char*)b + bn && (const char*)b < (const char*)a + an;
+}
+
+// Stacked experts' matrices: one GGUF tensor of experts * rows rows.
+int check_stack(const char* name, const mi_weight& w, int32_t experts, int32_t rows, int32_t cols) {
+  if ((int64_t)experts * rows > INT32_MAX)
+    return fail(MI_ERR_SHAPE, "%s: %d experts of %d rows are too many rows", name, experts, rows);
+  if (w.rows != experts * rows || w.cols != cols)
+    return fail(MI_ERR_SHAPE, "%s is %d x %d where %d experts of %d x %d are wanted", name, w.rows, w.cols, experts, rows,
+                cols);
+  const int rc = check_weight(name, w.kind, w.data, w.row_bytes, w.rows, w.cols);
+  if (rc) return rc;
+  // (every kind's tile takes an expert at its offset from there: rows are whole
+  // multiples of the alignment that their kind's loads need)
+  if ((uintptr_t)w.data & 15) return fail(MI_ERR_ALIGN, "%s: experts' matrices must be 16-byte aligned", name);
+  return MI_OK;
+}
+
+int check_counts(const char* name, int32_t experts, int64_t pairs) {
+  if (experts < 1 || experts > kMaxExperts) return fail(MI_ERR_SHAPE, "%s: %d experts, outside 1..%d", name, experts, kMaxExperts);
+  if (pairs < 1 || pairs > kMaxPairs) return fail(MI_ERR_SHAPE, "%s: %lld rows, outside 1..%d", name, (long long)pairs, kMaxPairs);
+  return MI_OK;
+}
+
+struct MatmulCarve {
+  size_t x, plan, total;
+};
+// Few rows: their activations in matvec form.  Many: by slot, and the plan.
+MatmulCarve matmul_carve(int32_t experts, int32_t cols, int32_t share, int32_t pairs) {
+  MatmulCarve c{};
+  size_t at = 0;
+  if (pairs <= kFewPairs) {
+    at += up256((size_t)xq_token_bytes(cols) * (pairs / share));
+  } else {
+    const GroupPlan g = group_plan(nullptr, pairs, experts, 1);  // (the most lists)
+    at += g.bytes;
+    c.x = at;
+    at += up256(group_prep_bytes(cols, g));
+  }
+  c.total = at;
+  return c;
+}
+
+struct MlpCarve {
+  size_t x, h, hx, part, plan, total;
+};
+// x: the input in the form its product reads; h: act(gate) * up in f32 (many
+// rows); hx: the same as the down projection reads it; part: what it gives.
+MlpCarve mlp_carve(int32_t experts, int32_t width, int32_t hidden, int32_t tokens, int32_t used) {
+  MlpCarve c{};
+  const size_t pairs = (size_t)tokens * used;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += up256(bytes);
+    return p;
+  };
+  if (pairs <= (size_t)kFewPairs) {
+    c.x = take((size_t)xq_token_bytes(width) * tokens);
+    c.hx = take((size_t)xq_token_bytes(hidden) * pairs);
+    c.part = take(4 * (size_t)width * pairs);
+  } else {
+    const GroupPlan g = group_plan(nullptr, (int32_t)pairs, experts, 1);
+    c.plan = take(g.bytes);
+    // (the input is dead where h's form is made, h where the down projection writes)
+    c.x = c.hx = take(std::max(group_prep_bytes(width, g), group_prep_bytes(hidden, g)));
+    c.h = c.part = take(4 * (size_t)std::max(width, hidden) * pairs);
+  }
+  c.total = at;
+  return c;
+}
+
+}  // namespace
+
+size_t experts_workspace(int32_t experts, int32_t width, int32_t hidden, int32_t tokens, int32_t used) {
+  return mlp_carve(experts, width, hidden, tokens, used).total;
+}
+
+int launch_experts_mlp(hipStream_t s, const mi_experts& d, const float* x, int32_t tokens, int32_t used,
+                       const int32_t* ids, const float* weights, float* out, bool add, void* work) {
+  const int32_t pairs = tokens * used;
+  const MlpCarve c = mlp_carve(d.experts, d.width, d.hidden, tokens, used);
+  char* base = (char*)work;
+  float* part = (float*)(base + c.part);
+  int rc;
+  if (pairs <= kFewPairs) {
+    if ((rc = launch_quantize(s, x, d.width, tokens, base + c.x))) return rc;
+    ExpertRows a{d.gate.data, d.up.data, d.gate.row_bytes, d.hidden, d.width, d.experts, base + c.x, used, pairs, d.act,
+                 ids, nullptr, base + c.hx};
+    if ((rc = launch_expert_rows(s, d.gate.kind, a))) return rc;
+    ExpertRows b{d.down.data, nullptr, d.down.row_bytes, d.width, d.hidden, d.experts, base + c.hx, 1, pairs, 0,
+                 ids, part, nullptr};
+    if ((rc = launch_expert_rows(s, d.down.kind, b))) return rc;
+  } else {
+    float* h = (float*)(base + c.h);
+    void *xp = base + c.x, *hp = base + c.hx;
+    const int ta = group_tiles(d.gate.kind, pairs, d.experts), tb = group_tiles(d.down.kind, pairs, d.experts);
+    GroupPlan g = group_plan(base + c.plan, pairs, d.experts, ta);
+    if ((rc = launch_group_plan(s, ids, pairs, d.experts, ta, g))) return rc;
+    if ((rc = launch_group_prep(s, x, d.width, pairs, used, g, xp))) return rc;
+    if ((rc = launch_group_tile(s, d.gate.kind, d.gate.data, d.up.data, d.gate.row_bytes, d.hidden, d.width, d.act, g, ta,
+                                xp, h)))
+      return rc;
+    if (tb != ta) {
+      // (other block lists; the slots may be others too, each pair's row is the same)
+      g = group_plan(base + c.plan, pairs, d.experts, tb);
+      if ((rc = launch_group_plan(s, ids, pairs, d.experts, tb, g))) return rc;
+    }
+    if ((rc = launch_group_prep(s, h, d.hidden, pairs, 1, g, hp))) return rc;
+    if ((rc = launch_group_tile(s, d.down.kind, d.down.data, nullptr, d.down.row_bytes, d.width, d.hidden, 0, g, tb, hp,
+                                part)))
+      return rc;
+  }
+  return launch_expert_sum(s, part, ids, weights, d.width, tokens, used, d.experts, add, out);
+}
+
+// The descriptor of a gated MLP of experts.
+int check_experts(const char* name, const mi_experts* d) {
+  if (!d) return fail(MI_ERR_ARG, "%s: null descriptor", name);
+  int rc = check_counts(name, d->experts, 1);
+  if (rc) return rc;
+  if (d->width <= 0 || d->hidden <= 0 || d->width % 64 || d->hidden % 64)
+    return fail(MI_ERR_SHAPE, "%s: width %d / hidden %d must be positive multiples of 64", name, d->width, d->hidden);
+  if (d->act != 0 && d->act != MI_ACT_GELU) return fail(MI_ERR_ARG, "%s: act %d is neither silu (0) nor gelu", name, d->act);
+  if ((rc = check_stack("experts' gate", d->gate, d->experts, d->hidden, d->width))) return rc;
+  if ((rc = check_stack("experts' up", d->up, d->experts, d->hidden, d->width))) return rc;
+  if ((rc = check_stack("experts' down", d->down, d->experts, d->width, d->hidden))) return rc;
+  if (d->gate.kind != d->up.kind)
+    return fail(MI_ERR_KIND, "%s: gate of type %d and up of type %d: they are of one", name, d->gate.kind, d->up.kind);
+  return MI_OK;
+}
+
+int check_router(const char* name, const float* router, int32_t width, int32_t experts, int32_t used, int32_t tokens,
+                 int32_t flags, float scale) {
+  if (!router) return fail(MI_ERR_ARG, "%s: null router", name);
+  if (width <= 0 || width % 4) return fail(MI_ERR_SHAPE, "%s: a router of %d values a row, not a multiple of 4", name, width);
+  if (tokens < 1 || tokens > kMaxPrefill) return fail(MI_ERR_ARG, "%s: tokens %d outside 1..%d", name, tokens, kMaxPrefill);
+  const int rc = check_counts(name, experts, 1);
+  if (rc) return rc;
+  if (used < 1 || used > std::min(experts, kMaxUsed))
+    return fail(MI_ERR_SHAPE, "%s: %d of %d experts a token, at most %d", name, used, experts, kMaxUsed);
+  if (flags & ~(MI_ROUTER_SIGMOID | MI_ROUTER_NORM)) return fail(MI_ERR_ARG, "%s: unknown router bits 0x%x", name, flags);
+  if (!std::isfinite(scale)) return fail(MI_ERR_ARG, "%s: the weights' scale has to be finite", name);
+  if ((uintptr_t)router & 15) return fail(MI_ERR_ALIGN, "%s: the router must be 16-byte aligned", name);
+  return MI_OK;
+}
+
+size_t router_workspace(int32_t experts, int32_t tokens) { return up256(sizeof(double) * (size_t)experts * tokens); }
+
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" {
+
+size_t mi_router_workspace(int32_t experts, int32_t tokens) {
+  if (experts < 1 || experts > kMaxExperts || tokens < 1 || tokens > kMaxPrefill) return 0;
+  return router_workspace(experts, tokens);
+}
+
+int mi_router(mi_stream stream, const float* x, const float* router, const float* bias, int32_t width, int32_t experts,
+              int32_t used, int32_t tokens, int32_t flags, float scale, int32_t* ids, float* weights, void* work,
+              size_t work_bytes) {
+  if (!x || !ids || !weights) return fail(MI_ERR_ARG, "router: null pointer");
+  int rc = check_router("router", router, width, experts, used, tokens, flags, scale);
+  if (rc) return rc;
+  if ((uintptr_t)x & 15) return fail(MI_ERR_ALIGN, "router: the input must be 16-byte aligned");
+  const size_t picks = 4 * (size_t)tokens * used, xb = 4 * (size_t)tokens * width, rb = 4 * (size_t)experts * width;
+  if (meet(ids, picks, weights, picks) || meet(ids, picks, bias, 4 * (size_t)experts) ||
+      meet(weights, picks, bias, 4 * (size_t)experts))
+    return fail(MI_ERR_ARG, "router: an output lies in another buffer");
+  const size_t need = router_workspace(experts, tokens);
+  if (!work || ((uintptr_t)work & 255) || work_bytes < need)
+    return fail(MI_ERR_WORKSPACE, "router: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);
+  if (meet(work, need, x, xb) || meet(work, need, router, rb) || meet(work, need, bias, 4 * (size_t)experts) ||
+      meet(work, need, ids, picks) || meet(work, need, weights, picks))
+    return fail(MI_ERR_ARG, "router: the workspace lies in another buffer");
+  return launch_router((hipStream_t)stream, x, router, bias, width, experts, used, tokens, flags, scale, ids, weights,
+                       work);
+}
+
+size_t mi_experts_matmul_workspace(int32_t experts, int32_t cols, int32_t share, int32_t pairs) {
+  if (experts < 1 || experts > kMaxExperts || cols <= 0 || cols % 64 || pairs < 1 || pairs > kMaxPairs || share < 1 ||
+      pairs % share)
+    return 0;
+  return matmul_carve(experts, cols, share, pairs).total;
+}
+
+int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_bytes, int32_t experts, int32_t rows,
+                      int32_t cols, const float* x, int32_t share, const int32_t* ids, int32_t pairs, float* y,
+                      void* work, size_t work_bytes) {
+  int rc = check_counts("experts_matmul", experts, pairs);
+  if (rc) return rc;
+  if (rows < 1) return fail(MI_ERR_SHAPE, "experts_matmul: experts of %d rows", rows);
+  if ((int64_t)experts * rows > INT32_MAX)
+    return fail(MI_ERR_SHAPE, "experts_matmul: %d experts of %d rows are too many rows", experts, rows);
+  if ((rc = check_stack("experts_matmul", mi_weight{w, kind, experts * rows, cols, row_bytes}, experts, rows, cols))) return rc;
+  if (!x || !ids || !y) return fail(MI_ERR_ARG, "experts_matmul: null pointer");
+  if (share < 1 || pairs % share)
+    return fail(MI_ERR_SHAPE, "experts_matmul: %d rows, %d for each row of the input", pairs, share);
+  if (((uintptr_t)x | (uintptr_t)y) & 15)
+    return fail(MI_ERR_ALIGN, "experts_matmul: the input and the output must be 16-byte aligned");
+  const size_t xb = 4 * (size_t)(pairs / share) * cols, yb = 4 * (size_t)pairs * rows;
+  if (meet(y, yb, x, xb) || meet(y, yb, ids, 4 * (size_t)pairs) || meet(y, yb, w, (size_t)experts * rows * row_bytes))
+    return fail(MI_ERR_ARG, "experts_matmul: the output lies in an input");
+  const MatmulCarve c = matmul_carve(experts, cols, share, pairs);
+  if (!work || ((uintptr_t)work & 255) || work_bytes < c.total)
+    return fail(MI_ERR_WORKSPACE, "experts_matmul: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, c.total);
+  if (meet(work, c.total, x, xb) || meet(work, c.total, y, yb) || meet(work, c.total, ids, 4 * (size_t)pairs))
+    return fail(MI_ERR_ARG, "experts_matmul: the workspace lies in another buffer");
+  hipStream_t s = (hipStream_t)stream;
+  char* base = (char*)work;
+  if (pairs <= kFewPairs) {
+    if ((rc = launch_quantize(s, x, cols, pairs / share, base + c.x))) return rc;
+    const ExpertRows a{w, nullptr, row_bytes, rows, cols, experts, base + c.x, share, pairs, 0, ids, y, nullptr};
+    return launch_expert_rows(s, kind, a);
+  }
+  const int tiles = group_tiles(kind, pairs, experts);
+  const GroupPlan g = group_plan(base + c.plan, pairs, experts, tiles);
+  if ((rc = launch_group_plan(s, ids, pairs, experts, tiles, g))) return rc;
+  if ((rc = launch_group_prep(s, x, cols, pairs, share, g, base + c.x))) return rc;
+  return launch_group_tile(s, kind, w, nullptr, row_bytes, rows, cols, 0, g, tiles, base + c.x, y);
+}
+
+size_t mi_experts_workspace(const mi_experts* d, int32_t tokens, int32_t used) {
+  if (!d || d->experts < 1 || d->experts > kMaxExperts || d->width <= 0 || d->hidden <= 0 || d->width % 64 ||
+      d->hidden % 64 || tokens < 1 || tokens > kMaxPrefill || used < 1 || used > kMaxUsed ||
+      (int64_t)tokens * used > kMaxPairs)
+    return 0;
+  return experts_workspace(d->experts, d->width, d->hidden, tokens, used);
+}
+
+int mi_experts_mlp(mi_stream stream, const mi_experts* d, const float* x, int32_t tokens, int32_t used,
+                   const int32_t* ids, const float* weights, float* out, int32_t epi, void* work, size_t work_bytes) {
+  int rc = check_experts("experts_mlp", d);
+  if (rc) return rc;
+  if (!x || !ids || !weights || !out) return fail(MI_ERR_ARG, "experts_mlp: null pointer");
+  if (tokens < 1 || tokens > kMaxPrefill)
+    return fail(MI_ERR_ARG, "experts_mlp: tokens %d outside 1..%d", tokens, kMaxPrefill);
+  if (used < 1 || used > kMaxUsed) return fail(MI_ERR_SHAPE, "experts_mlp: %d experts a token, outside 1..%d", used, kMaxUsed);
+  if ((rc = check_counts("experts_mlp", d->experts, (int64_t)tokens * used))) return rc;
+  if (epi != MI_EPI_NONE && epi != MI_EPI_ADD) return fail(MI_ERR_ARG, "experts_mlp: epilogue 0x%x is neither none nor add", epi);
+  if (((uintptr_t)x | (uintptr_t)out) & 15)
+    return fail(MI_ERR_ALIGN, "experts_mlp: the input and the output must be 16-byte aligned");
+  const size_t xb = 4 * (size_t)tokens * d->width, pb = 4 * (size_t)tokens * used;
+  if (meet(out, xb, ids, pb) || meet(out, xb, weights, pb)) return fail(MI_ERR_ARG, "experts_mlp: the output lies in an input");
+  const size_t need = experts_workspace(d->experts, d->width, d->hidden, tokens, used);
+  if (!work || ((uintptr_t)work & 255) || work_bytes < need)
+    return fail(MI_ERR_WORKSPACE, "experts_mlp: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);
+  if (meet(work, need, x, xb) || meet(work, need, out, xb) || meet(work, need, ids, pb) || meet(work, need, weights, pb))
+    return fail(MI_ERR_ARG, "experts_mlp: the workspace lies in another buffer");
+  return launch_experts_mlp((hipStream_t)stream, *d, x, tokens, used, ids, weights, out, epi == MI_EPI_ADD, work);
+}
+
+}  // extern "C"

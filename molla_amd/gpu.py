@@ -16,7 +16,7 @@ import ctypes
 import numpy as np
 import torch
 
-from ._lib import MiError, MiLayerDesc, MiQk, MiTree, MiWeight, check, lib
+from ._lib import MiError, MiExperts, MiLayerDesc, MiQk, MiTree, MiWeight, check, lib
 
 # ggml type numbers, src/molla/nn/quant.mojo:47-57
 Q_F32, Q_F16, Q_Q4_0, Q_Q4_1, Q_Q5_0, Q_Q5_1, Q_Q8_0, Q_Q4_K, Q_Q5_K, Q_Q6_K = 0, 1, 2, 3, 6, 7, 8, 12, 13, 14
@@ -420,6 +420,73 @@ def device_attend_tree(ctx: DeviceContext, q: torch.Tensor, k_cache: torch.Tenso
            _on(ctx, v_cache, "v_cache", f16, least), cache_stride,
            None if kv_index is None else _on(ctx, kv_index, "kv_index", i32), stride, heads, kv_heads, head_dim, scale,
            t, _on(ctx, out, "out", torch.float32, tokens * qw), work.data_ptr(), work.numel())
+
+
+# ---- sparse experts (no counterpart in the reference) ----
+ROUTER_SIGMOID, ROUTER_NORM = 1, 2
+
+
+def device_router(ctx: DeviceContext, x: torch.Tensor, router: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
+                  bias: torch.Tensor | None = None, sigmoid: bool = False, norm: bool = True, scale: float = 1.0,
+                  work: torch.Tensor | None = None) -> None:
+    """Which experts each row of x [tokens, width] takes (mi_router): router
+    [experts, width] f32; writes ids [tokens, used] (int32) and weights the same
+    (f32).  Scores are the softmax over the experts, or sigmoid each; bias [experts]
+    is added for the choice alone; norm: a token's weights sum to scale."""
+    f32 = torch.float32
+    if x.dim() != 2 or router.dim() != 2 or ids.dim() != 2 or x.shape[1] != router.shape[1]:
+        raise ValueError("router wants x [tokens, width], router [experts, width] and ids [tokens, used]")
+    (tokens, width), experts, used = x.shape, router.shape[0], ids.shape[1]
+    if ids.shape[0] != tokens or weights.shape != ids.shape:
+        raise ValueError(f"router wants ids and weights for {tokens} tokens, alike")
+    L = lib()
+    work = ctx.workspace(L.mi_router_workspace(experts, tokens)) if work is None else work
+    _queue(ctx, L.mi_router, _on(ctx, x, "x", f32), _on(ctx, router, "router", f32),
+           None if bias is None else _on(ctx, bias, "bias", f32, experts), width, experts, used, tokens,
+           (ROUTER_SIGMOID if sigmoid else 0) | (ROUTER_NORM if norm else 0), scale, _on(ctx, ids, "ids", torch.int32),
+           _on(ctx, weights, "weights", f32), _on(ctx, work, "work", torch.uint8), work.numel())
+
+
+def _stacked(w: Tensor, experts: int, name: str) -> int:
+    """Rows of one expert of a stacked tensor."""
+    if experts < 1 or w.rows % experts:
+        raise ValueError(f"{name} has {w.rows} rows, which are no {experts} experts")
+    return w.rows // experts
+
+
+def device_experts_matmul(ctx: DeviceContext, w: Tensor, experts: int, x: torch.Tensor, ids: torch.Tensor,
+                          out: torch.Tensor, work: torch.Tensor | None = None) -> None:
+    """Matrix products grouped by expert (mi_experts_matmul): w stacks `experts`
+    matrices; out [pairs, rows] row p is expert ids[p]'s matrix against x [pairs /
+    share, cols] row p / share.  A row whose id is no expert keeps what it held."""
+    f32 = torch.float32
+    rows, pairs = _stacked(w, experts, "w"), ids.numel()
+    if x.dim() != 2 or x.shape[1] != w.cols or not x.shape[0] or pairs % x.shape[0]:
+        raise ValueError(f"experts_matmul wants x of whole rows of {w.cols} for {pairs} ids")
+    share = pairs // x.shape[0]
+    L = lib()
+    work = ctx.workspace(L.mi_experts_matmul_workspace(experts, w.cols, share, pairs)) if work is None else work
+    _queue(ctx, L.mi_experts_matmul, w.kind, w.address, w.row_bytes(), experts, rows, w.cols, _on(ctx, x, "x", f32), share,
+           _on(ctx, ids, "ids", torch.int32), pairs, _on(ctx, out, "out", f32, pairs * rows),
+           _on(ctx, work, "work", torch.uint8), work.numel())
+
+
+def device_experts_mlp(ctx: DeviceContext, gate: Tensor, up: Tensor, down: Tensor, experts: int, x: torch.Tensor,
+                       ids: torch.Tensor, weights: torch.Tensor, out: torch.Tensor, act: int = 0, add: bool = False,
+                       work: torch.Tensor | None = None) -> None:
+    """The experts' gated MLP and its weighted sum (mi_experts_mlp): x and out
+    [tokens, width], ids and weights [tokens, used]; gate, up and down stack
+    `experts` matrices.  act: 0 silu, ACT_BIT gelu; add: onto what out holds."""
+    f32 = torch.float32
+    if x.dim() != 2 or ids.dim() != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:
+        raise ValueError("experts_mlp wants x [tokens, width] with ids and weights [tokens, used]")
+    (tokens, width), used = x.shape, ids.shape[1]
+    d = MiExperts(experts, width, _stacked(gate, experts, "gate"), act, gate.weight(), up.weight(), down.weight())
+    L, p = lib(), ctypes.byref(d)
+    work = ctx.workspace(L.mi_experts_workspace(p, tokens, used)) if work is None else work
+    _queue(ctx, L.mi_experts_mlp, p, _on(ctx, x, "x", f32), tokens, used, _on(ctx, ids, "ids", torch.int32),
+           _on(ctx, weights, "weights", f32), _on(ctx, out, "out", f32, tokens * width), EPI_ADD if add else EPI_NONE,
+           _on(ctx, work, "work", torch.uint8), work.numel())
 
 
 __all__ = [n for n in dir() if not n.startswith("_")] + ["MiError"]
