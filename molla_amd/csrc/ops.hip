@@ -1001,7 +1001,8 @@ int launch_store_kv(hipStream_t s, const float* k, const float* v, int32_t kv_wi
 static int launch_merge(hipStream_t s, const float* part_acc, const float* part_ml, int heads, int head_dim,
                         const int32_t* pos_dev, int count_host, int chunks, int tokens, float* out, void* xq_out,
                         void* hx_out, bool fold = false) {
-  const dim3 grid(heads, tokens), block(head_dim < 64 ? 64 : head_dim);
+  // (whole waves: their sums take every lane)
+  const dim3 grid(heads, tokens), block((head_dim + 63) / 64 * 64);
 #define MI_MERGE(B)                                                                                            \
   if (fold)                                                                                                    \
     hipLaunchKernelGGL((attend_merge_kernel<B, true>), grid, block, 0, s, part_acc, part_ml, heads, head_dim,    \
