@@ -291,6 +291,21 @@ typedef struct {
    * that norm are one launch.  Both are ignored at 1 token and above 8. */
   const float* next_norm;
   int32_t prenormed;
+  /* Sparse experts in place of the MLP (no counterpart in the reference; 0: none):
+   * gate, up and down stack `experts` matrices (mi_experts: gate and up of one kind,
+   * rows experts * hidden, down's experts * width, 16-byte aligned), of which each
+   * token takes experts_used, by mi_router over the normed row with these flags
+   * (MI_ROUTER_*), scale, matrix (f32[experts * width]) and bias (f32[experts], or
+   * NULL).  Not together with ungated; the residual is 16-byte aligned. */
+  int32_t experts, experts_used;
+  int32_t router_flags;
+  float router_scale;
+  const float* router;
+  const float* router_bias;
+  /* Attention over a window (0: all positions): a token at position p sees the
+   * positions up to p that are above p - window or below `first` (mi_attend_window).
+   * mi_decoder_layer_tree refuses it. */
+  int32_t window, first;
 } mi_layer_desc;
 
 /* One Llama layer for `tokens` independent sequences (batch decode, one token
@@ -461,6 +476,30 @@ size_t mi_layer_tree_workspace(const mi_layer_desc* desc, const mi_tree* tree);
 int mi_decoder_layer_tree(mi_stream stream, const mi_layer_desc* desc, float* resid, uint16_t* k_cache,
                           uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
                           const mi_tree* tree, void* work, size_t work_bytes);
+
+/* ---- attention over a window ------------------------------------------------
+ * Token t at position pos[t] (device int32[tokens]) sees the positions j <= pos[t]
+ * with j > pos[t] - window or j < first: the last `window` of them, its own among
+ * them, and the first few of the sequence (attention.mojo:52 AttnSpec's window;
+ * the first positions have no counterpart in the reference).  window is at least 1,
+ * first at least 0.  The caches as in mi_decoder_layer: position j of token t's
+ * sequence is row j of the cache at t * cache_stride halves, or pool cell
+ * kv_index[t * index_stride + j] (negative: not held, not seen); a stride of 0
+ * makes the tokens one sequence's chunk.  max_count bounds the positions: one at or
+ * above it is taken for the last, one below 0 sees nothing.  q: rows of heads *
+ * head_dim floats q_stride apart, out: the same contiguous, apart from q; both
+ * 16-byte aligned.  A token that sees nothing gets zeros, and what it does not see
+ * changes no bit of its result, whatever it holds.  A value that it sees and that
+ * is not finite makes its place of the result not finite; a key, or a q8_0 factor,
+ * leaves the heads over it undefined.  GQA groups and head widths as mi_attend.
+ * Workspace: mi_attend_window_workspace, 256-byte aligned (one_seq: whether the
+ * tokens are one sequence's chunk). */
+size_t mi_attend_window_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, int32_t window,
+                                  int32_t first, int32_t max_count, int32_t tokens, int32_t one_seq);
+int mi_attend_window(mi_stream stream, int32_t form, const float* q, int64_t q_stride, const uint16_t* k_cache,
+                     const uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
+                     int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, int32_t window, int32_t first,
+                     const int32_t* pos, int32_t max_count, int32_t tokens, float* out, void* work, size_t work_bytes);
 
 /* ---- sparse experts (no counterpart in the reference) ----------------------
  * An MLP of many experts, of which each token takes a few.  Experts are stacked

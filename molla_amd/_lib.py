@@ -28,7 +28,9 @@ class MiLayerDesc(ctypes.Structure):
                [("rope_factors", P), ("cache_form", I32)] + \
                [(n, P) for n in ("q_bias", "k_bias", "v_bias", "q_norm", "k_norm", "attn_post_norm",
                                  "ffn_post_norm")] + \
-               [("ungated", I32), ("act", I32), ("next_norm", P), ("prenormed", I32)]
+               [("ungated", I32), ("act", I32), ("next_norm", P), ("prenormed", I32), ("experts", I32),
+                ("experts_used", I32), ("router_flags", I32), ("router_scale", F), ("router", P), ("router_bias", P),
+                ("window", I32), ("first", I32)]
 
 
 class MiQk(ctypes.Structure):
@@ -92,6 +94,9 @@ SIGNATURES = {
     "mi_layer_tree_workspace": (SZ, [ctypes.POINTER(MiLayerDesc), ctypes.POINTER(MiTree)]),
     "mi_decoder_layer_tree": (ctypes.c_int, [P, ctypes.POINTER(MiLayerDesc), P, P, P, I64, P, I64,
                                              ctypes.POINTER(MiTree), P, SZ]),
+    "mi_attend_window_workspace": (SZ, [I32, I32, I32, I32, I32, I32, I32, I32, I32]),
+    "mi_attend_window": (ctypes.c_int, [P, I32, P, I64, P, P, I64, P, I64, I32, I32, I32, F, I32, I32, P, I32, I32, P, P,
+                                        SZ]),
     "mi_router_workspace": (SZ, [I32, I32]),
     "mi_router": (ctypes.c_int, [P, P, P, P, I32, I32, I32, I32, I32, F, P, P, P, SZ]),
     "mi_experts_matmul_workspace": (SZ, [I32, I32, I32, I32]),

@@ -34,6 +34,15 @@ class BlockSpec:
     eps: float = 1e-5
     ungated: bool = False  # block.mojo:80 gated: False computes act(up(x))
     act: int = 0  # block.mojo:83: 0 silu, gpu.ACT_BIT (8) gelu
+    # sparse experts in place of the MLP (mi_layer_desc): hidden is one expert's, gate,
+    # up and down stack `experts` matrices, and extras holds the router (and its bias)
+    experts: int = 0
+    experts_used: int = 0
+    router_flags: int = gpu.ROUTER_NORM
+    router_scale: float = 1.0
+    # attention over the last `window` positions and the first few (0: over all)
+    window: int = 0
+    first: int = 0
 
     @property
     def attn_scale(self) -> float:
@@ -52,7 +61,8 @@ class DeviceLayer:
 
     NAMES = ("wq", "wk", "wv", "wo", "gate", "up", "down")
 
-    OPTIONAL = ("q_bias", "k_bias", "v_bias", "q_norm", "k_norm", "attn_post_norm", "ffn_post_norm")
+    OPTIONAL = ("q_bias", "k_bias", "v_bias", "q_norm", "k_norm", "attn_post_norm", "ffn_post_norm", "router",
+                "router_bias")
 
     def __init__(self, spec: BlockSpec, attn_norm: torch.Tensor, ffn_norm: torch.Tensor, weights: dict,
                  rope_steps: torch.Tensor, rope_factors: torch.Tensor | None = None, extras: dict | None = None):
@@ -82,6 +92,9 @@ class DeviceLayer:
                 raise ValueError(f"{n} must be a device float32 tensor")
             setattr(d, n, t.data_ptr())
         d.ungated, d.act = int(spec.ungated), int(spec.act)
+        d.experts, d.experts_used = spec.experts, spec.experts_used
+        d.router_flags, d.router_scale = spec.router_flags, spec.router_scale
+        d.window, d.first = spec.window, spec.first
         if rope_factors is not None:
             if rope_factors.dtype != torch.float32 or rope_factors.numel() < spec.rope_dim // 2:
                 raise ValueError(f"rope wants {spec.rope_dim // 2} f32 frequency factors")

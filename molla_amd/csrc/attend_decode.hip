@@ -69,7 +69,7 @@ __device__ __forceinline__ df4 mfma16(dh8 a, dh8 b, df4 c) {
 // takes 4 rows x 32 bytes per 16 lanes, on distinct banks.
 template <int D>
 __device__ __forceinline__ int swz(int r) {
-  return (D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1)) | ((r >> 2) & 3);
+  return (D >= 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1)) | ((r >> 2) & 3);
 }
 
 // over the four lanes that share a column
@@ -101,12 +101,14 @@ __device__ __forceinline__ dh8 int8_halves(uint32_t x, uint32_t y) {
 // the context), starting at the s-th, and writes each head's unnormalised sum
 // with (maximum, sum) in base 2 to slot (token, head, share); (0, 0) for no
 // keys.
-template <int D, bool Q8, bool PAGED, int W>
-__global__ __launch_bounds__(64 * W, 2) void attend_decode_kernel(
+// WIN: the keys are those a window leaves (Window), numbered end to end; a value
+// that is masked or not held enters as zero, whatever lies there.
+template <int D, bool Q8, bool PAGED, int W, bool WIN>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_decode_kernel(
     const float* __restrict__ q, int64_t q_stride, const __half* __restrict__ kc, const __half* __restrict__ vc,
     int64_t cache_stride, int row_halves, int heads, int kv_heads, int group, float scale,
     const int32_t* __restrict__ pos, int count_host, const int32_t* __restrict__ kv_index, int64_t index_stride,
-    float* __restrict__ part_acc, float* __restrict__ part_ml) {
+    float* __restrict__ part_acc, float* __restrict__ part_ml, const Window win) {
   constexpr int kStep = kRun * W;  // keys a block takes at a time
   constexpr int KS = D / 32, NT = D / 16, PIECES = D / 8;
   constexpr int kFac = Q8 ? 2 * KS * kRun : 1;             // floats: factors of a run's keys and values
@@ -119,7 +121,9 @@ __global__ __launch_bounds__(64 * W, 2) void attend_decode_kernel(
   const int lm = lane & 15, lk = lane >> 4;
   const int share = blockIdx.x, shares = gridDim.x, kvh = blockIdx.y, t = blockIdx.z;
   const int64_t slot0 = ((int64_t)t * heads + (int64_t)kvh * group) * shares + share;
-  const int count = pos ? pos[t] + 1 : count_host;
+  int count = pos ? pos[t] + 1 : count_host;
+  int near = 0, skip = 0;  // WIN: keys from `near` on are `skip` positions further
+  if constexpr (WIN) count = win.keys(pos[t], near, skip);
   // the queries, first in line, also ahead of the position: column lm (past the
   // group, the last one)
   const float* qr = q + (int64_t)t * q_stride + ((int64_t)kvh * group + min(lm, group - 1)) * D + 8 * lk;
@@ -141,11 +145,13 @@ __global__ __launch_bounds__(64 * W, 2) void attend_decode_kernel(
   // the last one, masked below): read a run ahead of its keys and values, which
   // take theirs from the lane that has it
   auto cells_of = [&](int key) __attribute__((always_inline)) {
-    const int j = min(key + (lane & 31), count - 1);
+    int j = min(key + (lane & 31), count - 1);
+    if constexpr (WIN) j += j < near ? 0 : skip;
     return PAGED ? kv_index[j] : j;
   };
   auto row_of = [&](int key, int cells, int r) __attribute__((always_inline)) {
-    const int cell = PAGED ? max(__shfl(cells, r), 0) : min(key + r, count - 1);
+    int cell = PAGED ? max(__shfl(cells, r), 0) : min(key + r, count - 1);
+    if constexpr (WIN && !PAGED) cell += cell < near ? 0 : skip;
     return seq + (int64_t)cell * row_halves;
   };
 
@@ -156,7 +162,8 @@ __global__ __launch_bounds__(64 * W, 2) void attend_decode_kernel(
   constexpr int VW = Q8 ? kRun * D / 16 / 64 : kRun * PIECES / 64;
   KWord kw[2][KS];
   du4 vw[VW];
-  du2 fw = {0, 0};
+  typedef typename std::conditional<KS == 8, du4, du2>::type FWord;
+  FWord fw = {0, 0};
   auto load_k = [&](int key0, int cells) __attribute__((always_inline)) {
 #pragma unroll
     for (int a = 0; a < 2; a++) {
@@ -170,7 +177,7 @@ __global__ __launch_bounds__(64 * W, 2) void attend_decode_kernel(
   auto load_v = [&](int key0, int cells) __attribute__((always_inline)) {
     if constexpr (Q8) {
       const __half* c = (lane < 32 ? kc : vc) + row_of(key0, cells, lane & 31) + (kvw >> 1) + ((kvh * D) >> 5);
-      if constexpr (KS == 4) fw = *(const du2*)c;
+      if constexpr (KS >= 4) fw = *(const FWord*)c;
       else fw.x = *(const uint32_t*)c;
     }
 #pragma unroll
@@ -249,10 +256,10 @@ __global__ __launch_bounds__(64 * W, 2) void attend_decode_kernel(
       if constexpr (Q8) {
         // factors to LDS by (key | value, block, key), read back four keys a
         // lane; zero for a key past the end or not held, whose row is another's
-        if (!((held >> (lane & 31)) & 1)) fw = du2{0, 0};
+        if (!((held >> (lane & 31)) & 1)) fw = FWord{0, 0};
 #pragma unroll
         for (int b = 0; b < KS; b++)
-          fl[(lane >> 5) * KS * kRun + b * kRun + (lane & 31)] = half_bits_to_float(b < 2 ? fw.x >> (16 * b) : fw.y >> (16 * (b - 2)));
+          fl[(lane >> 5) * KS * kRun + b * kRun + (lane & 31)] = half_bits_to_float(fw[b >> 1] >> (16 * (b & 1)));
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int a = 0; a < 2; a++) {
@@ -321,6 +328,10 @@ __global__ __launch_bounds__(64 * W, 2) void attend_decode_kernel(
           *(__attribute__((address_space(3))) dh8*)(vl + 2 * row * D + 16 * ((pc + 1) ^ swz<D>(row))) = int8_halves(vw[j].z, vw[j].w);
         } else {
           const int row = i / PIECES, pc = i % PIECES;
+          if constexpr (WIN) {
+            const uint32_t keep = 0u - ((held >> row) & 1u);
+            vw[j] &= du4{keep, keep, keep, keep};
+          }
           *(__attribute__((address_space(3))) du4*)(vl + 2 * row * D + 16 * (pc ^ swz<D>(row))) = vw[j];
         }
       }
@@ -446,6 +457,11 @@ bool decode_attend_fits(int32_t group, int32_t head_dim) {
   return (group == 1 || group == 2 || group == 4 || group == 8) && (head_dim == 64 || head_dim == 128);
 }
 
+// With a window also heads of 256, for which a wave has the registers of two.
+bool decode_window_fits(int32_t group, int32_t head_dim) {
+  return decode_attend_fits(group, head_dim) || (decode_attend_fits(group, 128) && head_dim == 256);
+}
+
 // Two-wave blocks while every 64 keys of the context can have a compute unit of
 // their own: one unit takes in about 64 bytes a cycle, so that a short context is
 // better spread (us of a layer of width 256, two / four waves: 300 keys 26.3 / 27.4,
@@ -478,36 +494,56 @@ DecodePlan decode_attend_plan(int32_t kv_heads, int32_t tokens, int32_t max_coun
   return best;
 }
 
+namespace {
+
+template <int D, bool Q8, bool PAGED, bool WIN>
+void launch_w(hipStream_t s, dim3 grid, int waves, const float* q, int64_t q_stride, const uint16_t* k_cache,
+              const uint16_t* v_cache, int64_t cache_stride, int row, int heads, int kv_heads, float scale,
+              const int32_t* pos, int count_host, const int32_t* kv_index, int64_t index_stride, float* part_acc,
+              float* part_ml, const Window& win) {
+#define MI_DEC_W(W)                                                                                                  \
+  hipLaunchKernelGGL((attend_decode_kernel<D, Q8, PAGED, W, WIN>), grid, dim3(64 * W), 0, s, q, q_stride,            \
+                     (const __half*)k_cache, (const __half*)v_cache, cache_stride, row, heads, kv_heads,             \
+                     heads / kv_heads, scale, pos, count_host, kv_index, index_stride, part_acc, part_ml, win)
+  if (waves == 4) MI_DEC_W(4);
+  else MI_DEC_W(2);
+#undef MI_DEC_W
+}
+
+}  // namespace
+
 int launch_attend_decode(hipStream_t s, const float* q, int64_t q_stride, const uint16_t* k_cache,
                          const uint16_t* v_cache, int64_t cache_stride, int32_t heads, int32_t kv_heads,
                          int32_t head_dim, float scale, const int32_t* pos, int32_t count_host, DecodePlan plan,
                          int32_t tokens, float* part_acc, float* part_ml, int32_t form, const int32_t* kv_index,
-                         int64_t index_stride) {
+                         int64_t index_stride, const Window* win) {
   const int row = cache_row(form, kv_heads * head_dim);
   const dim3 grid(plan.shares, kv_heads, tokens);
-#define MI_DEC_W(DD, Q, P, W)                                                                                      \
-  hipLaunchKernelGGL((attend_decode_kernel<DD, Q, P, W>), grid, dim3(64 * W), 0, s, q, q_stride,                   \
-                     (const __half*)k_cache, (const __half*)v_cache, cache_stride, row, heads, kv_heads,           \
-                     heads / kv_heads, scale, pos, count_host, kv_index, index_stride, part_acc, part_ml)
-#define MI_DEC(DD, Q, P)                              \
-  if (plan.waves == 4) MI_DEC_W(DD, Q, P, 4);         \
-  else MI_DEC_W(DD, Q, P, 2);
-#define MI_DEC_F(DD)                         \
+  const Window w = win ? *win : Window{};
+#define MI_DEC(DD, Q, P, WN)                                                                                       \
+  launch_w<DD, Q, P, WN>(s, grid, plan.waves, q, q_stride, k_cache, v_cache, cache_stride, row, heads, kv_heads,   \
+                         scale, pos, count_host, kv_index, index_stride, part_acc, part_ml, w)
+#define MI_DEC_F(DD, WN)                     \
   if (form == MI_CACHE_Q8) {                 \
-    if (kv_index) { MI_DEC(DD, true, true) }    \
-    else { MI_DEC(DD, true, false) }            \
+    if (kv_index) MI_DEC(DD, true, true, WN);   \
+    else MI_DEC(DD, true, false, WN);           \
   } else {                                   \
-    if (kv_index) { MI_DEC(DD, false, true) }   \
-    else { MI_DEC(DD, false, false) }           \
+    if (kv_index) MI_DEC(DD, false, true, WN);  \
+    else MI_DEC(DD, false, false, WN);          \
   }
-  if (head_dim == 64) {
-    MI_DEC_F(64)
+  if (win && head_dim == 64) {
+    MI_DEC_F(64, true)
+  } else if (win && head_dim == 128) {
+    MI_DEC_F(128, true)
+  } else if (win) {
+    MI_DEC_F(256, true)
+  } else if (head_dim == 64) {
+    MI_DEC_F(64, false)
   } else {
-    MI_DEC_F(128)
+    MI_DEC_F(128, false)
   }
 #undef MI_DEC_F
 #undef MI_DEC
-#undef MI_DEC_W
   return hip_check(hipGetLastError(), "attend_decode launch");
 }
 

@@ -80,11 +80,20 @@ __device__ __forceinline__ ff16 mfma32(fh8 a, fh8 b, ff16 c) {
 // so that the lanes served together fall on distinct banks.
 template <int D>
 __device__ __forceinline__ int key_swz(int r) {
-  return D == 128 ? (r & 15) : ((r >> 1) & 7);
+  return D >= 128 ? (r & 15) : ((r >> 1) & 7);
 }
 template <int D>
 __device__ __forceinline__ int val_swz(int r) {
-  return (D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1)) | ((r >> 2) & 3);
+  return (D >= 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1)) | ((r >> 2) & 3);
+}
+
+// Whether a half of a 16-byte word is an infinity or NaN: its exponent is all ones,
+// and one more unit of it carries into the sign's place.
+__device__ __forceinline__ bool not_finite(fu4 v) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) any |= (v[i] & 0x7c007c00u) + 0x04000400u;
+  return (any & 0x80008000u) != 0;
 }
 
 struct IMax {
@@ -113,12 +122,20 @@ __device__ __forceinline__ void int8_halves(uint32_t w, fh2& a, fh2& b) {
 // host knows only the context), and writes each row's unnormalised sum with
 // (maximum, sum) in base 2 to part_acc / part_ml, slot (token, head, split);
 // with one split, the finished row to out.
-template <int D, bool Q8, bool PAGED>
-__global__ __launch_bounds__(256, 2) void attend_flash_kernel(
+//
+// WIN: each token sees what a Window leaves.  The slices are those of the first
+// positions and then those from the earliest window's on; a row that sees nothing
+// gets zeros.  An f16 value that is not finite enters the product as zero, with the
+// 16-byte word it lies in, and is added in float32 at the end to the rows that see
+// it, as q8_0's keys are that are left out: what a row does not see changes nothing
+// of it.
+template <int D, bool Q8, bool PAGED, bool WIN>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
     const float* __restrict__ q, int64_t q_stride, const __half* __restrict__ kc, const __half* __restrict__ vc,
     int row_halves, int heads, int kv_heads, int group, float scale, const int32_t* __restrict__ pos, int tokens,
     const int32_t* __restrict__ kv_index, float* __restrict__ part_acc, float* __restrict__ part_ml,
-    float* __restrict__ out) {
+    float* __restrict__ out, const Window win) {
+  static_assert(!Q8 || D <= 128, "a wave stages values of one q8_0 block");
   constexpr int PIECES = D / 8, NT = D / 32;
   constexpr int VB = Q8 ? 1 : 2;  // value buffers (q8_0 values take two halves: 32 KB at D = 128)
   constexpr int VH = Q8 ? 2 : 1;  // halves a value
@@ -126,8 +143,8 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
   __shared__ __align__(16) _Float16 vs[VB * VH][kSlice * D];
   __shared__ __align__(16) float kf[Q8 ? 2 : 1][Q8 ? NT : 1][kSlice];  // q8_0 key factors
   __shared__ int vexp[Q8 ? 4 : 1];                                     // X of each wave's dims
-  __shared__ int left_out;                                             // q8_0: some key's values were
-  __shared__ int cmax[4];
+  __shared__ int left_out;                                             // some key's values were
+  __shared__ int cmax[4], lmin[WIN ? 4 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int split = blockIdx.x, splits = gridDim.x, kvh = blockIdx.y, t0 = blockIdx.z * (kRows / group);
@@ -135,18 +152,39 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
   // this lane's query: row r = token t0 + r / group, head r % group
   const int r = 32 * wave + n, t = t0 + r / group, head = kvh * group + r % group;
   const bool live_row = t < tokens;
-  const int cnt = live_row ? pos[t] + 1 : 0;
+  const int cnt = live_row ? (WIN ? win.count(pos[t]) : pos[t] + 1) : 0;
+  // WIN: the lowest position of this row's window; the wave's least and largest
+  const int low = WIN ? max(cnt - win.window, 0) : 0;
+  const int wave_low = WIN ? -lanes::reduce<64>(cnt > 0 ? -low : -0x7fffffff, IMax{}) : 0;
+  const int wave_top = WIN ? lanes::reduce<64>(live_row ? low : 0, IMax{}) : 0;
   const int wave_max = lanes::reduce<64>(cnt, IMax{});
   const int wave_min = -lanes::reduce<64>(live_row ? -cnt : -0x7fffffff, IMax{});
   if (lane == 0) cmax[wave] = wave_max;
-  if (Q8 && tid == 0) left_out = 0;
+  if (WIN && lane == 0) lmin[wave] = wave_low;
+  if ((Q8 || WIN) && tid == 0) left_out = 0;
   __syncthreads();
   const int count = __builtin_amdgcn_readfirstlane(max(max(cmax[0], cmax[1]), max(cmax[2], cmax[3])));
-  const int slices = (count + kSlice - 1) / kSlice, per = (slices + splits - 1) / splits;
+  int slices = (count + kSlice - 1) / kSlice;
+  // WIN: slices behind the first positions' ones, up to the windows', are left out
+  int near = 0, skip = 0;
+  if constexpr (WIN) {
+    const int lo = __builtin_amdgcn_readfirstlane(min(min(lmin[0], lmin[1]), min(lmin[2], lmin[3]))) / kSlice;
+    near = min((int)(((int64_t)win.first + kSlice - 1) / kSlice), lo);
+    skip = lo - near;
+    slices -= skip;
+  }
+  auto slice_of = [&](int v) __attribute__((always_inline)) { return WIN && v >= near ? v + skip : v; };
+  const int per = (slices + splits - 1) / splits;
   const int s0 = split * per, s1 = min(s0 + per, slices);
 
-  if (s0 >= s1) {  // (uniform; only with several splits) no keys: no part in the fold
-    if (live_row && h == 0) *(float2*)(part_ml + (((int64_t)t * heads + head) * splits + split) * 2) = make_float2(0.0f, 0.0f);
+  if (s0 >= s1) {  // (uniform; with several splits, or rows that see nothing) no keys: no part in the fold
+    if (WIN && splits == 1) {
+      if (live_row)
+        for (int i = 0; i < D / 2; i += 4)
+          *(ff4*)(out + ((int64_t)t * heads + head) * D + D / 2 * h + i) = ff4{0.0f, 0.0f, 0.0f, 0.0f};
+    } else if (live_row && h == 0) {
+      *(float2*)(part_ml + (((int64_t)t * heads + head) * splits + split) * 2) = make_float2(0.0f, 0.0f);
+    }
     return;
   }
 
@@ -265,14 +303,20 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
 #pragma unroll
       for (int j = 0; j < PER; j++) {
         const int i = tid + 256 * j, row = i / PIECES, pc = i % PIECES;
+        if constexpr (WIN) {
+          if (__builtin_expect(not_finite(vr[j]), 0)) {
+            vr[j] = fu4{0, 0, 0, 0};
+            left_out = 1;
+          }
+        }
         *(fu4*)(vs[buf] + row * D + 8 * (pc ^ val_swz<D>(row))) = vr[j];
       }
     }
   };
 
   // the first slice on its way behind the queries, ahead of their conversion
-  load(kc, s0, kr, kfr);
-  load(vc, s0, vr, vfr);
+  load(kc, slice_of(s0), kr, kfr);
+  load(vc, slice_of(s0), vr, vfr);
   __builtin_amdgcn_sched_barrier(0);
 
   // The query, scaled by the power of two that brings its largest value to
@@ -378,13 +422,14 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
       }
     }
     // lanes past their token's end, or on a cell that is not held, take no part
-    const bool full = !PAGED && base + 32 <= wave_min;
+    const bool full = !PAGED && base + 32 <= wave_min && (!WIN || base >= wave_top || base + 32 <= win.first);
     const int rel = cnt - base - 4 * h;
+    const int from = WIN ? low - base - 4 * h : 0, firsts = WIN ? win.first - base - 4 * h : 0;
     uint32_t held = 0xffffffffu;
     if constexpr (PAGED) held = (uint32_t)__ballot(kv_index[min(base + n, count - 1)] >= 0) >> (4 * h);
     auto live = [&](int j) __attribute__((always_inline)) {
       const int at = 8 * (j >> 2) + (j & 3);
-      return at < rel && (!PAGED || ((held >> at) & 1));
+      return at < rel && (!WIN || at >= from || at < firsts) && (!PAGED || ((held >> at) & 1));
     };
     if (!full) {
 #pragma unroll
@@ -439,11 +484,12 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
   store_k(0);
   store_v(0);
   __syncthreads();
-  for (int sl = s0; sl < s1; sl++) {
-    const int buf = (sl - s0) & 1, base = sl * kSlice;
-    const bool more = sl + 1 < s1;          // uniform
-    const bool mine = base < wave_max;      // this wave has tokens that reach the slice
-    if (more) load(kc, sl + 1, kr, kfr);
+  for (int sv = s0; sv < s1; sv++) {
+    const int buf = (sv - s0) & 1, sl = slice_of(sv), base = sl * kSlice;
+    const bool more = sv + 1 < s1;          // uniform
+    // this wave has tokens that reach the slice
+    const bool mine = base < wave_max && (!WIN || base + kSlice > wave_low || base < win.first);
+    if (more) load(kc, slice_of(sv + 1), kr, kfr);
     // the slice's weights, 32 keys at a time (both tiles' scores at once are 32
     // more registers than a wave has)
 #pragma unroll
@@ -451,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
       if (mine && base + 32 * kt < wave_max) tile(kt, sl, buf);
       if (kt == 0 && more) {
         store_k(1 - buf);
-        int next = sl + 1;
+        int next = slice_of(sv + 1);
         asm volatile("" : "+s"(next));  // (the keys' row offsets are not kept for it)
         load(vc, next, vr, vfr);
       }
@@ -470,15 +516,16 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
       int tid = threadIdx.x;
       asm volatile("" : "+v"(tid));
       const int lane = tid & 63, h = lane >> 5, r = 32 * (tid >> 6) + (lane & 31);
-      const int t = t0 + r / group, head = kvh * group + r % group, cnt = t < tokens ? pos[t] + 1 : 0;
+      const int t = t0 + r / group, head = kvh * group + r % group;
+      const int cnt = t < tokens ? (WIN ? win.count(pos[t]) : pos[t] + 1) : 0;
       const int e = __builtin_amdgcn_frexp_expf(c2) - __builtin_amdgcn_frexp_expf(fabsf(scale) * kLog2e);
       const float sc = ldexpf(scale < 0.0f ? -1.0f : 1.0f, -e);
       const float* qr = q + (int64_t)min(t, tokens - 1) * q_stride + (int64_t)head * D + 8 * h;
 #pragma unroll
       for (int dt = 0; dt < NT; dt++) {
         int x = -100;
-        for (int sl = s0; sl < s1; sl++) {
-          const int cell = cell_of(sl, lane);
+        for (int sv = s0; sv < s1; sv++) {
+          const int sl = slice_of(sv), cell = cell_of(sl, lane);
           float f = __half2float(vc[row_of(cell) + (kvw >> 1) + ((kvh * D) >> 5) + dt]);
           if (sl * kSlice + lane >= count || cell < 0) f = 0.0f;
           for (uint64_t outs = __ballot(track(f, x)); outs; outs &= outs - 1) {
@@ -497,7 +544,8 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
             const float p = __builtin_amdgcn_exp2f((s - mc) * c2) * kLift;
             const float fk = __shfl(f, k) * ldexpf(1.0f, 8 - xo[dt]);
             const int8_t* vb = (const int8_t*)(vc + row) + kvh * D + 32 * dt + 4 * h;
-            if (sl * kSlice + k < cnt) {
+            const int key = sl * kSlice + k;
+            if (key < cnt && (!WIN || key >= cnt - win.window || key < win.first)) {
 #pragma unroll
               for (int j = 0; j < 16; j++)
                 o[dt][j] = fmaf(p, (float)vb[8 * (j >> 2) + (j & 3)] * fk, o[dt][j]);
@@ -508,11 +556,46 @@ __global__ __launch_bounds__(256, 2) void attend_flash_kernel(
     }
   }
 
+  // f16 over a window: the words that were left out, to the rows that see their keys
+  if constexpr (WIN && !Q8) {
+    if (__builtin_expect(left_out, 0)) {
+      const int e = __builtin_amdgcn_frexp_expf(c2) - __builtin_amdgcn_frexp_expf(fabsf(scale) * kLog2e);
+      const float sc = ldexpf(scale < 0.0f ? -1.0f : 1.0f, -e);
+      const float* qr = q + (int64_t)min(t, tokens - 1) * q_stride + (int64_t)head * D + 8 * h;
+      for (int sv = s0; sv < s1; sv++) {
+        const int sl = slice_of(sv), cell = cell_of(sl, lane);
+        uint32_t words = 0;  // of this lane's key
+        if (sl * kSlice + lane < count && cell >= 0)
+          for (int w = 0; w < PIECES; w++)
+            words |= (uint32_t)not_finite(*(const fu4*)(vc + row_of(cell) + kvh * D + 8 * w)) << w;
+        for (uint64_t outs = __ballot(words != 0); outs; outs &= outs - 1) {
+          const int k = __builtin_ctzll(outs), key = sl * kSlice + k;
+          const int64_t row = row_of(__shfl(cell, k)) + kvh * D;
+          const uint32_t which = __shfl((int)words, k);
+          float s = 0.0f;
+#pragma nounroll
+          for (int st = 0; st < D / 16; st++)
+            for (int u = 0; u < 8; u++) s = fmaf(__half2float(kc[row + 16 * st + 8 * h + u]), sc * qr[16 * st + u], s);
+          s = other_sum(s);
+          const float p = __builtin_amdgcn_exp2f((s - mc) * c2) * kLift;
+          if (key < cnt && (key >= cnt - win.window || key < win.first)) {
+#pragma unroll
+            for (int dt = 0; dt < NT; dt++)
+#pragma unroll
+              for (int j = 0; j < 16; j++)
+                if ((which >> (4 * dt + (j >> 2))) & 1)
+                  o[dt][j] = fmaf(p, __half2float(vc[row + 32 * dt + 8 * (j >> 2) + 4 * h + (j & 3)]), o[dt][j]);
+          }
+        }
+      }
+    }
+  }
+
   l = other_sum(l);
   if (!live_row) return;
   const int64_t rowi = (int64_t)t * heads + head;
   float* dst = splits == 1 ? out + rowi * D : part_acc + (rowi * splits + split) * D;
-  const float w = (splits == 1 ? 1.0f / l : 1.0f) * (1.0f / kLift);
+  const float w = (splits == 1 ? (WIN && l == 0.0f ? 0.0f : 1.0f / l) : 1.0f) * (1.0f / kLift);
 #pragma unroll
   for (int dt = 0; dt < NT; dt++) {
     const float f = Q8 ? w * ldexpf(1.0f, xo[dt] - 8) : w;
@@ -556,20 +639,22 @@ __global__ __launch_bounds__(256) void attend_combine_kernel(const float* __rest
       for (int e = 0; e < 4; e++) o[e] = fmaf(a[e], w, o[e]);
     }
   }
-  const float w = 1.0f / l;
+  const float w = l != 0.0f ? 1.0f / l : 0.0f;  // (zeros for a row that sees nothing)
   ((ff4*)out)[(int64_t)row * TPR + d4] = o * w;
 }
 
+}  // namespace
+
 // Shares of the keys: enough that the blocks fill two a compute unit, at
-// most one for each slice of the context, and at most 16 (each is another
-// partial result of every row to write and fold).
-int flash_splits(int kv_heads, int tiles, int max_count) {
-  const int slices = (max_count + kSlice - 1) / kSlice;
+// most one for each slice of the context (of what a tile's windows reach), and at
+// most 16 (each is another partial result of every row to write and fold).
+int flash_splits(int32_t heads, int32_t kv_heads, int32_t max_count, int32_t tokens, const Window* win) {
+  const int group = heads / kv_heads, tq = kRows / group, tiles = (tokens + tq - 1) / tq;
+  int slices = (max_count + kSlice - 1) / kSlice;
+  if (win) slices = (int)std::min<int64_t>(slices, ((int64_t)win->window + tq + win->first) / kSlice + 3);
   const int want = 2 * cu_count() / std::max(1, kv_heads * tiles);
   return std::max(1, std::min({want, slices, 16}));
 }
-
-}  // namespace
 
 bool flash_fits(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t tokens) {
   const int group = heads / kv_heads;
@@ -580,39 +665,49 @@ bool flash_fits(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t token
 int launch_attend_flash(hipStream_t s, const float* q, int64_t q_stride, const uint16_t* k_cache,
                         const uint16_t* v_cache, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
                         const int32_t* pos, int32_t max_count, int32_t tokens, float* out, float* part_acc,
-                        float* part_ml, int32_t form, const int32_t* kv_index) {
+                        float* part_ml, int32_t form, const int32_t* kv_index, const Window* win) {
   const int group = heads / kv_heads, tq = kRows / group, tiles = (tokens + tq - 1) / tq;
-  const int splits = flash_splits(kv_heads, tiles, max_count);
+  const int splits = flash_splits(heads, kv_heads, max_count, tokens, win);
   const int row = cache_row(form, kv_heads * head_dim);
   const dim3 grid(splits, kv_heads, tiles);
-#define MI_FLASH(DD, Q, P)                                                                                       \
-  hipLaunchKernelGGL((attend_flash_kernel<DD, Q, P>), grid, dim3(256), 0, s, q, q_stride, (const __half*)k_cache, \
-                     (const __half*)v_cache, row, heads, kv_heads, group, scale, pos, tokens, kv_index, part_acc, \
-                     part_ml, out)
-#define MI_FLASH_F(DD)                         \
-  if (form == MI_CACHE_Q8) {                   \
-    if (kv_index) MI_FLASH(DD, true, true);    \
-    else MI_FLASH(DD, true, false);            \
-  } else {                                     \
-    if (kv_index) MI_FLASH(DD, false, true);   \
-    else MI_FLASH(DD, false, false);           \
+  const Window w = win ? *win : Window{};
+#define MI_FLASH(DD, Q, P, WN)                                                                                   \
+  hipLaunchKernelGGL((attend_flash_kernel<DD, Q, P, WN>), grid, dim3(256), 0, s, q, q_stride,                    \
+                     (const __half*)k_cache, (const __half*)v_cache, row, heads, kv_heads, group, scale, pos, tokens, \
+                     kv_index, part_acc, part_ml, out, w)
+#define MI_FLASH_F(DD, WN)                         \
+  if (form == MI_CACHE_Q8) {                       \
+    if (kv_index) MI_FLASH(DD, true, true, WN);    \
+    else MI_FLASH(DD, true, false, WN);            \
+  } else {                                         \
+    if (kv_index) MI_FLASH(DD, false, true, WN);   \
+    else MI_FLASH(DD, false, false, WN);           \
   }
-  if (head_dim == 64) {
-    MI_FLASH_F(64)
+  if (win && head_dim == 256) {
+    // (f16 caches only: a wave would stage two q8_0 blocks' values)
+    if (kv_index) MI_FLASH(256, false, true, true);
+    else MI_FLASH(256, false, false, true);
+  } else if (win && head_dim == 64) {
+    MI_FLASH_F(64, true)
+  } else if (win) {
+    MI_FLASH_F(128, true)
+  } else if (head_dim == 64) {
+    MI_FLASH_F(64, false)
   } else {
-    MI_FLASH_F(128)
+    MI_FLASH_F(128, false)
   }
 #undef MI_FLASH_F
 #undef MI_FLASH
   int rc = hip_check(hipGetLastError(), "attend_flash launch");
   if (rc || splits == 1) return rc;
   const int rows = tokens * heads, rpb = 256 / (head_dim / 4);
-  if (head_dim == 64)
-    hipLaunchKernelGGL(attend_combine_kernel<64>, dim3((rows + rpb - 1) / rpb), dim3(256), 0, s, part_acc, part_ml, rows,
-                       splits, out);
-  else
-    hipLaunchKernelGGL(attend_combine_kernel<128>, dim3((rows + rpb - 1) / rpb), dim3(256), 0, s, part_acc, part_ml, rows,
-                       splits, out);
+#define MI_COMBINE(DD)                                                                                               \
+  hipLaunchKernelGGL(attend_combine_kernel<DD>, dim3((rows + rpb - 1) / rpb), dim3(256), 0, s, part_acc, part_ml, rows, \
+                     splits, out)
+  if (head_dim == 64) MI_COMBINE(64);
+  else if (head_dim == 128) MI_COMBINE(128);
+  else MI_COMBINE(256);
+#undef MI_COMBINE
   return hip_check(hipGetLastError(), "attend_combine launch");
 }
 

@@ -19,6 +19,9 @@
 //   attn   attention slices (attend_workspace); over trees their attention's
 //          workspace and its output in f32
 //   trig   rope (cos, sin) of this position
+//   route  with sparse experts, in place of up, gate, xq2 and part: the normed row
+//          and another of its size in f32, the router's choice and the experts' own
+//          workspace (experts_carve)
 //   xq2    4 * hidden * tokens: the down projection's input, when the gate/up
 //          launch writes it (it cannot share xq, which that launch reads)
 // Above 8 tokens (prefill_layer) the activations stay f32 and the pieces are
@@ -26,7 +29,7 @@
 // prefill matmul's own workspace (prefill_carve).
 #include <algorithm>
 
-#include "mi_internal.h"
+#include "experts.h"
 #include "matvec_rows.h"
 
 namespace mi {
@@ -48,30 +51,67 @@ size_t tree_part(const mi_layer_desc* d, const mi_tree* tree) {
   return up256(mi_attend_tree_workspace(d->heads, d->kv_heads, d->head_dim, d->cache_form, tree));
 }
 size_t attend_part(const mi_layer_desc* d, int32_t max_count, int32_t tokens, const mi_tree* tree) {
-  return tree ? tree_part(d, tree) : up256(attend_workspace(d->heads, d->head_dim, max_count, tokens));
+  if (tree) return tree_part(d, tree);
+  if (!d->window) return up256(attend_workspace(d->heads, d->head_dim, max_count, tokens));
+  // (of one sequence's chunk or of many sequences: whichever is larger)
+  const Window w{d->window, d->first, max_count};
+  return up256(std::max(attend_window_workspace(d->heads, d->kv_heads, d->head_dim, d->cache_form, w, tokens, true),
+                        attend_window_workspace(d->heads, d->kv_heads, d->head_dim, d->cache_form, w, tokens, false)));
+}
+
+// Sparse experts' part of a workspace: the normed row, a row for what is normed
+// ahead of the residual, the router's choice, and the larger of its scratch and
+// the MLP's.
+struct ExpertsCarve {
+  size_t xn, tmp, ids, weights, work, total;
+};
+ExpertsCarve experts_carve(const mi_layer_desc* d, int32_t tokens) {
+  ExpertsCarve c{};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += up256(bytes);
+    return p;
+  };
+  c.xn = take(sizeof(float) * (size_t)d->width * tokens);
+  c.tmp = take(sizeof(float) * (size_t)d->width * tokens);
+  c.ids = take(sizeof(int32_t) * (size_t)d->experts_used * tokens);
+  c.weights = take(sizeof(float) * (size_t)d->experts_used * tokens);
+  c.work = take(std::max(router_workspace(d->experts, tokens),
+                         experts_workspace(d->experts, d->width, d->hidden, tokens, d->experts_used)));
+  c.total = at;
+  return c;
 }
 
 struct Carve {
-  size_t xq, qkv, up, gate, attn, trig, xq2, part, total;
+  size_t xq, qkv, up, gate, attn, trig, xq2, part, route, total;
 };
 
 Carve carve(const mi_layer_desc* d, int32_t max_count, int32_t tokens, const mi_tree* tree = nullptr) {
   const int64_t qw = (int64_t)d->heads * d->head_dim, kvw = (int64_t)d->kv_heads * d->head_dim;
-  const int64_t widest = std::max<int64_t>({d->width, qw, d->hidden});
-  Carve c;
+  const bool sparse = d->experts > 0;
+  const int64_t widest = std::max<int64_t>({d->width, qw, sparse ? 0 : d->hidden});
+  Carve c{};
   size_t at = 0;
   c.xq = at;  // at 2..8 tokens followed by the hx form (for wo's f16 matrix-core tile)
   at += up256((size_t)xq_token_bytes((int32_t)widest) * tokens * (tokens > 1 ? 2 : 1));
   c.qkv = at;
   at += up256(sizeof(float) * (size_t)(qw + 2 * kvw) * tokens);
-  c.up = at;
-  at += up256(sizeof(float) * (size_t)d->hidden * tokens);
-  c.gate = at;
-  at += up256(sizeof(float) * (size_t)d->hidden * tokens);
+  if (!sparse) {
+    c.up = at;
+    at += up256(sizeof(float) * (size_t)d->hidden * tokens);
+    c.gate = at;
+    at += up256(sizeof(float) * (size_t)d->hidden * tokens);
+  }
   c.attn = at;
   at += attend_part(d, max_count, tokens, tree) + (tree ? up256(sizeof(float) * (size_t)qw * tokens) : 0);
   c.trig = at;
   at += up256(sizeof(float) * (size_t)d->rope_dim);
+  if (sparse) {
+    c.route = at;
+    c.total = at + experts_carve(d, tokens).total;
+    return c;
+  }
   c.xq2 = at;  // down's input; at 2..8 tokens followed by its hx form
   at += up256((size_t)xq_token_bytes(d->hidden) * tokens * (tokens > 1 ? 2 : 1));
   c.part = at;  // split-K partial sums of the down projection (batch 2..8)
@@ -85,12 +125,13 @@ Carve carve(const mi_layer_desc* d, int32_t max_count, int32_t tokens, const mi_
 
 // A prefill chunk (tokens > 8): f32 activations for the prefill matmul.
 struct PrefillCarve {
-  size_t xn, qkv, attn_out, up, h, attn, mm, total;
+  size_t xn, qkv, attn_out, up, h, attn, mm, route, total;
 };
 
 PrefillCarve prefill_carve(const mi_layer_desc* d, int32_t max_count, int32_t tokens, const mi_tree* tree = nullptr) {
   const int64_t qw = (int64_t)d->heads * d->head_dim, kvw = (int64_t)d->kv_heads * d->head_dim;
-  PrefillCarve c;
+  const bool sparse = d->experts > 0;
+  PrefillCarve c{};
   size_t at = 0;
   c.xn = at;
   at += up256(sizeof(float) * (size_t)d->width * tokens);
@@ -98,20 +139,45 @@ PrefillCarve prefill_carve(const mi_layer_desc* d, int32_t max_count, int32_t to
   at += up256(sizeof(float) * (size_t)(qw + 2 * kvw) * tokens);
   c.attn_out = at;
   at += up256(sizeof(float) * (size_t)qw * tokens);
-  c.up = at;
-  at += up256(sizeof(float) * (size_t)d->hidden * tokens);
-  c.h = at;
-  at += up256(sizeof(float) * (size_t)d->hidden * tokens);
+  if (!sparse) {
+    c.up = at;
+    at += up256(sizeof(float) * (size_t)d->hidden * tokens);
+    c.h = at;
+    at += up256(sizeof(float) * (size_t)d->hidden * tokens);
+  }
   c.attn = at;
   at += attend_part(d, max_count, tokens, tree);
+  if (sparse) {
+    c.route = at;
+    at += experts_carve(d, tokens).total;
+  }
   c.mm = at;
   size_t mm = 0;
   const int32_t shapes[5][2] = {{(int32_t)(qw + 2 * kvw), d->width}, {(int32_t)qw, d->width},
                                 {d->width, (int32_t)qw}, {d->hidden, d->width}, {d->width, d->hidden}};
-  for (auto& sh : shapes) mm = std::max(mm, prefill_workspace(sh[0], sh[1], tokens));
+  for (int i = 0; i < (sparse ? 3 : 5); i++) mm = std::max(mm, prefill_workspace(shapes[i][0], shapes[i][1], tokens));
   at += up256(mm);
   c.total = at;
   return c;
+}
+
+mi_experts experts_of(const mi_layer_desc* d) {
+  return mi_experts{d->experts, d->width, d->hidden, d->act, d->gate, d->up, d->down};
+}
+
+// Sparse experts and the attention's window: what a workspace's size takes of them.
+int check_sparse(const mi_layer_desc* d, int32_t tokens) {
+  if (d->window < 0 || d->first < 0)
+    return fail(MI_ERR_ARG, "layer: a window of %d and the first %d positions", d->window, d->first);
+  if (d->experts < 0) return fail(MI_ERR_SHAPE, "layer: %d experts", d->experts);
+  if (!d->experts) return MI_OK;
+  if (d->ungated) return fail(MI_ERR_ARG, "layer: experts without a gate");
+  const int rc = check_router("layer", d->router, d->width, d->experts, d->experts_used, tokens, d->router_flags,
+                              d->router_scale);
+  if (rc) return rc;
+  if ((int64_t)tokens * d->experts_used > kMaxPairs)
+    return fail(MI_ERR_SHAPE, "layer: %d tokens of %d experts are more than %d rows", tokens, d->experts_used, kMaxPairs);
+  return MI_OK;
 }
 
 int check_desc(const mi_layer_desc* d) {
@@ -150,6 +216,7 @@ int check_desc(const mi_layer_desc* d) {
               {"down", d->down, d->width, d->hidden}};
   for (auto& e : want) {
     if (d->ungated && &e.w == &d->gate) continue;  // act(up(x)): no gate
+    if (d->experts && (&e.w == &d->gate || &e.w == &d->up || &e.w == &d->down)) continue;  // (below)
     // block.mojo:230-247 _shape: a projection of the wrong size is refused.
     if (e.w.rows != e.rows || e.w.cols != e.cols)
       return fail(MI_ERR_SHAPE, "layer: %s is %d x %d where the layer wants %d x %d", e.name, e.w.rows,
@@ -157,13 +224,19 @@ int check_desc(const mi_layer_desc* d) {
     int rc = check_weight(e.name, e.w.kind, e.w.data, e.w.row_bytes, e.w.rows, e.w.cols);
     if (rc) return rc;
   }
-  return MI_OK;
+  int rc = check_sparse(d, 1);
+  if (!rc && d->experts) {
+    const mi_experts x = experts_of(d);
+    rc = check_experts("layer", &x);
+  }
+  return rc;
 }
 
 // Whether the layer uses any part beyond the Llama layer (q|k|v biases,
 // q/k norms, post norms, a non-gated or gelu MLP).
 bool extended(const mi_layer_desc* d) {
-  return d->q_bias || d->q_norm || d->attn_post_norm || d->ffn_post_norm || d->ungated || d->act;
+  if (d->q_bias || d->q_norm || d->attn_post_norm) return true;
+  return !d->experts && (d->ffn_post_norm || d->ungated || d->act);
 }
 
 // Where a layer's keys and values are: the caches and, over trees of drafted
@@ -224,6 +297,36 @@ int tree_attention(hipStream_t s, const mi_layer_desc* d, float* qkv, const Laye
   return launch_tree_attend(s, a, work);
 }
 
+// A layer's attention over the caches: all positions, or a window of them.
+int layer_attend(hipStream_t s, const mi_layer_desc* d, const float* qkv, int64_t qkv_stride, const LayerCache& kv,
+                 const int32_t* pos, int32_t max_count, int32_t tokens, float* out, void* xq, void* work,
+                 void* hx = nullptr) {
+  if (d->window)
+    return launch_attend_window(s, qkv, qkv_stride, kv.k, kv.v, kv.stride, d->heads, d->kv_heads, d->head_dim,
+                                d->attn_scale, pos, Window{d->window, d->first, max_count}, tokens, out, xq, work,
+                                d->cache_form, kv.kv_index, kv.index_stride, hx);
+  return launch_attend(s, qkv, qkv_stride, kv.k, kv.v, kv.stride, d->heads, d->kv_heads, d->head_dim, d->attn_scale, pos,
+                       -1, max_count, tokens, out, xq, work, d->cache_form, kv.kv_index, kv.index_stride, hx);
+}
+
+// The sparse experts' half of a layer: norm, router, the experts' MLP and its sum
+// onto the residual (normed ahead of it with a post norm).  base: experts_carve.
+int experts_layer(hipStream_t s, const mi_layer_desc* d, float* resid, int32_t tokens, char* base) {
+  const ExpertsCarve c = experts_carve(d, tokens);
+  float *xn = (float*)(base + c.xn), *tmp = (float*)(base + c.tmp), *weights = (float*)(base + c.weights);
+  int32_t* ids = (int32_t*)(base + c.ids);
+  int rc = launch_rms_norm(s, resid, d->ffn_norm, d->width, tokens, d->eps, xn, nullptr);
+  if (rc) return rc;
+  if ((rc = launch_router(s, xn, d->router, d->router_bias, d->width, d->experts, d->experts_used, tokens, d->router_flags,
+                          d->router_scale, ids, weights, base + c.work)))
+    return rc;
+  const bool post = d->ffn_post_norm != nullptr;
+  if ((rc = launch_experts_mlp(s, experts_of(d), xn, tokens, d->experts_used, ids, weights, post ? tmp : resid, !post,
+                               base + c.work)))
+    return rc;
+  return post ? launch_norm_add(s, resid, tmp, d->width, tokens, d->ffn_post_norm, d->eps) : MI_OK;
+}
+
 }  // namespace
 
 // The layer with the optional parts of other families at 1..8 tokens, as
@@ -271,11 +374,9 @@ static int extended_layer(hipStream_t s, const mi_layer_desc* d, float* resid, c
                                 tokens, qkv_stride, kv.k, kv.v, kv.stride, d->rope_factors, d->cache_form,
                                 kv.kv_index, kv.index_stride)))
       return rc;
-    if ((rc = launch_attend(s, qkv, qkv_stride, kv.k, kv.v, kv.stride, d->heads, d->kv_heads, d->head_dim,
-                            d->attn_scale, pos, -1, max_count, tokens, nullptr, xq, attn, d->cache_form, kv.kv_index,
-                            kv.index_stride)))
-      return rc;
+    if ((rc = layer_attend(s, d, qkv, qkv_stride, kv, pos, max_count, tokens, nullptr, xq, attn))) return rc;
   }
+  if (d->experts) up = (float*)(base + c.route + experts_carve(d, tokens).tmp);
   if (d->attn_post_norm) {
     // wo into a scratch row (the up buffer is free until the MLP), normed into the stream
     if ((rc = launch_matvec(s, d->wo.kind, d->wo.data, d->wo.row_bytes, d->width, qw, xq, tokens, up, d->width,
@@ -286,6 +387,7 @@ static int extended_layer(hipStream_t s, const mi_layer_desc* d, float* resid, c
                                  d->width, MI_EPI_ADD, nullptr))) {
     return rc;
   }
+  if (d->experts) return experts_layer(s, d, resid, tokens, base + c.route);
   // mlp_layer (block.mojo:429)
   if ((rc = launch_rms_norm(s, resid, d->ffn_norm, d->width, tokens, d->eps, nullptr, xq))) return rc;
   if ((rc = launch_matvec(s, d->up.kind, d->up.data, d->up.row_bytes, d->hidden, d->width, xq, tokens, up,
@@ -387,10 +489,7 @@ static int prefill_layer(hipStream_t s, const mi_layer_desc* d, float* resid, co
                                 tokens, qkv_stride, kv.k, kv.v, kv.stride, d->rope_factors, d->cache_form,
                                 kv.kv_index, kv.index_stride)))
       return rc;
-    if ((rc = launch_attend(s, qkv, qkv_stride, kv.k, kv.v, kv.stride, d->heads, d->kv_heads, d->head_dim,
-                            d->attn_scale, pos, -1, max_count, tokens, attn_out, nullptr, attn, d->cache_form,
-                            kv.kv_index, kv.index_stride)))
-      return rc;
+    if ((rc = layer_attend(s, d, qkv, qkv_stride, kv, pos, max_count, tokens, attn_out, nullptr, attn))) return rc;
   }
   if (d->attn_post_norm) {  // wo into xn (free once q, k, v are made), normed into the stream
     if ((rc = mat(d->wo, d->width, qw, attn_out, xn, d->width, MI_EPI_NONE, nullptr))) return rc;
@@ -398,6 +497,7 @@ static int prefill_layer(hipStream_t s, const mi_layer_desc* d, float* resid, co
   } else if ((rc = mat(d->wo, d->width, qw, attn_out, resid, d->width, MI_EPI_ADD, nullptr))) {
     return rc;
   }
+  if (d->experts) return experts_layer(s, d, resid, tokens, base + c.route);
   // mlp_layer (block.mojo:429)
   if ((rc = launch_rms_norm(s, resid, d->ffn_norm, d->width, tokens, d->eps, xn, nullptr))) return rc;
   if (d->ungated || d->act || d->ffn_post_norm) {
@@ -511,9 +611,12 @@ static int decoder_layer(mi_stream stream, const mi_layer_desc* d, float* resid,
   int rc = check_desc(d);
   if (rc) return rc;
   if (!resid || !k_cache || !v_cache || !pos) return fail(MI_ERR_ARG, "layer: null pointer");
+  if (d->experts && ((uintptr_t)resid & 15))
+    return fail(MI_ERR_ALIGN, "layer: with experts the residual must be 16-byte aligned");
   if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || cache_stride % 8)
     return fail(MI_ERR_ALIGN, "layer: caches must be 16-byte aligned with a stride of a multiple of 8 halves");
   if (tokens < 1 || tokens > kMaxPrefill) return fail(MI_ERR_ARG, "layer: tokens %d outside 1..%d", tokens, kMaxPrefill);
+  if ((rc = check_sparse(d, tokens))) return rc;
   if (max_count <= 0) return fail(MI_ERR_SHAPE, "layer: max_count must be positive");
   const int64_t kvw = (int64_t)d->kv_heads * d->head_dim;
   const int64_t crow = cache_row(d->cache_form, (int32_t)kvw);  // halves per position
@@ -754,19 +857,18 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, cons
     float* out = (float*)((char*)attn + tree_part(d, kv.tree));
     if ((rc = tree_attention(s, d, qkv, kv, out, attn))) return rc;
     if ((rc = launch_quantize(s, out, qw, tokens, xq, hx))) return rc;
-  } else if ((rc = launch_attend(s, qkv, qkv_stride, kv.k, kv.v, kv.stride, d->heads, d->kv_heads, d->head_dim,
-                                 d->attn_scale, pos, -1, max_count, tokens, nullptr, xq, attn, d->cache_form,
-                                 kv.kv_index, kv.index_stride, hx))) {
+  } else if ((rc = layer_attend(s, d, qkv, qkv_stride, kv, pos, max_count, tokens, nullptr, xq, attn, hx))) {
     // count = pos + 1 per sequence: the attention kernels read pos and add one.
     return rc;
   }
-  const bool glu_tile = tokens >= 4 && d->gate.kind == MI_Q4_K && d->up.kind == MI_Q4_K &&
+  const bool glu_tile = tokens >= 4 && !d->experts && d->gate.kind == MI_Q4_K && d->up.kind == MI_Q4_K &&
                         d->gate.row_bytes == d->up.row_bytes && htile_glu_fits(d->hidden, d->width, tokens);
   const bool wo_split = glu_tile && wo_split_norm(d, qw, tokens);
   if (!wo_split && (rc = launch_matvec(s, d->wo.kind, d->wo.data, d->wo.row_bytes, d->width, qw, xq, tokens, resid,
                                        d->width, MI_EPI_ADD, nullptr, hx)))
     return rc;
 
+  if (d->experts) return experts_layer(s, d, resid, tokens, base + c.route);
   // mlp_layer (block.mojo:429), gated silu
   if (tokens == 1 && d->gate.kind == MI_Q4_K && d->up.kind == MI_Q4_K && d->gate.row_bytes == d->up.row_bytes &&
       q4k_glu_norm_fits(d->hidden, d->width, resid, d->ffn_norm)) {
@@ -837,7 +939,7 @@ static int llama_layer(hipStream_t s, const mi_layer_desc* d, float* resid, cons
 extern "C" {
 
 size_t mi_layer_workspace(const mi_layer_desc* desc, int32_t max_count, int32_t tokens) {
-  if (!desc || max_count <= 0 || tokens <= 0 || tokens > kMaxPrefill) return 0;
+  if (!desc || max_count <= 0 || tokens <= 0 || tokens > kMaxPrefill || check_sparse(desc, tokens)) return 0;
   if (tokens > kMaxTokens) return prefill_carve(desc, max_count, tokens).total;
   return carve(desc, max_count, tokens).total;
 }
@@ -860,7 +962,7 @@ int mi_decoder_layer_paged(mi_stream stream, const mi_layer_desc* d, float* resi
 }
 
 size_t mi_layer_tree_workspace(const mi_layer_desc* desc, const mi_tree* tree) {
-  if (!desc || !tree || tree->tokens > kMaxPrefill || !tree_part(desc, tree)) return 0;
+  if (!desc || !tree || tree->tokens > kMaxPrefill || !tree_part(desc, tree) || check_sparse(desc, tree->tokens)) return 0;
   const int32_t n = tree->tokens;
   return n > kMaxTokens ? prefill_carve(desc, tree->max_count, n, tree).total : carve(desc, tree->max_count, n, tree).total;
 }
@@ -871,12 +973,16 @@ int mi_decoder_layer_tree(mi_stream stream, const mi_layer_desc* d, float* resid
   int rc = check_desc(d);
   if (rc) return rc;
   if (!resid || !k_cache || !v_cache) return fail(MI_ERR_ARG, "layer: null pointer");
+  if (d->experts && ((uintptr_t)resid & 15))
+    return fail(MI_ERR_ALIGN, "layer: with experts the residual must be 16-byte aligned");
   if ((rc = check_tree("layer", tree, true))) return rc;
   if ((rc = check_tree_caches("layer", d->cache_form, d->heads, d->kv_heads, d->head_dim, d->attn_scale, k_cache, v_cache,
                               cache_stride, kv_index, index_stride, tree)))
     return rc;
   if (tree->tokens > kMaxPrefill)
     return fail(MI_ERR_ARG, "layer: tokens %d outside 1..%d", tree->tokens, kMaxPrefill);
+  if (d->window) return fail(MI_ERR_ARG, "layer: no window over trees");
+  if ((rc = check_sparse(d, tree->tokens))) return rc;
   const LayerCache kv{k_cache, v_cache, cache_stride, kv_index, index_stride, tree};
   return run_layer((hipStream_t)stream, d, resid, kv, tree->pos, tree->max_count, tree->tokens, work, work_bytes);
 }

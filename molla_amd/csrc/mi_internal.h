@@ -255,12 +255,35 @@ int launch_attend(hipStream_t s, const float* q, int64_t q_stride, const uint16_
                   int32_t max_count, int32_t tokens, float* out, void* xq_out, void* work,
                   int32_t form = MI_CACHE_F16, const int32_t* kv_index = nullptr, int64_t index_stride = 0,
                   void* hx_out = nullptr);
+// A window of attention: a token at position p sees the positions up to p that are
+// above p - window or below `first`.  `limit` bounds the positions (max_count).
+struct Window {
+  int32_t window, first, limit;
+  // positions up to pos, of those there are
+  __device__ __forceinline__ int count(int pos) const { return max(min(pos, limit - 1) + 1, 0); }
+  // The keys of a token at `pos`, numbered end to end:
+  // key v is position v below `near`, position v + skip from there on.
+  __device__ __forceinline__ int keys(int pos, int& near, int& skip) const {
+    const int count = this->count(pos);
+    const int low = count > window ? count - window : 0;
+    near = first < low ? first : low;
+    skip = low - near;
+    return count - skip;
+  }
+  // the most keys a token sees
+  int most() const {
+    const int64_t n = (int64_t)window + first;
+    return n < limit ? (int)n : limit;
+  }
+};
+
 // Decode attention at head widths 64 and 128, either cache form
 // (attend_decode.hip): each token's keys in `shares` parts, whose (maximum,
 // sum) in base 2 and values go to part_ml / part_acc slot (token, head, share);
 // a share without keys leaves the sum 0 and no values.  Never more shares than
 // the context has 64-key slices (launch_attend's workspace).
 bool decode_attend_fits(int32_t group, int32_t head_dim);
+bool decode_window_fits(int32_t group, int32_t head_dim);
 struct DecodePlan {
   int32_t waves, shares;  // of a block; of the keys
 };
@@ -269,7 +292,7 @@ int launch_attend_decode(hipStream_t s, const float* q, int64_t q_stride, const 
                          const uint16_t* v_cache, int64_t cache_stride, int32_t heads, int32_t kv_heads,
                          int32_t head_dim, float scale, const int32_t* pos, int32_t count_host, DecodePlan plan,
                          int32_t tokens, float* part_acc, float* part_ml, int32_t form, const int32_t* kv_index,
-                         int64_t index_stride);
+                         int64_t index_stride, const Window* win = nullptr);
 // One sequence's chunk of more than kMaxTokens tokens at head widths 64 and
 // 128, either cache form (attend_flash.hip); cache rows from the sequence's
 // start or through kv_index.  part_acc / part_ml as launch_attend carves them.
@@ -277,7 +300,17 @@ bool flash_fits(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t token
 int launch_attend_flash(hipStream_t s, const float* q, int64_t q_stride, const uint16_t* k_cache,
                         const uint16_t* v_cache, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
                         const int32_t* pos, int32_t max_count, int32_t tokens, float* out, float* part_acc,
-                        float* part_ml, int32_t form, const int32_t* kv_index);
+                        float* part_ml, int32_t form, const int32_t* kv_index, const Window* win = nullptr);
+int flash_splits(int32_t heads, int32_t kv_heads, int32_t max_count, int32_t tokens, const Window* win);
+// Attention over a window (mi_attend_window, and the layer's): the paths above,
+// and how many parts of a (token, head) each leaves.  Arguments as launch_attend.
+size_t attend_window_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const Window& win,
+                               int32_t tokens, bool one_seq);
+int launch_attend_window(hipStream_t s, const float* q, int64_t q_stride, const uint16_t* k_cache,
+                         const uint16_t* v_cache, int64_t cache_stride, int32_t heads, int32_t kv_heads,
+                         int32_t head_dim, float scale, const int32_t* pos, const Window& win, int32_t tokens, float* out,
+                         void* xq_out, void* work, int32_t form, const int32_t* kv_index, int64_t index_stride,
+                         void* hx_out = nullptr);
 int launch_argmax(hipStream_t s, const float* x, int32_t n, int32_t tokens, int32_t* out);
 size_t argmax_workspace(int32_t n, int32_t tokens);
 int launch_argmax_ws(hipStream_t s, const float* x, int32_t n, int32_t tokens, int32_t* out, void* work,

@@ -324,18 +324,29 @@ __device__ __forceinline__ int kv_cell(const int32_t* __restrict__ kv_index, int
 // stages the slice once and scores tq consecutive tokens against it, each
 // with its own count, so a prefill chunk reads every slice once per tq
 // tokens instead of once per token.
-template <int GROUP>
+//
+// WIN (a token a block): the keys are those a Window leaves, numbered end to end
+// (win_key), and values of masked keys are staged as zeros.
+__device__ __forceinline__ int win_key(int j, int near, int skip) { return j < near ? j : j + skip; }
+
+template <int GROUP, bool WIN = false>
 __global__ __launch_bounds__(kAttnThreads) void attend_split_kernel(
     const float* __restrict__ q, int64_t q_stride, const __half* __restrict__ kc,
     const __half* __restrict__ vc, int64_t cache_stride, int heads, int kv_heads, int head_dim,
     float scale, const int32_t* __restrict__ pos_dev, int count_host, int max_chunks,
     float* __restrict__ part_acc, float* __restrict__ part_ml, const int32_t* __restrict__ kv_index,
-    int64_t index_stride, int tokens, int tq) {
+    int64_t index_stride, int tokens, int tq, const Window win) {
+  int near = 0, skip = 0;
+  auto key_of = [&](int j) __attribute__((always_inline)) { return WIN ? win_key(j, near, skip) : j; };
+  auto count_of = [&](int t) __attribute__((always_inline)) {
+    if constexpr (WIN) return win.keys(pos_dev[t], near, skip);
+    return pos_dev ? pos_dev[t] + 1 : count_host;
+  };
   const int c = blockIdx.x, kvh = blockIdx.y;
   const int t0 = blockIdx.z * tq, t1 = min(t0 + tq, tokens);
   // a position p attends over p + 1 slots; the block stages for its widest
   int count_max = 0;
-  for (int t = t0; t < t1; t++) count_max = max(count_max, pos_dev ? pos_dev[t] + 1 : count_host);
+  for (int t = t0; t < t1; t++) count_max = max(count_max, count_of(t));
   const int kk = attn_slice(head_dim);
   const int start = c * kk;
   if (start >= count_max) return;
@@ -369,10 +380,11 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_kernel(
     for (int j = 0; j < kBatch; j++) {
       const int i = min(b0 + tid + j * kAttnThreads, total - 1);
       const int key = min(i / pieces, nk_max - 1), pc = i % pieces;
-      const int cell = max(kv_cell(kv_index, index_stride, t0, start + key), 0);
+      const int found = kv_cell(kv_index, index_stride, t0, key_of(start + key)), cell = max(found, 0);
       const int64_t off = (int64_t)cell * kvw + pc * 8;
       kv[j] = *(const uint4*)(kbase + off);
       vv[j] = *(const uint4*)(vbase + off);
+      if (WIN && (found < 0 || i / pieces >= nk_max)) vv[j] = make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int j = 0; j < kBatch; j++) {
@@ -386,7 +398,7 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_kernel(
   }
   const int halfD = D >> 1;
   for (int t = t0; t < t1; t++) {
-    const int count = pos_dev ? pos_dev[t] + 1 : count_host;
+    const int count = count_of(t);
     if (start >= count) continue;  // uniform over the block: no keys of this slice for t
     const int nk = min(kk, count - start);
     if (t == t0) {
@@ -420,7 +432,7 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_kernel(
           sdot = fmaf(qb.w, k3.y, sdot);
         }
       }
-      const bool live = lane < nk && (!kv_index || kv_cell(kv_index, index_stride, t, start + lane) >= 0);
+      const bool live = lane < nk && (!kv_index || kv_cell(kv_index, index_stride, t, key_of(start + lane)) >= 0);
       const float sc = live ? sdot * scale : -INFINITY;
       float m = sc;
 #pragma unroll
@@ -430,6 +442,7 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_kernel(
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
       if (lane < kk) Ps[g * kk + lane] = pr;
+      if (WIN && l == 0.0f) m = -3e38f;  // (nothing held: no part in the fold)
       if (lane == 0) {
         part_ml[(slot_base + (int64_t)g * max_chunks) * 2 + 0] = m;
         part_ml[(slot_base + (int64_t)g * max_chunks) * 2 + 1] = l;
@@ -470,16 +483,20 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_kernel(
 // bytes of the f16 form); a key or value element is read as float(q) *
 // float(factor), which is gpu.mojo:1168 cache_load, and then used exactly
 // as the f16 kernel uses a widened half.
-template <int GROUP>
+template <int GROUP, bool WIN = false>
 __global__ __launch_bounds__(kAttnThreads) void attend_split_q8_kernel(
     const float* __restrict__ q, int64_t q_stride, const __half* __restrict__ kc,
     const __half* __restrict__ vc, int64_t cache_stride, int row, int heads, int kv_heads, int head_dim,
     float scale, const int32_t* __restrict__ pos_dev, int count_host, int max_chunks,
     float* __restrict__ part_acc, float* __restrict__ part_ml, const int32_t* __restrict__ kv_index,
-    int64_t index_stride) {
+    int64_t index_stride, const Window win) {
 #pragma clang fp contract(off)
   const int c = blockIdx.x, kvh = blockIdx.y, t = blockIdx.z;
-  const int count = pos_dev ? pos_dev[t] + 1 : count_host;
+  int near = 0, skip = 0;
+  int count;
+  if constexpr (WIN) count = win.keys(pos_dev[t], near, skip);
+  else count = pos_dev ? pos_dev[t] + 1 : count_host;
+  auto key_of = [&](int j) __attribute__((always_inline)) { return WIN ? win_key(j, near, skip) : j; };
   const int kk = attn_slice(head_dim);
   const int start = c * kk;
   if (start >= count) return;
@@ -511,7 +528,7 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_q8_kernel(
     for (int j = 0; j < 2; j++) {
       const int i = min(b0 + tid + j * kAttnThreads, total - 1);
       const int key = min(i / pieces, nk - 1), pc = i % pieces;
-      const int cell = max(kv_cell(kv_index, index_stride, t, start + key), 0);
+      const int cell = max(kv_cell(kv_index, index_stride, t, key_of(start + key)), 0);
       const int64_t off = (int64_t)cell * row * 2 + (int64_t)kvh * D + pc * 16;  // bytes
       kv[j] = *(const uint4*)((const int8_t*)kseq + off);
       vv[j] = *(const uint4*)((const int8_t*)vseq + off);
@@ -528,10 +545,10 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_q8_kernel(
   }
   for (int i = tid; i < kk * NB; i += kAttnThreads) {
     const int key = min(i / NB, nk - 1), b = i % NB;
-    const int cell = max(kv_cell(kv_index, index_stride, t, start + key), 0);
+    const int found = kv_cell(kv_index, index_stride, t, key_of(start + key)), cell = max(found, 0);
     const int64_t at = (int64_t)cell * row + (kvw >> 1) + (kvh * D >> 5) + b;  // halves
     Ksc[i] = __half2float(kseq[at]);
-    Vsc[i] = __half2float(vseq[at]);
+    Vsc[i] = WIN && (found < 0 || i / NB >= nk) ? 0.0f : __half2float(vseq[at]);
   }
   if (tid < nq4) ((float4*)Qs)[tid] = qv;
   for (int i = tid + kAttnThreads; i < nq4; i += kAttnThreads) ((float4*)Qs)[i] = q4[i];
@@ -551,7 +568,7 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_q8_kernel(
         for (int i = 0; i < 16; i++) sdot = fmaf(qg[d + i], (float)b[i] * f, sdot);
       }
     }
-    const bool live = lane < nk && (!kv_index || kv_cell(kv_index, index_stride, t, start + lane) >= 0);
+    const bool live = lane < nk && (!kv_index || kv_cell(kv_index, index_stride, t, key_of(start + lane)) >= 0);
     const float sc = live ? sdot * scale : -INFINITY;
     float m = sc;
 #pragma unroll
@@ -561,6 +578,7 @@ __global__ __launch_bounds__(kAttnThreads) void attend_split_q8_kernel(
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
     if (lane < kk) Ps[g * kk + lane] = pr;
+    if (WIN && l == 0.0f) m = -3e38f;
     if (lane == 0) {
       part_ml[(slot_base + (int64_t)g * max_chunks) * 2 + 0] = m;
       part_ml[(slot_base + (int64_t)g * max_chunks) * 2 + 1] = l;
@@ -622,12 +640,12 @@ __global__ __launch_bounds__(256) void store_kv_q8_kernel(const float* __restric
 // 12-32 us slower (batch 1 to 8) than 40 or 48.
 // FOLD: the slices are attend_decode.hip's shares, max_chunks of them whatever
 // the position, their maxima in base 2 and a sum of 0 where no key fell in
-// (whose values were never written).
-template <int B, bool FOLD>
+// (whose values were never written).  WIN: the slices of what a Window leaves.
+template <int B, bool FOLD, bool WIN = false>
 __global__ void attend_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml,
                                     int heads, int head_dim, const int32_t* __restrict__ pos_dev,
                                     int count_host, int max_chunks, float* __restrict__ out,
-                                    uint8_t* __restrict__ xq, uint8_t* __restrict__ hx) {
+                                    uint8_t* __restrict__ xq, uint8_t* __restrict__ hx, const Window win) {
   const int h = blockIdx.x, t = blockIdx.y;
   const int64_t slot = ((int64_t)t * heads + h) * max_chunks;
   const int d = threadIdx.x, lane = d & 63;
@@ -638,7 +656,11 @@ __global__ void attend_merge_kernel(const float* __restrict__ part_acc, const fl
 #pragma unroll
   for (int k = 0; k < B; k++) a[k] = pa[(int64_t)min(k, max_chunks - 1) * head_dim];
   float2 ml = pml[min(lane, max_chunks - 1)];
-  const int count = pos_dev ? pos_dev[t] + 1 : count_host;  // a position p attends over p + 1 slots
+  int count = pos_dev ? pos_dev[t] + 1 : count_host;  // a position p attends over p + 1 slots
+  if constexpr (WIN && !FOLD) {
+    int near, skip;
+    count = win.keys(pos_dev[t], near, skip);
+  }
   const int kk = attn_slice(head_dim);
   const int chunks = FOLD ? max_chunks : min((count + kk - 1) / kk, max_chunks);
   // the largest slice max over every round
@@ -669,7 +691,8 @@ __global__ void attend_merge_kernel(const float* __restrict__ part_acc, const fl
     }
   }
   L = lanes::reduce<64>(L, lanes::Add{});
-  o *= 1.0f / L;
+  if constexpr (WIN) o = L != 0.0f ? o * (1.0f / L) : 0.0f;  // (zeros for a token that sees nothing)
+  else o *= 1.0f / L;
   const int width = heads * head_dim;
   if (live && out) out[(int64_t)t * width + (int64_t)h * head_dim + d] = o;
   if (xq)
@@ -1000,16 +1023,18 @@ int launch_store_kv(hipStream_t s, const float* k, const float* v, int32_t kv_wi
 // attend_merge_kernel with B the slice count rounded up to 8 (at most 64)
 static int launch_merge(hipStream_t s, const float* part_acc, const float* part_ml, int heads, int head_dim,
                         const int32_t* pos_dev, int count_host, int chunks, int tokens, float* out, void* xq_out,
-                        void* hx_out, bool fold = false) {
+                        void* hx_out, bool fold = false, const Window* win = nullptr) {
   // (whole waves: their sums take every lane)
   const dim3 grid(heads, tokens), block((head_dim + 63) / 64 * 64);
-#define MI_MERGE(B)                                                                                            \
-  if (fold)                                                                                                    \
-    hipLaunchKernelGGL((attend_merge_kernel<B, true>), grid, block, 0, s, part_acc, part_ml, heads, head_dim,    \
-                       pos_dev, count_host, chunks, out, (uint8_t*)xq_out, (uint8_t*)hx_out);                    \
-  else                                                                                                         \
-    hipLaunchKernelGGL((attend_merge_kernel<B, false>), grid, block, 0, s, part_acc, part_ml, heads, head_dim,   \
-                       pos_dev, count_host, chunks, out, (uint8_t*)xq_out, (uint8_t*)hx_out)
+#define MI_MERGE_W(B, F, WN)                                                                                   \
+  hipLaunchKernelGGL((attend_merge_kernel<B, F, WN>), grid, block, 0, s, part_acc, part_ml, heads, head_dim,    \
+                     pos_dev, count_host, chunks, out, (uint8_t*)xq_out, (uint8_t*)hx_out, w)
+#define MI_MERGE(B)                             \
+  if (fold && win) MI_MERGE_W(B, true, true);   \
+  else if (fold) MI_MERGE_W(B, true, false);    \
+  else if (win) MI_MERGE_W(B, false, true);     \
+  else MI_MERGE_W(B, false, false)
+  const Window w = win ? *win : Window{};
   switch ((std::min(chunks, 64) + 7) / 8) {
     case 1: MI_MERGE(8); break;
     case 2: MI_MERGE(16); break;
@@ -1021,6 +1046,7 @@ static int launch_merge(hipStream_t s, const float* part_acc, const float* part_
     default: MI_MERGE(64); break;
   }
 #undef MI_MERGE
+#undef MI_MERGE_W
   return hip_check(hipGetLastError(), "attend_merge launch");
 }
 
@@ -1073,11 +1099,11 @@ int launch_attend(hipStream_t s, const float* q, int64_t q_stride, const uint16_
   if (q8)                                                                                                  \
     hipLaunchKernelGGL(attend_split_q8_kernel<G>, grid, dim3(kAttnThreads), shmem, s, q, q_stride, kc, vc,  \
                        cache_stride, row, heads, kv_heads, head_dim, scale, pos_dev, count_host, chunks,    \
-                       part_acc, part_ml, kv_index, index_stride);                                         \
+                       part_acc, part_ml, kv_index, index_stride, Window{});                               \
   else                                                                                                     \
     hipLaunchKernelGGL(attend_split_kernel<G>, grid, dim3(kAttnThreads), shmem, s, q, q_stride, kc, vc,     \
                        cache_stride, heads, kv_heads, head_dim, scale, pos_dev, count_host, chunks,         \
-                       part_acc, part_ml, kv_index, index_stride, tokens, tq)
+                       part_acc, part_ml, kv_index, index_stride, tokens, tq, Window{})
   switch (group) {
     case 1: MI_ATTEND(1); break;
     case 2: MI_ATTEND(2); break;
@@ -1090,6 +1116,93 @@ int launch_attend(hipStream_t s, const float* q, int64_t q_stride, const uint16_
   if (rc) return rc;
   return launch_merge(s, part_acc, part_ml, heads, head_dim, pos_dev, count_host, chunks, tokens, out, xq_out,
                       hx_out);
+}
+
+// Attention over a window.  The paths of launch_attend, with what the window leaves
+// in place of the context, and heads of 256: decode shares at up to 8 tokens, and at
+// any count where each token has a sequence of its own (or the chunk kernel does not
+// take the cache); a sequence's chunk; slices for the other widths.
+namespace {
+enum WindowPath { kShares, kChunk, kSlices };
+struct WindowPlan {
+  WindowPath path;
+  int parts;  // of a (token, head)
+  DecodePlan decode;
+};
+WindowPlan window_plan(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const Window& win, int32_t tokens,
+                       bool one_seq) {
+  const int group = heads / kv_heads;
+  const bool q8 = form == MI_CACHE_Q8, mfma = decode_window_fits(group, head_dim);
+  WindowPlan p{};
+  if (mfma && tokens > kMaxTokens && one_seq && !(q8 && head_dim == 256)) {
+    p.path = kChunk;
+    p.parts = flash_splits(heads, kv_heads, win.limit, tokens, &win);
+  } else if (mfma) {
+    p.path = kShares;
+    p.decode = decode_attend_plan(kv_heads, tokens, win.most(), q8);
+    p.parts = p.decode.shares;
+  } else {
+    p.path = kSlices;
+    const int kk = attn_slice(head_dim);
+    p.parts = (win.most() + kk - 1) / kk;
+  }
+  return p;
+}
+size_t window_acc_bytes(const WindowPlan& p, int32_t heads, int32_t head_dim, int32_t tokens) {
+  return ((size_t)tokens * heads * p.parts * head_dim * sizeof(float) + 255) & ~(size_t)255;
+}
+}  // namespace
+
+size_t attend_window_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const Window& win,
+                               int32_t tokens, bool one_seq) {
+  const WindowPlan p = window_plan(heads, kv_heads, head_dim, form, win, tokens, one_seq);
+  return window_acc_bytes(p, heads, head_dim, tokens) + (size_t)tokens * heads * p.parts * 2 * sizeof(float);
+}
+
+int launch_attend_window(hipStream_t s, const float* q, int64_t q_stride, const uint16_t* k_cache,
+                         const uint16_t* v_cache, int64_t cache_stride, int32_t heads, int32_t kv_heads,
+                         int32_t head_dim, float scale, const int32_t* pos, const Window& win, int32_t tokens, float* out,
+                         void* xq_out, void* work, int32_t form, const int32_t* kv_index, int64_t index_stride,
+                         void* hx_out) {
+  const bool one_seq = kv_index ? index_stride == 0 : cache_stride == 0;
+  const WindowPlan p = window_plan(heads, kv_heads, head_dim, form, win, tokens, one_seq);
+  float* part_acc = (float*)work;
+  float* part_ml = (float*)((char*)work + window_acc_bytes(p, heads, head_dim, tokens));
+  if (p.path == kChunk)
+    return launch_attend_flash(s, q, q_stride, k_cache, v_cache, heads, kv_heads, head_dim, scale, pos, win.limit,
+                               tokens, out, part_acc, part_ml, form, kv_index, &win);
+  if (p.path == kShares) {
+    const int rc = launch_attend_decode(s, q, q_stride, k_cache, v_cache, cache_stride, heads, kv_heads, head_dim, scale,
+                                        pos, 0, p.decode, tokens, part_acc, part_ml, form, kv_index, index_stride, &win);
+    if (rc) return rc;
+  } else {
+    const int group = heads / kv_heads, row = cache_row(form, kv_heads * head_dim);
+    const bool q8 = form == MI_CACHE_Q8;
+    const dim3 grid(p.parts, kv_heads, tokens);
+    const size_t shmem = q8 ? attn_q8_lds_bytes(head_dim, group) : attn_lds_bytes(head_dim, group);
+    const __half *kc = (const __half*)k_cache, *vc = (const __half*)v_cache;
+#define MI_WIN(G)                                                                                                   \
+  if (q8)                                                                                                           \
+    hipLaunchKernelGGL((attend_split_q8_kernel<G, true>), grid, dim3(kAttnThreads), shmem, s, q, q_stride, kc, vc,   \
+                       cache_stride, row, heads, kv_heads, head_dim, scale, pos, 0, p.parts, part_acc, part_ml,     \
+                       kv_index, index_stride, win);                                                                \
+  else                                                                                                              \
+    hipLaunchKernelGGL((attend_split_kernel<G, true>), grid, dim3(kAttnThreads), shmem, s, q, q_stride, kc, vc,      \
+                       cache_stride, heads, kv_heads, head_dim, scale, pos, 0, p.parts, part_acc, part_ml, kv_index, \
+                       index_stride, tokens, 1, win)
+    switch (group) {
+      case 1: MI_WIN(1); break;
+      case 2: MI_WIN(2); break;
+      case 4: MI_WIN(4); break;
+      case 8: MI_WIN(8); break;
+      default: return fail(MI_ERR_SHAPE, "attend: %d query heads per key head is not 1, 2, 4 or 8", group);
+    }
+#undef MI_WIN
+    const int rc = hip_check(hipGetLastError(), "attend_window launch");
+    if (rc) return rc;
+  }
+  return launch_merge(s, part_acc, part_ml, heads, head_dim, pos, 0, p.parts, tokens, out, xq_out, hx_out,
+                      p.path == kShares, &win);
 }
 
 int launch_argmax(hipStream_t s, const float* x, int32_t n, int32_t tokens, int32_t* out) {

@@ -409,6 +409,56 @@ int mi_attend_form(mi_stream stream, int32_t form, const float* q, const uint16_
                        kv_heads, head_dim, scale, nullptr, count, count, 1, out, nullptr, work, form);
 }
 
+// The shape of attention over a window.
+static int check_window(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, int32_t window, int32_t first,
+                        int32_t max_count, int32_t tokens) {
+  const int rc = check_attn("attend_window", heads, kv_heads, head_dim);
+  if (rc) return rc;
+  if ((int64_t)heads * head_dim > kMaxHeadsWidth)
+    return fail(MI_ERR_SHAPE, "attend_window: rows of %lld values", (long long)heads * head_dim);
+  if (cache_row(form, kv_heads * head_dim) < 0) return fail(MI_ERR_SHAPE, "attend_window: unknown cache form %d", form);
+  if (window < 1 || first < 0)
+    return fail(MI_ERR_ARG, "attend_window: a window of %d and the first %d positions", window, first);
+  if (max_count < 1) return fail(MI_ERR_SHAPE, "attend_window: max_count must be positive");
+  if (tokens < 1 || tokens > kMaxPrefill) return fail(MI_ERR_ARG, "attend_window: tokens %d outside 1..%d", tokens, kMaxPrefill);
+  return MI_OK;
+}
+
+size_t mi_attend_window_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, int32_t window,
+                                  int32_t first, int32_t max_count, int32_t tokens, int32_t one_seq) {
+  if (check_window(heads, kv_heads, head_dim, form, window, first, max_count, tokens)) return 0;
+  return attend_window_workspace(heads, kv_heads, head_dim, form, Window{window, first, max_count}, tokens, one_seq != 0);
+}
+
+int mi_attend_window(mi_stream stream, int32_t form, const float* q, int64_t q_stride, const uint16_t* k_cache,
+                     const uint16_t* v_cache, int64_t cache_stride, const int32_t* kv_index, int64_t index_stride,
+                     int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, int32_t window, int32_t first,
+                     const int32_t* pos, int32_t max_count, int32_t tokens, float* out, void* work, size_t work_bytes) {
+  if (!q || !k_cache || !v_cache || !pos || !out) return fail(MI_ERR_ARG, "attend_window: null pointer");
+  const int rc = check_window(heads, kv_heads, head_dim, form, window, first, max_count, tokens);
+  if (rc) return rc;
+  if (!std::isfinite(scale)) return fail(MI_ERR_ARG, "attend_window: the scale of the scores has to be finite");
+  const int64_t qw = (int64_t)heads * head_dim, row = cache_row(form, kv_heads * head_dim);
+  if (q_stride < qw) return fail(MI_ERR_SHAPE, "attend_window: row stride too small");
+  if (cache_stride < 0 || index_stride < 0) return fail(MI_ERR_SHAPE, "attend_window: negative stride");
+  const int64_t stride = kv_index ? index_stride : cache_stride;
+  if (tokens > 1 && stride != 0 && stride < (kv_index ? max_count : max_count * row))
+    return fail(MI_ERR_SHAPE, "attend_window: a sequence's stride holds fewer than %d positions", max_count);
+  if ((((uintptr_t)q | (uintptr_t)out) & 15) || q_stride % 4)
+    return fail(MI_ERR_ALIGN, "attend_window: the queries and the output must be 16-byte aligned");
+  if ((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) || (!kv_index && cache_stride % 8))
+    return fail(MI_ERR_ALIGN, "attend_window: the caches must be 16-byte aligned with a stride of a multiple of 8 halves");
+  // (a tile's queries are read by several blocks, one of which may have written its rows)
+  if (out < q + (tokens - 1) * q_stride + qw && q < out + tokens * qw)
+    return fail(MI_ERR_ARG, "attend_window: the output may not lie among the queries");
+  const Window win{window, first, max_count};
+  const size_t need = attend_window_workspace(heads, kv_heads, head_dim, form, win, tokens, stride == 0);
+  if (!work || ((uintptr_t)work & 255) || work_bytes < need)
+    return fail(MI_ERR_WORKSPACE, "attend_window: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);
+  return launch_attend_window((hipStream_t)stream, q, q_stride, k_cache, v_cache, cache_stride, heads, kv_heads, head_dim,
+                              scale, pos, win, tokens, out, nullptr, work, form, kv_index, index_stride);
+}
+
 int mi_argmax(mi_stream stream, const float* x, int32_t n, int32_t tokens, int32_t* out) {
   if (!x || !out) return fail(MI_ERR_ARG, "argmax: null pointer");
   if (n <= 0 || tokens <= 0) return fail(MI_ERR_SHAPE, "argmax: empty row");

@@ -422,6 +422,41 @@ def device_attend_tree(ctx: DeviceContext, q: torch.Tensor, k_cache: torch.Tenso
            t, _on(ctx, out, "out", torch.float32, tokens * qw), work.data_ptr(), work.numel())
 
 
+def device_attend_window(ctx: DeviceContext, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, heads: int,
+                         kv_heads: int, head_dim: int, scale: float, window: int, first: int, pos: torch.Tensor,
+                         max_count: int, out: torch.Tensor, cache_stride: int = 0, kv_index: torch.Tensor | None = None,
+                         form: int = CACHE_F16, work: torch.Tensor | None = None) -> None:
+    """Attention over the last `window` positions and the first few (mi_attend_window):
+    the token of row t of q [tokens, heads * head_dim] (rows of any stride) is at
+    position pos[t] (int32) of its sequence and sees the positions up to its own that
+    are above pos[t] - window or below `first`.  Its sequence's cache lies cache_stride
+    halves after the one before, or kv_index [tokens, positions] lists its pool cells;
+    a cache_stride of 0, or one list [positions], makes the rows one sequence's chunk.
+    max_count bounds the positions.  out is as q, contiguous."""
+    f16, i32 = torch.float16, torch.int32
+    tokens, qw = pos.numel(), heads * head_dim
+    row = cache_row(form, kv_heads * head_dim)
+    stride = 0
+    if kv_index is not None:
+        if kv_index.dim() not in (1, 2) or (kv_index.dim() == 2 and kv_index.shape[0] != tokens):
+            raise ValueError(f"attend_window wants one list of cells, or one for each of {tokens} tokens")
+        if kv_index.shape[-1] < max_count:
+            raise ValueError(f"attend_window: a list of {kv_index.shape[-1]} cells for {max_count} positions")
+        stride = kv_index.shape[1] if kv_index.dim() == 2 else 0
+        least = 1
+    else:
+        least = (tokens - 1) * cache_stride + max_count * row
+    L = lib()
+    if work is None:
+        work = ctx.workspace(L.mi_attend_window_workspace(heads, kv_heads, head_dim, form, window, first, max_count, tokens,
+                                                          int((cache_stride if kv_index is None else stride) == 0)))
+    _queue(ctx, L.mi_attend_window, form, q.data_ptr(), _rows(ctx, q, "q", tokens, qw),
+           _on(ctx, k_cache, "k_cache", f16, least), _on(ctx, v_cache, "v_cache", f16, least), cache_stride,
+           None if kv_index is None else _on(ctx, kv_index, "kv_index", i32), stride, heads, kv_heads, head_dim, scale,
+           window, first, _on(ctx, pos, "pos", i32), max_count, tokens, _on(ctx, out, "out", torch.float32, tokens * qw),
+           _on(ctx, work, "work", torch.uint8), work.numel())
+
+
 # ---- sparse experts (no counterpart in the reference) ----
 ROUTER_SIGMOID, ROUTER_NORM = 1, 2
 
