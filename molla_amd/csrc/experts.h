@@ -13,18 +13,28 @@ constexpr int kFewPairs = 64;          // up to here the row kernel: a lane each
 int launch_router(hipStream_t s, const float* x, const float* router, const float* bias, int32_t width, int32_t experts,
                   int32_t used, int32_t tokens, int32_t flags, float scale, int32_t* ids, float* weights, void* work);
 
-// A few pairs' products (experts.hip): y[p] = W[ids[p]] . x[p / share], x in
-// matvec form; with w1, act(w0) * w1 in matvec form to xq_out instead.
+// A few pairs' products (experts_rows.h), x in matvec form (xq), or one row of floats
+// for every pair (x; one_row_fits): y[p] = W[ids[p]] .
+// x[p / share]; with w1, act(w0) * w1 in matvec form to xq_out instead; with
+// weights, y[t] (+)= sum over k < used of weights[t * used + k] * W[ids[t * used +
+// k]] . x[t * used + k].
 struct ExpertRows {
   const void *w0, *w1;
   int64_t row_bytes;
   int32_t rows, cols, experts;
   const void* xq;
-  int32_t share, pairs, act;
+  const float* x;
+  int32_t share, pairs;
   const int32_t* ids;
   float* y;
+  // GLU
+  int32_t act;
   void* xq_out;
+  // the weighted sum
+  const float* weights;
+  int32_t used, add;
 };
+bool one_row_fits(int32_t cols, int32_t share, int32_t pairs);
 int launch_expert_rows(hipStream_t s, int kind, const ExpertRows& a);
 int launch_expert_sum(hipStream_t s, const float* part, const int32_t* ids, const float* weights, int32_t width,
                       int32_t tokens, int32_t used, int32_t experts, bool add, float* out);

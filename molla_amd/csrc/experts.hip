@@ -1,6 +1,6 @@
-// experts.hip -- a sparse-expert MLP: which experts a token takes (the router),
-// the lists that group a call's rows by expert, and products of a few rows with
-// the experts' quantized matrices; gfx950.  (Many rows: experts_tile.hip.)
+// experts.hip -- a sparse-expert MLP: which experts a token takes (the router), the
+// lists that group a call's rows by expert, and the weighted sum of their products;
+// gfx950.  (Products of a few rows: experts_rows.h, of many: experts_tile.hip.)
 //
 // A pair is one expert that one token takes: pair p of a call belongs to row
 // p / share of its input.  Experts are stacked: expert e's matrix is rows
@@ -10,7 +10,6 @@
 #include <algorithm>
 
 #include "experts.h"
-#include "matvec_rows.h"
 
 namespace mi {
 namespace {
@@ -19,6 +18,11 @@ namespace {
 // logits[t][e] = x[t] . router[e], products and sums in float64: which of two
 // near scores is larger must not hang on the order of a sum.
 constexpr int kRouteTok = 4;  // tokens a wave takes
+// Products of a call from which the matrix cores take it, whose blocks are a longer
+// chain.  us a call, a wave an expert / matrix cores: 128 experts of 4096 values, 128
+// tokens 17.4 / 21.5, 256 29.0 / 21.6; 64 of 2048, 256 tokens 11.5 / 13.6, 512 17.8 /
+// 14.0; 8 of 4096, 2048 tokens 16.8 / 19.0.
+constexpr int64_t kRouteTile = 1 << 26;
 __global__ __launch_bounds__(256) void router_logits_kernel(const float* __restrict__ x,
                                                             const float* __restrict__ router, int width, int experts,
                                                             int tokens, double* __restrict__ logits) {
@@ -44,10 +48,110 @@ __global__ __launch_bounds__(256) void router_logits_kernel(const float* __restr
   }
 }
 
-__device__ __forceinline__ double swap_half(double v, int xor_lane) {
-  const uint64_t b = __double_as_longlong(v);
-  const uint32_t lo = __shfl_xor((int)(uint32_t)b, xor_lane), hi = __shfl_xor((int)(uint32_t)(b >> 32), xor_lane);
-  return __longlong_as_double((long long)(lo | ((uint64_t)hi << 32)));
+// The same on the matrix cores (v_mfma_f64_16x16x4_f64), for many tokens: a wave takes
+// 16 tokens x 16 NE experts, the block's eight waves every eighth step of 32 values,
+// and their sums meet in LDS, added in wave order.  Lane l holds row or column l % 16
+// and four values in turn of its quarter of 16 (the order of K is the same for both);
+// result j of lane l is row 4 j + l / 16, column l % 16.
+typedef double rd4 __attribute__((ext_vector_type(4)));
+constexpr int kRouteWaves = 8;
+template <int NE>
+__global__ __launch_bounds__(64 * kRouteWaves) void router_tile_kernel(const float* __restrict__ x,
+                                                                      const float* __restrict__ router, int width,
+                                                                      int experts, int tokens,
+                                                                      double* __restrict__ logits) {
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  __shared__ double part[kRouteWaves][4 * NE][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, q = lane >> 4;
+  const int t0 = blockIdx.y * 16, e0 = blockIdx.x * (16 * NE);
+  const float* xr = x + (int64_t)min(t0 + n, tokens - 1) * width;
+  const float* wr[NE];
+#pragma unroll
+  for (int k = 0; k < NE; k++) wr[k] = router + (int64_t)min(e0 + 16 * k + n, experts - 1) * width;
+  const int steps = (width + 31) / 32;
+  struct Step {
+    f4 a[2], b[NE][2];
+  };
+  // (past the end of a row: the last values, and zeros where they are used)
+  auto load = [&](Step& v, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int at = min(32 * s + 16 * h + 4 * q, width - 4);
+      v.a[h] = *(const f4*)(xr + at);
+#pragma unroll
+      for (int k = 0; k < NE; k++) v.b[k][h] = *(const f4*)(wr[k] + at);
+    }
+  };
+  rd4 acc[NE];
+#pragma unroll
+  for (int k = 0; k < NE; k++) acc[k] = rd4{0.0, 0.0, 0.0, 0.0};
+  auto use = [&](Step& v, int s) __attribute__((always_inline)) {
+    if (32 * s + 32 > width) {  // (uniform)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        if (32 * s + 16 * h + 4 * q >= width) {
+          v.a[h] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < NE; k++) v.b[k][h] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int k = 0; k < NE; k++)
+          acc[k] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v.a[h][i], (double)v.b[k][h][i], acc[k], 0, 0, 0);
+  };
+  // two steps on their way (past the last one: it again, and its use is left out)
+  Step st[3];
+  load(st[0], min(wave, steps - 1));
+  load(st[1], min(wave + kRouteWaves, steps - 1));
+  for (int s = wave; s < steps; s += 3 * kRouteWaves) {
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+      const int now = s + i * kRouteWaves;
+      load(st[(i + 2) % 3], min(now + 2 * kRouteWaves, steps - 1));
+      __builtin_amdgcn_sched_barrier(0);
+      if (now < steps) use(st[i], now);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < NE; k++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) part[wave][4 * k + j][lane] = acc[k][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 256 * NE; i += 64 * kRouteWaves) {
+    const int l = i & 63, j = (i >> 6) & 3, k = i >> 8;
+    double v = part[0][4 * k + j][l];
+#pragma unroll
+    for (int w = 1; w < kRouteWaves; w++) v += part[w][4 * k + j][l];
+    const int t = t0 + 4 * j + (l >> 4), e = e0 + 16 * k + (l & 15);
+    if (t < tokens && e < experts) logits[(int64_t)t * experts + e] = v;
+  }
+}
+
+// The largest of a float64 over the wave, in every lane.
+template <int CTRL>
+__device__ __forceinline__ double max_dpp(double v) {
+  return fmax(v, lanes::dpp_d<CTRL>(v));
+}
+__device__ __forceinline__ double wave_max(double v) {
+  v = max_dpp<lanes::kXor1>(v);
+  v = max_dpp<lanes::kXor2>(v);
+  v = max_dpp<lanes::kHalfMirror>(v);
+  v = max_dpp<lanes::kMirror>(v);
+  uint64_t b = __double_as_longlong(v);
+  auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  v = fmax(__longlong_as_double((long long)(lo[0] | ((uint64_t)hi[0] << 32))),
+           __longlong_as_double((long long)(lo[1] | ((uint64_t)hi[1] << 32))));
+  b = __double_as_longlong(v);
+  lo = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+  hi = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  return fmax(__longlong_as_double((long long)(lo[0] | ((uint64_t)hi[0] << 32))),
+              __longlong_as_double((long long)(lo[1] | ((uint64_t)hi[1] << 32))));
 }
 
 // A wave a token: its logits (expert lane + 64 k in place k), their scores, then
@@ -62,18 +166,20 @@ __global__ __launch_bounds__(64) void router_pick_kernel(const double* __restric
   const int64_t t = blockIdx.x;
   const double* row = logits + t * experts;
   double p[PER], score[PER];
+  float add[PER];
   double top = -INFINITY;
 #pragma unroll
   for (int k = 0; k < PER; k++) {
-    p[k] = lane + 64 * k < experts ? row[lane + 64 * k] : -INFINITY;
+    const int e = lane + 64 * k;
+    p[k] = e < experts ? row[e] : -INFINITY;
+    add[k] = bias && e < experts ? bias[e] : 0.0f;
     top = fmax(top, p[k]);
   }
   if (flags & MI_ROUTER_SIGMOID) {
 #pragma unroll
     for (int k = 0; k < PER; k++) p[k] = 1.0 / (1.0 + exp(-p[k]));
   } else {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmax(top, swap_half(top, o));
+    top = wave_max(top);
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < PER; k++) {
@@ -84,42 +190,48 @@ __global__ __launch_bounds__(64) void router_pick_kernel(const double* __restric
 #pragma unroll
     for (int k = 0; k < PER; k++) p[k] /= sum;
   }
+  uint32_t left = 0;  // bit k: this lane's expert of place k, not taken yet
 #pragma unroll
   for (int k = 0; k < PER; k++) {
-    const int e = lane + 64 * k;
-    score[k] = e < experts ? p[k] + (bias ? (double)bias[e] : 0.0) : -INFINITY;
+    score[k] = p[k] + (double)add[k];
     if (!(score[k] == score[k])) score[k] = -INFINITY;
+    if (lane + 64 * k < experts) left |= 1u << k;
   }
-  uint32_t taken = 0;  // bit k: this lane's expert of place k
-  double mine = 0.0, total = 0.0;
+  int mine = 0;  // lane u: pick u
+  double weight = 0.0;
   for (int u = 0; u < used; u++) {
     double best = -INFINITY;
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int k = PER - 1; k >= 0; k--) {
-      const int e = lane + 64 * k;
-      if (e < experts && !((taken >> k) & 1) && score[k] >= best) best = score[k], at = e;
-    }
-    for (int o = 32; o; o >>= 1) {
-      const double b = swap_half(best, o);
-      const int a = __shfl_xor(at, o);
-      if (b > best || (b == best && a < at)) best = b, at = a;
-    }
-    // (at is an expert: fewer than `experts` are taken)
-    double w = 0.0;
 #pragma unroll
     for (int k = 0; k < PER; k++)
-      if (lane + 64 * k == at) taken |= 1u << k, w = p[k];
-    const uint64_t b = __double_as_longlong(w);
-    const uint32_t lo = __shfl((int)(uint32_t)b, at & 63), hi = __shfl((int)(uint32_t)(b >> 32), at & 63);
-    w = __longlong_as_double((long long)(lo | ((uint64_t)hi << 32)));
-    total += w;
-    if (lane == u) mine = w;
-    if (lane == 0) ids[t * used + u] = at;
+      if ((left >> k) & 1) best = fmax(best, score[k]);
+    best = wave_max(best);
+    int at = 0;
+    double w = 0.0;
+    bool found = false;
+    // (fewer than `experts` are taken: one of what is left has the largest score)
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const uint64_t has = __ballot(((left >> k) & 1) && score[k] == best);
+      if (!found && has) {
+        found = true;
+        const int l = __builtin_ctzll(has);
+        at = l + 64 * k;
+        const uint64_t b = __double_as_longlong(p[k]);
+        w = __longlong_as_double((long long)((uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l) |
+                                             ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l) << 32)));
+        if (lane == l) left &= ~(1u << k);
+      }
+    }
+    if (lane == u) mine = at, weight = w;
+  }
+  double total = 1.0;
+  if (flags & MI_ROUTER_NORM) {
+    total = lanes::reduce_sum<64>(weight);
+    if (total == 0.0) total = 1.0;
   }
   if (lane < used) {
-    if (flags & MI_ROUTER_NORM) mine = total != 0.0 ? mine / total : 0.0;
-    weights[t * used + lane] = (float)(mine * (double)scale);
+    ids[t * used + lane] = mine;
+    weights[t * used + lane] = (float)(weight / total * (double)scale);
   }
 }
 
@@ -173,80 +285,7 @@ __global__ __launch_bounds__(kPlanThreads) void group_plan_kernel(const int32_t*
   }
 }
 
-// ---- a few rows ----------------------------------------------------------------
-// Up to 64 pairs: block (x, p) takes 32 rows of the expert of pair p, if no
-// earlier pair has the same one, against every pair that has it.  SUB lanes share
-// a row, a unit (64 values; 128 for Q6_K) each, in turns where there are more; R
-// rows of each matrix a lane, so that an activation read serves them all.  The
-// arithmetic is matvec_units.h's: exact integer dots of a unit, one rounding a
-// block.
-// GLU: act(w0) * w1 of the 32 rows, written in matvec form (a group of xq_out's
-// row p), the input of the next product.
-template <int KIND, int SUB, int R, bool GLU>
-__global__ __launch_bounds__(32 * SUB / R) void experts_rows_kernel(
-    const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1, int64_t expert_bytes, int64_t rb, int rows, int cols,
-    const uint8_t* __restrict__ xq, int share, const int32_t* __restrict__ ids, int pairs, int experts, int act,
-    float* __restrict__ y, uint8_t* __restrict__ xq_out) {
-  using Unit = typename mv::UnitOf<KIND, 1>::type;
-  constexpr int NSUB = 64 / SUB, M = GLU ? 2 : 1;
-  __shared__ float grp[2][GLU ? 32 : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int first = blockIdx.y, id = lane < pairs ? ids[lane] : -1;
-  const int e = __builtin_amdgcn_readfirstlane(__shfl(id, first));
-  uint64_t todo = __ballot(id == e);
-  if ((uint32_t)e >= (uint32_t)experts || (todo & ((1ull << first) - 1))) return;  // (uniform over the block)
-  const int sub = lane / SUB, sl = lane % SUB;
-  const int local = wave * NSUB * R + sub;  // row r of this lane: + r * NSUB
-  const int row0 = blockIdx.x * 32 + local, units = cols / Unit::kElems;
-  const uint8_t* base[M] = {w0 + e * expert_bytes};
-  if constexpr (GLU) base[1] = w1 + e * expert_bytes;
-  Unit un[M * R];
-  auto load = [&](int u) __attribute__((always_inline)) {
-#pragma unroll
-    for (int m = 0; m < M; m++)
-#pragma unroll
-      for (int r = 0; r < R; r++) un[m * R + r].load(base[m], rb, min(row0 + r * NSUB, rows - 1), rows - 1, u);
-  };
-  const bool fits = units <= SUB;  // the weights stay for every pair
-  load(min(sl, units - 1));
-  for (int it = 0; todo; todo &= todo - 1, it ^= 1) {
-    const int p = __builtin_ctzll(todo);
-    const mv::XAcc xa{xq + (int64_t)(p / share) * xq_token_bytes(cols), 0, (int64_t)(cols >> 5) * 16};
-    float acc[M * R] = {};
-    for (int u0 = 0; u0 < units; u0 += SUB) {
-      const int u = min(u0 + sl, units - 1);
-      if (!fits) load(u);
-      const bool live = u0 + sl < units;
-#pragma unroll
-      for (int k = 0; k < M * R; k++) {
-        float a[1][1] = {{0.0f}};
-        un[k].template compute<1>(xa, u, a);
-        acc[k] += live ? a[0][0] : 0.0f;
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < M * R; k++) acc[k] = lanes::reduce<SUB>(acc[k], lanes::Add{});
-    if constexpr (GLU) {
-      if (sl == 0) {
-#pragma unroll
-        for (int r = 0; r < R; r++)
-          grp[it][local + r * NSUB] = ((act & MI_ACT_GELU) ? mv::gelu(acc[r]) : mv::silu(acc[r])) * acc[R + r];
-      }
-      // (buffers take turns: a wave that writes one again has passed the barrier
-      // behind wave 0's last reading of it)
-      __syncthreads();
-      if (wave == 0)
-        quantize_group32(grp[it][lane & 31], lane & 31, blockIdx.x, rows >> 5, xq_out + (int64_t)p * xq_token_bytes(rows),
-                         lane < 32);
-    } else {
-#pragma unroll
-      for (int r = 0; r < R; r++)
-        if (sl == 0 && row0 + r * NSUB < rows) y[(int64_t)p * rows + row0 + r * NSUB] = acc[r];
-    }
-  }
-}
-
+// ---- the weighted sum of many rows' products ------------------------------------
 // out[t] (+)= sum over k of weights[t][k] * part[t * used + k], in the order of k;
 // a pair without an expert takes no part.
 __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restrict__ part, const int32_t* __restrict__ ids,
@@ -268,43 +307,7 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
   *o = add ? *o + v : v;
 }
 
-template <int KIND, int SUB, bool GLU>
-int launch_rows_sub(hipStream_t s, const ExpertRows& a) {
-  constexpr int R = 4;
-  hipLaunchKernelGGL((experts_rows_kernel<KIND, SUB, R, GLU>), dim3((a.rows + 31) / 32, a.pairs), dim3(32 * SUB / R), 0, s,
-                     (const uint8_t*)a.w0, (const uint8_t*)a.w1, a.rows * a.row_bytes, a.row_bytes, a.rows, a.cols,
-                     (const uint8_t*)a.xq, a.share, a.ids, a.pairs, a.experts, a.act, a.y, (uint8_t*)a.xq_out);
-  return hip_check(hipGetLastError(), "experts rows launch");
-}
-
-template <int KIND>
-int launch_rows_kind(hipStream_t s, const ExpertRows& a) {
-  const int units = a.cols / mv::UnitOf<KIND, 1>::type::kElems;
-  if (a.w1) {
-    if (units <= 16) return launch_rows_sub<KIND, 16, true>(s, a);
-    if (units <= 32) return launch_rows_sub<KIND, 32, true>(s, a);
-    return launch_rows_sub<KIND, 64, true>(s, a);
-  }
-  if (units <= 16) return launch_rows_sub<KIND, 16, false>(s, a);
-  if (units <= 32) return launch_rows_sub<KIND, 32, false>(s, a);
-  return launch_rows_sub<KIND, 64, false>(s, a);
-}
-
 }  // namespace
-
-int launch_expert_rows(hipStream_t s, int kind, const ExpertRows& a) {
-  switch (kind) {
-    case MI_Q4_K: return launch_rows_kind<MI_Q4_K>(s, a);
-    case MI_Q5_K: return launch_rows_kind<MI_Q5_K>(s, a);
-    case MI_Q6_K: return launch_rows_kind<MI_Q6_K>(s, a);
-    case MI_Q8_0: return launch_rows_kind<MI_Q8_0>(s, a);
-    case MI_Q4_0: return launch_rows_kind<MI_Q4_0>(s, a);
-    case MI_Q4_1: return launch_rows_kind<MI_Q4_1>(s, a);
-    case MI_Q5_0: return launch_rows_kind<MI_Q5_0>(s, a);
-    case MI_Q5_1: return launch_rows_kind<MI_Q5_1>(s, a);
-  }
-  return fail(MI_ERR_KIND, "experts: ggml type %d has no device kernel", kind);
-}
 
 int launch_expert_sum(hipStream_t s, const float* part, const int32_t* ids, const float* weights, int32_t width,
                       int32_t tokens, int32_t used, int32_t experts, bool add, float* out) {
@@ -323,8 +326,16 @@ int launch_group_plan(hipStream_t s, const int32_t* ids, int32_t pairs, int32_t 
 int launch_router(hipStream_t s, const float* x, const float* router, const float* bias, int32_t width, int32_t experts,
                   int32_t used, int32_t tokens, int32_t flags, float scale, int32_t* ids, float* weights, void* work) {
   double* logits = (double*)work;
-  hipLaunchKernelGGL(router_logits_kernel, dim3((experts + 3) / 4, (tokens + kRouteTok - 1) / kRouteTok), dim3(256), 0, s, x,
-                     router, width, experts, tokens, logits);
+  const int tiles = (tokens + 15) / 16;
+  if ((int64_t)tokens * experts * width < kRouteTile)
+    hipLaunchKernelGGL(router_logits_kernel, dim3((experts + 3) / 4, (tokens + kRouteTok - 1) / kRouteTok), dim3(256), 0, s,
+                       x, router, width, experts, tokens, logits);
+  else if ((int64_t)tiles * ((experts + 63) / 64) < cu_count() || experts <= 16)
+    hipLaunchKernelGGL(router_tile_kernel<1>, dim3((experts + 15) / 16, tiles), dim3(64 * kRouteWaves), 0, s, x, router, width,
+                       experts, tokens, logits);
+  else
+    hipLaunchKernelGGL(router_tile_kernel<4>, dim3((experts + 63) / 64, tiles), dim3(64 * kRouteWaves), 0, s, x, router, width,
+                       experts, tokens, logits);
   int rc = hip_check(hipGetLastError(), "router launch");
   if (rc) return rc;
 #define MI_PICK(P)                                                                                             \

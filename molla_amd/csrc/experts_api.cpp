@@ -61,7 +61,7 @@ struct MlpCarve {
   size_t x, h, hx, part, plan, total;
 };
 // x: the input in the form its product reads; h: act(gate) * up in f32 (many
-// rows); hx: the same as the down projection reads it; part: what it gives.
+// rows); hx: the same as the down projection reads it; part: what that gives.
 MlpCarve mlp_carve(int32_t experts, int32_t width, int32_t hidden, int32_t tokens, int32_t used) {
   MlpCarve c{};
   const size_t pairs = (size_t)tokens * used;
@@ -74,7 +74,6 @@ MlpCarve mlp_carve(int32_t experts, int32_t width, int32_t hidden, int32_t token
   if (pairs <= (size_t)kFewPairs) {
     c.x = take((size_t)xq_token_bytes(width) * tokens);
     c.hx = take((size_t)xq_token_bytes(hidden) * pairs);
-    c.part = take(4 * (size_t)width * pairs);
   } else {
     const GroupPlan g = group_plan(nullptr, (int32_t)pairs, experts, 1);
     c.plan = take(g.bytes);
@@ -97,36 +96,58 @@ int launch_experts_mlp(hipStream_t s, const mi_experts& d, const float* x, int32
   const int32_t pairs = tokens * used;
   const MlpCarve c = mlp_carve(d.experts, d.width, d.hidden, tokens, used);
   char* base = (char*)work;
-  float* part = (float*)(base + c.part);
   int rc;
   if (pairs <= kFewPairs) {
-    if ((rc = launch_quantize(s, x, d.width, tokens, base + c.x))) return rc;
-    ExpertRows a{d.gate.data, d.up.data, d.gate.row_bytes, d.hidden, d.width, d.experts, base + c.x, used, pairs, d.act,
-                 ids, nullptr, base + c.hx};
+    const bool one = one_row_fits(d.width, used, pairs);
+    if (!one && (rc = launch_quantize(s, x, d.width, tokens, base + c.x))) return rc;
+    ExpertRows a{};
+    a.w0 = d.gate.data;
+    a.w1 = d.up.data;
+    a.row_bytes = d.gate.row_bytes;
+    a.rows = d.hidden;
+    a.cols = d.width;
+    a.experts = d.experts;
+    a.xq = base + c.x;
+    a.x = one ? x : nullptr;
+    a.share = used;
+    a.pairs = pairs;
+    a.ids = ids;
+    a.act = d.act;
+    a.xq_out = base + c.hx;
     if ((rc = launch_expert_rows(s, d.gate.kind, a))) return rc;
-    ExpertRows b{d.down.data, nullptr, d.down.row_bytes, d.width, d.hidden, d.experts, base + c.hx, 1, pairs, 0,
-                 ids, part, nullptr};
-    if ((rc = launch_expert_rows(s, d.down.kind, b))) return rc;
-  } else {
-    float* h = (float*)(base + c.h);
-    void *xp = base + c.x, *hp = base + c.hx;
-    const int ta = group_tiles(d.gate.kind, pairs, d.experts), tb = group_tiles(d.down.kind, pairs, d.experts);
-    GroupPlan g = group_plan(base + c.plan, pairs, d.experts, ta);
-    if ((rc = launch_group_plan(s, ids, pairs, d.experts, ta, g))) return rc;
-    if ((rc = launch_group_prep(s, x, d.width, pairs, used, g, xp))) return rc;
-    if ((rc = launch_group_tile(s, d.gate.kind, d.gate.data, d.up.data, d.gate.row_bytes, d.hidden, d.width, d.act, g, ta,
-                                xp, h)))
-      return rc;
-    if (tb != ta) {
-      // (other block lists; the slots may be others too, each pair's row is the same)
-      g = group_plan(base + c.plan, pairs, d.experts, tb);
-      if ((rc = launch_group_plan(s, ids, pairs, d.experts, tb, g))) return rc;
-    }
-    if ((rc = launch_group_prep(s, h, d.hidden, pairs, 1, g, hp))) return rc;
-    if ((rc = launch_group_tile(s, d.down.kind, d.down.data, nullptr, d.down.row_bytes, d.width, d.hidden, 0, g, tb, hp,
-                                part)))
-      return rc;
+    ExpertRows b{};
+    b.w0 = d.down.data;
+    b.row_bytes = d.down.row_bytes;
+    b.rows = d.width;
+    b.cols = d.hidden;
+    b.experts = d.experts;
+    b.xq = base + c.hx;
+    b.pairs = pairs;
+    b.ids = ids;
+    b.y = out;
+    b.weights = weights;
+    b.used = used;
+    b.add = add;
+    return launch_expert_rows(s, d.down.kind, b);
   }
+  float *h = (float*)(base + c.h), *part = (float*)(base + c.part);
+  void *xp = base + c.x, *hp = base + c.hx;
+  const int ta = group_tiles(d.gate.kind, pairs, d.experts), tb = group_tiles(d.down.kind, pairs, d.experts);
+  GroupPlan g = group_plan(base + c.plan, pairs, d.experts, ta);
+  if ((rc = launch_group_plan(s, ids, pairs, d.experts, ta, g))) return rc;
+  if ((rc = launch_group_prep(s, x, d.width, pairs, used, g, xp))) return rc;
+  if ((rc = launch_group_tile(s, d.gate.kind, d.gate.data, d.up.data, d.gate.row_bytes, d.hidden, d.width, d.act, g, ta,
+                              xp, h)))
+    return rc;
+  if (tb != ta) {
+    // (other block lists; the slots may be others too, each pair's row is the same)
+    g = group_plan(base + c.plan, pairs, d.experts, tb);
+    if ((rc = launch_group_plan(s, ids, pairs, d.experts, tb, g))) return rc;
+  }
+  if ((rc = launch_group_prep(s, h, d.hidden, pairs, 1, g, hp))) return rc;
+  if ((rc = launch_group_tile(s, d.down.kind, d.down.data, nullptr, d.down.row_bytes, d.width, d.hidden, 0, g, tb, hp,
+                              part)))
+    return rc;
   return launch_expert_sum(s, part, ids, weights, d.width, tokens, used, d.experts, add, out);
 }
 
@@ -227,8 +248,20 @@ int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_byt
   hipStream_t s = (hipStream_t)stream;
   char* base = (char*)work;
   if (pairs <= kFewPairs) {
-    if ((rc = launch_quantize(s, x, cols, pairs / share, base + c.x))) return rc;
-    const ExpertRows a{w, nullptr, row_bytes, rows, cols, experts, base + c.x, share, pairs, 0, ids, y, nullptr};
+    const bool one = one_row_fits(cols, share, pairs);
+    if (!one && (rc = launch_quantize(s, x, cols, pairs / share, base + c.x))) return rc;
+    ExpertRows a{};
+    a.w0 = w;
+    a.row_bytes = row_bytes;
+    a.rows = rows;
+    a.cols = cols;
+    a.experts = experts;
+    a.xq = base + c.x;
+    a.x = one ? x : nullptr;
+    a.share = share;
+    a.pairs = pairs;
+    a.ids = ids;
+    a.y = y;
     return launch_expert_rows(s, kind, a);
   }
   const int tiles = group_tiles(kind, pairs, experts);
