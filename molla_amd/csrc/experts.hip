@@ -236,16 +236,30 @@ __global__ __launch_bounds__(64) void router_pick_kernel(const double* __restric
 }
 
 // ---- a call's rows by expert -------------------------------------------------
-// One block: counts, their starts in tiles of 32 slots, the blocks' lists, and
-// each pair's slot.  Which of an expert's slots a pair gets changes nothing of
-// its row (a row's products depend on its own values only).
+// The first block: counts, their starts in tiles of 32 slots, the blocks' lists, and
+// the pair of each slot (-1 behind an expert's last).  Which of an expert's slots a
+// pair gets changes nothing of its row (a row's products depend on its own values
+// only).  The others: the largest size in each row of x.
 constexpr int kPlanThreads = 1024;
 __global__ __launch_bounds__(kPlanThreads) void group_plan_kernel(const int32_t* __restrict__ ids, int pairs, int experts,
-                                                                  int tiles_a_block, int32_t* __restrict__ slot,
-                                                                  int32_t* __restrict__ order,
-                                                                  int4* __restrict__ tiles, int32_t* __restrict__ count) {
+                                                                  int tiles_a_block, int32_t* __restrict__ order,
+                                                                  int4* __restrict__ tiles, int32_t* __restrict__ count,
+                                                                  const float* __restrict__ x, int rows, int cols,
+                                                                  float* __restrict__ xtop) {
   __shared__ int cnt[kMaxExperts], at[kMaxExperts], wave_sum[2][kPlanThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (blockIdx.x > 0) {  // a wave a row
+    for (int r = (blockIdx.x - 1) * (kPlanThreads / 64) + wave; r < rows; r += (gridDim.x - 1) * (kPlanThreads / 64)) {
+      float m = 0.0f;
+      for (int i = 4 * lane; i < cols; i += 256) {
+        const float4 v = *(const float4*)(x + (int64_t)r * cols + i);
+        m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+      }
+      m = lanes::reduce<64>(m, lanes::Max{});
+      if (lane == 0) xtop[r] = m;
+    }
+    return;
+  }
   for (int e = tid; e < experts; e += kPlanThreads) cnt[e] = 0;
   __syncthreads();
   for (int p = tid; p < pairs; p += kPlanThreads) {
@@ -267,30 +281,30 @@ __global__ __launch_bounds__(kPlanThreads) void group_plan_kernel(const int32_t*
   int a0 = 0, b0 = 0;
   for (int w = 0; w < wave; w++) a0 += wave_sum[0][w], b0 += wave_sum[1][w];
   const int first = a0 + a - t32, entry = b0 + b - blocks;
-  if (tid == kPlanThreads - 1) *count = entry + blocks;
+  if (tid == kPlanThreads - 1) {
+    count[0] = entry + blocks;
+    count[1] = (first + t32) * 32;  // slots
+  }
   if (tid < experts) {
     at[tid] = first * 32;
     for (int k = 0; k < blocks; k++)
       tiles[entry + k] = make_int4(tid, first + k * tiles_a_block, first * 32 + n, 0);
+    for (int k = n; k < t32 * 32; k++) order[first * 32 + k] = -1;
   }
   __syncthreads();
   for (int p = tid; p < pairs; p += kPlanThreads) {
     const int e = ids[p];
-    int s = -1;
-    if ((uint32_t)e < (uint32_t)experts) {
-      s = atomicAdd(&at[e], 1);
-      order[s] = p;
-    }
-    slot[p] = s;
+    if ((uint32_t)e < (uint32_t)experts) order[atomicAdd(&at[e], 1)] = p;
   }
 }
 
 // ---- the weighted sum of many rows' products ------------------------------------
-// out[t] (+)= sum over k of weights[t][k] * part[t * used + k], in the order of k;
-// a pair without an expert takes no part.
+// out[t] (+)= sum over k of weights[t][k] * part[t * used + k], in the order of k, a
+// pair's splits added up first; a pair without an expert takes no part.
 __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restrict__ part, const int32_t* __restrict__ ids,
                                                           const float* __restrict__ weights, int width, int used,
-                                                          int experts, int add, float* __restrict__ out) {
+                                                          int experts, int add, int splits, int64_t split_stride,
+                                                          float* __restrict__ out) {
   const int i = 4 * (blockIdx.x * 256 + threadIdx.x);
   const int64_t t = blockIdx.y;
   if (i >= width) return;
@@ -299,7 +313,9 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
   for (int k = 0; k < used; k++) {
     if ((uint32_t)ids[t * used + k] >= (uint32_t)experts) continue;
     const float w = weights[t * used + k];
-    const f4 a = *(const f4*)(part + (t * used + k) * width + i);
+    const float* p = part + (t * used + k) * width + i;
+    f4 a = *(const f4*)p;
+    for (int z = 1; z < splits; z++) a += *(const f4*)(p + z * split_stride);
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] = fmaf(w, a[e], v[e]);
   }
@@ -310,16 +326,17 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
 }  // namespace
 
 int launch_expert_sum(hipStream_t s, const float* part, const int32_t* ids, const float* weights, int32_t width,
-                      int32_t tokens, int32_t used, int32_t experts, bool add, float* out) {
+                      int32_t tokens, int32_t used, int32_t experts, bool add, int32_t splits, float* out) {
   hipLaunchKernelGGL(experts_sum_kernel, dim3((width / 4 + 255) / 256, tokens), dim3(256), 0, s, part, ids, weights, width,
-                     used, experts, add ? 1 : 0, out);
+                     used, experts, add ? 1 : 0, splits, (int64_t)tokens * used * width, out);
   return hip_check(hipGetLastError(), "experts sum launch");
 }
 
 int launch_group_plan(hipStream_t s, const int32_t* ids, int32_t pairs, int32_t experts, int32_t tiles_a_block,
-                      const GroupPlan& g) {
-  hipLaunchKernelGGL(group_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, ids, pairs, experts, tiles_a_block, g.slot,
-                     g.order, (int4*)g.tiles, g.count);
+                      const GroupPlan& g, const float* x, int32_t rows, int32_t cols) {
+  const int more = x ? std::min((rows + kPlanThreads / 64 - 1) / (kPlanThreads / 64), 4 * cu_count()) : 0;
+  hipLaunchKernelGGL(group_plan_kernel, dim3(1 + more), dim3(kPlanThreads), 0, s, ids, pairs, experts, tiles_a_block,
+                     g.order, (int4*)g.tiles, g.count, x, rows, cols, g.xtop);
   return hip_check(hipGetLastError(), "group plan launch");
 }
 

@@ -58,11 +58,13 @@ MatmulCarve matmul_carve(int32_t experts, int32_t cols, int32_t share, int32_t p
 }
 
 struct MlpCarve {
-  size_t x, h, hx, part, plan, total;
+  size_t x, h, hx, part, plan, top, total;
+  int gate_tiles, down_tiles, splits;  // many rows: tiles a block, parts of down's K
 };
 // x: the input in the form its product reads; h: act(gate) * up in f32 (many
-// rows); hx: the same as the down projection reads it; part: what that gives.
-MlpCarve mlp_carve(int32_t experts, int32_t width, int32_t hidden, int32_t tokens, int32_t used) {
+// rows), top: the largest sizes in its rows; hx: the same as the down projection reads it; part: what that gives.
+MlpCarve mlp_carve(const mi_experts& d, int32_t tokens, int32_t used) {
+  const int32_t experts = d.experts, width = d.width, hidden = d.hidden;
   MlpCarve c{};
   const size_t pairs = (size_t)tokens * used;
   size_t at = 0;
@@ -75,11 +77,15 @@ MlpCarve mlp_carve(int32_t experts, int32_t width, int32_t hidden, int32_t token
     c.x = take((size_t)xq_token_bytes(width) * tokens);
     c.hx = take((size_t)xq_token_bytes(hidden) * pairs);
   } else {
+    c.gate_tiles = group_tiles(d.gate.kind, (int32_t)pairs, experts);
+    c.down_tiles = group_tiles(d.down.kind, (int32_t)pairs, experts);
+    c.splits = group_splits(d.down.kind, width, hidden, (int32_t)pairs, experts, c.down_tiles);
     const GroupPlan g = group_plan(nullptr, (int32_t)pairs, experts, 1);
     c.plan = take(g.bytes);
+    c.top = take(4 * pairs * group_tops(d.gate.kind, hidden, c.gate_tiles));
     // (the input is dead where h's form is made, h where the down projection writes)
     c.x = c.hx = take(std::max(group_prep_bytes(width, g), group_prep_bytes(hidden, g)));
-    c.h = c.part = take(4 * (size_t)std::max(width, hidden) * pairs);
+    c.h = c.part = take(4 * (size_t)std::max<int64_t>((int64_t)width * c.splits, hidden) * pairs);
   }
   c.total = at;
   return c;
@@ -87,14 +93,12 @@ MlpCarve mlp_carve(int32_t experts, int32_t width, int32_t hidden, int32_t token
 
 }  // namespace
 
-size_t experts_workspace(int32_t experts, int32_t width, int32_t hidden, int32_t tokens, int32_t used) {
-  return mlp_carve(experts, width, hidden, tokens, used).total;
-}
+size_t experts_workspace(const mi_experts& d, int32_t tokens, int32_t used) { return mlp_carve(d, tokens, used).total; }
 
 int launch_experts_mlp(hipStream_t s, const mi_experts& d, const float* x, int32_t tokens, int32_t used,
                        const int32_t* ids, const float* weights, float* out, bool add, void* work) {
   const int32_t pairs = tokens * used;
-  const MlpCarve c = mlp_carve(d.experts, d.width, d.hidden, tokens, used);
+  const MlpCarve c = mlp_carve(d, tokens, used);
   char* base = (char*)work;
   int rc;
   if (pairs <= kFewPairs) {
@@ -130,25 +134,25 @@ int launch_experts_mlp(hipStream_t s, const mi_experts& d, const float* x, int32
     b.add = add;
     return launch_expert_rows(s, d.down.kind, b);
   }
-  float *h = (float*)(base + c.h), *part = (float*)(base + c.part);
+  float *h = (float*)(base + c.h), *part = (float*)(base + c.part), *top = (float*)(base + c.top);
   void *xp = base + c.x, *hp = base + c.hx;
-  const int ta = group_tiles(d.gate.kind, pairs, d.experts), tb = group_tiles(d.down.kind, pairs, d.experts);
+  const int ta = c.gate_tiles, tb = c.down_tiles;
   GroupPlan g = group_plan(base + c.plan, pairs, d.experts, ta);
-  if ((rc = launch_group_plan(s, ids, pairs, d.experts, ta, g))) return rc;
-  if ((rc = launch_group_prep(s, x, d.width, pairs, used, g, xp))) return rc;
+  if ((rc = launch_group_plan(s, ids, pairs, d.experts, ta, g, x, tokens, d.width))) return rc;
+  if ((rc = launch_group_prep(s, x, d.width, pairs, used, g.xtop, 1, g, xp))) return rc;
   if ((rc = launch_group_tile(s, d.gate.kind, d.gate.data, d.up.data, d.gate.row_bytes, d.hidden, d.width, d.act, g, ta,
-                              xp, h)))
+                              pairs, 1, xp, h, top)))
     return rc;
   if (tb != ta) {
     // (other block lists; the slots may be others too, each pair's row is the same)
     g = group_plan(base + c.plan, pairs, d.experts, tb);
-    if ((rc = launch_group_plan(s, ids, pairs, d.experts, tb, g))) return rc;
+    if ((rc = launch_group_plan(s, ids, pairs, d.experts, tb, g, nullptr, 0, 0))) return rc;
   }
-  if ((rc = launch_group_prep(s, h, d.hidden, pairs, 1, g, hp))) return rc;
-  if ((rc = launch_group_tile(s, d.down.kind, d.down.data, nullptr, d.down.row_bytes, d.width, d.hidden, 0, g, tb, hp,
-                              part)))
+  if ((rc = launch_group_prep(s, h, d.hidden, pairs, 1, top, group_tops(d.gate.kind, d.hidden, ta), g, hp))) return rc;
+  if ((rc = launch_group_tile(s, d.down.kind, d.down.data, nullptr, d.down.row_bytes, d.width, d.hidden, 0, g, tb, pairs,
+                              c.splits, hp, part)))
     return rc;
-  return launch_expert_sum(s, part, ids, weights, d.width, tokens, used, d.experts, add, out);
+  return launch_expert_sum(s, part, ids, weights, d.width, tokens, used, d.experts, add, c.splits, out);
 }
 
 // The descriptor of a gated MLP of experts.
@@ -266,9 +270,9 @@ int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_byt
   }
   const int tiles = group_tiles(kind, pairs, experts);
   const GroupPlan g = group_plan(base + c.plan, pairs, experts, tiles);
-  if ((rc = launch_group_plan(s, ids, pairs, experts, tiles, g))) return rc;
-  if ((rc = launch_group_prep(s, x, cols, pairs, share, g, base + c.x))) return rc;
-  return launch_group_tile(s, kind, w, nullptr, row_bytes, rows, cols, 0, g, tiles, base + c.x, y);
+  if ((rc = launch_group_plan(s, ids, pairs, experts, tiles, g, x, pairs / share, cols))) return rc;
+  if ((rc = launch_group_prep(s, x, cols, pairs, share, g.xtop, 1, g, base + c.x))) return rc;
+  return launch_group_tile(s, kind, w, nullptr, row_bytes, rows, cols, 0, g, tiles, pairs, 1, base + c.x, y);
 }
 
 size_t mi_experts_workspace(const mi_experts* d, int32_t tokens, int32_t used) {
@@ -276,7 +280,7 @@ size_t mi_experts_workspace(const mi_experts* d, int32_t tokens, int32_t used) {
       d->hidden % 64 || tokens < 1 || tokens > kMaxPrefill || used < 1 || used > kMaxUsed ||
       (int64_t)tokens * used > kMaxPairs)
     return 0;
-  return experts_workspace(d->experts, d->width, d->hidden, tokens, used);
+  return experts_workspace(*d, tokens, used);
 }
 
 int mi_experts_mlp(mi_stream stream, const mi_experts* d, const float* x, int32_t tokens, int32_t used,
@@ -293,7 +297,7 @@ int mi_experts_mlp(mi_stream stream, const mi_experts* d, const float* x, int32_
     return fail(MI_ERR_ALIGN, "experts_mlp: the input and the output must be 16-byte aligned");
   const size_t xb = 4 * (size_t)tokens * d->width, pb = 4 * (size_t)tokens * used;
   if (meet(out, xb, ids, pb) || meet(out, xb, weights, pb)) return fail(MI_ERR_ARG, "experts_mlp: the output lies in an input");
-  const size_t need = experts_workspace(d->experts, d->width, d->hidden, tokens, used);
+  const size_t need = experts_workspace(*d, tokens, used);
   if (!work || ((uintptr_t)work & 255) || work_bytes < need)
     return fail(MI_ERR_WORKSPACE, "experts_mlp: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);
   if (meet(work, need, x, xb) || meet(work, need, out, xb) || meet(work, need, ids, pb) || meet(work, need, weights, pb))

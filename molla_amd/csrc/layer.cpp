@@ -59,6 +59,10 @@ size_t attend_part(const mi_layer_desc* d, int32_t max_count, int32_t tokens, co
                         attend_window_workspace(d->heads, d->kv_heads, d->head_dim, d->cache_form, w, tokens, false)));
 }
 
+mi_experts experts_of(const mi_layer_desc* d) {
+  return mi_experts{d->experts, d->width, d->hidden, d->act, d->gate, d->up, d->down};
+}
+
 // Sparse experts' part of a workspace: the normed row, a row for what is normed
 // ahead of the residual, the router's choice, and the larger of its scratch and
 // the MLP's.
@@ -78,7 +82,7 @@ ExpertsCarve experts_carve(const mi_layer_desc* d, int32_t tokens) {
   c.ids = take(sizeof(int32_t) * (size_t)d->experts_used * tokens);
   c.weights = take(sizeof(float) * (size_t)d->experts_used * tokens);
   c.work = take(std::max(router_workspace(d->experts, tokens),
-                         experts_workspace(d->experts, d->width, d->hidden, tokens, d->experts_used)));
+                         experts_workspace(experts_of(d), tokens, d->experts_used)));
   c.total = at;
   return c;
 }
@@ -159,10 +163,6 @@ PrefillCarve prefill_carve(const mi_layer_desc* d, int32_t max_count, int32_t to
   at += up256(mm);
   c.total = at;
   return c;
-}
-
-mi_experts experts_of(const mi_layer_desc* d) {
-  return mi_experts{d->experts, d->width, d->hidden, d->act, d->gate, d->up, d->down};
 }
 
 // Sparse experts and the attention's window: what a workspace's size takes of them.

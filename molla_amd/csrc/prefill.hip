@@ -63,7 +63,7 @@ int launch_kind(hipStream_t s, const RowSegs& sg, int cols, int tokens, const vo
   const dim3 block(sh.wr * sh.ks * 64);
 #define MI_PF(R, T, W, G)                                                                                  \
   hipLaunchKernelGGL((prefill_kernel<KIND, R, T, W, G>), grid, block, 0, s, sg, cols, tokens,               \
-                     (const uint8_t*)work, cps, y, ldy, epi, aux, splits > 1 ? part : nullptr, NoGroups{})
+                     (const uint8_t*)work, cps, y, ldy, epi, aux, splits > 1 ? part : nullptr)
   if (sh.tt == 1) MI_PF(1, 1, 4, 2);
   else if (sh.rt == 1 && sh.tt == 2) MI_PF(1, 2, 4, 2);
   else if constexpr (KIND == MI_Q6_K) {
@@ -124,8 +124,7 @@ size_t prefill_prep_bytes(int32_t cols, int32_t tokens) { return prep_layout(col
 
 int prefill_prepare(hipStream_t s, const float* x, int32_t cols, int32_t tokens, void* work) {
   const Prep P = prep_layout(cols, tokens);
-  hipLaunchKernelGGL(prefill_prep_kernel<NoSlots>, dim3(P.ttp * kTileTok), dim3(256), 0, s, x, cols, tokens,
-                     (uint8_t*)work, NoSlots{});
+  hipLaunchKernelGGL(prefill_prep_kernel, dim3(P.ttp * kTileTok), dim3(256), 0, s, x, cols, tokens, (uint8_t*)work);
   return hip_check(hipGetLastError(), "prefill activation launch");
 }
 

@@ -413,6 +413,9 @@ __device__ __forceinline__ void split_half(float v, _Float16& hi, _Float16& lo) 
   lo = (_Float16)(v - (float)hi);
 }
 
+// The exponent of a token's scale, from its largest |x| (below)
+__device__ __forceinline__ int scale_exp(float mx) { return mx > 0.0f ? min(max(ilogbf(mx) - 13, -100), 100) : 0; }
+
 // A token's activations, one block a token (256 threads, 8 consecutive values
 // a thread and round): its scale, the power of two 2^e with the largest
 // |x| * 2^-e in [2^13, 2^14) (e clamped so that the scale stays a normal
@@ -420,31 +423,13 @@ __device__ __forceinline__ void split_half(float v, _Float16& hi, _Float16& lo) 
 // means of its 32-value groups.  A row of up to 16384 values stays in
 // registers between the maximum and the split (one launch and one reading of
 // x, where two launches were 9.8 us at 256 x 4096).
-//
-// GROUPED: block p takes pair p's row x[p / share] to the slot of the pair
-// (slots[p]; below 0: none).  Slots without a pair are not written: their
-// products stay in rows that nothing reads.
 constexpr int kPrepRounds = 8;
-struct NoSlots {};
-struct Slots {
-  const int32_t* slot;
-  int share;
-};
-template <class S>
 __global__ __launch_bounds__(256) void prefill_prep_kernel(const float* __restrict__ x, int cols, int tokens,
-                                                           uint8_t* __restrict__ work, const S sl) {
-  constexpr bool GROUPED = std::is_same<S, Slots>::value;
+                                                           uint8_t* __restrict__ work) {
   const Prep P = prep_layout(cols, tokens);
-  int t = blockIdx.x;
-  int64_t from = t;
-  if constexpr (GROUPED) {
-    t = sl.slot[blockIdx.x];
-    if (t < 0) return;
-    from = blockIdx.x / sl.share;
-  }
-  const int tile = t >> 5, m = t & 31;
+  const int t = blockIdx.x, tile = t >> 5, m = t & 31;
   const int n8 = cols >> 3;  // runs of 8 values
-  const float* row = x + from * cols;
+  const float* row = x + (int64_t)t * cols;
   typedef float v4f __attribute__((ext_vector_type(4)));
   __shared__ float red[4];
   v4f v[kPrepRounds][2];
@@ -474,7 +459,7 @@ __global__ __launch_bounds__(256) void prefill_prep_kernel(const float* __restri
     __syncthreads();
     mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   }
-  const int e = mx > 0.0f ? min(max(ilogbf(mx) - 13, -100), 100) : 0;
+  const int e = scale_exp(mx);
   if (threadIdx.x == 0) ((float*)(work + P.xs))[t] = ldexpf(1.0f, e);
   uint8_t* xp = work + P.xp + (size_t)tile * P.ks * 2048 + 16 * m;
   _Float16* xm = (_Float16*)(work + P.xm) + (size_t)tile * P.nch * 512 + 8 * m;
@@ -538,7 +523,11 @@ __global__ __launch_bounds__(256) void prefill_prep_kernel(const float* __restri
 // those stacked at sg.w[0], each of sg.end[0] rows; tokens are slots, of which
 // block y takes TT tiles from tiles[y].first on, and slot s goes to row order[s]
 // of y.  GLU (epi has MI_EPI_GLU): the lower half of a block's rows are those of
-// sg.w[0], the upper half the same ones of sg.w[1], and y gets act(lower) * upper.
+// sg.w[0], the upper half the same ones of sg.w[1], and y gets act(lower) * upper;
+// top the largest size among a row's values of each block x, for the next product's
+// activations (top_stride apart.  An atomic maximum a row, from every block, cost 70 us
+// of 714 at 1018 rows of 2 x 14336 x 4096.)  K may be split over blockIdx.z: part z
+// starts split_stride floats behind the one before.
 struct NoGroups {};
 struct GroupTile {
   int32_t expert, first, end, pad;  // first: a tile of 32 slots; end: behind the expert's last slot
@@ -547,32 +536,31 @@ struct Groups {
   const GroupTile* tiles;
   const int32_t* count;  // of them
   const int32_t* order;
-  int64_t expert_bytes;
+  int64_t expert_bytes, split_stride, top_stride;
+  float* top;
 };
-template <int KIND, int RT, int TT, int WR, int KS, class G = NoGroups, bool GLU = false>
-__global__ __launch_bounds__(WR * KS * 64, (WR * KS + 3) / 4) void prefill_kernel(
-    const RowSegs sg, int cols, int tokens, const uint8_t* __restrict__ work, int chunks_per_split,
-    float* __restrict__ y, int64_t ldy, int epi, const float* __restrict__ aux, float* __restrict__ part, const G gr) {
+template <int RT, int TT, int WR, int KS>
+struct BlockLds {
+  static constexpr int kStageBytes = TT * 4 * 2 * 1024;  // one buffer: TT tiles x 4 steps x 2 halves
+  static constexpr int kX = KS * 2 * kStageBytes, kSum = TT * 32 * WR * RT * 32 * 4;
+  static_assert(kX <= 65536, "the transfer's LDS address is 16 bits");
+  static constexpr int kBytes = kX > kSum ? kX : kSum;
+};
+template <int KIND, int RT, int TT, int WR, int KS, class G, bool GLU>
+__device__ __forceinline__ void prefill_block(
+    const RowSegs& sg, int cols, int tokens, const uint8_t* __restrict__ work, int chunks_per_split,
+    float* __restrict__ y, int64_t ldy, int epi, const float* __restrict__ aux, float* __restrict__ part, const G& gr,
+    const GroupTile& gt, uint8_t* lds) {
   constexpr bool GROUPED = std::is_same<G, Groups>::value;
   using K = typename KindOf<KIND>::T;
   constexpr int S = K::SLOTS;
-  constexpr int kStageBytes = TT * 4 * 2 * 1024;  // one LDS buffer: TT tiles x 4 steps x 2 halves
+  constexpr int kStageBytes = BlockLds<RT, TT, WR, KS>::kStageBytes;
   constexpr int kBlockRows = WR * RT * 32;
-  constexpr int kX = KS * 2 * kStageBytes;
-  static_assert(kX <= 65536, "the transfer's LDS address is 16 bits");
-  constexpr int kSum = TT * 32 * kBlockRows * 4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kX > kSum ? kX : kSum];
   const Prep P = prep_layout(cols, tokens);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave / WR, wr = wave % WR;
   const int n = lane & 31, kh = lane >> 5;
-  int tile0 = blockIdx.y * TT;
-  GroupTile gt{};
-  if constexpr (GROUPED) {
-    if ((int)blockIdx.y >= *gr.count) return;
-    gt = gr.tiles[blockIdx.y];
-    tile0 = gt.first;
-  }
+  const int tile0 = GROUPED ? gt.first : blockIdx.y * TT;
   const int nst = cols / kStage;
   const int ch0 = blockIdx.z * chunks_per_split, ch1 = min(ch0 + chunks_per_split, P.nch);
   const int rounds = (ch1 - ch0 + KS - 1) / KS;
@@ -813,18 +801,35 @@ __global__ __launch_bounds__(WR * KS * 64, (WR * KS + 3) / 4) void prefill_kerne
     constexpr int kMine = GLU ? kBlockRows / 2 : kBlockRows;
     static_assert(!GLU || (WR % 2 == 0 && kMine % 64 == 0), "two matrices a block");
     const int row0 = blockIdx.x * kMine;
-#pragma unroll 4
-    for (int tl = wave; tl < TT * 32; tl += WR * KS) {
-      if (t0 + tl >= gt.end) break;
-      const float sc = xs[t0 + tl];
-      float* to = y + (int64_t)gr.order[t0 + tl] * ldy;
+    // four of a wave's tokens at a time, their loads together (tokens past the end: the
+    // last one again, not stored)
+    constexpr int kStep = WR * KS;
+#pragma unroll 1
+    for (int tl0 = wave; tl0 < TT * 32 && t0 + tl0 < gt.end; tl0 += 4 * kStep) {
+      float most[4] = {};
 #pragma unroll
-      for (int k = 0; k < kMine / 64; k++) {
-        const int r = row0 + 64 * k + lane;
-        const float* at = (const float*)lds + tl * kBlockRows + 64 * k + lane;
-        float v = *at * sc;
-        if constexpr (GLU) v = ((epi & MI_ACT_GELU) ? mv::gelu(v) : mv::silu(v)) * (at[kMine] * sc);
-        if (r < rows) to[r] = v;
+      for (int u = 0; u < 4; u++) {
+        const bool live = t0 + tl0 + u * kStep < gt.end;  // (uniform)
+        const int tl = live ? tl0 + u * kStep : tl0;
+        const float sc = xs[t0 + tl];
+        float* to = y + (int64_t)gr.order[t0 + tl] * ldy + blockIdx.z * gr.split_stride;
+#pragma unroll
+        for (int k = 0; k < kMine / 64; k++) {
+          const int r = row0 + 64 * k + lane;
+          const float* at = (const float*)lds + tl * kBlockRows + 64 * k + lane;
+          float v = *at * sc;
+          if constexpr (GLU) v = ((epi & MI_ACT_GELU) ? mv::gelu(v) : mv::silu(v)) * (at[kMine] * sc);
+          if (r < rows && live) to[r] = v;
+          if constexpr (GLU) most[u] = fmaxf(most[u], r < rows ? fabsf(v) : 0.0f);
+        }
+      }
+      if constexpr (GLU) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const float m = lanes::reduce<64>(most[u], lanes::Max{});
+          const int s = t0 + tl0 + u * kStep;
+          if (lane == 0 && s < gt.end) gr.top[blockIdx.x * gr.top_stride + gr.order[s]] = m;
+        }
       }
     }
   } else {
@@ -844,6 +849,38 @@ __global__ __launch_bounds__(WR * KS * 64, (WR * KS + 3) / 4) void prefill_kerne
       }
     }
   }
+}
+
+template <int KIND, int RT, int TT, int WR, int KS>
+__global__ __launch_bounds__(WR * KS * 64, (WR * KS + 3) / 4) void prefill_kernel(
+    const RowSegs sg, int cols, int tokens, const uint8_t* __restrict__ work, int chunks_per_split,
+    float* __restrict__ y, int64_t ldy, int epi, const float* __restrict__ aux, float* __restrict__ part) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[BlockLds<RT, TT, WR, KS>::kBytes];
+  prefill_block<KIND, RT, TT, WR, KS, NoGroups, false>(sg, cols, tokens, work, chunks_per_split, y, ldy, epi, aux, part,
+                                                       NoGroups{}, GroupTile{}, lds);
+}
+
+// A block takes as many tiles as its list has left, not always TT: half of an expert's
+// last block is empty on average, and the products are what bounds the rest.
+template <int KIND, int RT, int TT, int WR, int KS, bool GLU>
+__global__ __launch_bounds__(WR * KS * 64, (WR * KS + 3) / 4) void group_kernel(
+    const RowSegs sg, int cols, int slots, const uint8_t* __restrict__ work, int chunks_per_split, float* __restrict__ y,
+    int64_t ldy, int epi, const Groups gr) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[BlockLds<RT, TT, WR, KS>::kBytes];
+  if ((int)blockIdx.y >= *gr.count) return;
+  const GroupTile gt = gr.tiles[blockIdx.y];
+  const int left = (gt.end - 32 * gt.first + 31) >> 5;
+#define MI_GROUP(T)                                                                                                  \
+  prefill_block<KIND, RT, T, WR, KS, Groups, GLU>(sg, cols, slots, work, chunks_per_split, y, ldy, epi, nullptr, nullptr, \
+                                                  gr, gt, lds)
+  if constexpr (TT > 2) {
+    if (left > 3) return MI_GROUP(4);
+    if (left > 2) return MI_GROUP(3);
+  }
+  if constexpr (TT > 1)
+    if (left > 1) return MI_GROUP(2);
+  MI_GROUP(1);
+#undef MI_GROUP
 }
 
 }  // namespace
