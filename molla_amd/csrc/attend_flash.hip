@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
 
   // 32 keys of slice sl: their scores, the running maximum and sum, the
   // weights' halves, and the weighted values
-  auto tile = [&](int kt, int sl, int buf) __attribute__((always_inline)) {
+  auto tile = [&](int kt, int sl, int buf, uint64_t cells_held) __attribute__((always_inline)) {
     const int base = sl * kSlice + 32 * kt;
     // (opaque, so that the pieces' addresses are formed here and not kept in
     // registers across the loop, of which there are none to spare)
@@ -422,11 +422,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
       }
     }
     // lanes past their token's end, or on a cell that is not held, take no part
-    const bool full = !PAGED && base + 32 <= wave_min && (!WIN || base >= wave_top || base + 32 <= win.first);
+    const bool full = (WIN ? (uint32_t)(cells_held >> (32 * kt)) == 0xffffffffu : !PAGED) && base + 32 <= wave_min &&
+                      (!WIN || base >= wave_top || base + 32 <= win.first);
     const int rel = cnt - base - 4 * h;
     const int from = WIN ? low - base - 4 * h : 0, firsts = WIN ? win.first - base - 4 * h : 0;
     uint32_t held = 0xffffffffu;
-    if constexpr (PAGED) held = (uint32_t)__ballot(kv_index[min(base + n, count - 1)] >= 0) >> (4 * h);
+    if constexpr (WIN) held = (uint32_t)(cells_held >> (32 * kt)) >> (4 * h);
+    else if constexpr (PAGED) held = (uint32_t)__ballot(kv_index[min(base + n, count - 1)] >= 0) >> (4 * h);
     auto live = [&](int j) __attribute__((always_inline)) {
       const int at = 8 * (j >> 2) + (j & 3);
       return at < rel && (!WIN || at >= from || at < firsts) && (!PAGED || ((held >> at) & 1));
@@ -484,17 +486,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
   store_k(0);
   store_v(0);
   __syncthreads();
+  // WIN: which of a slice's cells are held, read a slice ahead (in the tile it was a
+  // load's latency each time: MI_HELD_US)
+  int cell = WIN && PAGED ? cell_of(slice_of(s0), lane) : 0;
   for (int sv = s0; sv < s1; sv++) {
     const int buf = (sv - s0) & 1, sl = slice_of(sv), base = sl * kSlice;
     const bool more = sv + 1 < s1;          // uniform
     // this wave has tokens that reach the slice
     const bool mine = base < wave_max && (!WIN || base + kSlice > wave_low || base < win.first);
+    const uint64_t cells_held = WIN && PAGED ? __ballot(cell >= 0) : ~0ull;
     if (more) load(kc, slice_of(sv + 1), kr, kfr);
+    if (WIN && PAGED && more) cell = cell_of(slice_of(sv + 1), lane);
     // the slice's weights, 32 keys at a time (both tiles' scores at once are 32
     // more registers than a wave has)
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
-      if (mine && base + 32 * kt < wave_max) tile(kt, sl, buf);
+      if (mine && base + 32 * kt < wave_max) tile(kt, sl, buf, cells_held);
       if (kt == 0 && more) {
         store_k(1 - buf);
         int next = slice_of(sv + 1);

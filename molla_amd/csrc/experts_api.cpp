@@ -38,26 +38,34 @@ int check_counts(const char* name, int32_t experts, int64_t pairs) {
   return MI_OK;
 }
 
+// Whether a call's pairs take the row kernel: up to three an expert, on average, or
+// where the products are small beside the tile's chain of launches.  us of an MLP, rows
+// / tile: 8 experts of 4096 x 14336, 16 pairs Q4_K 246 / 279, with Q6_K down 305 / 440,
+// Q8_0 328 / 575, 24 pairs 345 / 316, 420 / 442, 434 / 580, 32 pairs 444 / 318, 536 /
+// 439, 537 / 582; 16 of 2048 x 4096, 48 pairs Q4_K 124 / 108, Q8_0 132 / 186; 64 of 2048
+// x 1024, 64 pairs 52 / 89, 69 / 151; 4 of 1024 x 2048, 24 pairs 41 / 43, 32 pairs 55 /
+// 41.
+bool few_pairs(int64_t pairs, int32_t experts, int64_t weights) {
+  return pairs <= kFewPairs && (pairs <= 3 * (int64_t)experts || pairs * weights <= 48 << 20);
+}
+
 struct MatmulCarve {
   size_t x, plan, total;
 };
-// Few rows: their activations in matvec form.  Many: by slot, and the plan.
-MatmulCarve matmul_carve(int32_t experts, int32_t cols, int32_t share, int32_t pairs) {
+// Few rows: their activations in matvec form.  Many: by slot, and the plan.  (The
+// larger of the two where it hangs on the rows.)
+MatmulCarve matmul_carve(int32_t experts, int32_t cols, int32_t share, int32_t pairs, bool few) {
   MatmulCarve c{};
-  size_t at = 0;
-  if (pairs <= kFewPairs) {
-    at += up256((size_t)xq_token_bytes(cols) * (pairs / share));
-  } else {
-    const GroupPlan g = group_plan(nullptr, pairs, experts, 1);  // (the most lists)
-    at += g.bytes;
-    c.x = at;
-    at += up256(group_prep_bytes(cols, g));
-  }
-  c.total = at;
+  const size_t rows = up256((size_t)xq_token_bytes(cols) * (pairs / share));
+  const GroupPlan g = group_plan(nullptr, pairs, experts, 1);  // (the most lists)
+  const size_t tile = g.bytes + up256(group_prep_bytes(cols, g));
+  c.x = few ? 0 : g.bytes;
+  c.total = pairs > kFewPairs ? tile : few_pairs(pairs, experts, INT32_MAX) ? rows : std::max(rows, tile);
   return c;
 }
 
 struct MlpCarve {
+  bool few;
   size_t x, h, hx, part, plan, top, total;
   int gate_tiles, down_tiles, splits;  // many rows: tiles a block, parts of down's K
 };
@@ -73,7 +81,8 @@ MlpCarve mlp_carve(const mi_experts& d, int32_t tokens, int32_t used) {
     at += up256(bytes);
     return p;
   };
-  if (pairs <= (size_t)kFewPairs) {
+  c.few = few_pairs(pairs, experts, (int64_t)width * hidden);
+  if (c.few) {
     c.x = take((size_t)xq_token_bytes(width) * tokens);
     c.hx = take((size_t)xq_token_bytes(hidden) * pairs);
   } else {
@@ -101,7 +110,7 @@ int launch_experts_mlp(hipStream_t s, const mi_experts& d, const float* x, int32
   const MlpCarve c = mlp_carve(d, tokens, used);
   char* base = (char*)work;
   int rc;
-  if (pairs <= kFewPairs) {
+  if (c.few) {
     const bool one = one_row_fits(d.width, used, pairs);
     if (!one && (rc = launch_quantize(s, x, d.width, tokens, base + c.x))) return rc;
     ExpertRows a{};
@@ -224,7 +233,7 @@ size_t mi_experts_matmul_workspace(int32_t experts, int32_t cols, int32_t share,
   if (experts < 1 || experts > kMaxExperts || cols <= 0 || cols % 64 || pairs < 1 || pairs > kMaxPairs || share < 1 ||
       pairs % share)
     return 0;
-  return matmul_carve(experts, cols, share, pairs).total;
+  return matmul_carve(experts, cols, share, pairs, true).total;
 }
 
 int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_bytes, int32_t experts, int32_t rows,
@@ -244,14 +253,15 @@ int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_byt
   const size_t xb = 4 * (size_t)(pairs / share) * cols, yb = 4 * (size_t)pairs * rows;
   if (meet(y, yb, x, xb) || meet(y, yb, ids, 4 * (size_t)pairs) || meet(y, yb, w, (size_t)experts * rows * row_bytes))
     return fail(MI_ERR_ARG, "experts_matmul: the output lies in an input");
-  const MatmulCarve c = matmul_carve(experts, cols, share, pairs);
+  const bool few = few_pairs(pairs, experts, (int64_t)rows * cols);
+  const MatmulCarve c = matmul_carve(experts, cols, share, pairs, few);
   if (!work || ((uintptr_t)work & 255) || work_bytes < c.total)
     return fail(MI_ERR_WORKSPACE, "experts_matmul: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, c.total);
   if (meet(work, c.total, x, xb) || meet(work, c.total, y, yb) || meet(work, c.total, ids, 4 * (size_t)pairs))
     return fail(MI_ERR_ARG, "experts_matmul: the workspace lies in another buffer");
   hipStream_t s = (hipStream_t)stream;
   char* base = (char*)work;
-  if (pairs <= kFewPairs) {
+  if (few) {
     const bool one = one_row_fits(cols, share, pairs);
     if (!one && (rc = launch_quantize(s, x, cols, pairs / share, base + c.x))) return rc;
     ExpertRows a{};
