@@ -14,7 +14,7 @@ int prep_slots(const GroupPlan& g) { return g.slots + (kPadTiles - 1) * kTileTok
 // (and its arithmetic), the rows' largest sizes known: a wave takes 8 slots x 8 runs of
 // 8 values, so that the 16-byte pieces of a step's 8 neighbouring slots leave as whole
 // 128-byte lines.  (A row a block left them to blocks on different chiplets, an eighth
-// of a line each: 1018 rows of 14336 columns in 64 us, of 4096 in 16; now MI_PREP_US.)
+// of a line each: 1018 rows of 14336 columns in 64 us, of 4096 in 16; now 37 together.)
 constexpr int kPrepCols = 1024;
 __global__ __launch_bounds__(256) void group_prep_kernel(const float* __restrict__ x, int cols, int slots, int share,
                                                          const int32_t* __restrict__ order,
