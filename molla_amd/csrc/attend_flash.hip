@@ -68,6 +68,11 @@ constexpr int kRows = 128;    // query rows a block
 // scaled back.  (A lift in the exponential's argument rounds that to 2^-21, weights
 // to 3e-7; after it, it takes 2 us of a layer's 470 at a chunk of 256.)
 constexpr float kLift = 16384.0f;
+// Over a window a row's maximum stays until a score passes it by a factor of 2^4 (the
+// row's other sums are not taken to the new one in most tiles: 256 tokens of 32 heads of
+// 128 over 4096 positions 70 -> 66 us), so weights reach 2^4 and are lifted by 2^11: a
+// weight to 2^-36 of the largest, or 2^-24 of itself.
+constexpr float kGrow = 4.0f, kGrowLift = 2048.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ ff16 mfma32(fh8 a, fh8 b, ff16 c) {
@@ -137,6 +142,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
     float* __restrict__ out, const Window win) {
   static_assert(!Q8 || D <= 128, "a wave stages values of one q8_0 block");
   constexpr int PIECES = D / 8, NT = D / 32;
+  constexpr float lift = WIN ? kGrowLift : kLift;
   constexpr int VB = Q8 ? 1 : 2;  // value buffers (q8_0 values take two halves: 32 KB at D = 128)
   constexpr int VH = Q8 ? 2 : 1;  // halves a value
   __shared__ __align__(16) _Float16 ks[2][kSlice * D];
@@ -424,7 +430,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
     // lanes past their token's end, or on a cell that is not held, take no part
     const bool full = (WIN ? (uint32_t)(cells_held >> (32 * kt)) == 0xffffffffu : !PAGED) && base + 32 <= wave_min &&
                       (!WIN || base >= wave_top || base + 32 <= win.first);
-    const int rel = cnt - base - 4 * h;
+    int rel = cnt - base - 4 * h;
     const int from = WIN ? low - base - 4 * h : 0, firsts = WIN ? win.first - base - 4 * h : 0;
     uint32_t held = 0xffffffffu;
     if constexpr (WIN) held = (uint32_t)(cells_held >> (32 * kt)) >> (4 * h);
@@ -433,16 +439,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
       const int at = 8 * (j >> 2) + (j & 3);
       return at < rel && (!WIN || at >= from || at < firsts) && (!PAGED || ((held >> at) & 1));
     };
+    // (WIN: the masks' bits, made behind a branch that the asm keeps: taken in every
+    // tile, the masks are 7 % of a window's time)
+    uint32_t lives = 0;
     if (!full) {
-      if constexpr (WIN) asm volatile("");  // (keeps the branch: taken in every tile, the masks are 7 %)
+      if constexpr (WIN) {
+        asm volatile("" : "+v"(rel));
 #pragma unroll
-      for (int j = 0; j < 16; j++) s[j] = live(j) ? s[j] : -INFINITY;
+        for (int j = 0; j < 16; j++) lives |= (uint32_t)live(j) << j;
+        asm volatile("" : "+v"(lives));
+      }
+#pragma unroll
+      for (int j = 0; j < 16; j++) s[j] = (WIN ? (lives >> j) & 1 : live(j)) ? s[j] : -INFINITY;
     }
     float m = s[0];
 #pragma unroll
     for (int j = 1; j < 16; j++) m = fmaxf(m, s[j]);
     m = other_max(m);
-    const float mn = fmaxf(mc, m);
+    const float mn = !WIN || (m - mc) * c2 > kGrow ? fmaxf(mc, m) : mc;
     if (__any(mn != mc)) {
       const float a = __builtin_amdgcn_exp2f((mc - mn) * c2);
       l *= a;
@@ -456,17 +470,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
 #pragma unroll
     for (int j = 0; j < 16; j++) s[j] = __builtin_amdgcn_exp2f((s[j] - mc) * c2);
     if (!full) {
-      if constexpr (WIN) asm volatile("");
+      if constexpr (WIN) asm volatile("" : "+v"(lives));
 #pragma unroll
-      for (int j = 0; j < 16; j++) s[j] = live(j) ? s[j] : 0.0f;
+      for (int j = 0; j < 16; j++) s[j] = (WIN ? (lives >> j) & 1 : live(j)) ? s[j] : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < 16; j++) {
       const float p = s[j];
       l += p;
-      const _Float16 hi = (_Float16)fmaf(p, kLift, 0.0f);  // (one instruction)
+      const _Float16 hi = (_Float16)fmaf(p, lift, 0.0f);  // (one instruction)
       ph[j >> 3][j & 7] = hi;
-      pl[j >> 3][j & 7] = (_Float16)fmaf(p, kLift, -(float)hi);
+      pl[j >> 3][j & 7] = (_Float16)fmaf(p, lift, -(float)hi);
     }
     if constexpr (Q8) {
 #pragma unroll
@@ -556,7 +570,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
               s = fmaf(__half2float(kfac[st >> 1]), b, s);
             }
             s = other_sum(s);
-            const float p = __builtin_amdgcn_exp2f((s - mc) * c2) * kLift;
+            const float p = __builtin_amdgcn_exp2f((s - mc) * c2) * lift;
             const float fk = __shfl(f, k) * ldexpf(1.0f, 8 - xo[dt]);
             const int8_t* vb = (const int8_t*)(vc + row) + kvh * D + 32 * dt + 4 * h;
             const int key = sl * kSlice + k;
@@ -592,7 +606,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
           for (int st = 0; st < D / 16; st++)
             for (int u = 0; u < 8; u++) s = fmaf(__half2float(kc[row + 16 * st + 8 * h + u]), sc * qr[16 * st + u], s);
           s = other_sum(s);
-          const float p = __builtin_amdgcn_exp2f((s - mc) * c2) * kLift;
+          const float p = __builtin_amdgcn_exp2f((s - mc) * c2) * lift;
           if (key < cnt && (key >= cnt - win.window || key < win.first)) {
 #pragma unroll
             for (int dt = 0; dt < NT; dt++)
@@ -610,7 +624,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
   if (!live_row) return;
   const int64_t rowi = (int64_t)t * heads + head;
   float* dst = splits == 1 ? out + rowi * D : part_acc + (rowi * splits + split) * D;
-  const float w = (splits == 1 ? (WIN && l == 0.0f ? 0.0f : 1.0f / l) : 1.0f) * (1.0f / kLift);
+  const float w = (splits == 1 ? (WIN && l == 0.0f ? 0.0f : 1.0f / l) : 1.0f) * (1.0f / lift);
 #pragma unroll
   for (int dt = 0; dt < NT; dt++) {
     const float f = Q8 ? w * ldexpf(1.0f, xo[dt] - 8) : w;
