@@ -39,6 +39,14 @@ int launch_expert_rows(hipStream_t s, int kind, const ExpertRows& a);
 int launch_expert_sum(hipStream_t s, const float* part, const int32_t* ids, const float* weights, int32_t width,
                       int32_t tokens, int32_t used, int32_t experts, bool add, int32_t splits, float* out);
 
+// A few pairs' products on the matrix cores (experts_pack.hip): y[z][p] = W[ids[p]] .
+// x[p / share] over part z of the columns; with w1, act(w0) * w1.
+int launch_expert_pack(hipStream_t s, int kind, const void* w0, const void* w1, int64_t row_bytes, int32_t rows,
+                       int32_t cols, int32_t experts, const float* x, int32_t share, const int32_t* ids, int32_t pairs,
+                       int32_t act, int32_t splits, float* y);
+bool pack_fits(int kind);
+int pack_splits(int32_t rows, int32_t cols, int32_t pairs, int32_t experts);
+
 // The lists of many pairs by expert: order[slot] (the pair, -1 behind an expert's
 // last), the blocks' tiles (experts_tile.hip), count (of lists, of slots), and the
 // largest size in each row of x.

@@ -49,6 +49,26 @@ bool few_pairs(int64_t pairs, int32_t experts, int64_t weights) {
   return pairs <= kFewPairs && (pairs <= 3 * (int64_t)experts || pairs * weights <= 48 << 20);
 }
 
+// Whether they take the matrix cores instead, eight rows an operand (experts_pack.hip):
+// from where an expert's weights, unpacked once for all its pairs there, cost the row
+// kernel more.  us of an MLP, rows (or the tile, the last) / packed, by pairs: 8 experts
+// of 4096 x 14336 Q4_K 4 pairs 86 / 101, 8 173 / 144, 16 244 / 198, 32 345 / 217, 64 330
+// / 320; with Q6_K down 8 206 / 239, 12 272 / 279, 16 303 / 283, 32 448 / 390, 48 444 /
+// 456; all Q6_K 16 405 / 435, 24 565 / 435, 48 698 / 660, 64 701 / 751; 16 of 2048 x 4096
+// Q4_K 16 48 / 53, 24 69 / 63, 64 102 / 76; 64 of 2048 x 1024 48 43 / 53, 64 50 / 64.  A
+// product of 8 of 14336 x 4096: Q4_K 12 61 / 67, 16 72 / 65, 64 108 / 101; Q6_K 16 152 /
+// 165, 24 196 / 166, 64 262 / 258.
+bool pack_pairs(int kind, int64_t pairs, int32_t experts) {
+  if (!pack_fits(kind) || pairs > kFewPairs) return false;
+  return kind == MI_Q4_K ? 2 * pairs >= 3 * (int64_t)experts && pairs <= 8 * (int64_t)experts
+                         : pairs >= 3 * (int64_t)experts && pairs <= 6 * (int64_t)experts;
+}
+bool pack_mlp(const mi_experts& d, int64_t pairs) {
+  if (!pack_pairs(d.gate.kind, pairs, d.experts)) return false;
+  return d.down.kind == MI_Q4_K ||
+         (d.down.kind == MI_Q6_K && pairs >= 2 * (int64_t)d.experts && pairs <= 5 * (int64_t)d.experts);
+}
+
 struct MatmulCarve {
   size_t x, plan, total;
 };
@@ -65,12 +85,13 @@ MatmulCarve matmul_carve(int32_t experts, int32_t cols, int32_t share, int32_t p
 }
 
 struct MlpCarve {
-  bool few;
+  bool few, pack;
   size_t x, h, hx, part, plan, top, total;
-  int gate_tiles, down_tiles, splits;  // many rows: tiles a block, parts of down's K
+  int gate_tiles, down_tiles, splits;  // many rows: tiles a block; parts of down's K
 };
-// x: the input in the form its product reads; h: act(gate) * up in f32 (many
-// rows), top: the largest sizes in its rows; hx: the same as the down projection reads it; part: what that gives.
+// Packed: h and part alone.  x: the input in the form its product reads; h: act(gate) *
+// up in f32, top: the largest sizes in its rows; hx: the same as the down projection
+// reads it; part: what that gives.
 MlpCarve mlp_carve(const mi_experts& d, int32_t tokens, int32_t used) {
   const int32_t experts = d.experts, width = d.width, hidden = d.hidden;
   MlpCarve c{};
@@ -82,7 +103,12 @@ MlpCarve mlp_carve(const mi_experts& d, int32_t tokens, int32_t used) {
     return p;
   };
   c.few = few_pairs(pairs, experts, (int64_t)width * hidden);
-  if (c.few) {
+  c.pack = pack_mlp(d, pairs);
+  if (c.pack) {
+    c.splits = pack_splits(width, hidden, pairs, experts);
+    c.h = take(4 * (size_t)hidden * pairs);
+    c.part = take(4 * (size_t)width * pairs * c.splits);
+  } else if (c.few) {
     c.x = take((size_t)xq_token_bytes(width) * tokens);
     c.hx = take((size_t)xq_token_bytes(hidden) * pairs);
   } else {
@@ -110,6 +136,16 @@ int launch_experts_mlp(hipStream_t s, const mi_experts& d, const float* x, int32
   const MlpCarve c = mlp_carve(d, tokens, used);
   char* base = (char*)work;
   int rc;
+  if (c.pack) {
+    float *h = (float*)(base + c.h), *part = (float*)(base + c.part);
+    if ((rc = launch_expert_pack(s, d.gate.kind, d.gate.data, d.up.data, d.gate.row_bytes, d.hidden, d.width, d.experts, x,
+                                 used, ids, pairs, d.act, 1, h)))
+      return rc;
+    if ((rc = launch_expert_pack(s, d.down.kind, d.down.data, nullptr, d.down.row_bytes, d.width, d.hidden, d.experts, h, 1,
+                                 ids, pairs, 0, c.splits, part)))
+      return rc;
+    return launch_expert_sum(s, part, ids, weights, d.width, tokens, used, d.experts, add, c.splits, out);
+  }
   if (c.few) {
     const bool one = one_row_fits(d.width, used, pairs);
     if (!one && (rc = launch_quantize(s, x, d.width, tokens, base + c.x))) return rc;
@@ -261,6 +297,8 @@ int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_byt
     return fail(MI_ERR_ARG, "experts_matmul: the workspace lies in another buffer");
   hipStream_t s = (hipStream_t)stream;
   char* base = (char*)work;
+  if (pack_pairs(kind, pairs, experts))
+    return launch_expert_pack(s, kind, w, nullptr, row_bytes, rows, cols, experts, x, share, ids, pairs, 0, 1, y);
   if (few) {
     const bool one = one_row_fits(cols, share, pairs);
     if (!one && (rc = launch_quantize(s, x, cols, pairs / share, base + c.x))) return rc;

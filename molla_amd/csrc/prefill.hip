@@ -6,6 +6,97 @@
 namespace mi {
 namespace {
 
+// A token's activations, one block a token (256 threads, 8 consecutive values
+// a thread and round): its scale, the power of two 2^e with the largest
+// |x| * 2^-e in [2^13, 2^14) (e clamped so that the scale stays a normal
+// float; 1 for a zero or padding token), xs[t] = 2^e; its halves; and the
+// means of its 32-value groups.  A row of up to 16384 values stays in
+// registers between the maximum and the split (one launch and one reading of
+// x, where two launches were 9.8 us at 256 x 4096).
+constexpr int kPrepRounds = 8;
+__global__ __launch_bounds__(256) void prefill_prep_kernel(const float* __restrict__ x, int cols, int tokens,
+                                                           uint8_t* __restrict__ work) {
+  const Prep P = prep_layout(cols, tokens);
+  const int t = blockIdx.x, tile = t >> 5, m = t & 31;
+  const int n8 = cols >> 3;  // runs of 8 values
+  const float* row = x + (int64_t)t * cols;
+  typedef float v4f __attribute__((ext_vector_type(4)));
+  __shared__ float red[4];
+  v4f v[kPrepRounds][2];
+  float mx = 0.0f;
+  if (t < tokens) {
+#pragma unroll
+    for (int k = 0; k < kPrepRounds; k++) {
+      const int i = min((int)threadIdx.x + 256 * k, n8 - 1);  // (a repeated run changes no maximum)
+      if (256 * k < n8) {
+        v[k][0] = *(const v4f*)(row + 8 * i);
+        v[k][1] = *(const v4f*)(row + 8 * i + 4);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kPrepRounds; k++)
+      if (256 * k < n8) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(v[k][i >> 2][i & 3]));
+      }
+    for (int i = threadIdx.x + 256 * kPrepRounds; i < n8; i += 256) {
+      const v4f a = *(const v4f*)(row + 8 * i), b = *(const v4f*)(row + 8 * i + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) mx = fmaxf(mx, fmaxf(fabsf(a[e]), fabsf(b[e])));
+    }
+    mx = lanes::reduce<64>(mx, lanes::Max{});
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+  const int e = scale_exp(mx);
+  if (threadIdx.x == 0) ((float*)(work + P.xs))[t] = ldexpf(1.0f, e);
+  uint8_t* xp = work + P.xp + (size_t)tile * P.ks * 2048 + 16 * m;
+  _Float16* xm = (_Float16*)(work + P.xm) + (size_t)tile * P.nch * 512 + 8 * m;
+  auto put = [&](int i, v4f a, v4f b) __attribute__((always_inline)) {
+    // run i: values 8 i .. +8, half wave (i >> 1) & 1 of step 2 (i >> 2) + (i & 1)
+    v8h hi, lo;
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      constexpr int order[4] = {0, 2, 1, 3};  // the order of K (above)
+      const int c = order[k & 3];
+      const float f = ldexpf(k < 4 ? a[c] : b[c], -e);
+      _Float16 h, l;
+      split_half(f, h, l);
+      hi[k] = h;
+      lo[k] = l;
+      sum += f;
+    }
+    uint8_t* dst = xp + (size_t)(2 * (i >> 2) + (i & 1)) * 2048 + 512 * ((i >> 1) & 1);
+    *(v8h*)dst = hi;
+    *(v8h*)(dst + 1024) = lo;
+    // the mean of the group's 32 values (a mean, since 32 values of up to
+    // 2^14 overflow a half): four neighbouring lanes
+    sum = lanes::reduce<4>(sum, lanes::Add{}) * (1.0f / 32.0f);
+    _Float16 h, l;
+    split_half(sum, h, l);
+    const int g = i >> 2;
+    if ((i & 3) == 0) {
+      xm[(size_t)(g >> 3) * 512 + (g & 7)] = h;
+      xm[(size_t)(g >> 3) * 512 + 256 + (g & 7)] = l;
+    }
+  };
+  // (n8 is a multiple of 8: a group's four lanes go together)
+#pragma unroll
+  for (int k = 0; k < kPrepRounds; k++) {
+    const int i = threadIdx.x + 256 * k;
+    if (i < n8) put(i, t < tokens ? v[k][0] : v4f{}, t < tokens ? v[k][1] : v4f{});
+  }
+  for (int i = threadIdx.x + 256 * kPrepRounds; i < n8; i += 256)
+    put(i, t < tokens ? *(const v4f*)(row + 8 * i) : v4f{}, t < tokens ? *(const v4f*)(row + 8 * i + 4) : v4f{});
+  // groups past cols in the last chunk
+  for (int g = (cols >> 5) + threadIdx.x; g < 8 * P.nch; g += 256) {
+    xm[(size_t)(g >> 3) * 512 + (g & 7)] = (_Float16)0.0f;
+    xm[(size_t)(g >> 3) * 512 + 256 + (g & 7)] = (_Float16)0.0f;
+  }
+}
+
 // Adds the splits' partial sums in split order and applies the epilogue.
 __global__ __launch_bounds__(256) void prefill_reduce_kernel(const float* __restrict__ part, int splits, int rows,
                                                              int tokens, float* __restrict__ y, int64_t ldy, int epi,
