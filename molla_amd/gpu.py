@@ -12,6 +12,7 @@ GPU every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -72,6 +73,8 @@ class Tensor:
         return MiWeight(self.address, self.kind, self.rows, self.cols, self.row_bytes())
 
 
+# (a size of its two numbers alone; asked of the library each time it is 0.4 us of a call)
+@functools.lru_cache(maxsize=1024)
 def row_bytes(kind: int, cols: int) -> int:
     rb = lib().mi_row_bytes(kind, cols)
     if rb < 0:
@@ -210,6 +213,7 @@ def device_rope(ctx: DeviceContext, x: torch.Tensor, heads: int, head_dim: int, 
 CACHE_F16, CACHE_Q8 = 0, 1  # repack.mojo:174-181
 
 
+@functools.lru_cache(maxsize=1024)
 def cache_row(form: int, kv_width: int) -> int:
     """repack.mojo:221 cache_row: halves one cached position occupies."""
     row = lib().mi_cache_row(form, kv_width)
