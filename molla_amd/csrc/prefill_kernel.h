@@ -662,6 +662,15 @@ __device__ __forceinline__ void prefill_block(
     __syncthreads();
   };
 
+  // a list's rows and their scales, for the end (read there they were two latencies)
+  __shared__ int row_of[GROUPED ? TT * 32 : 1];
+  __shared__ float scale_of[GROUPED ? TT * 32 : 1];
+  if constexpr (GROUPED) {
+    if ((int)threadIdx.x < TT * 32) {
+      row_of[threadIdx.x] = gr.order[tile0 * 32 + threadIdx.x];
+      scale_of[threadIdx.x] = ((const float*)(work + P.xs))[tile0 * 32 + threadIdx.x];
+    }
+  }
   load_x(stage_of(0, 0), 0);
 #pragma unroll
   for (int rt = 0; rt < RT; rt++) {
@@ -720,8 +729,8 @@ __device__ __forceinline__ void prefill_block(
       for (int u = 0; u < 4; u++) {
         const bool live = t0 + tl0 + u * kStep < gt.end;  // (uniform)
         const int tl = live ? tl0 + u * kStep : tl0;
-        const float sc = xs[t0 + tl];
-        float* to = y + (int64_t)gr.order[t0 + tl] * ldy + blockIdx.z * gr.split_stride;
+        const float sc = scale_of[tl];
+        float* to = y + (int64_t)row_of[tl] * ldy + blockIdx.z * gr.split_stride;
 #pragma unroll
         for (int k = 0; k < kMine / 64; k++) {
           const int r = row0 + 64 * k + lane;
@@ -737,7 +746,7 @@ __device__ __forceinline__ void prefill_block(
         for (int u = 0; u < 4; u++) {
           const float m = lanes::reduce<64>(most[u], lanes::Max{});
           const int s = t0 + tl0 + u * kStep;
-          if (lane == 0 && s < gt.end) gr.top[blockIdx.x * gr.top_stride + gr.order[s]] = m;
+          if (lane == 0 && s < gt.end) gr.top[blockIdx.x * gr.top_stride + row_of[s - t0]] = m;
         }
       }
     }
@@ -776,8 +785,11 @@ __global__ __launch_bounds__(WR * KS * 64, (WR * KS + 3) / 4) void group_kernel(
     const RowSegs sg, int cols, int slots, const uint8_t* __restrict__ work, int chunks_per_split, float* __restrict__ y,
     int64_t ldy, int epi, const Groups gr) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[BlockLds<RT, TT, WR, KS>::kBytes];
-  if ((int)blockIdx.y >= *gr.count) return;
-  const GroupTile gt = gr.tiles[blockIdx.y];
+  // (both loads at once: there are lists for the whole grid, those past the count unwritten)
+  GroupTile gt = gr.tiles[blockIdx.y];
+  int count = *gr.count;
+  asm volatile("" : "+s"(gt.expert), "+s"(gt.first), "+s"(gt.end), "+s"(count));
+  if ((int)blockIdx.y >= count) return;
   const int left = (gt.end - 32 * gt.first + 31) >> 5;
 #define MI_GROUP(T)                                                                                                  \
   prefill_block<KIND, RT, T, WR, KS, Groups, GLU>(sg, cols, slots, work, chunks_per_split, y, ldy, epi, nullptr, nullptr, \
