@@ -123,17 +123,18 @@ int launch_kind(hipStream_t s, const RowSegs& sg, int cols, int act, const Group
 
 // By the rows of an expert, on average.  us a product by tiles a block 1 / 2 / 4 (Q4_K's
 // 2: (2, 2, 4, 2)), 64 experts of 2048x1024 and 8 of 14336x4096:
-//   rows           16             38             64             100            160
-//   Q4_K 64   48 / 60 / 82   64 / 81 / 95   89 / 97 / 126  126 / 143 / 145  189 / 196 / 203
-//   Q4_K 8   109 / 137 / 234  151 / 154 / 246  236 / 215 / 268  323 / 287 / 370  470 / 428 / 516
-//   Q6_K 64   83 / 97 / 106  112 / 109 / 146  155 / 136 / 158  226 / 197 / 181  357 / 298 / 269
-//   Q6_K 8   254 / 280 / 352  352 / 290 / 356  503 / 407 / 379  701 / 495 / 528  1053 / 741 / 695
-//   Q8_0 64   67 / 77 / 92   91 / 86 / 104  127 / 105 / 139  186 / 150 / 160  312 / 245 / 242
-//   Q8_0 8   216 / 247 / 305  299 / 256 / 311  422 / 359 / 331  593 / 464 / 451  840 / 616 / 600
+//   rows           16              38              64              100             160
+//   Q4_K 64   49 / 53         63 / 76         85 / 87         125 / 125       180 / 174
+//   Q4_K 8    119 / 114       158 / 149       245 / 209       332 / 286       477 / 400
+//   Q6_K 64   88 / 92 / 83    114 / 101 / 100 153 / 128 / 124 216 / 177 / 152 330 / 259 / 213
+//   Q6_K 8    255 / 264 / 270 354 / 280 / 306 503 / 381 / 313 697 / 475 / 421 1045 / 706 / 589
+//   Q8_0 64   68 / 69 / 67    88 / 78 / 84    119 / 98 / 98   170 / 132 / 127 270 / 203 / 192
+//   Q8_0 8    221 / 220 / 238 299 / 249 / 255 426 / 332 / 279 588 / 436 / 381 833 / 585 / 502
+// (24 rows: Q6_K 102 / 92, 307 / 266, Q8_0 77 / 73, 261 / 240.)
 int group_tiles(int kind, int32_t pairs, int32_t experts) {
   const int each = pairs / experts;
   if (long_scales(kind)) return each < 56 ? 1 : 2;
-  return each < 24 ? 1 : each < 80 ? 2 : 4;
+  return each < 24 ? 1 : each < 56 ? 2 : 4;
 }
 
 // Parts of K (in whole 256-value chunks): while the blocks that the experts take on
