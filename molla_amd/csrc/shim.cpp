@@ -453,6 +453,19 @@ int mi_attend_window(mi_stream stream, int32_t form, const float* q, int64_t q_s
     return fail(MI_ERR_ARG, "attend_window: the output may not lie among the queries");
   const Window win{window, first, max_count};
   const size_t need = attend_window_workspace(heads, kv_heads, head_dim, form, win, tokens, stride == 0);
+  // (the lists of one sequence's chunk are one)
+  const size_t lists = kv_index ? 4 * ((size_t)(stride ? tokens - 1 : 0) * stride + max_count) : 0;
+  const struct {
+    const void* at;
+    size_t bytes;
+  } in[] = {{q, 4 * ((size_t)(tokens - 1) * q_stride + qw)}, {pos, 4 * (size_t)tokens}, {kv_index, lists}},
+    written[] = {{work, need}, {out, 4 * (size_t)tokens * qw}};
+  for (const auto& w : written)
+    for (const auto& b : in)
+      if (b.at && (const char*)w.at < (const char*)b.at + b.bytes && (const char*)b.at < (const char*)w.at + w.bytes)
+        return fail(MI_ERR_ARG, "attend_window: the output or the workspace lies in an input");
+  if ((const char*)work < (const char*)out + written[1].bytes && (const char*)out < (const char*)work + need)
+    return fail(MI_ERR_ARG, "attend_window: the workspace lies in the output");
   if (!work || ((uintptr_t)work & 255) || work_bytes < need)
     return fail(MI_ERR_WORKSPACE, "attend_window: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);
   return launch_attend_window((hipStream_t)stream, q, q_stride, k_cache, v_cache, cache_stride, heads, kv_heads, head_dim,
