@@ -538,7 +538,8 @@ int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_byt
  * added to out.  A pair whose id is no expert takes no part; the sum runs in the
  * order of k.  gate and up are of one kind, their rows experts * hidden, down's
  * experts * width.  out may be x.  Workspace: mi_experts_workspace, 256-byte
- * aligned; x and out 16-byte aligned. */
+ * aligned (one for the most tokens holds calls of fewer, here and for the other
+ * calls of this section and the one above); x and out 16-byte aligned. */
 typedef struct {
   int32_t experts;
   int32_t width, hidden; /* of one expert, multiples of 64 (256 for the K-quants) */

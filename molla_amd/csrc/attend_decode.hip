@@ -494,6 +494,9 @@ DecodePlan decode_attend_plan(int32_t kv_heads, int32_t tokens, int32_t max_coun
   return best;
 }
 
+// The most shares that a plan for up to max_count keys has.
+int64_t most_shares(int32_t max_count) { return std::min<int64_t>((max_count - 1) / (2 * kRun) + 1, kMaxShares); }
+
 namespace {
 
 template <int D, bool Q8, bool PAGED, bool WIN>

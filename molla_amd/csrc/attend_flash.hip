@@ -677,12 +677,23 @@ __global__ __launch_bounds__(256) void attend_combine_kernel(const float* __rest
 // Shares of the keys: enough that the blocks fill two a compute unit, at
 // most one for each slice of the context (of what a tile's windows reach), and at
 // most 16 (each is another partial result of every row to write and fold).
+static int flash_slices(int32_t max_count, int tq, const Window* win) {
+  const int slices = (max_count + kSlice - 1) / kSlice;
+  return win ? (int)std::min<int64_t>(slices, ((int64_t)win->window + tq + win->first) / kSlice + 3) : slices;
+}
 int flash_splits(int32_t heads, int32_t kv_heads, int32_t max_count, int32_t tokens, const Window* win) {
   const int group = heads / kv_heads, tq = kRows / group, tiles = (tokens + tq - 1) / tq;
-  int slices = (max_count + kSlice - 1) / kSlice;
-  if (win) slices = (int)std::min<int64_t>(slices, ((int64_t)win->window + tq + win->first) / kSlice + 3);
+  const int slices = flash_slices(max_count, tq, win);
   const int want = 2 * cu_count() / std::max(1, kv_heads * tiles);
   return std::max(1, std::min({want, slices, 16}));
+}
+
+// The most (token, split) pairs of calls of up to `tokens` tokens: splits times the
+// tiles' tokens are no more than fill the chip.
+int64_t flash_most_slots(int32_t heads, int32_t kv_heads, int32_t max_count, int32_t tokens, const Window* win) {
+  const int tq = kRows / (heads / kv_heads);
+  const int64_t each = std::min(flash_slices(max_count, tq, win), 16);
+  return std::max<int64_t>(tokens, std::min(tokens * each, (int64_t)tq * 2 * cu_count() / kv_heads));
 }
 
 bool flash_fits(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t tokens) {

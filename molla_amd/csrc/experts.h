@@ -45,6 +45,7 @@ int launch_expert_pack(hipStream_t s, int kind, const void* w0, const void* w1, 
                        int32_t cols, int32_t experts, const float* x, int32_t share, const int32_t* ids, int32_t pairs,
                        int32_t act, int32_t splits, float* y);
 bool pack_fits(int kind);
+int pack_most_splits(int32_t cols);
 int pack_splits(int32_t rows, int32_t cols, int32_t pairs, int32_t experts);
 
 // The lists of many pairs by expert: order[slot] (the pair, -1 behind an expert's
@@ -68,6 +69,7 @@ GroupPlan group_plan(void* work, int32_t pairs, int32_t experts, int32_t tiles_a
 int group_tiles(int kind, int32_t pairs, int32_t experts);  // 32-slot tiles a block
 // Parts of K of a product whose sum a later launch takes.
 int group_splits(int kind, int32_t rows, int32_t cols, int32_t pairs, int32_t experts, int32_t tiles_a_block);
+int group_most_splits(int32_t cols);
 size_t group_prep_bytes(int32_t cols, const GroupPlan& g);
 // Row p / share of x for pair p, whose largest size is that among top[j * pairs + p /
 // share], j < tops.

@@ -128,7 +128,25 @@ MlpCarve mlp_carve(const mi_experts& d, int32_t tokens, int32_t used) {
 
 }  // namespace
 
-size_t experts_workspace(const mi_experts& d, int32_t tokens, int32_t used) { return mlp_carve(d, tokens, used).total; }
+// Of calls of up to as many tokens: a workspace of the largest holds a smaller call's,
+// which may take another way or be cut into more parts.
+size_t experts_workspace(const mi_experts& d, int32_t tokens, int32_t used) {
+  const int64_t pairs = (int64_t)tokens * used, some = std::min<int64_t>(pairs, kFewPairs);
+  const int32_t width = d.width, hidden = d.hidden;
+  size_t most = up256((size_t)xq_token_bytes(width) * std::min<int64_t>(tokens, kFewPairs)) +
+                up256((size_t)xq_token_bytes(hidden) * some);
+  if (pack_fits(d.gate.kind) && pack_fits(d.down.kind))
+    most = std::max(most, up256(4 * (size_t)hidden * some) + up256(4 * (size_t)width * some * pack_most_splits(hidden)));
+  if (!few_pairs(pairs, d.experts, (int64_t)width * hidden)) {
+    const GroupPlan g = group_plan(nullptr, (int32_t)pairs, d.experts, 1);
+    const size_t top = 4 * (size_t)pairs * group_tops(d.gate.kind, hidden, 1);
+    const int64_t row = std::max<int64_t>((int64_t)width * group_most_splits(hidden), hidden);
+    most = std::max(most, up256(g.bytes) + up256(top) +
+                              up256(std::max(group_prep_bytes(width, g), group_prep_bytes(hidden, g))) +
+                              up256(4 * (size_t)row * pairs));
+  }
+  return most;
+}
 
 int launch_experts_mlp(hipStream_t s, const mi_experts& d, const float* x, int32_t tokens, int32_t used,
                        const int32_t* ids, const float* weights, float* out, bool add, void* work) {

@@ -148,6 +148,13 @@ int group_splits(int kind, int32_t rows, int32_t cols, int32_t pairs, int32_t ex
   return z;
 }
 
+int group_most_splits(int32_t cols) {
+  const int nch = (cols + kChunk - 1) / kChunk;
+  int z = 1;
+  while (z < 8 && nch >= 16 * z) z *= 2;
+  return z;
+}
+
 GroupPlan group_plan(void* work, int32_t pairs, int32_t experts, int32_t tiles_a_block) {
   GroupPlan g{};
   const int64_t some = std::min(pairs, experts);  // experts that have a pair

@@ -287,6 +287,7 @@ bool decode_window_fits(int32_t group, int32_t head_dim);
 struct DecodePlan {
   int32_t waves, shares;  // of a block; of the keys
 };
+int64_t most_shares(int32_t max_count);
 DecodePlan decode_attend_plan(int32_t kv_heads, int32_t tokens, int32_t max_count, bool q8);
 int launch_attend_decode(hipStream_t s, const float* q, int64_t q_stride, const uint16_t* k_cache,
                          const uint16_t* v_cache, int64_t cache_stride, int32_t heads, int32_t kv_heads,
@@ -301,6 +302,7 @@ int launch_attend_flash(hipStream_t s, const float* q, int64_t q_stride, const u
                         const uint16_t* v_cache, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
                         const int32_t* pos, int32_t max_count, int32_t tokens, float* out, float* part_acc,
                         float* part_ml, int32_t form, const int32_t* kv_index, const Window* win = nullptr);
+int64_t flash_most_slots(int32_t heads, int32_t kv_heads, int32_t max_count, int32_t tokens, const Window* win);
 int flash_splits(int32_t heads, int32_t kv_heads, int32_t max_count, int32_t tokens, const Window* win);
 // Attention over a window (mi_attend_window, and the layer's): the paths above,
 // and how many parts of a (token, head) each leaves.  Arguments as launch_attend.

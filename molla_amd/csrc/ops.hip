@@ -1129,6 +1129,9 @@ struct WindowPlan {
   int parts;  // of a (token, head)
   DecodePlan decode;
 };
+// Blocks a compute unit, at most, that shares of a window's keys make: what bounds the
+// partial results of many sequences (a plan never gains by more).
+constexpr int kWindowBlocks = 8;
 WindowPlan window_plan(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const Window& win, int32_t tokens,
                        bool one_seq) {
   const int group = heads / kv_heads;
@@ -1140,6 +1143,7 @@ WindowPlan window_plan(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_
   } else if (mfma) {
     p.path = kShares;
     p.decode = decode_attend_plan(kv_heads, tokens, win.most(), q8);
+    p.decode.shares = std::min(p.decode.shares, std::max(1, kWindowBlocks * cu_count() / (kv_heads * tokens)));
     p.parts = p.decode.shares;
   } else {
     p.path = kSlices;
@@ -1153,10 +1157,23 @@ size_t window_acc_bytes(const WindowPlan& p, int32_t heads, int32_t head_dim, in
 }
 }  // namespace
 
+// Of calls of up to as many tokens and positions: a workspace of the largest holds a
+// smaller call's, which may well be cut into more parts.
 size_t attend_window_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, const Window& win,
                                int32_t tokens, bool one_seq) {
-  const WindowPlan p = window_plan(heads, kv_heads, head_dim, form, win, tokens, one_seq);
-  return window_acc_bytes(p, heads, head_dim, tokens) + (size_t)tokens * heads * p.parts * 2 * sizeof(float);
+  const int group = heads / kv_heads, cus = cu_count();
+  int64_t slots;  // (token, part)
+  if (!decode_window_fits(group, head_dim)) {
+    slots = (int64_t)tokens * window_plan(heads, kv_heads, head_dim, form, win, tokens, one_seq).parts;
+  } else {
+    const bool chunk = one_seq && !(form == MI_CACHE_Q8 && head_dim == 256);
+    const int64_t shared = chunk ? std::min(tokens, kMaxTokens) : tokens;
+    slots = std::max(shared, std::min(shared * most_shares(win.most()), (int64_t)kWindowBlocks * cus / kv_heads));
+    if (chunk && tokens > kMaxTokens)
+      slots = std::max(slots, flash_most_slots(heads, kv_heads, win.limit, tokens, &win));
+  }
+  const size_t acc = ((size_t)slots * heads * head_dim * sizeof(float) + 255) & ~(size_t)255;
+  return acc + (size_t)slots * heads * 2 * sizeof(float);
 }
 
 int launch_attend_window(hipStream_t s, const float* q, int64_t q_stride, const uint16_t* k_cache,
