@@ -313,7 +313,8 @@ class DeviceSession:
         if n_all < 1 or start + n_all > self.context:
             raise ValueError(f"prompt of {n_all} at {start} does not fit a context of {self.context}")
         chunk = max(1, min(chunk, n_all))
-        need = max(layer_workspace(l, self.context, chunk) for l in m.layers)
+        # (a shorter last chunk may be cut into more parts than a whole one)
+        need = max(layer_workspace(l, self.context, n) for l in m.layers for n in {chunk, n_all % chunk or chunk})
         if getattr(self, "_pwork", None) is None or self._pwork.numel() < need + 256:
             self._pwork = torch.empty(need + 256, dtype=torch.uint8, device=c.device)
             self._px = torch.empty(chunk * s.width, dtype=torch.float32, device=c.device)
