@@ -49,19 +49,20 @@ __global__ __launch_bounds__(256) void router_logits_kernel(const float* __restr
 }
 
 // The same on the matrix cores (v_mfma_f64_16x16x4_f64), for many tokens: a wave takes
-// 16 tokens x 16 NE experts, the block's eight waves every eighth step of 32 values,
-// and their sums meet in LDS, added in wave order.  Lane l holds row or column l % 16
+// 16 tokens x 16 NE experts, the block's W waves every W-th step of 32 values, and their
+// sums meet in LDS, added in wave order (2048 tokens, 128 experts of 4096 values, NE = 4:
+// four waves 47 us, eight 53, sixteen 103; 32 tokens a wave, K in two parts, 47; one or
+// five steps ahead 49, 57).  Lane l holds row or column l % 16
 // and four values in turn of its quarter of 16 (the order of K is the same for both);
 // result j of lane l is row 4 j + l / 16, column l % 16.
 typedef double rd4 __attribute__((ext_vector_type(4)));
-constexpr int kRouteWaves = 8;
-template <int NE>
-__global__ __launch_bounds__(64 * kRouteWaves) void router_tile_kernel(const float* __restrict__ x,
+template <int NE, int W>
+__global__ __launch_bounds__(64 * W) void router_tile_kernel(const float* __restrict__ x,
                                                                       const float* __restrict__ router, int width,
                                                                       int experts, int tokens,
                                                                       double* __restrict__ logits) {
   typedef float f4 __attribute__((ext_vector_type(4)));
-  __shared__ double part[kRouteWaves][4 * NE][64];
+  __shared__ double part[W][4 * NE][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, q = lane >> 4;
   const int t0 = blockIdx.y * 16, e0 = blockIdx.x * (16 * NE);
@@ -107,12 +108,12 @@ __global__ __launch_bounds__(64 * kRouteWaves) void router_tile_kernel(const flo
   // two steps on their way (past the last one: it again, and its use is left out)
   Step st[3];
   load(st[0], min(wave, steps - 1));
-  load(st[1], min(wave + kRouteWaves, steps - 1));
-  for (int s = wave; s < steps; s += 3 * kRouteWaves) {
+  load(st[1], min(wave + W, steps - 1));
+  for (int s = wave; s < steps; s += 3 * W) {
 #pragma unroll
     for (int i = 0; i < 3; i++) {
-      const int now = s + i * kRouteWaves;
-      load(st[(i + 2) % 3], min(now + 2 * kRouteWaves, steps - 1));
+      const int now = s + i * W;
+      load(st[(i + 2) % 3], min(now + 2 * W, steps - 1));
       __builtin_amdgcn_sched_barrier(0);
       if (now < steps) use(st[i], now);
     }
@@ -122,11 +123,11 @@ __global__ __launch_bounds__(64 * kRouteWaves) void router_tile_kernel(const flo
 #pragma unroll
     for (int j = 0; j < 4; j++) part[wave][4 * k + j][lane] = acc[k][j];
   __syncthreads();
-  for (int i = threadIdx.x; i < 256 * NE; i += 64 * kRouteWaves) {
+  for (int i = threadIdx.x; i < 256 * NE; i += 64 * W) {
     const int l = i & 63, j = (i >> 6) & 3, k = i >> 8;
     double v = part[0][4 * k + j][l];
 #pragma unroll
-    for (int w = 1; w < kRouteWaves; w++) v += part[w][4 * k + j][l];
+    for (int w = 1; w < W; w++) v += part[w][4 * k + j][l];
     const int t = t0 + 4 * j + (l >> 4), e = e0 + 16 * k + (l & 15);
     if (t < tokens && e < experts) logits[(int64_t)t * experts + e] = v;
   }
@@ -347,11 +348,17 @@ int launch_router(hipStream_t s, const float* x, const float* router, const floa
   if ((int64_t)tokens * experts * width < kRouteTile)
     hipLaunchKernelGGL(router_logits_kernel, dim3((experts + 3) / 4, (tokens + kRouteTok - 1) / kRouteTok), dim3(256), 0, s,
                        x, router, width, experts, tokens, logits);
+  // (the widest blocks that give every compute unit one: 1024 tokens, 128 experts of 4096
+  // values 42 us a call at NE = 1, 31 at 2; 2048 tokens, 64 of 2048 25, 20)
+  else if (experts > 16 && (int64_t)tiles * ((experts + 63) / 64) < cu_count() &&
+           (int64_t)tiles * ((experts + 31) / 32) >= cu_count())
+    hipLaunchKernelGGL((router_tile_kernel<2, 4>), dim3((experts + 31) / 32, tiles), dim3(256), 0, s, x, router, width,
+                       experts, tokens, logits);
   else if ((int64_t)tiles * ((experts + 63) / 64) < cu_count() || experts <= 16)
-    hipLaunchKernelGGL(router_tile_kernel<1>, dim3((experts + 15) / 16, tiles), dim3(64 * kRouteWaves), 0, s, x, router, width,
+    hipLaunchKernelGGL((router_tile_kernel<1, 8>), dim3((experts + 15) / 16, tiles), dim3(512), 0, s, x, router, width,
                        experts, tokens, logits);
   else
-    hipLaunchKernelGGL(router_tile_kernel<4>, dim3((experts + 63) / 64, tiles), dim3(64 * kRouteWaves), 0, s, x, router, width,
+    hipLaunchKernelGGL((router_tile_kernel<4, 4>), dim3((experts + 63) / 64, tiles), dim3(256), 0, s, x, router, width,
                        experts, tokens, logits);
   int rc = hip_check(hipGetLastError(), "router launch");
   if (rc) return rc;
