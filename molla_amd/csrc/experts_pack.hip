@@ -10,8 +10,8 @@
 //
 // What bounds it is the experts' weights, so nothing waits for anything else: a block
 // takes its expert's rows of x as floats, kPackCols columns at a time, makes their halves
-// itself (no launch ahead, no list of rows: as in the row kernel, the block of an
-// expert's first pair takes them all) and keeps them in LDS, the next columns on their
+// itself (no launch ahead, no list of rows: a block finds its eight among the ids) and
+// keeps them in LDS, the next columns on their
 // way, while each wave streams its own 32 rows of weights, one or two superblocks
 // ahead.  A chunk has a power of two a row, of the largest size in it.
 //
@@ -125,8 +125,11 @@ __global__ __launch_bounds__(64 * kPackWaves, 2) void experts_pack_kernel(
   const int n = lane & 15, kq = lane >> 4;
   const int first = blockIdx.y, id = lane < pairs ? ids[lane] : -1;
   const int e = __builtin_amdgcn_readlane(id, first);
+  // (uniform over the block) every eighth pair's block takes it and the seven behind it
   uint64_t mine = __ballot(id == e);
-  if ((uint32_t)e >= (uint32_t)experts || (mine & ((1ull << first) - 1))) return;  // (uniform over the block)
+  const uint64_t before = mine & ((1ull << first) - 1);
+  if ((uint32_t)e >= (uint32_t)experts || __builtin_popcountll(before) % kPackRows) return;
+  mine ^= before;
 
   // this wave's rows: two tiles of 16 of one matrix, or the same 16 of both
   const int row0 = (blockIdx.x * kPackWaves + wave) * (GLU ? 16 : 32);
@@ -138,170 +141,166 @@ __global__ __launch_bounds__(64 * kPackWaves, 2) void experts_pack_kernel(
   const int c0 = blockIdx.z * chunks_per_split, c1 = min(c0 + chunks_per_split, chunks);
   const int sb0 = c0 * kSb, sb1 = min(c1 * kSb, nsb);
 
-  while (mine) {
-    // the next eight pairs of the expert
-    int count = 0;
-    __syncthreads();  // (the last ones' list has been read)
-    for (; mine && count < kPackRows; mine &= mine - 1, count++)
-      if ((int)threadIdx.x == count) pair_of[count] = __builtin_ctzll(mine);
-    // rows that are not there
-    if (count < kPackRows) {
-      for (int i = threadIdx.x; i < (int)(sizeof(xl) / 16); i += 64 * kPackWaves) ((v4u*)xl)[i] = v4u{0, 0, 0, 0};
-      for (int i = threadIdx.x; i < (int)(sizeof(xm) / 16); i += 64 * kPackWaves) ((v4u*)xm)[i] = v4u{0, 0, 0, 0};
+  int count = 0;
+  for (; mine && count < kPackRows; mine &= mine - 1, count++)
+    if ((int)threadIdx.x == count) pair_of[count] = __builtin_ctzll(mine);
+  // rows that are not there
+  if (count < kPackRows) {
+    for (int i = threadIdx.x; i < (int)(sizeof(xl) / 16); i += 64 * kPackWaves) ((v4u*)xl)[i] = v4u{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < (int)(sizeof(xm) / 16); i += 64 * kPackWaves) ((v4u*)xm)[i] = v4u{0, 0, 0, 0};
+  }
+  __syncthreads();
+
+  Unit un[S][RT];
+  auto load = [&](Unit(&u)[RT], int sb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) u[rt].load(wrow[rt], min(sb, sb1 - 1), kq);
+  };
+#pragma unroll
+  for (int k = 0; k < S - 1; k++) load(un[k], sb0 + k);
+
+  // A chunk's activations: a row has 32 lanes, lane c takes its runs 32 k + c of 8 values
+  const int m = 2 * wave + (lane >> 5), c = lane & 31;
+  const bool there = m < count;
+  const float* xrow = x + (int64_t)(pair_of[min(m, count - 1)] / share) * cols;
+  v4f v[kRuns][2];
+  auto load_x = [&](int ch) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < kRuns; k++) {
+      const float* p = xrow + min(ch * kPackCols + 8 * (32 * k + c), cols - 8);
+      v[k][0] = *(const v4f*)p;
+      v[k][1] = *(const v4f*)(p + 4);
     }
-    __syncthreads();
-
-    Unit un[S][RT];
-    auto load = [&](Unit(&u)[RT], int sb) __attribute__((always_inline)) {
+  };
+  auto store_x = [&](int ch, int buf) __attribute__((always_inline)) {
+    float mx = 0.0f;
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++) u[rt].load(wrow[rt], min(sb, sb1 - 1), kq);
-    };
+    for (int k = 0; k < kRuns; k++) {
+      if (ch * kPackCols + 8 * (32 * k + c) >= cols) v[k][0] = v[k][1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < S - 1; k++) load(un[k], sb0 + k);
-
-    // A chunk's activations: a row has 32 lanes, lane c takes its runs 32 k + c of 8 values
-    const int m = 2 * wave + (lane >> 5), c = lane & 31;
-    const bool there = m < count;
-    const float* xrow = x + (int64_t)(pair_of[min(m, count - 1)] / share) * cols;
-    v4f v[kRuns][2];
-    auto load_x = [&](int ch) __attribute__((always_inline)) {
-#pragma unroll
-      for (int k = 0; k < kRuns; k++) {
-        const float* p = xrow + min(ch * kPackCols + 8 * (32 * k + c), cols - 8);
-        v[k][0] = *(const v4f*)p;
-        v[k][1] = *(const v4f*)(p + 4);
-      }
-    };
-    auto store_x = [&](int ch, int buf) __attribute__((always_inline)) {
-      float mx = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kRuns; k++) {
-        if (ch * kPackCols + 8 * (32 * k + c) >= cols) v[k][0] = v[k][1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[k][j >> 2][j & 3]));
-      }
-      const int ex = scale_exp(lanes::reduce<32>(mx, lanes::Max{}));
-      if (c == 0) scale[buf][m] = there ? ldexpf(1.0f, ex) : 0.0f;
-#pragma unroll
-      for (int k = 0; k < kRuns; k++) {
-        v8h hi, lo;
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          constexpr int kOrder[4] = {0, 2, 1, 3};  // the order of K
-          const float f = ldexpf(v[k][j >> 2][kOrder[j & 3]], -ex);
-          _Float16 h, l;
-          split_half(f, h, l);
-          hi[j] = h;
-          lo[j] = l;
-          sum += f;
-        }
-        sum = lanes::reduce<4>(sum, lanes::Add{}) * (1.0f / 32.0f);
-        if (!there) continue;
-        const int i = 32 * k + c, sb = i >> 5, g = (i >> 2) & 7, r = i & 3;  // superblock, group, run of it
-        uint8_t* dst = &xl[buf][sb][4 * (g >> 2) + 2 * Unit::up_of(g) + (r & 1)][256 * (2 * Unit::which_of(g) + (r >> 1)) + 16 * m];
-        *(v8h*)dst = hi;
-        *(v8h*)(dst + 16 * kPackRows) = lo;
-        if (Unit::MINS && r == 0) {
-          _Float16 h, l;
-          split_half(sum, h, l);
-          xm[buf][sb][m][g] = h;
-          xm[buf][sb][kPackRows + m][g] = l;
-        }
-      }
-    };
-
-    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    v4f tot[RT], out[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) out[rt] = zero;
-    auto use = [&](const Unit(&u)[RT], int local, int buf) __attribute__((always_inline)) {
-      v4f acc[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; rt++) acc[rt] = zero;
-      const uint8_t* at = &xl[buf][local][0][16 * lane];
-#pragma unroll
-      for (int st = 0; st < 8; st++) {
-        const v8h a = *(const v8h*)(at + 1024 * st);
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-          v8h b0, b1;
-          u[rt].codes(st >> 2, (st >> 1) & 1, st & 1, kq, b0, b1);
-          acc[rt] = mfma16(a, b0, acc[rt]);
-          if constexpr (Unit::LIMBS == 2) acc[rt] = mfma16(a, b1, acc[rt]);
-        }
-      }
-      if constexpr (Unit::MINS) {
-        // (lanes past the first 16 hold values 8..31 of the mins' step: zeros)
-        const v8h am = kq == 0 ? *(const v8h*)xm[buf][local][n] : v8h{0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-          const v4f cm = mfma16(am, u[rt].mins(), zero);
-          const float dm = -32.0f * u[rt].dmin();
-#pragma unroll
-          for (int j = 0; j < 4; j++) tot[rt][j] = fmaf(dm, cm[j], tot[rt][j]);
-        }
-      }
-#pragma unroll
-      for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) tot[rt][j] = fmaf(u[rt].d(), acc[rt][j], tot[rt][j]);
-    };
-
-    load_x(c0);
-    store_x(c0, 0);
-    __syncthreads();
-    int ch = c0, local = 0;
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) tot[rt] = zero;
-    load_x(min(c0 + 1, chunks - 1));
-    // superblock sb, after sending for sb + S - 1; at a chunk's end the next one's halves
-    auto step = [&](int sb, Unit(&now)[RT], Unit(&refill)[RT]) __attribute__((always_inline)) {
-      if (sb >= sb1) return;
-      load(refill, sb + S - 1);
-      __builtin_amdgcn_sched_barrier(0);
-      const int buf = (ch - c0) & 1;
-      use(now, local, buf);
-      if (++local < kSb && sb + 1 < sb1) return;
-#pragma unroll
-      for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          out[rt][j] = fmaf(scale[buf][(4 * kq + j) & 7], tot[rt][j], out[rt][j]);
-          tot[rt][j] = 0.0f;
-        }
-      local = 0;
-      if (++ch >= c1) return;
-      store_x(ch, 1 - buf);  // (read before the last barrier)
-      __syncthreads();
-      load_x(min(ch + 1, chunks - 1));
-    };
-    for (int sb = sb0; sb < sb1; sb += S) {
-#pragma unroll
-      for (int k = 0; k < S; k++) step(sb + k, un[k], un[(k + S - 1) % S]);
+      for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[k][j >> 2][j & 3]));
     }
+    const int ex = scale_exp(lanes::reduce<32>(mx, lanes::Max{}));
+    if (c == 0) scale[buf][m] = there ? ldexpf(1.0f, ex) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < kRuns; k++) {
+      v8h hi, lo;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        constexpr int kOrder[4] = {0, 2, 1, 3};  // the order of K
+        const float f = ldexpf(v[k][j >> 2][kOrder[j & 3]], -ex);
+        _Float16 h, l;
+        split_half(f, h, l);
+        hi[j] = h;
+        lo[j] = l;
+        sum += f;
+      }
+      sum = lanes::reduce<4>(sum, lanes::Add{}) * (1.0f / 32.0f);
+      if (!there) continue;
+      const int i = 32 * k + c, sb = i >> 5, g = (i >> 2) & 7, r = i & 3;  // superblock, group, run of it
+      uint8_t* dst = &xl[buf][sb][4 * (g >> 2) + 2 * Unit::up_of(g) + (r & 1)][256 * (2 * Unit::which_of(g) + (r >> 1)) + 16 * m];
+      *(v8h*)dst = hi;
+      *(v8h*)(dst + 16 * kPackRows) = lo;
+      if (Unit::MINS && r == 0) {
+        _Float16 h, l;
+        split_half(sum, h, l);
+        xm[buf][sb][m][g] = h;
+        xm[buf][sb][kPackRows + m][g] = l;
+      }
+    }
+  };
 
-    // high and low halves' sums: 32 lanes apart
+  const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  v4f tot[RT], out[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) out[rt] = zero;
+  auto use = [&](const Unit(&u)[RT], int local, int buf) __attribute__((always_inline)) {
+    v4f acc[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) acc[rt] = zero;
+    const uint8_t* at = &xl[buf][local][0][16 * lane];
+#pragma unroll
+    for (int st = 0; st < 8; st++) {
+      const v8h a = *(const v8h*)(at + 1024 * st);
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++) {
+        v8h b0, b1;
+        u[rt].codes(st >> 2, (st >> 1) & 1, st & 1, kq, b0, b1);
+        acc[rt] = mfma16(a, b0, acc[rt]);
+        if constexpr (Unit::LIMBS == 2) acc[rt] = mfma16(a, b1, acc[rt]);
+      }
+    }
+    if constexpr (Unit::MINS) {
+      // (lanes past the first 16 hold values 8..31 of the mins' step: zeros)
+      const v8h am = kq == 0 ? *(const v8h*)xm[buf][local][n] : v8h{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++) {
+        const v4f cm = mfma16(am, u[rt].mins(), zero);
+        const float dm = -32.0f * u[rt].dmin();
+#pragma unroll
+        for (int j = 0; j < 4; j++) tot[rt][j] = fmaf(dm, cm[j], tot[rt][j]);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) tot[rt][j] = fmaf(u[rt].d(), acc[rt][j], tot[rt][j]);
+  };
+
+  load_x(c0);
+  store_x(c0, 0);
+  __syncthreads();
+  int ch = c0, local = 0;
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) tot[rt] = zero;
+  load_x(min(c0 + 1, chunks - 1));
+  // superblock sb, after sending for sb + S - 1; at a chunk's end the next one's halves
+  auto step = [&](int sb, Unit(&now)[RT], Unit(&refill)[RT]) __attribute__((always_inline)) {
+    if (sb >= sb1) return;
+    load(refill, sb + S - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const int buf = (ch - c0) & 1;
+    use(now, local, buf);
+    if (++local < kSb && sb + 1 < sb1) return;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(out[rt][j]), __float_as_uint(out[rt][j]), false, false);
-        out[rt][j] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+        out[rt][j] = fmaf(scale[buf][(4 * kq + j) & 7], tot[rt][j], out[rt][j]);
+        tot[rt][j] = 0.0f;
       }
-    if (lane < 32) {
+    local = 0;
+    if (++ch >= c1) return;
+    store_x(ch, 1 - buf);  // (read before the last barrier)
+    __syncthreads();
+    load_x(min(ch + 1, chunks - 1));
+  };
+  for (int sb = sb0; sb < sb1; sb += S) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int k = 4 * kq + j;
-        if (k >= count) continue;
-        float* to = y + blockIdx.z * split_stride + (int64_t)pair_of[k] * rows + row0 + n;
-        if constexpr (GLU) {
-          if (row0 + n < rows) *to = ((act & MI_ACT_GELU) ? mv::gelu(out[0][j]) : mv::silu(out[0][j])) * out[1][j];
-        } else {
+    for (int k = 0; k < S; k++) step(sb + k, un[k], un[(k + S - 1) % S]);
+  }
+
+  // high and low halves' sums: 32 lanes apart
 #pragma unroll
-          for (int rt = 0; rt < RT; rt++)
-            if (row0 + 16 * rt + n < rows) to[16 * rt] = out[rt][j];
-        }
+  for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(out[rt][j]), __float_as_uint(out[rt][j]), false, false);
+      out[rt][j] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    }
+  if (lane < 32) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int k = 4 * kq + j;
+      if (k >= count) continue;
+      float* to = y + blockIdx.z * split_stride + (int64_t)pair_of[k] * rows + row0 + n;
+      if constexpr (GLU) {
+        if (row0 + n < rows) *to = ((act & MI_ACT_GELU) ? mv::gelu(out[0][j]) : mv::silu(out[0][j])) * out[1][j];
+      } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+          if (row0 + 16 * rt + n < rows) to[16 * rt] = out[rt][j];
       }
     }
   }
