@@ -52,12 +52,11 @@ bool few_pairs(int64_t pairs, int32_t experts, int64_t weights) {
 // Whether they take the matrix cores instead, eight rows an operand (experts_pack.hip):
 // from where an expert's weights, unpacked once for all its pairs there, cost the row
 // kernel more.  us of an MLP, rows (or the tile, the last) / packed, by pairs: 8 experts
-// of 4096 x 14336 Q4_K 4 pairs 86 / 101, 8 173 / 144, 16 244 / 198, 32 345 / 217, 64 330
-// / 320; with Q6_K down 8 206 / 239, 12 272 / 279, 16 303 / 283, 32 448 / 390, 48 444 /
-// 456; all Q6_K 16 405 / 435, 24 565 / 435, 48 698 / 660, 64 701 / 751; 16 of 2048 x 4096
-// Q4_K 16 48 / 53, 24 69 / 63, 64 102 / 76; 64 of 2048 x 1024 48 43 / 53, 64 50 / 64.  A
-// product of 8 of 14336 x 4096: Q4_K 12 61 / 67, 16 72 / 65, 64 108 / 101; Q6_K 16 152 /
-// 165, 24 196 / 166, 64 262 / 258.
+// of 4096 x 14336 Q4_K 12 pairs 221 / 193, 16 244 / 213, 32 345 / 228, 64 330 / 289; with
+// Q6_K down 12 272 / 269, 16 303 / 288, 32 448 / 377, 48 444 / 452; all Q6_K 16 405 /
+// 435, 24 565 / 436, 48 698 / 691; 16 of 2048 x 4096 Q4_K 16 48 / 53, 24 69 / 67, 64 102 /
+// 76; 64 of 2048 x 1024 48 43 / 53, 64 50 / 64.  A product of 8 of 14336 x 4096: Q4_K 12
+// 61 / 63, 16 72 / 63, 64 108 / 88; Q6_K 16 152 / 165, 24 196 / 166, 64 262 / 258.
 bool pack_pairs(int kind, int64_t pairs, int32_t experts) {
   if (!pack_fits(kind) || pairs > kFewPairs) return false;
   return kind == MI_Q4_K ? 2 * pairs >= 3 * (int64_t)experts && pairs <= 8 * (int64_t)experts

@@ -312,10 +312,10 @@ bool pack_fits(int kind) { return kind == MI_Q4_K || kind == MI_Q6_K; }
 
 int pack_most_splits(int32_t cols) { return std::min((cols + kPackCols - 1) / kPackCols, 8); }
 
-// Parts of the columns: two blocks a CU, where the chunks allow it.
+// Parts of the columns: three blocks a CU, where the chunks allow it.
 int pack_splits(int32_t rows, int32_t cols, int32_t pairs, int32_t experts) {
   const int chunks = (cols + kPackCols - 1) / kPackCols, blocks = (rows + 127) / 128 * std::min(pairs, experts);
-  const int most = std::min(std::max(2 * cu_count() / blocks, 1), pack_most_splits(cols)), each = (chunks + most - 1) / most;
+  const int most = std::min(std::max(3 * cu_count() / blocks, 1), pack_most_splits(cols)), each = (chunks + most - 1) / most;
   return (chunks + each - 1) / each;
 }
 
