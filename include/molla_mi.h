@@ -489,8 +489,11 @@ int mi_decoder_layer_tree(mi_stream stream, const mi_layer_desc* desc, float* re
  * above it is taken for the last, one below 0 sees nothing.  q: rows of heads *
  * head_dim floats q_stride apart, out: the same contiguous, apart from q; both
  * 16-byte aligned.  A token that sees nothing gets zeros, and what it does not see
- * changes no bit of its result, whatever it holds.  A value that it sees and that
- * is not finite makes its place of the result not finite; a key, or a q8_0 factor,
+ * changes no bit of its result, whatever it holds.  (One exception: the tokens of a
+ * chunk over a q8_0 cache take their values at a power of two in common, so a finite
+ * factor that another one of them sees, 2^22 times those that this one does, may
+ * change how its sums round; not their accuracy.)  A value that it sees and that is
+ * not finite makes its place of the result not finite; a key, or a q8_0 factor,
  * leaves the heads over it undefined.  GQA groups and head widths as mi_attend.
  * Workspace: mi_attend_window_workspace, 256-byte aligned (one_seq: whether the
  * tokens are one sequence's chunk); neither it nor out shares a byte with an input. */

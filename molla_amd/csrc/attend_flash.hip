@@ -133,7 +133,9 @@ __device__ __forceinline__ void int8_halves(uint32_t w, fh2& a, fh2& b) {
 // gets zeros.  An f16 value that is not finite enters the product as zero, with the
 // 16-byte word it lies in, and is added in float32 at the end to the rows that see
 // it, as q8_0's keys are that are left out: what a row does not see changes nothing
-// of it.
+// of it.  (Over q8_0 X, and with it which keys are left out, goes by the factors that
+// some row of the tile sees: 2048 tokens of 32 heads of 128 over a window of 4096 1316 us
+// without that look, 1331 with it; 64-wide heads 86 and 86.)
 template <int D, bool Q8, bool PAGED, bool WIN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
     const float* __restrict__ q, int64_t q_stride, const __half* __restrict__ kc, const __half* __restrict__ vc,
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
   __shared__ __align__(16) float kf[Q8 ? 2 : 1][Q8 ? NT : 1][kSlice];  // q8_0 key factors
   __shared__ int vexp[Q8 ? 4 : 1];                                     // X of each wave's dims
   __shared__ int left_out;                                             // some key's values were
-  __shared__ int cmax[4], lmin[WIN ? 4 : 1];
+  __shared__ int cmax[4], lmin[WIN ? 4 : 1], gaps[WIN && Q8 ? 4 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int split = blockIdx.x, splits = gridDim.x, kvh = blockIdx.y, t0 = blockIdx.z * (kRows / group);
@@ -167,18 +169,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
   const int wave_min = -lanes::reduce<64>(live_row ? -cnt : -0x7fffffff, IMax{});
   if (lane == 0) cmax[wave] = wave_max;
   if (WIN && lane == 0) lmin[wave] = wave_low;
+  if constexpr (WIN && Q8) {
+    // whether this window and the one of the token before leave positions between them:
+    // where none do, the tile's windows are one run (a token that sees nothing may
+    // stand behind others, as padding does)
+    const int before = t > t0 && live_row ? win.count(pos[t - 1]) : cnt;
+    const bool gap = cnt > 0 && (before <= 0 || low > before || max(before - win.window, 0) > cnt);
+    const uint64_t any = __ballot(gap);
+    if (lane == 0) gaps[wave] = any != 0;
+  }
   if ((Q8 || WIN) && tid == 0) left_out = 0;
   __syncthreads();
   const int count = __builtin_amdgcn_readfirstlane(max(max(cmax[0], cmax[1]), max(cmax[2], cmax[3])));
   int slices = (count + kSlice - 1) / kSlice;
   // WIN: slices behind the first positions' ones, up to the windows', are left out
-  int near = 0, skip = 0;
+  int near = 0, skip = 0, least = 0;  // least: the lowest position of the tile's windows
   if constexpr (WIN) {
-    const int lo = __builtin_amdgcn_readfirstlane(min(min(lmin[0], lmin[1]), min(lmin[2], lmin[3]))) / kSlice;
+    least = __builtin_amdgcn_readfirstlane(min(min(lmin[0], lmin[1]), min(lmin[2], lmin[3])));
+    const int lo = least / kSlice;
     near = min((int)(((int64_t)win.first + kSlice - 1) / kSlice), lo);
     skip = lo - near;
     slices -= skip;
   }
+  bool apart = false;  // WIN, q8_0: the tile's windows leave positions between them
+  if constexpr (WIN && Q8) apart = __builtin_amdgcn_readfirstlane(gaps[0] | gaps[1] | gaps[2] | gaps[3]);
   auto slice_of = [&](int v) __attribute__((always_inline)) { return WIN && v >= near ? v + skip : v; };
   const int per = (slices + splits - 1) / splits;
   const int s0 = split * per, s1 = min(s0 + per, slices);
@@ -208,14 +222,33 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
   constexpr int PER = Q8 ? D / 64 : kSlice * PIECES / 256;  // 16-byte words of K (and of V)
   fu4 kr[PER], vr[PER];
   uint16_t kfr = 0, vfr = 0;  // the factor's bits (converted when stored: a use here would wait for the load)
-  uint64_t dead = 0;  // q8_0: the loaded slice's keys that no row reaches
+  uint64_t dead = 0;  // q8_0: the loaded values' keys that no row sees
   const int kvw = kv_heads * D;
   auto cell_of = [&](int sl, int key) __attribute__((always_inline)) {
     const int j = min(sl * kSlice + key, count - 1);
     return PAGED ? kv_index[j] : j;  // (negative: not held)
   };
   auto row_of = [&](int cell) __attribute__((always_inline)) { return (int64_t)max(cell, 0) * row_halves; };
-  auto load = [&](const __half* __restrict__ c, int sl, fu4 (&w)[PER], uint16_t& f) __attribute__((always_inline)) {
+  // q8_0: whether no row of the tile sees key `lane` of slice sl, which lies in `cell`:
+  // its factor may then be anything, and has no part in X
+  auto unseen = [&](int sl, int cell) __attribute__((always_inline)) {
+    const int key = sl * kSlice + lane;
+    bool no = key >= count || (PAGED && cell < 0);
+    if constexpr (WIN && Q8) {
+      if (apart) {  // (uniform)
+        bool in = key < win.first;
+        for (int i = 0; i < kRows / group && t0 + i < tokens; i++) {
+          const int c = win.count(pos[t0 + i]);
+          in |= key < c && key >= c - win.window;
+        }
+        no |= !in;
+      } else {
+        no |= key < least && key >= win.first;
+      }
+    }
+    return no;
+  };
+  auto load = [&](const __half* __restrict__ c, int sl, fu4 (&w)[PER], uint16_t& f, bool of_values) __attribute__((always_inline)) {
     if constexpr (Q8) {
       const int cell = cell_of(sl, lane);
       const __half* rowp = c + row_of(cell);
@@ -223,7 +256,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
 #pragma unroll
       for (int j = 0; j < PER; j++) w[j] = *(const fu4*)(b + 16 * j);
       f = ((const uint16_t*)rowp)[(kvw >> 1) + ((kvh * D + wave * (D / 4)) >> 5)];
-      dead = __ballot(sl * kSlice + lane >= count || (PAGED && cell < 0));
+      if (of_values) dead = __ballot(unseen(sl, cell));
     } else {
 #pragma unroll
       for (int j = 0; j < PER; j++) {
@@ -321,8 +354,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
   };
 
   // the first slice on its way behind the queries, ahead of their conversion
-  load(kc, slice_of(s0), kr, kfr);
-  load(vc, slice_of(s0), vr, vfr);
+  load(kc, slice_of(s0), kr, kfr, false);
+  load(vc, slice_of(s0), vr, vfr, true);
   __builtin_amdgcn_sched_barrier(0);
 
   // The query, scaled by the power of two that brings its largest value to
@@ -517,7 +550,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
     // this wave has tokens that reach the slice
     const bool mine = base < wave_max && (!WIN || base + kSlice > wave_low || base < win.first);
     const uint64_t cells_held = WIN && PAGED ? __ballot(cell >= 0) : ~0ull;
-    if (more) load(kc, slice_of(sv + 1), kr, kfr);
+    if (more) load(kc, slice_of(sv + 1), kr, kfr, false);
     if (WIN && PAGED && more) cell = cell_of(slice_of(sv + 1), lane);
     // the slice's weights, 32 keys at a time (both tiles' scores at once are 32
     // more registers than a wave has)
@@ -528,7 +561,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
         store_k(1 - buf);
         int next = slice_of(sv + 1);
         asm volatile("" : "+s"(next));  // (the keys' row offsets are not kept for it)
-        load(vc, next, vr, vfr);
+        load(vc, next, vr, vfr, true);
       }
     }
     if (Q8) __syncthreads();  // the one value buffer has been read
@@ -556,7 +589,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_flash_kernel(
         for (int sv = s0; sv < s1; sv++) {
           const int sl = slice_of(sv), cell = cell_of(sl, lane);
           float f = __half2float(vc[row_of(cell) + (kvw >> 1) + ((kvh * D) >> 5) + dt]);
-          if (sl * kSlice + lane >= count || cell < 0) f = 0.0f;
+          if (unseen(sl, cell)) f = 0.0f;
           for (uint64_t outs = __ballot(track(f, x)); outs; outs &= outs - 1) {
             const int k = __builtin_ctzll(outs);
             const int64_t row = row_of(__shfl(cell, k));
