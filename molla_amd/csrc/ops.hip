@@ -679,14 +679,19 @@ __global__ void attend_merge_kernel(const float* __restrict__ part_acc, const fl
     }
     const int n = min(chunks - c0, B);
     const float e = FOLD ? __builtin_amdgcn_exp2f(ml.x - M) : expf(ml.x - M);
-    const float w = lane < n && (!FOLD || ml.y != 0.0f) ? e : 0.0f;
+    const bool written = lane < n && (!FOLD || ml.y != 0.0f);
+    const float w = written ? e : 0.0f;
+    // WIN: a share that was written counts where its weight is zero too: a value in it
+    // that is not finite stays so
+    const uint64_t counts = WIN ? __ballot(written) : 0;
     L += lane < n ? ml.y * w : 0.0f;
 #pragma unroll
     for (int k = 0; k < B; k++) {
       // (a mask where a share may not have been written, and not a branch for each:
       // with the share kernel's own fold a layer of 2304 keys 29.4 -> 28.3 us)
       const uint32_t wk = __builtin_amdgcn_readlane(__float_as_int(w), k);
-      if (FOLD) o = fmaf(__uint_as_float(__float_as_uint(a[k]) & (wk ? 0xffffffffu : 0u)), __uint_as_float(wk), o);
+      const bool use = WIN ? (counts >> k) & 1 : wk != 0;
+      if (FOLD) o = fmaf(__uint_as_float(__float_as_uint(a[k]) & (use ? 0xffffffffu : 0u)), __uint_as_float(wk), o);
       else if (k < n) o = fmaf(a[k], __uint_as_float(wk), o);
     }
   }
