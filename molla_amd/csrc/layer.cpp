@@ -180,11 +180,7 @@ int check_sparse(const mi_layer_desc* d, int32_t tokens) {
   return MI_OK;
 }
 
-int check_desc(const mi_layer_desc* d) {
-  if (!d) return fail(MI_ERR_ARG, "layer: null descriptor");
-  if (d->width <= 0 || d->hidden <= 0 || d->width % 256 || d->hidden % 256)
-    return fail(MI_ERR_SHAPE, "layer: width %d / hidden %d must be positive multiples of 256", d->width,
-                d->hidden);
+int check_heads(const mi_layer_desc* d) {
   if (d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads)
     return fail(MI_ERR_SHAPE, "layer: %d query heads over %d key heads", d->heads, d->kv_heads);
   const int group = d->heads / d->kv_heads;
@@ -192,6 +188,16 @@ int check_desc(const mi_layer_desc* d) {
     return fail(MI_ERR_SHAPE, "layer: %d query heads per key head is not 1, 2, 4 or 8", group);
   if (d->head_dim <= 0 || d->head_dim % 32 || d->head_dim > 512)
     return fail(MI_ERR_SHAPE, "layer: head_dim %d", d->head_dim);
+  return MI_OK;
+}
+
+int check_desc(const mi_layer_desc* d) {
+  if (!d) return fail(MI_ERR_ARG, "layer: null descriptor");
+  if (d->width <= 0 || d->hidden <= 0 || d->width % 256 || d->hidden % 256)
+    return fail(MI_ERR_SHAPE, "layer: width %d / hidden %d must be positive multiples of 256", d->width,
+                d->hidden);
+  int rc = check_heads(d);
+  if (rc) return rc;
   if (cache_row(d->cache_form, d->kv_heads * d->head_dim) < 0)
     return fail(MI_ERR_SHAPE, "layer: cache form %d has no row for %d key heads of %d", d->cache_form, d->kv_heads,
                 d->head_dim);
@@ -224,7 +230,7 @@ int check_desc(const mi_layer_desc* d) {
     int rc = check_weight(e.name, e.w.kind, e.w.data, e.w.row_bytes, e.w.rows, e.w.cols);
     if (rc) return rc;
   }
-  int rc = check_sparse(d, 1);
+  rc = check_sparse(d, 1);
   if (!rc && d->experts) {
     const mi_experts x = experts_of(d);
     rc = check_experts("layer", &x);
@@ -940,6 +946,7 @@ extern "C" {
 
 size_t mi_layer_workspace(const mi_layer_desc* desc, int32_t max_count, int32_t tokens) {
   if (!desc || max_count <= 0 || tokens <= 0 || tokens > kMaxPrefill || check_sparse(desc, tokens)) return 0;
+  if (desc->window && check_heads(desc)) return 0;  // (a window's plan divides by them)
   if (tokens > kMaxTokens) return prefill_carve(desc, max_count, tokens).total;
   return carve(desc, max_count, tokens).total;
 }
