@@ -711,7 +711,7 @@ __global__ __launch_bounds__(256) void attend_combine_kernel(const float* __rest
 // most one for each slice of the context (of what a tile's windows reach), and at
 // most 16 (each is another partial result of every row to write and fold).
 static int flash_slices(int32_t max_count, int tq, const Window* win) {
-  const int slices = (max_count + kSlice - 1) / kSlice;
+  const int slices = (max_count - 1) / kSlice + 1;
   return win ? (int)std::min<int64_t>(slices, ((int64_t)win->window + tq + win->first) / kSlice + 3) : slices;
 }
 int flash_splits(int32_t heads, int32_t kv_heads, int32_t max_count, int32_t tokens, const Window* win) {

@@ -1153,7 +1153,7 @@ WindowPlan window_plan(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_
   } else {
     p.path = kSlices;
     const int kk = attn_slice(head_dim);
-    p.parts = (win.most() + kk - 1) / kk;
+    p.parts = (win.most() - 1) / kk + 1;  // (at least one key, and up to 2^31 - 1)
   }
   return p;
 }
