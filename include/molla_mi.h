@@ -251,7 +251,7 @@ typedef struct {
 
 typedef struct {
   int32_t width;    /* residual stream, 4096 for an 8B */
-  int32_t hidden;   /* MLP inner width, 14336 */
+  int32_t hidden;   /* MLP inner width, 14336; of one expert where there are experts */
   int32_t heads, kv_heads, head_dim; /* 32, 8, 128 */
   int32_t rope_dim; /* rotated elements per head, usually head_dim */
   int32_t neox;     /* 0 = adjacent pairs (Llama), 1 = half-split pairs */

@@ -193,7 +193,8 @@ int check_heads(const mi_layer_desc* d) {
 
 int check_desc(const mi_layer_desc* d) {
   if (!d) return fail(MI_ERR_ARG, "layer: null descriptor");
-  if (d->width <= 0 || d->hidden <= 0 || d->width % 256 || d->hidden % 256)
+  // (experts' width is check_experts's: none of their kernels asks for whole 256s)
+  if (d->width <= 0 || d->width % 256 || (!d->experts && (d->hidden <= 0 || d->hidden % 256)))
     return fail(MI_ERR_SHAPE, "layer: width %d / hidden %d must be positive multiples of 256", d->width,
                 d->hidden);
   int rc = check_heads(d);
