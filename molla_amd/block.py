@@ -91,6 +91,16 @@ class DeviceLayer:
             if t.dtype != torch.float32 or not t.is_cuda:
                 raise ValueError(f"{n} must be a device float32 tensor")
             setattr(d, n, t.data_ptr())
+        if spec.experts > 0:
+            # (the descriptor has no lengths: a short or a transposed one would be read as it lies)
+            shapes = {"router": (spec.experts, spec.width), "router_bias": (spec.experts,)}
+            for n, shape in shapes.items():
+                t = self.extras.get(n)
+                if t is None and n == "router":
+                    raise ValueError(f"a layer of {spec.experts} experts wants its router")
+                flat = (math.prod(shape),)
+                if t is not None and (tuple(t.shape) not in (shape, flat) or not t.is_contiguous()):
+                    raise ValueError(f"{n} must be {shape}, or {flat[0]} values one after another")
         d.ungated, d.act = int(spec.ungated), int(spec.act)
         d.experts, d.experts_used = spec.experts, spec.experts_used
         d.router_flags, d.router_scale = spec.router_flags, spec.router_scale
