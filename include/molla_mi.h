@@ -496,7 +496,8 @@ int mi_decoder_layer_tree(mi_stream stream, const mi_layer_desc* desc, float* re
  * not finite makes its place of the result not finite; a key, or a q8_0 factor,
  * leaves the heads over it undefined.  GQA groups and head widths as mi_attend.
  * Workspace: mi_attend_window_workspace, 256-byte aligned (one_seq: whether the
- * tokens are one sequence's chunk); neither it nor out shares a byte with an input. */
+ * tokens are one sequence's chunk); neither it nor out shares a byte with an input
+ * (of a pool of cells that is the caller's to see to: its size is not known here). */
 size_t mi_attend_window_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, int32_t window,
                                   int32_t first, int32_t max_count, int32_t tokens, int32_t one_seq);
 int mi_attend_window(mi_stream stream, int32_t form, const float* q, int64_t q_stride, const uint16_t* k_cache,

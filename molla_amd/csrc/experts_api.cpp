@@ -310,7 +310,8 @@ int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_byt
   const MatmulCarve c = matmul_carve(experts, cols, share, pairs, few);
   if (!work || ((uintptr_t)work & 255) || work_bytes < c.total)
     return fail(MI_ERR_WORKSPACE, "experts_matmul: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, c.total);
-  if (meet(work, c.total, x, xb) || meet(work, c.total, y, yb) || meet(work, c.total, ids, 4 * (size_t)pairs))
+  if (meet(work, c.total, x, xb) || meet(work, c.total, y, yb) || meet(work, c.total, ids, 4 * (size_t)pairs) ||
+      meet(work, c.total, w, (size_t)experts * rows * row_bytes))
     return fail(MI_ERR_ARG, "experts_matmul: the workspace lies in another buffer");
   hipStream_t s = (hipStream_t)stream;
   char* base = (char*)work;
@@ -361,11 +362,19 @@ int mi_experts_mlp(mi_stream stream, const mi_experts* d, const float* x, int32_
   if (((uintptr_t)x | (uintptr_t)out) & 15)
     return fail(MI_ERR_ALIGN, "experts_mlp: the input and the output must be 16-byte aligned");
   const size_t xb = 4 * (size_t)tokens * d->width, pb = 4 * (size_t)tokens * used;
-  if (meet(out, xb, ids, pb) || meet(out, xb, weights, pb)) return fail(MI_ERR_ARG, "experts_mlp: the output lies in an input");
+  // (of the experts' matrices)
+  auto in_stacks = [d](const void* p, size_t n) {
+    for (const mi_weight* w : {&d->gate, &d->up, &d->down})
+      if (meet(p, n, w->data, (size_t)w->rows * w->row_bytes)) return true;
+    return false;
+  };
+  if (meet(out, xb, ids, pb) || meet(out, xb, weights, pb) || in_stacks(out, xb))
+    return fail(MI_ERR_ARG, "experts_mlp: the output lies in an input");
   const size_t need = experts_workspace(*d, tokens, used);
   if (!work || ((uintptr_t)work & 255) || work_bytes < need)
     return fail(MI_ERR_WORKSPACE, "experts_mlp: workspace of %zu bytes (256-aligned), %zu needed", work_bytes, need);
-  if (meet(work, need, x, xb) || meet(work, need, out, xb) || meet(work, need, ids, pb) || meet(work, need, weights, pb))
+  if (meet(work, need, x, xb) || meet(work, need, out, xb) || meet(work, need, ids, pb) || meet(work, need, weights, pb) ||
+      in_stacks(work, need))
     return fail(MI_ERR_ARG, "experts_mlp: the workspace lies in another buffer");
   return launch_experts_mlp((hipStream_t)stream, *d, x, tokens, used, ids, weights, out, epi == MI_EPI_ADD, work);
 }

@@ -409,6 +409,14 @@ int mi_attend_form(mi_stream stream, int32_t form, const float* q, const uint16_
                        kv_heads, head_dim, scale, nullptr, count, count, 1, out, nullptr, work, form);
 }
 
+// Whether `bytes` from `at` on share one with `count` runs of `run` bytes, `stride` apart
+// from `first` on.
+static bool runs_meet(uintptr_t at, size_t bytes, uintptr_t first, size_t run, size_t stride, int64_t count) {
+  // the first run that ends behind `at`
+  const int64_t r = at < first + run ? 0 : stride ? (int64_t)((at - first - run) / stride + 1) : count;
+  return r < count && first + r * stride < at + bytes;
+}
+
 // The shape of attention over a window.
 static int check_window(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t form, int32_t window, int32_t first,
                         int32_t max_count, int32_t tokens) {
@@ -464,6 +472,13 @@ int mi_attend_window(mi_stream stream, int32_t form, const float* q, int64_t q_s
     for (const auto& b : in)
       if (b.at && (const char*)w.at < (const char*)b.at + b.bytes && (const char*)b.at < (const char*)w.at + w.bytes)
         return fail(MI_ERR_ARG, "attend_window: the output or the workspace lies in an input");
+  // (the sequences' caches, between which there may be anything; how far a pool of cells
+  // reaches is not known here)
+  for (const auto& w : written)
+    for (const uint16_t* c : {k_cache, v_cache})
+      if (!kv_index && w.at && runs_meet((uintptr_t)w.at, w.bytes, (uintptr_t)c, 2 * (size_t)max_count * row,
+                                         2 * (size_t)stride, stride ? tokens : 1))
+        return fail(MI_ERR_ARG, "attend_window: the output or the workspace lies in a cache");
   if ((const char*)work < (const char*)out + written[1].bytes && (const char*)out < (const char*)work + need)
     return fail(MI_ERR_ARG, "attend_window: the workspace lies in the output");
   if (!work || ((uintptr_t)work & 255) || work_bytes < need)
