@@ -1,4 +1,4 @@
-"""Checks the gfx950 assembly of prefill.hip: every direct load to LDS
+"""Checks the gfx950 assembly of prefill_kernel.h's kernels: every direct load to LDS
 (global_load_lds, issued by inline assembly that the compiler does not count)
 has landed before the barrier after which other waves read it.
 
@@ -16,6 +16,9 @@ order of execution.
 m0 holds an LDS load's address, and the compiler does not know that the assembly
 writes it: it may appear only where a load sets it, with nothing but an s_nop
 before the load.
+
+That address is 16 bits, and the buffers take up to all 65536 bytes: they start at 0,
+as the kernel's one LDS object.  A kernel's LDS is therefore as large as that object.
 """
 
 import re
@@ -25,6 +28,8 @@ LDS_LOAD = re.compile(r"(global|buffer)_load_lds_|(global|buffer)_load_\S+\s.*\b
 LOAD = re.compile(r"(global|buffer)_load_")
 M0 = re.compile(r"\bm0\b")
 VMCNT = re.compile(r"vmcnt\((\d+)\)")
+KERNEL = re.compile(r"\.amdhsa_kernel \S*?\d(prefill|group)_kernelILi\d+ELi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)E")
+LDS_SIZE = re.compile(r"\.amdhsa_group_segment_fixed_size (\d+)")
 
 
 def check(lines):
@@ -76,9 +81,29 @@ def check(lines):
     return seen, bad
 
 
+def check_lds(lines):
+    """(kernels seen, messages about those whose LDS is not BlockLds's one object)."""
+    seen, bad, want = 0, [], None
+    for at, raw in enumerate(lines, 1):
+        found = KERNEL.search(raw)
+        if found:
+            rt, tt, wr, ks = (int(v) for v in found.groups()[1:])
+            want = max(ks * 2 * tt * 8192, tt * 32 * wr * rt * 32 * 4) + (tt * 256 if found.group(1) == "group" else 0)
+        size = LDS_SIZE.search(raw)
+        if size and want is not None:
+            seen += 1
+            if int(size.group(1)) != want:
+                bad.append(f"line {at}: {size.group(1)} bytes of LDS, where one object of {want} is expected")
+        if size:
+            want = None
+    return seen, bad
+
+
 def main(path):
     with open(path) as f:
-        seen, bad = check(f.read().splitlines())
+        lines = f.read().splitlines()
+    seen, bad = check(lines)
+    bad += check_lds(lines)[1]
     for b in bad:
         print(f"{path}: {b}", file=sys.stderr)
     if not seen:

@@ -454,6 +454,9 @@ struct BlockLds {
   static constexpr int kX = KS * 2 * kStageBytes, kSum = TT * 32 * WR * RT * 32 * 4;
   static_assert(kX <= 65536, "the transfer's LDS address is 16 bits");
   static constexpr int kBytes = kX > kSum ? kX : kSum;
+  // (grouped: a list's rows and their scales behind them.  The buffers start at 0, as
+  // their kernel has one LDS object: check_waits.py looks at its size in every build)
+  static constexpr int kLists = TT * 32 * 8;
 };
 template <int KIND, int RT, int TT, int WR, int KS, class G, bool GLU>
 __device__ __forceinline__ void prefill_block(
@@ -663,8 +666,8 @@ __device__ __forceinline__ void prefill_block(
   };
 
   // a list's rows and their scales, for the end (read there they were two latencies)
-  __shared__ int row_of[GROUPED ? TT * 32 : 1];
-  __shared__ float scale_of[GROUPED ? TT * 32 : 1];
+  int* const row_of = (int*)(lds + BlockLds<RT, TT, WR, KS>::kBytes);
+  float* const scale_of = (float*)(row_of + TT * 32);
   if constexpr (GROUPED) {
     if ((int)threadIdx.x < TT * 32) {
       row_of[threadIdx.x] = gr.order[tile0 * 32 + threadIdx.x];
@@ -784,7 +787,7 @@ template <int KIND, int RT, int TT, int WR, int KS, bool GLU>
 __global__ __launch_bounds__(WR * KS * 64, (WR * KS + 3) / 4) void group_kernel(
     const RowSegs sg, int cols, int slots, const uint8_t* __restrict__ work, int chunks_per_split, float* __restrict__ y,
     int64_t ldy, int epi, const Groups gr) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[BlockLds<RT, TT, WR, KS>::kBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[BlockLds<RT, TT, WR, KS>::kBytes + BlockLds<RT, TT, WR, KS>::kLists];
   // (both loads at once: there are lists for the whole grid, those past the count unwritten)
   GroupTile gt = gr.tiles[blockIdx.y];
   int count = *gr.count;
