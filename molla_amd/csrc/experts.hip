@@ -18,11 +18,14 @@ namespace {
 // logits[t][e] = x[t] . router[e], products and sums in float64: which of two
 // near scores is larger must not hang on the order of a sum.
 constexpr int kRouteTok = 4;  // tokens a wave takes
-// Products of a call from which the matrix cores take it, whose blocks are a longer
-// chain.  us a call, a wave an expert / matrix cores: 128 experts of 4096 values, 128
-// tokens 17.4 / 21.5, 256 29.0 / 21.6; 64 of 2048, 256 tokens 11.5 / 13.6, 512 17.8 /
-// 14.0; 8 of 4096, 2048 tokens 16.8 / 19.0.
-constexpr int64_t kRouteTile = 1 << 26;
+// Scores (tokens times experts) of a call from which the matrix cores take it.  Both
+// kernels' time grows with the width, a wave an expert's with the scores besides, the
+// matrix cores' little before the chip is full.  us a call, a wave an expert / matrix
+// cores, with the choice: 128 experts of 4096 values, 128 tokens 17.4 / 23.5, 192 22.4 /
+// 23.4, 224 25.0 / 23.6, 256 28.5 / 23.9; 64 of 2048, 384 tokens 14.1 / 15.1, 448 15.9 /
+// 15.2, 512 17.1 / 15.2; 8 of 4096, 2048 tokens 18.5 / 19.7, 3584 25.6 / 21.4; 128 of
+// 8192, 224 tokens 41.6 / 37.0; of 1024, 256 tokens 12.6 / 13.2; of 512, 512 14.2 / 11.2.
+constexpr int64_t kRouteTile = 28672;
 __global__ __launch_bounds__(256) void router_logits_kernel(const float* __restrict__ x,
                                                             const float* __restrict__ router, int width, int experts,
                                                             int tokens, double* __restrict__ logits) {
@@ -345,7 +348,7 @@ int launch_router(hipStream_t s, const float* x, const float* router, const floa
                   int32_t used, int32_t tokens, int32_t flags, float scale, int32_t* ids, float* weights, void* work) {
   double* logits = (double*)work;
   const int tiles = (tokens + 15) / 16;
-  if ((int64_t)tokens * experts * width < kRouteTile)
+  if ((int64_t)tokens * experts < kRouteTile)
     hipLaunchKernelGGL(router_logits_kernel, dim3((experts + 3) / 4, (tokens + kRouteTok - 1) / kRouteTok), dim3(256), 0, s,
                        x, router, width, experts, tokens, logits);
   // (the widest blocks that give every compute unit one: 1024 tokens, 128 experts of 4096
