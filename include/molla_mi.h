@@ -73,7 +73,12 @@ enum { MI_EPI_NONE = 0, MI_EPI_BIAS = 1, MI_EPI_ADD = 2, MI_EPI_GLU = 4, MI_ACT_
 
 /* ---- library ------------------------------------------------------------- */
 
-int mi_version(void);                 /* (major << 16) | minor */
+/* (major << 16) | minor of this header.  A descriptor may grow at its end from one
+ * minor number to the next, and a call reads all of it: a caller compares mi_version()
+ * with the MI_VERSION that it was built with, ahead of its first call.  (1: mi_layer_desc
+ * up to prenormed; 2: up to first.) */
+#define MI_VERSION 2
+int mi_version(void);
 const char* mi_last_error(void);      /* last refusal / HIP error on this thread */
 int mi_sync(mi_stream stream);        /* hipStreamSynchronize; ctx.synchronize() in the reference */
 int mi_block_elements(int kind);      /* quant.mojo:78 */

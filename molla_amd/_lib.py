@@ -51,6 +51,8 @@ class MiExperts(ctypes.Structure):
                [(n, MiWeight) for n in ("gate", "up", "down")]
 
 
+VERSION = 2  # MI_VERSION of the header that these structs and signatures follow
+
 # Every symbol include/molla_mi.h declares, with its C signature.
 SIGNATURES = {
     "mi_version": (ctypes.c_int, []),
@@ -127,6 +129,9 @@ def lib():
             fn = getattr(l, name)
             fn.restype = res
             fn.argtypes = args
+        if l.mi_version() != VERSION:
+            raise RuntimeError(f"{LIB_PATH} is of version {l.mi_version()}, its callers here of {VERSION}: "
+                               "build it again (`make -C molla_amd/csrc`)")
         _lib = l
     return _lib
 

@@ -126,7 +126,7 @@ using namespace mi;
 
 extern "C" {
 
-int mi_version(void) { return (0 << 16) | 1; }
+int mi_version(void) { return MI_VERSION; }
 
 const char* mi_last_error(void) { return g_err; }
 
