@@ -544,11 +544,12 @@ int mi_experts_matmul(mi_stream stream, int kind, const void* w, int64_t row_byt
 
 /* The experts' gated MLP: out[t] = sum over k < used of weights[t * used + k] *
  * down[e](act(gate[e] x[t]) * (up[e] x[t])), e = ids[t * used + k]; with MI_EPI_ADD
- * added to out.  A pair whose id is no expert takes no part; the sum runs in the
- * order of k.  gate and up are of one kind, their rows experts * hidden, down's
- * experts * width.  out may be x.  Workspace: mi_experts_workspace, 256-byte
- * aligned (one for the most tokens holds calls of fewer, here and for the other
- * calls of this section and the one above); x and out 16-byte aligned. */
+ * added to out.  A pair whose id is no expert takes no part.  The order of the sum
+ * goes by the sizes and kinds alone: a call gives the same bits each time.  gate and
+ * up are of one kind, their rows experts * hidden, down's experts * width.  out may be
+ * x.  Workspace: mi_experts_workspace, 256-byte aligned (one for the most tokens holds
+ * calls of fewer, here and for the other calls of this section and the one above); x
+ * and out 16-byte aligned. */
 typedef struct {
   int32_t experts;
   int32_t width, hidden; /* of one expert, multiples of 64 (256 for the K-quants) */
